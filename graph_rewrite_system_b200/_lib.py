@@ -6,6 +6,7 @@ operation of this package.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from pathlib import Path
 import re
@@ -153,6 +154,23 @@ class pinned_stream:
 
     def __exit__(self, *exc):
         _PINNED_STREAM.pop()
+
+
+def on_device(t: torch.Tensor):
+    """Context that makes t's device current for a launch (the library's
+    launches and device queries go to the current device)."""
+    if t.device.index is None or t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def scratch(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
+    """Uninitialised bytes for one call that is enqueued on `stream`: when that
+    is not torch's current stream, the allocator is told of the use."""
+    work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if nbytes and stream != torch.cuda.current_stream(device).cuda_stream:
+        work.record_stream(torch.cuda.ExternalStream(stream, device=device))
+    return work
 
 
 def require_cuda(*tensors: torch.Tensor | None) -> None:

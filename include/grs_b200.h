@@ -588,6 +588,73 @@ GRS_API int grs_shard_route(const int64_t* child_proposal, const int64_t* summar
 GRS_API int grs_rows_copy(int nseg, const int64_t* segments, const int64_t* n_dev,
                           int64_t n_max, void* stream);
 
+/* ---- prompts, long shared prefixes, next-token logits --------------------
+ * No reference counterpart: the reference's model reads its action history
+ * one token at a time and scores rewrites, not tokens.
+ *
+ * Causal attention over packed prompts: query [tokens, heads, D], key/value
+ * [tokens, kv_heads, D], output [tokens, heads, D] (strides per token and
+ * head in elements; D contiguous, 1..256).  heads is a multiple of kv_heads;
+ * query head i reads K/V head i / (heads / kv_heads).  offsets int32
+ * [sequences + 1], ascending: sequence j is the tokens offsets[j] ..
+ * offsets[j+1] - 1, and its token i attends to its own tokens up to i.
+ * Sequences may be empty.  Output rows of tokens outside every sequence are
+ * left as they were, or zeroed with clear_rest; what their query, key and
+ * value rows hold (NaN too) reaches no other row.  Any content of offsets is
+ * safe: it moves no access out of the tensors.  `status` (device int32, may be
+ * null) receives GRS_ERR_TIMEOUT if a bounded in-kernel wait gives up.
+ * The output overlaps none of the inputs. */
+GRS_API int grs_prompt_attention(int dtype, const void* query, int64_t q_st, int64_t q_sh,
+                                 const void* key, int64_t k_st, int64_t k_sh, const void* value,
+                                 int64_t v_st, int64_t v_sh, const int32_t* offsets,
+                                 int sequences, void* out, int64_t o_st, int64_t o_sh, int tokens,
+                                 int heads, int kv_heads, int head_width, float scale,
+                                 int clear_rest, int32_t* status, void* stream);
+
+/* One query per beam, query/output [batch, heads, D], against the prefix
+ * key/value [num_prefix, kv_heads, D] that every beam shares, then the first
+ * lengths[b] tokens of the beam's pages (key/value cache [num_pages,
+ * page_size, kv_heads, D] of one layout; block_table int32 [batch,
+ * max_blocks]; max_blocks 0: no pages), then the beam's current token
+ * (current_key/value [batch, kv_heads, D] of one layout, or null;
+ * current_valid uint8 [batch], null = all valid).  Heads group as in
+ * grs_prompt_attention.  Beams with no key are written as zeros.  Page ids
+ * outside [0, num_pages) set GRS_ERR_BAD_PAGE in `status` and their tokens
+ * are skipped; lengths outside [0, max_blocks * page_size] set GRS_ERR_LENGTH
+ * and are clamped.  The workspace (fp32 partial sums of the prefix slices)
+ * is the call's own until it has run. */
+GRS_API int64_t grs_shared_prefix_workspace_bytes(int batch, int heads, int kv_heads,
+                                                  int head_width, int num_prefix);
+GRS_API int grs_shared_prefix_attention(
+    int dtype, const void* query, int64_t q_sb, int64_t q_sh, const void* prefix_key,
+    int64_t pk_st, int64_t pk_sh, const void* prefix_value, int64_t pv_st, int64_t pv_sh,
+    int num_prefix, const void* key_cache, const void* value_cache, int64_t kc_sp, int64_t kc_st,
+    int64_t kc_sh, const int32_t* block_table, int64_t bt_stride, int max_blocks,
+    const int32_t* lengths, int num_pages, int page_size, const void* current_key,
+    const void* current_value, int64_t ck_sb, int64_t ck_sh, const uint8_t* current_valid,
+    void* output, int64_t o_sb, int64_t o_sh, int batch, int heads, int kv_heads, int head_width,
+    float scale, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
+/* Next-token logits [rows, vocab] (bf16 or fp32, row strides in elements)
+ * adjusted into out (which may be logits itself).  For every token v of row b:
+ * if v is among the first lengths[b] history tokens (tokens int32 or int64
+ * [rows, history]; ids outside [0, vocab) are ignored), x = x > 0 ? x / r :
+ * x * r with the repetition penalty r; with c its count among the history
+ * tokens from prompt_lengths[b] on (null: from 0 on), c > 0 subtracts
+ * frequency * c + presence; then bias[v] is added (fp32, row stride bias_sb, 0
+ * = one row for all); then v is set to `fill` when bit v of the row's allowed
+ * words (int32 [rows, ceil(vocab / 32)], row stride a_sb) is clear.  lengths
+ * null: whole rows.  repetition/presence/frequency: fp32 [rows], or null for
+ * the scalar.  Arithmetic in fp32, rounded once. */
+GRS_API int grs_adjust_logits(int dtype, const void* logits, int64_t l_sb, void* out, int64_t o_sb,
+                              int rows, int vocab, const void* tokens, int tokens_are_i64,
+                              int64_t t_sb, int history, const int32_t* lengths,
+                              const int32_t* prompt_lengths, const float* repetition,
+                              const float* presence, const float* frequency,
+                              float repetition_all, float presence_all, float frequency_all,
+                              const float* bias, int64_t bias_sb, const int32_t* allowed,
+                              int64_t a_sb, float fill, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
