@@ -8,8 +8,10 @@
 // the beam's own keys, joins all parts by their weights and writes the output.
 #include <algorithm>
 #include <climits>
+#include <cmath>
+#include <type_traits>
 
-#include "grouped_attention.cuh"
+#include "grouped_attention_tc.cuh"
 
 namespace grs {
 
@@ -108,6 +110,7 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
   float norm = l * own;
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i] *= own;
+#pragma unroll 4
   for (int i = 0; i < a.slices; ++i) {
     const int64_t at = ((int64_t)i * a.batch + b) * a.heads + head;
     const float w = exp2f(a.part_lse[at] - base);
@@ -127,23 +130,65 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
   }
 }
 
-// Slices of the prefix: enough CTAs for two waves of 148 SMs, none shorter
-// than 256 keys.
-static int prefix_slices(int batch, int group, int kv_heads, int keys) {
-  if (keys <= 0) return 0;
+// How the prefix is cut: `parts` partial sums, `keys` per slice (two parts per
+// slice when the tensor-core kernel's slots halve it).
+struct PrefixPlan {
+  int slices, parts, keys;
+};
+
+// fp32 rows: enough CTAs for two waves of 148 SMs, none shorter than 256 keys.
+static PrefixPlan rows_plan(int batch, int group, int kv_heads, int keys) {
+  if (keys <= 0) return {0, 0, 0};
   const int64_t tiles = ((int64_t)batch * group + 63) / 64 * kv_heads;
-  const int64_t want = (2 * 148 + tiles - 1) / tiles;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (keys + 255) / 256));
+  const int64_t want =
+      std::max<int64_t>(1, std::min<int64_t>((2 * 148 + tiles - 1) / tiles, (keys + 255) / 256));
+  const int each = (int)(((keys + want - 1) / want + 127) / 128 * 128);
+  const int slices = (keys + each - 1) / each;
+  return {slices, slices, each};
 }
 
-static size_t part_bytes(int slices, int batch, int heads, int D) {
-  return (size_t)slices * batch * heads * D * 4;
+// Tensor cores: the count whose waves of 148 CTAs take the fewest 128-key
+// blocks, each wave paying about four blocks for its start and end and every
+// part the write and read of its fp32 sums (a block takes about 1.1 us).
+static PrefixPlan tc_plan(int batch, int heads, int kv_heads, int D, int keys) {
+  if (keys <= 0) return {0, 0, 0};
+  const int group = heads / kv_heads;
+  const bool split = grouped_tc_split(batch, group);
+  const int pps = std::max(1, 128 / group) * (split ? 1 : 2);
+  const int64_t tiles = ((int64_t)batch + pps - 1) / pps * kv_heads;
+  // slots of a split slice take turns on half the blocks each
+  const int blocks = (keys + 127) / 128, per = split ? 2 : 1;
+  const double join = 8.0 * batch * heads * D / 6.5e12 / 1.1e-6 + 0.02;
+  double best = 1e30;
+  int slices = 1;
+  for (int z = 1; z <= std::min(64, (blocks + per - 1) / per); ++z) {
+    const int64_t waves = (tiles * z + 147) / 148;
+    const int64_t each = ((blocks + z - 1) / z + per - 1) / per;
+    const double cost = (double)waves * (each + 4) + join * z * per;
+    if (cost < best) {
+      best = cost;
+      slices = z;
+    }
+  }
+  const int each = (blocks + slices - 1) / slices;
+  slices = (blocks + each - 1) / each;
+  return {slices, slices * per, each * 128};
+}
+
+static size_t plan_bytes(const PrefixPlan& p, int batch, int heads, int D) {
+  return (size_t)p.parts * batch * heads * (D + 1) * 4;
 }
 
 template <typename T>
-static int shared_prefix(const PagesArgs<T>& p, const GroupedArgs<T>& prefix, cudaStream_t stream) {
+static int shared_prefix(const PagesArgs<T>& p, const GroupedArgs<T>& prefix, bool tensor_cores,
+                         cudaStream_t stream) {
   if (prefix.slices > 0) {
-    const int status = grouped_rows_launch<T>(prefix, stream);
+    int status = GRS_OK;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      status = tensor_cores ? grouped_tc_launch(prefix, stream)
+                            : grouped_rows_launch<T>(prefix, stream);
+    else
+      status = grouped_rows_launch<T>(prefix, stream);
     if (status != GRS_OK) return status;
   }
   const int64_t rows = (int64_t)p.batch * p.heads;
@@ -161,9 +206,12 @@ static int shared_prefix(const PagesArgs<T>& p, const GroupedArgs<T>& prefix, cu
 extern "C" int64_t grs_shared_prefix_workspace_bytes(int batch, int heads, int kv_heads,
                                                      int head_width, int num_prefix) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || num_prefix <= 0) return 0;
-  const int slices = grs::prefix_slices(batch, heads / kv_heads, kv_heads, num_prefix);
-  return (int64_t)(grs::part_bytes(slices, batch, heads, head_width) +
-                   (size_t)slices * batch * heads * 4);
+  // either kernel may take the call, by the alignment of its tensors
+  return (int64_t)std::max(
+      grs::plan_bytes(grs::rows_plan(batch, heads / kv_heads, kv_heads, num_prefix), batch, heads,
+                      head_width),
+      grs::plan_bytes(grs::tc_plan(batch, heads, kv_heads, head_width, num_prefix), batch, heads,
+                      head_width));
 }
 
 extern "C" int grs_shared_prefix_attention(
@@ -177,7 +225,7 @@ extern "C" int grs_shared_prefix_attention(
     int64_t workspace_bytes, int32_t* status, void* stream) {
   using namespace grs;
   if (batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_width <= 0 ||
-      head_width > 256 || num_prefix < 0 || max_blocks < 0 || num_pages < 0 ||
+      head_width > 256 || !std::isfinite(scale) || num_prefix < 0 || max_blocks < 0 || num_pages < 0 ||
       (max_blocks > 0 && (page_size <= 0 || !block_table || !lengths || !key_cache ||
                           !value_cache || (int64_t)max_blocks * page_size > INT_MAX / 2)) ||
       (num_prefix > 0 && (!prefix_key || !prefix_value)) || (current_key && !current_value))
@@ -186,11 +234,10 @@ extern "C" int grs_shared_prefix_attention(
   if (!query || !output) return GRS_ERR_SHAPE;
   const int64_t need =
       grs_shared_prefix_workspace_bytes(batch, heads, kv_heads, head_width, num_prefix);
-  if (need > 0 && (!workspace || workspace_bytes < need)) return GRS_ERR_WORKSPACE;
+  if (need > 0 && (!workspace || workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return GRS_ERR_WORKSPACE;
   const int group = heads / kv_heads;
-  const int slices = prefix_slices(batch, group, kv_heads, num_prefix);
-  float* part = static_cast<float*>(workspace);
-  float* lse = slices ? part + part_bytes(slices, batch, heads, head_width) / 4 : nullptr;
   const float scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const auto go = [&](auto zero) {
@@ -201,8 +248,14 @@ extern "C" int grs_shared_prefix_attention(
     g.v = static_cast<const T*>(prefix_value); g.v_st = pv_st; g.v_sh = pv_sh;
     g.positions = batch; g.keys = num_prefix; g.heads = heads; g.kv_heads = kv_heads;
     g.group = group; g.D = head_width; g.scale_log2 = scale_log2;
-    g.part = part; g.part_lse = lse; g.slices = slices; g.status = status;
-    g.slice_keys = slices ? ((num_prefix + slices - 1) / slices + 127) / 128 * 128 : 0;
+    bool tensor_cores = false;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) tensor_cores = grouped_tc_takes(g);
+    const PrefixPlan plan = tensor_cores ? tc_plan(batch, heads, kv_heads, head_width, num_prefix)
+                                         : rows_plan(batch, group, kv_heads, num_prefix);
+    float* part = static_cast<float*>(workspace);
+    float* lse = plan.parts ? part + (size_t)plan.parts * batch * heads * head_width : nullptr;
+    g.part = part; g.part_lse = lse; g.slices = plan.slices; g.slice_keys = plan.keys;
+    g.status = status;
     PagesArgs<T> p = {};
     p.q = g.q; p.q_sb = q_sb; p.q_sh = q_sh;
     p.kc = static_cast<const T*>(key_cache); p.vc = static_cast<const T*>(value_cache);
@@ -211,11 +264,11 @@ extern "C" int grs_shared_prefix_attention(
     p.lengths = max_blocks ? lengths : nullptr; p.num_pages = num_pages; p.page = page_size;
     p.ck = static_cast<const T*>(current_key); p.cv = static_cast<const T*>(current_value);
     p.ck_sb = ck_sb; p.ck_sh = ck_sh; p.cvalid = current_valid;
-    p.part = part; p.part_lse = lse; p.slices = slices;
+    p.part = part; p.part_lse = lse; p.slices = plan.parts;
     p.out = static_cast<T*>(output); p.o_sb = o_sb; p.o_sh = o_sh;
     p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.group = group; p.D = head_width;
     p.scale_log2 = scale_log2; p.status = status;
-    return shared_prefix<T>(p, g, s);
+    return shared_prefix<T>(p, g, tensor_cores, s);
   };
   if (dtype == GRS_DTYPE_F32) return go(float{});
   if (dtype == GRS_DTYPE_BF16) return go(__nv_bfloat16{});

@@ -1,5 +1,8 @@
 // Causal attention over packed prompts: the host side of grs_prompt_attention.
-#include "grouped_attention.cuh"
+#include <cmath>
+#include <type_traits>
+
+#include "grouped_attention_tc.cuh"
 
 namespace grs {
 namespace {
@@ -21,6 +24,8 @@ int prompt_attention(const void* query, int64_t q_st, int64_t q_sh, const void* 
   a.out = static_cast<T*>(out); a.o_sp = o_st; a.o_sh = o_sh;
   a.clear_rest = clear_rest;
   a.status = status;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    if (grouped_tc_takes(a)) return grouped_tc_launch(a, stream);
   return grouped_rows_launch<T>(a, stream);
 }
 
@@ -35,7 +40,8 @@ extern "C" int grs_prompt_attention(int dtype, const void* query, int64_t q_st, 
                                     int kv_heads, int head_width, float scale, int clear_rest,
                                     int32_t* status, void* stream) {
   if (tokens < 0 || sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads ||
-      head_width <= 0 || head_width > 256)
+      head_width <= 0 || head_width > 256 ||
+      !std::isfinite(scale))
     return GRS_ERR_SHAPE;
   if (tokens == 0) return GRS_OK;
   if (!query || !key || !value || !offsets || !out) return GRS_ERR_SHAPE;

@@ -12,12 +12,10 @@ tensors raise.
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import _lib
-from .prompt_attention import _check_heads, _check_out, _check_rows, _status_for
+from .prompt_attention import _check_heads, _check_out, _check_rows, _check_scale, _status_for
 
 
 def shared_prefix_attention(
@@ -111,6 +109,7 @@ def shared_prefix_attention(
         _check_out(out, query, *(t for t in inputs if t is not None and t.numel()))
     if not out.numel():
         return out
+    scale = _check_scale(scale, width)
     word = _status_for(query.device, status)
     lib = _lib.lib()
     with _lib.on_device(query):
@@ -125,7 +124,7 @@ def shared_prefix_attention(
             0 if block_table is None else block_table.stride(0), columns, _lib.ptr(lengths),
             pages, page, _lib.ptr(current_key), _lib.ptr(current_value), *cur_strides,
             _lib.ptr(current_valid), out.data_ptr(), out.stride(0), out.stride(1), batch, heads,
-            kv_heads, width, 1.0 / math.sqrt(width) if scale is None else float(scale),
+            kv_heads, width, scale,
             work.data_ptr(), work.numel(), word.data_ptr(), stream)
     _lib.check(code, "shared-prefix attention")
     return out

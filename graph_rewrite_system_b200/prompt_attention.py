@@ -59,6 +59,13 @@ def _check_heads(query: torch.Tensor, kv_heads: int) -> None:
         raise ValueError("query heads must be a multiple of the key/value heads")
 
 
+def _check_scale(scale: float | None, width: int) -> float:
+    scale = 1.0 / math.sqrt(width) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    return scale
+
+
 def prompt_attention(
     query: torch.Tensor,
     key: torch.Tensor,
@@ -103,6 +110,7 @@ def prompt_attention(
         _check_out(out, query, key, value)
     if not out.numel():
         return out
+    scale = _check_scale(scale, width)
     word = _status_for(query.device, status)
     with _lib.on_device(query):
         code = _lib.lib().grs_prompt_attention(
@@ -110,7 +118,7 @@ def prompt_attention(
             key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
             value.stride(1), offsets.data_ptr(), offsets.numel() - 1, out.data_ptr(),
             out.stride(0), out.stride(1), tokens, heads, kv_heads, width,
-            1.0 / math.sqrt(width) if scale is None else float(scale), int(fresh),
+            scale, int(fresh),
             word.data_ptr(), _lib.stream_of(query))
     _lib.check(code, "prompt attention")
     return out

@@ -40,13 +40,14 @@ PROMPT = dict(query=_z(6, 4, 32), key=_z(6, 2, 32), value=_z(6, 2, 32), offsets=
     dict(offsets=_offsets(0, 1, 6)[::2]), dict(offsets=_offsets(0, 6)[None]),
     dict(out=_z(6, 4, 31)), dict(out=_z(6, 4, 32, dtype=torch.float32)),
     dict(out=_z(1, 4, 32).expand(6, 4, 32)), dict(out=PROMPT["query"]),
-    dict(status=torch.zeros(1, dtype=torch.int64)),
+    dict(status=torch.zeros(1, dtype=torch.int64)), dict(scale=float("nan")),
+    dict(scale=float("inf")),
 ])
 def test_prompt_refusals(lifted, change):
     from graph_rewrite_system_b200.prompt_attention import prompt_attention
 
     args = {**PROMPT, **change}
-    rest = {n: args.pop(n) for n in ("out", "status") if n in args}
+    rest = {n: args.pop(n) for n in ("out", "status", "scale") if n in args}
     rest.setdefault("status", torch.zeros(1, dtype=torch.int32))
     with pytest.raises(ValueError):
         prompt_attention(**args, **rest)
@@ -81,7 +82,7 @@ PREFIX = dict(query=_z(3, 4, 32), prefix_key=_z(9, 2, 32), prefix_value=_z(9, 2,
     dict(current_key=_z(2, 3, 32).transpose(0, 1)),
     dict(current_key=None, current_value=None),
     dict(current_valid=torch.ones(3)), dict(current_valid=torch.ones(2, dtype=torch.bool)),
-    dict(out=_z(3, 4, 33)), dict(out=PREFIX["query"]), dict(out=_z(3, 1, 32).expand(3, 4, 32)),
+    dict(scale=float("nan")), dict(out=_z(3, 4, 33)), dict(out=PREFIX["query"]), dict(out=_z(3, 1, 32).expand(3, 4, 32)),
     dict(block_table=torch.zeros(3, 1, dtype=torch.int32).expand(3, 1 << 27)),
 ])
 def test_prefix_refusals(lifted, change):
@@ -139,7 +140,7 @@ def test_c_abi_refusals():
                   width=32, scale=1.0, clear=0, status=None, stream=None)
     for change in (dict(dtype=7), dict(heads=3), dict(kv=0), dict(heads=0), dict(width=0),
                    dict(width=257), dict(tokens=-1), dict(sequences=-1), dict(q=None),
-                   dict(offsets=None), dict(out=None)):
+                   dict(offsets=None), dict(out=None), dict(scale=float("inf"))):
         assert lib.grs_prompt_attention(*{**prompt, **change}.values()) == shape, change
     assert lib.grs_prompt_attention(*{**prompt, "tokens": 0}.values()) == 0
     prefix = dict(dtype=0, q=256, q_sb=1, q_sh=1, pk=256, pk_st=1, pk_sh=1, pv=256, pv_st=1,
@@ -151,7 +152,7 @@ def test_c_abi_refusals():
                    dict(n=-1), dict(pk=None), dict(kc=None), dict(bt=None), dict(lengths=None),
                    dict(page=0), dict(blocks=1 << 30), dict(ck=256), dict(q=None), dict(out=None)):
         assert lib.grs_shared_prefix_attention(*{**prefix, **change}.values()) == shape, change
-    for change in (dict(work=None), dict(bytes=8)):
+    for change in (dict(work=None), dict(bytes=8), dict(work=260)):
         assert lib.grs_shared_prefix_attention(*{**prefix, **change}.values()) == work, change
     assert lib.grs_shared_prefix_attention(*{**prefix, "batch": 0}.values()) == 0
     assert lib.grs_shared_prefix_workspace_bytes(2, 4, 2, 32, 0) == 0

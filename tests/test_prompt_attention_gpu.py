@@ -114,7 +114,11 @@ def test_rows_behind_the_last_sequence(cuda_device, dtype):
     # rows before the first sequence are nobody's either
     out.fill_(7.0)
     prompt_attention(q, k, v, off[1:], out=out)
-    assert (out[:60] == 7).all() and torch.equal(out[60:135], got[60:135])
+    assert (out[:60] == 7).all()
+    # (another packing: the key blocks start elsewhere, so sums may round apart)
+    out[:60] = got[:60]
+    out[135:] = 0
+    _check(out, clean, offsets)
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
