@@ -6,7 +6,6 @@ operation of this package.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from pathlib import Path
 import re
@@ -156,20 +155,26 @@ class pinned_stream:
         _PINNED_STREAM.pop()
 
 
-def on_device(t: torch.Tensor):
-    """Context that makes t's device current for a launch (the library's
-    launches and device queries go to the current device)."""
-    if t.device.index is None or t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def current_device() -> int:
+    """Index of the current device (the library launches on it)."""
+    return torch._C._cuda_getDevice()
 
 
-def scratch(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
-    """Uninitialised bytes for one call that is enqueued on `stream`: when that
-    is not torch's current stream, the allocator is told of the use."""
-    work = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    if nbytes and stream != torch.cuda.current_stream(device).cuda_stream:
-        work.record_stream(torch.cuda.ExternalStream(stream, device=device))
+def stream_on(index: int) -> int:
+    """Raw handle of the pinned stream, else of torch's current stream of
+    device `index` (what ``stream_of`` gives, without building stream objects)."""
+    if _PINNED_STREAM:
+        return _PINNED_STREAM[-1]
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def scratch(like: torch.Tensor, nbytes: int, stream: int) -> torch.Tensor:
+    """Uninitialised bytes on like's device for one call enqueued on `stream`:
+    when that is not torch's current stream, the allocator is told of the use."""
+    work = like.new_empty(nbytes, dtype=torch.uint8)
+    if _PINNED_STREAM and nbytes:
+        if stream != torch.cuda.current_stream(like.device).cuda_stream:
+            work.record_stream(torch.cuda.ExternalStream(stream, device=like.device))
     return work
 
 

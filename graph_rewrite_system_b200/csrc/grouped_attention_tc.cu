@@ -14,6 +14,7 @@
 //
 //   warps 0-3   softmax and epilogue of slot 0      warp 8  TMA loads
 //   warps 4-7   softmax and epilogue of slot 1      warp 9  MMA issue
+//   warp 10     zeroes the value rows behind a causal tile's last key
 // The launch's 384 x 168 registers are split 216 to a softmax thread, which
 // holds a row's 128 scores, and 72 to the other warpgroup (256 x 216 + 128 x
 // 72 = 64512 = 384 x 168).
@@ -75,6 +76,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   extern __shared__ uint8_t gtc_smem_raw[];
   __shared__ __align__(8) uint64_t q_full, kv_full[S::kStages], kv_empty[S::kStages];
   __shared__ __align__(8) uint64_t s_full[2], p_full[2], drain_bar;
+  __shared__ __align__(8) uint64_t last_full, last_clean;   // the causal tile's last V block
   __shared__ uint32_t tmem_slot;
   __shared__ int failed, drain_failed;
   // per slot: first and last key of any row, last first and first last key
@@ -112,9 +114,13 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       in_hi[s] = INT_MAX;
     }
     mbar_init(&drain_bar, 1);
+    mbar_init(&last_full, 1);
+    mbar_init(&last_clean, 1);
     failed = drain_failed = 0;
     mbar_init_fence();
   }
+  // the kernel that joins the slices may start as SMs fall free
+  if (!kCausal) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
   __syncthreads();
   int begin = 0, end = 0, position = -1;
@@ -158,6 +164,13 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const bool any0 = last[0] > first[0], any1 = last[1] > first[1];
   const int lo = any0 && any1 ? min(first[0], first[1]) : any0 ? first[0] : first[1];
   const int hi = any0 && any1 ? max(last[0], last[1]) : any0 ? last[0] : last[1];
+  // Value rows past the tile's last key (rows behind the last sequence, the
+  // next sequence, later tokens) meet only zero weights, but they may hold
+  // NaN: the last V block is cleared of them before its product.
+  const int end_row = kCausal && (any0 || any1)
+                          ? max(hi_key[0], hi_key[1]) - origin[0] - (hi - 1) * GTC_KEYS
+                          : GTC_KEYS;
+  const bool clear = end_row < GTC_KEYS;
   volatile int* gave_up = &failed;
 
   if (warp >= 8) {
@@ -172,22 +185,24 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                         p_tile + s * pps, &q_full);
         int g = 0;
         int armed[S::kStages] = {};
-        const auto load = [&](const CUtensorMap* map, int key) {
+        bool last_armed = false;
+        const auto load = [&](const CUtensorMap* map, int key, bool is_last = false) {
           const int st = g % S::kStages, r = g / S::kStages;
           if (*gave_up) return;
           if (r > 0 && !mbar_wait(&kv_empty[st], (r - 1) & 1)) {
             failed = 1;
             return;
           }
-          mbar_arrive_expect_tx(&kv_full[st], S::kTile);
+          uint64_t* bar = is_last ? &last_full : &kv_full[st];
+          mbar_arrive_expect_tx(bar, S::kTile);
           for (int b = 0; b < S::kBoxes; ++b)
-            tma_load_3d(ring + st * S::kTile + b * S::kBox, map, b * 64, h, key, &kv_full[st]);
-          armed[st] = r + 1;
+            tma_load_3d(ring + st * S::kTile + b * S::kBox, map, b * 64, h, key, bar);
+          if (is_last) last_armed = true; else armed[st] = r + 1;
           ++g;
         };
         if (!kSplit) {
           for (int j = lo - 1; j < hi; ++j) {
-            if (j >= lo) load(&tm_v, origin[0] + j * GTC_KEYS);
+            if (j >= lo) load(&tm_v, origin[0] + j * GTC_KEYS, clear && j == hi - 1);
             if (j + 1 < hi) load(&tm_k, origin[0] + (j + 1) * GTC_KEYS);
           }
         } else {
@@ -199,6 +214,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
         // every load in flight lands before the CTA exits
         if (!mbar_wait(&q_full, 0)) drain_failed = 1;
+        if (last_armed && !mbar_wait(&last_full, 0)) drain_failed = 1;
         for (int s = 0; s < S::kStages; ++s)
           if (armed[s] > 0 && !mbar_wait(&kv_full[s], (armed[s] - 1) & 1)) drain_failed = 1;
       }
@@ -240,7 +256,14 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (!kSplit) {
           for (int j = lo - 1; j < hi && ok; ++j) {
             const int gv = j >= lo ? g++ : -1, gk = j + 1 < hi ? g++ : -1;
-            if (gv >= 0) arrived(gv);
+            if (gv >= 0) {
+              if (clear && j == hi - 1) {
+                if (!mbar_wait(&last_clean, 0)) ok = false;
+                tc_fence_after();
+              } else {
+                arrived(gv);
+              }
+            }
   #pragma unroll
             for (int s = 0; s < 2; ++s) {
               if (j >= first[s] && j < last[s]) values(s, gv, j - first[s]);
@@ -274,6 +297,21 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         // no MMA may still use TMEM or shared memory when they are given back
         mma_commit(&drain_bar);
         if (!mbar_wait(&drain_bar, 0)) drain_failed = 1;
+      }
+    } else if (kCausal && warp == 10 && clear) {
+      const int at = 1 + 2 * (hi - 1 - lo);   // its place in the ring
+      // (the stream may still be a whole tile's work away from its last block)
+      bool ok = false;
+      while (!ok && !*gave_up) ok = mbar_wait_warp(&last_full, 0);
+      if (ok) {
+        uint8_t* block = ring + (at % S::kStages) * S::kTile;
+        constexpr int kPieces = S::kRow / 16;
+        for (int b = 0; b < S::kBoxes; ++b)
+          for (int i = end_row * kPieces + lane; i < GTC_KEYS * kPieces; i += 32)
+            *reinterpret_cast<uint4*>(block + b * S::kBox + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&last_clean);
       }
     }
   } else {                               // softmax and epilogue, one row per thread

@@ -21,7 +21,8 @@ struct PagesArgs {
   const T* kc; const T* vc; int64_t kc_sp, kc_st, kc_sh;
   const int32_t* bt; int64_t bt_s; int max_blocks; const int32_t* lengths; int num_pages, page;
   const T* ck; const T* cv; int64_t ck_sb, ck_sh; const uint8_t* cvalid;
-  const float* part; const float* part_lse; int slices;
+  const float* part; const float* part_lse; int slices;   // parts of the prefix
+  float* page_part; float* page_lse;                      // the same arrays, for page slices
   T* out; int64_t o_sb, o_sh;
   int batch, heads, kv_heads, group, D;
   float scale_log2;
@@ -130,6 +131,329 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
   }
 }
 
+// ---- bf16 pages on the tensor cores -------------------------------------------
+// One CTA of `warps` warps per (beam, K/V head, 16 query heads), each warp
+// taking every warps-th run of 32 tokens.  The pages are read once and nothing
+// else is large, so memory bounds it: every lane fetches 16-byte pieces of the
+// rows straight into mma.m16n8k16 operands, without shared memory.  A product
+// does not care in which order its inner dimension is summed, so lane t of a
+// quad takes the pieces t, t + 4, ... of a key row for its K fragments (the
+// query fragments are loaded in the same order), and for V the lane's column
+// index picks the piece and the eight elements of a piece go to eight
+// different n-tiles; two keys' pieces are interleaved by byte permutes.  The
+// weights leave the score product in the layout of the value product's A
+// operand.  The warps' sums meet in shared memory and are joined there with
+// the prefix slices; only that join waits for the prefix kernel.
+constexpr int PG_HEADS = 16;
+
+__device__ __forceinline__ void pg_mma(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float pg_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pg_pack(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+template <int DP>
+struct PgShape {
+  static constexpr int kPiece = DP >= 64 ? 8 : 4;         // V elements of a lane's piece
+  static constexpr int kRuns = DP / (8 * kPiece);         // pieces of a lane
+  static constexpr int kKey = DP / 32;                    // 16-byte K pieces of a lane
+  static constexpr int kStride = DP + 4;                  // row of the joined sums (floats)
+};
+
+template <int DP>
+__global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16> a, int rows) {
+  using S = PgShape<DP>;
+  using T = __nv_bfloat16;
+  extern __shared__ float pg_smem[];
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int chunks = (a.group + PG_HEADS - 1) / PG_HEADS;
+  const int b = blockIdx.x / (a.kv_heads * chunks);
+  const int h = blockIdx.x / chunks % a.kv_heads;
+  const int head0 = h * a.group + blockIdx.x % chunks * PG_HEADS;
+  const int n_heads = min(PG_HEADS, (h + 1) * a.group - head0);
+
+  // query fragments: rows g and g + 8, pieces t, t + 4, ...
+  uint32_t qa[2 * S::kKey][4];
+#pragma unroll
+  for (int i = 0; i < S::kKey; ++i) {
+    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+    const int d = 8 * (t + 4 * i);
+    const T* q = a.q + (int64_t)b * a.q_sb + (int64_t)(head0 + g) * a.q_sh + d;
+    if (d < a.D && g < n_heads) lo = *reinterpret_cast<const uint4*>(q);
+    if (d < a.D && g + 8 < n_heads) hi = *reinterpret_cast<const uint4*>(q + 8 * a.q_sh);
+    qa[2 * i][0] = lo.x;
+    qa[2 * i][1] = hi.x;
+    qa[2 * i][2] = lo.y;
+    qa[2 * i][3] = hi.y;
+    qa[2 * i + 1][0] = lo.z;
+    qa[2 * i + 1][1] = hi.z;
+    qa[2 * i + 1][2] = lo.w;
+    qa[2 * i + 1][3] = hi.w;
+  }
+
+  const int room = a.max_blocks * a.page;
+  int past = a.lengths ? a.lengths[b] : 0;
+  if (past < 0 || past > room) {
+    if (threadIdx.x == 0) set_status(a.status, GRS_ERR_LENGTH);
+    past = min(max(past, 0), room);
+  }
+  const bool cur = a.ck != nullptr && (a.cvalid == nullptr || a.cvalid[b] != 0);
+  const int total = past + (cur ? 1 : 0);
+  const int runs = (total + 31) / 32;
+  const int run_lo = (int)((int64_t)runs * blockIdx.y / gridDim.y);
+  const int run_hi = (int)((int64_t)runs * (blockIdx.y + 1) / gridDim.y);
+  const T* cur_k = cur ? a.ck + (int64_t)b * a.ck_sb + (int64_t)h * a.ck_sh : nullptr;
+  const int64_t paged_v = a.vc - a.kc, cur_v = a.cv - a.ck;   // value row behind a key row
+  const auto place = [&](int run) -> const T* {               // key row of token 32 run + lane
+    const int tok = run * 32 + lane;
+    if (run >= run_hi || tok >= total) return nullptr;
+    if (tok >= past) return cur_k;
+    const int page = __ldg(a.bt + (int64_t)b * a.bt_s + tok / a.page);
+    if (page < 0 || page >= a.num_pages) {
+      set_status(a.status, GRS_ERR_BAD_PAGE);
+      return nullptr;
+    }
+    return a.kc + (int64_t)page * a.kc_sp + (int64_t)(tok % a.page) * a.kc_st +
+           (int64_t)h * a.kc_sh;
+  };
+
+  float acc[DP / 8][4];
+#pragma unroll
+  for (int i = 0; i < DP / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const T* next = place(run_lo + warp);
+  for (int run = run_lo + warp; run < run_hi; run += warps) {
+    const T* mine = next;
+    next = place(run + warps);
+    const unsigned valid = __ballot_sync(0xffffffffu, mine != nullptr);
+    const unsigned long long at = reinterpret_cast<unsigned long long>(mine);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (((valid >> (16 * half)) & 0xffffu) == 0) continue;
+      uint4 kr[2][S::kKey];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const T* k = reinterpret_cast<const T*>(
+            __shfl_sync(0xffffffffu, at, 16 * half + 8 * n + g));
+#pragma unroll
+        for (int i = 0; i < S::kKey; ++i) {
+          const int d = 8 * (t + 4 * i);
+          kr[n][i] = make_uint4(0, 0, 0, 0);
+          if (k && d < a.D) kr[n][i] = __ldg(reinterpret_cast<const uint4*>(k + d));
+        }
+      }
+      // values of keys 2t, 2t + 1, 2t + 8, 2t + 9
+      uint32_t vr[4][S::kRuns][S::kPiece / 2];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int j = 16 * half + 2 * t + (n & 1) + 8 * (n >> 1);
+        const T* k = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, at, j));
+        const T* v = k + (run * 32 + j >= past ? cur_v : paged_v);
+#pragma unroll
+        for (int i = 0; i < S::kRuns; ++i) {
+          const int d = S::kPiece * (g + 8 * i);
+          if constexpr (S::kPiece == 8) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (k && d < a.D) w = __ldg(reinterpret_cast<const uint4*>(v + d));
+            vr[n][i][0] = w.x;
+            vr[n][i][1] = w.y;
+            vr[n][i][2] = w.z;
+            vr[n][i][3] = w.w;
+          } else {
+            uint2 w = make_uint2(0, 0);
+            if (k && d < a.D) w = __ldg(reinterpret_cast<const uint2*>(v + d));
+            vr[n][i][0] = w.x;
+            vr[n][i][1] = w.y;
+          }
+        }
+      }
+      float s[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < S::kKey; ++i) {
+          pg_mma(s[n], qa[2 * i], kr[n][i].x, kr[n][i].y);
+          pg_mma(s[n], qa[2 * i + 1], kr[n][i].z, kr[n][i].w);
+        }
+      }
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const bool ok = (valid >> (16 * half + 8 * n + 2 * t + (c & 1))) & 1;
+          s[n][c] = ok ? s[n][c] * a.scale_log2 : -INFINITY;
+          top[c >> 1] = fmaxf(top[c >> 1], s[n][c]);
+        }
+      float base[2];
+      bool grown = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+        grown |= top[r] > m[r];
+      }
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float now = fmaxf(m[r], top[r]);
+          const float keep = now == -INFINITY ? 1.f : pg_exp2(m[r] - now);
+          m[r] = now;
+          l[r] *= keep;
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i) {
+            acc[i][2 * r] *= keep;
+            acc[i][2 * r + 1] *= keep;
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) base[r] = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          s[n][c] = pg_exp2(s[n][c] - base[c >> 1]);
+          l[c >> 1] += s[n][c];
+        }
+      const uint32_t pa[4] = {pg_pack(s[0][0], s[0][1]), pg_pack(s[0][2], s[0][3]),
+                              pg_pack(s[1][0], s[1][1]), pg_pack(s[1][2], s[1][3])};
+#pragma unroll
+      for (int i = 0; i < S::kRuns; ++i)
+#pragma unroll
+        for (int e = 0; e < S::kPiece; ++e) {
+          const unsigned pick = (e & 1) ? 0x7632u : 0x5410u;
+          pg_mma(acc[i * S::kPiece + e], pa,
+                 __byte_perm(vr[0][i][e >> 1], vr[1][i][e >> 1], pick),
+                 __byte_perm(vr[2][i][e >> 1], vr[3][i][e >> 1], pick));
+        }
+    }
+  }
+
+  // each warp's state into shared memory
+  float* sums = pg_smem;                                   // [warps][rows][kStride]
+  float* tops = sums + warps * rows * S::kStride;
+  float* totals = tops + warps * rows;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    const int head = g + 8 * r;
+    if (head >= rows) continue;
+    float* row = sums + (warp * rows + head) * S::kStride;
+#pragma unroll
+    for (int i = 0; i < S::kRuns; ++i)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < S::kPiece; e += 4)
+          *reinterpret_cast<float4*>(row + S::kPiece * (2 * t + c + 8 * i) + e) = make_float4(
+              acc[i * S::kPiece + e][2 * r + c], acc[i * S::kPiece + e + 1][2 * r + c],
+              acc[i * S::kPiece + e + 2][2 * r + c], acc[i * S::kPiece + e + 3][2 * r + c]);
+    if (t == 0) {
+      tops[warp * rows + head] = m[r];
+      totals[warp * rows + head] = l[r];
+    }
+  }
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");   // the prefix slices are written
+
+  // a warp per head joins the warps' sums with the prefix slices, lane = 4 columns
+  const bool last = gridDim.y == 1;
+  const int64_t stride = (int64_t)a.batch * a.heads;
+  for (int head = warp; head < n_heads; head += warps) {
+    const int64_t at = (int64_t)b * a.heads + head0 + head;
+    const int parts = last ? a.slices : 0;
+    float top = -INFINITY;
+    for (int i = lane; i < warps; i += 32) top = fmaxf(top, tops[i * rows + head]);
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[i * stride + at]);
+    top = warp_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    float norm = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int d = 4 * lane;
+    for (int i = 0; i < warps; ++i) {
+      const float w = pg_exp2(tops[i * rows + head] - base);
+      norm = fmaf(w, totals[i * rows + head], norm);
+      if (d < DP) {
+        const float4 y = *reinterpret_cast<const float4*>(sums + (i * rows + head) * S::kStride + d);
+        x.x = fmaf(w, y.x, x.x);
+        x.y = fmaf(w, y.y, x.y);
+        x.z = fmaf(w, y.z, x.z);
+        x.w = fmaf(w, y.w, x.w);
+      }
+    }
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) {
+      const float w = pg_exp2(a.part_lse[i * stride + at] - base);
+      norm += w;
+      if (d < a.D) {
+        const float4 y = *reinterpret_cast<const float4*>(a.part + (i * stride + at) * a.D + d);
+        x.x = fmaf(w, y.x, x.x);
+        x.y = fmaf(w, y.y, x.y);
+        x.z = fmaf(w, y.z, x.z);
+        x.w = fmaf(w, y.w, x.w);
+      }
+    }
+    const float inv = norm == 0.f ? 0.f : 1.f / norm;
+    x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    if (last) {
+      if (d < a.D)
+        *reinterpret_cast<uint2*>(a.out + (int64_t)b * a.o_sb + (int64_t)(head0 + head) * a.o_sh +
+                                  d) = make_uint2(pg_pack(x.x, x.y), pg_pack(x.z, x.w));
+    } else {
+      const int64_t to = (a.slices + blockIdx.y) * stride + at;
+      if (d < a.D) *reinterpret_cast<float4*>(a.page_part + to * a.D + d) = x;
+      if (lane == 0) a.page_lse[to] = norm == 0.f ? -INFINITY : base + log2f(norm);
+    }
+  }
+}
+
+// The join alone, for pages that are cut into slices too: a warp per (beam,
+// head) over all parts.
+__global__ void __launch_bounds__(128) join_parts_kernel(PagesArgs<__nv_bfloat16> a, int parts) {
+  const int lane = threadIdx.x & 31;
+  const int64_t stride = (int64_t)a.batch * a.heads;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (at >= stride) return;
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[i * stride + at]);
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  float norm = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int d = 4 * lane;
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i) {
+    const float w = pg_exp2(a.part_lse[i * stride + at] - base);
+    norm += w;
+    if (d < a.D) {
+      const float4 y = *reinterpret_cast<const float4*>(a.part + (i * stride + at) * a.D + d);
+      x.x = fmaf(w, y.x, x.x);
+      x.y = fmaf(w, y.y, x.y);
+      x.z = fmaf(w, y.z, x.z);
+      x.w = fmaf(w, y.w, x.w);
+    }
+  }
+  const float inv = norm == 0.f ? 0.f : 1.f / norm;
+  if (d < a.D)
+    *reinterpret_cast<uint2*>(a.out + at / a.heads * a.o_sb + at % a.heads * a.o_sh + d) =
+        make_uint2(pg_pack(x.x * inv, x.y * inv), pg_pack(x.z * inv, x.w * inv));
+}
+
 // How the prefix is cut: `parts` partial sums, `keys` per slice (two parts per
 // slice when the tensor-core kernel's slots halve it).
 struct PrefixPlan {
@@ -175,13 +499,72 @@ static PrefixPlan tc_plan(int batch, int heads, int kv_heads, int D, int keys) {
   return {slices, slices * per, each * 128};
 }
 
-static size_t plan_bytes(const PrefixPlan& p, int batch, int heads, int D) {
-  return (size_t)p.parts * batch * heads * (D + 1) * 4;
+// Slices of each beam's pages: enough CTAs of a long table to fill 148 SMs
+// four times when there are few beams, none for less than 256 tokens.
+static int pages_slices(int batch, int heads, int kv_heads, int64_t room) {
+  const int group = heads / kv_heads;
+  const int64_t tasks = (int64_t)batch * kv_heads * ((group + PG_HEADS - 1) / PG_HEADS);
+  const int64_t want = (4 * 148 + tasks - 1) / tasks;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), room / 256));
+}
+
+static bool aligned(const void* p, int64_t bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+
+// 16-byte pieces of query, cache and current rows, 8-byte pieces of the output
+static bool pages_mma_takes(const PagesArgs<__nv_bfloat16>& p) {
+  return p.D % 8 == 0 && p.D <= 128 && aligned(p.q, 16) && p.q_sb % 8 == 0 && p.q_sh % 8 == 0 &&
+         aligned(p.kc, 16) && aligned(p.vc, 16) && p.kc_sp % 8 == 0 && p.kc_st % 8 == 0 &&
+         p.kc_sh % 8 == 0 && aligned(p.ck, 16) && aligned(p.cv, 16) && p.ck_sb % 8 == 0 &&
+         p.ck_sh % 8 == 0 && aligned(p.out, 8) && p.o_sb % 4 == 0 && p.o_sh % 4 == 0;
+}
+
+template <int DP>
+static int pages_mma_run(const PagesArgs<__nv_bfloat16>& p, int page_slices, bool after_prefix,
+                         cudaStream_t stream) {
+  const int64_t tasks = (int64_t)p.batch * p.kv_heads * ((p.group + PG_HEADS - 1) / PG_HEADS);
+  if (tasks > INT_MAX || page_slices > 65535) return GRS_ERR_SHAPE;
+  // warps of a CTA: a run of 32 tokens each, more when there are few CTAs
+  const int64_t runs = ((int64_t)p.max_blocks * p.page + 1 + 31) / 32;
+  const int warps = runs <= 2 && tasks * page_slices >= 4 * 148 ? 2 : tasks * page_slices >= 2 * 148 ? 4 : 8;
+  const int rows = p.group <= 8 ? 8 : PG_HEADS;
+  const int smem = warps * rows * (PgShape<DP>::kStride + 2) * 4;
+  if (cudaFuncSetAttribute(pages_mma_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           8 * PG_HEADS * (PgShape<DP>::kStride + 2) * 4) != cudaSuccess)
+    return GRS_ERR_CUDA;
+  // starts under the prefix kernel's tail; its join waits for the slices
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)tasks, page_slices);
+  config.blockDim = dim3(32 * warps);
+  config.dynamicSmemBytes = smem;
+  config.stream = counted(stream);
+  config.attrs = &attr;
+  config.numAttrs = after_prefix ? 1 : 0;
+  if (cudaLaunchKernelEx(&config, pages_mma_kernel<DP>, p, rows) != cudaSuccess)
+    return GRS_ERR_CUDA;
+  if (page_slices > 1) {
+    const int64_t n = (int64_t)p.batch * p.heads;
+    join_parts_kernel<<<(unsigned)((n + 3) / 4), 128, 0, counted(stream)>>>(p, p.slices +
+                                                                                  page_slices);
+  }
+  GRS_CUDA_CHECK_LAUNCH();
+  return GRS_OK;
+}
+
+static int pages_mma_launch(const PagesArgs<__nv_bfloat16>& p, int page_slices, bool after_prefix,
+                            cudaStream_t stream) {
+  if (p.D <= 32) return pages_mma_run<32>(p, page_slices, after_prefix, stream);
+  if (p.D <= 64) return pages_mma_run<64>(p, page_slices, after_prefix, stream);
+  return pages_mma_run<128>(p, page_slices, after_prefix, stream);
 }
 
 template <typename T>
 static int shared_prefix(const PagesArgs<T>& p, const GroupedArgs<T>& prefix, bool tensor_cores,
-                         cudaStream_t stream) {
+                         int page_slices, cudaStream_t stream) {
   if (prefix.slices > 0) {
     int status = GRS_OK;
     if constexpr (std::is_same<T, __nv_bfloat16>::value)
@@ -191,6 +574,8 @@ static int shared_prefix(const PagesArgs<T>& p, const GroupedArgs<T>& prefix, bo
       status = grouped_rows_launch<T>(prefix, stream);
     if (status != GRS_OK) return status;
   }
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    if (pages_mma_takes(p)) return pages_mma_launch(p, page_slices, prefix.slices > 0, stream);
   const int64_t rows = (int64_t)p.batch * p.heads;
   const unsigned grid = (unsigned)((rows + 3) / 4);
   if (p.D <= 32) pages_rows_kernel<T, 32><<<grid, 128, 0, counted(stream)>>>(p);
@@ -204,14 +589,15 @@ static int shared_prefix(const PagesArgs<T>& p, const GroupedArgs<T>& prefix, bo
 }  // namespace grs
 
 extern "C" int64_t grs_shared_prefix_workspace_bytes(int batch, int heads, int kv_heads,
-                                                     int head_width, int num_prefix) {
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || num_prefix <= 0) return 0;
-  // either kernel may take the call, by the alignment of its tensors
-  return (int64_t)std::max(
-      grs::plan_bytes(grs::rows_plan(batch, heads / kv_heads, kv_heads, num_prefix), batch, heads,
-                      head_width),
-      grs::plan_bytes(grs::tc_plan(batch, heads, kv_heads, head_width, num_prefix), batch, heads,
-                      head_width));
+                                                     int head_width, int num_prefix,
+                                                     int64_t page_tokens) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  // any of the kernels may take the call, by the alignment of its tensors
+  const int parts = std::max(
+      grs::rows_plan(batch, heads / kv_heads, kv_heads, num_prefix).parts,
+      grs::tc_plan(batch, heads, kv_heads, head_width, num_prefix).parts);
+  const int pages = grs::pages_slices(batch, heads, kv_heads, page_tokens);
+  return (int64_t)(parts + (pages > 1 ? pages : 0)) * batch * heads * (head_width + 1) * 4;
 }
 
 extern "C" int grs_shared_prefix_attention(
@@ -232,8 +618,9 @@ extern "C" int grs_shared_prefix_attention(
     return GRS_ERR_SHAPE;
   if (batch == 0) return GRS_OK;
   if (!query || !output) return GRS_ERR_SHAPE;
-  const int64_t need =
-      grs_shared_prefix_workspace_bytes(batch, heads, kv_heads, head_width, num_prefix);
+  const int64_t room = (int64_t)max_blocks * page_size;
+  const int64_t need = grs_shared_prefix_workspace_bytes(batch, heads, kv_heads, head_width,
+                                                         num_prefix, room);
   if (need > 0 && (!workspace || workspace_bytes < need ||
                    (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return GRS_ERR_WORKSPACE;
@@ -253,7 +640,9 @@ extern "C" int grs_shared_prefix_attention(
     const PrefixPlan plan = tensor_cores ? tc_plan(batch, heads, kv_heads, head_width, num_prefix)
                                          : rows_plan(batch, group, kv_heads, num_prefix);
     float* part = static_cast<float*>(workspace);
-    float* lse = plan.parts ? part + (size_t)plan.parts * batch * heads * head_width : nullptr;
+    const int page_slices = pages_slices(batch, heads, kv_heads, room);
+    const int64_t parts = plan.parts + (page_slices > 1 ? page_slices : 0);
+    float* lse = part + parts * batch * heads * head_width;
     g.part = part; g.part_lse = lse; g.slices = plan.slices; g.slice_keys = plan.keys;
     g.status = status;
     PagesArgs<T> p = {};
@@ -264,11 +653,11 @@ extern "C" int grs_shared_prefix_attention(
     p.lengths = max_blocks ? lengths : nullptr; p.num_pages = num_pages; p.page = page_size;
     p.ck = static_cast<const T*>(current_key); p.cv = static_cast<const T*>(current_value);
     p.ck_sb = ck_sb; p.ck_sh = ck_sh; p.cvalid = current_valid;
-    p.part = part; p.part_lse = lse; p.slices = plan.parts;
+    p.part = p.page_part = part; p.part_lse = p.page_lse = lse; p.slices = plan.parts;
     p.out = static_cast<T*>(output); p.o_sb = o_sb; p.o_sh = o_sh;
     p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.group = group; p.D = head_width;
     p.scale_log2 = scale_log2; p.status = status;
-    return shared_prefix<T>(p, g, tensor_cores, s);
+    return shared_prefix<T>(p, g, tensor_cores, page_slices, s);
   };
   if (dtype == GRS_DTYPE_F32) return go(float{});
   if (dtype == GRS_DTYPE_BF16) return go(__nv_bfloat16{});

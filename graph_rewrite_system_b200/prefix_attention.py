@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .prompt_attention import _check_heads, _check_out, _check_rows, _check_scale, _status_for
+from .prompt_attention import _check_heads, _check_scale, _out_rows, _rows, _status_for
 
 
 def shared_prefix_attention(
@@ -52,79 +52,94 @@ def shared_prefix_attention(
     ``check_decode_status`` reads).  ``out`` must not overlap the inputs.  The
     call does not synchronise and can be captured into a CUDA graph.
     """
-    _lib.require_cuda(query, prefix_key, prefix_value, key_cache, value_cache, block_table,
-                      lengths, current_key, current_value, current_valid, out, status)
+    device = query.get_device()
+    if device < 0:
+        _lib.require_cuda(query)
+    if device != _lib.current_device():
+        with torch.cuda.device(device):
+            return shared_prefix_attention(
+                query, prefix_key, prefix_value, key_cache, value_cache, block_table, lengths,
+                current_key=current_key, current_value=current_value,
+                current_valid=current_valid, scale=scale, out=out, status=status)
     if query.dim() != 3 or prefix_key.dim() != 3:
         raise ValueError("query must be [batch, heads, D], the prefix [keys, kv_heads, D]")
-    batch, heads, width = query.shape
-    num_prefix, kv_heads = prefix_key.shape[:2]
-    _check_heads(query, kv_heads)
-    _check_rows("query", query, query, tuple(query.shape))
-    _check_rows("prefix_key", prefix_key, query, (num_prefix, kv_heads, width))
-    _check_rows("prefix_value", prefix_value, query, (num_prefix, kv_heads, width))
-    paged = (key_cache, value_cache, block_table, lengths)
-    if any(t is None for t in paged) != all(t is None for t in paged):
-        raise ValueError("caches, block table and lengths must be supplied together")
-    columns = pages = page = 0
-    strides = (0, 0, 0)
-    if key_cache is not None:
+    shape = query.shape
+    batch, heads, width = shape
+    num_prefix, kv_heads, _ = prefix_key.shape
+    code, dtype = _check_heads(query, heads, kv_heads, width), query.dtype
+    q = _rows("query", query, device, dtype, shape)
+    pk = _rows("prefix_key", prefix_key, device, dtype, (num_prefix, kv_heads, width))
+    pv = _rows("prefix_value", prefix_value, device, dtype, (num_prefix, kv_heads, width))
+
+    columns = pages = page = table_row = 0
+    c = (0, 0, 0)
+    table = past = None
+    if key_cache is None or value_cache is None or block_table is None or lengths is None:
+        if not (key_cache is value_cache is block_table is lengths):
+            raise ValueError("caches, block table and lengths must be supplied together")
+    else:
         if key_cache.dim() != 4:
             raise ValueError("caches must be [pages, page, kv_heads, D]")
         pages, page = key_cache.shape[:2]
-        _check_rows("key_cache", key_cache, query, (pages, page, kv_heads, width))
-        _check_rows("value_cache", value_cache, query, (pages, page, kv_heads, width))
-        if key_cache.stride() != value_cache.stride():
+        c = _rows("key_cache", key_cache, device, dtype, (pages, page, kv_heads, width))
+        if c != _rows("value_cache", value_cache, device, dtype, (pages, page, kv_heads, width)):
             raise ValueError("key/value caches must share a layout")
-        strides = key_cache.stride()[:3]
-        if (block_table.dtype != torch.int32 or block_table.dim() != 2
-                or block_table.shape[0] != batch or block_table.device != query.device
-                or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
-            raise ValueError("block_table must be int32 [batch, columns] with contiguous rows")
-        if (lengths.dtype != torch.int32 or tuple(lengths.shape) != (batch,)
-                or not lengths.is_contiguous() or lengths.device != query.device):
-            raise ValueError("lengths must be contiguous int32 [batch]")
-        columns = block_table.shape[1] if page else 0
+        if (block_table.dtype is not torch.int32 or block_table.dim() != 2
+                or block_table.get_device() != device):
+            _lib.require_cuda(block_table)
+            raise ValueError("block_table must be int32 [batch, columns] on the query's device")
+        rows, columns = block_table.shape
+        table_row, step = block_table.stride()
+        if rows != batch or (columns > 1 and step != 1):
+            raise ValueError("block_table must be [batch, columns] with contiguous rows")
+        if (lengths.dtype is not torch.int32 or lengths.shape != (batch,)
+                or not lengths.is_contiguous() or lengths.get_device() != device):
+            _lib.require_cuda(lengths)
+            raise ValueError("lengths must be contiguous int32 [batch] on the query's device")
         if columns * page >= 1 << 30:
             raise ValueError("a block table row holds at most 2^30 tokens")
+        columns = columns if page else 0
+        table, past = block_table.data_ptr(), lengths.data_ptr()
+
+    cur = (0, 0)
+    valid = None
     if (current_key is None) != (current_value is None):
         raise ValueError("current key/value must be supplied together")
-    cur_strides = (0, 0)
     if current_key is not None:
-        _check_rows("current_key", current_key, query, (batch, kv_heads, width))
-        _check_rows("current_value", current_value, query, (batch, kv_heads, width))
-        if current_key.stride() != current_value.stride():
+        cur = _rows("current_key", current_key, device, dtype, (batch, kv_heads, width))
+        if cur != _rows("current_value", current_value, device, dtype, (batch, kv_heads, width)):
             raise ValueError("current key/value must share a layout")
-        cur_strides = current_key.stride()[:2]
     if current_valid is not None:
         if current_key is None:
             raise ValueError("current_valid comes with the current key/value")
         if (current_valid.dtype not in (torch.bool, torch.uint8)
-                or tuple(current_valid.shape) != (batch,) or not current_valid.is_contiguous()
-                or current_valid.device != query.device):
+                or current_valid.shape != (batch,) or not current_valid.is_contiguous()
+                or current_valid.get_device() != device):
+            _lib.require_cuda(current_valid)
             raise ValueError("current_valid must be contiguous bool or uint8 [batch]")
-    if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    else:
-        inputs = (prefix_key, prefix_value, key_cache, value_cache, current_key, current_value)
-        _check_out(out, query, *(t for t in inputs if t is not None and t.numel()))
-    if not out.numel():
-        return out
+        valid = current_valid.data_ptr()
     scale = _check_scale(scale, width)
-    word = _status_for(query.device, status)
-    lib = _lib.lib()
-    with _lib.on_device(query):
-        stream = _lib.stream_of(query)
-        need = lib.grs_shared_prefix_workspace_bytes(batch, heads, kv_heads, width, num_prefix)
-        work = _lib.scratch(need, query.device, stream)
-        code = lib.grs_shared_prefix_attention(
-            _lib.DTYPE_CODES[query.dtype], query.data_ptr(), query.stride(0), query.stride(1),
-            prefix_key.data_ptr(), prefix_key.stride(0), prefix_key.stride(1),
-            prefix_value.data_ptr(), prefix_value.stride(0), prefix_value.stride(1), num_prefix,
-            _lib.ptr(key_cache), _lib.ptr(value_cache), *strides, _lib.ptr(block_table),
-            0 if block_table is None else block_table.stride(0), columns, _lib.ptr(lengths),
-            pages, page, _lib.ptr(current_key), _lib.ptr(current_value), *cur_strides,
-            _lib.ptr(current_valid), out.data_ptr(), out.stride(0), out.stride(1), batch, heads,
-            kv_heads, width, scale,
-            work.data_ptr(), work.numel(), word.data_ptr(), stream)
-    _lib.check(code, "shared-prefix attention")
+    if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        o = (heads * width, width)
+    else:
+        o = _out_rows(out, device, dtype, shape, query, prefix_key, prefix_value, key_cache,
+                      value_cache, current_key, current_value)
+    if not batch:
+        return out
+    word = _status_for(query, status)
+    lib, stream = _lib.lib(), _lib.stream_on(device)
+    work = None
+    need = lib.grs_shared_prefix_workspace_bytes(batch, heads, kv_heads, width, num_prefix,
+                                                 columns * page)
+    if need:
+        scratch = _lib.scratch(query, need, stream)
+        work = scratch.data_ptr()
+    _lib.check(lib.grs_shared_prefix_attention(
+        code, query.data_ptr(), q[0], q[1], prefix_key.data_ptr(), pk[0], pk[1],
+        prefix_value.data_ptr(), pv[0], pv[1], num_prefix, _lib.ptr(key_cache),
+        _lib.ptr(value_cache), c[0], c[1], c[2], table, table_row, columns, past, pages, page,
+        _lib.ptr(current_key), _lib.ptr(current_value), cur[0], cur[1], valid, out.data_ptr(),
+        o[0], o[1], batch, heads, kv_heads, width, scale, work, need, word, stream),
+        "shared-prefix attention")
     return out

@@ -17,46 +17,70 @@ import math
 import torch
 
 from . import _lib
-from .paged_attention import _status_word
+from .paged_attention import _STATUS, _status_word
 
 
-def _status_for(device: torch.device, status: torch.Tensor | None) -> torch.Tensor:
-    """The caller's status word, or the device's (``check_decode_status``)."""
+def _status_for(query: torch.Tensor, status: torch.Tensor | None) -> int:
+    """Address of the caller's status word, or of the device's
+    (``check_decode_status``)."""
     if status is not None:
-        if status.dtype != torch.int32 or status.numel() != 1 or status.device != device:
+        if (status.dtype is not torch.int32 or status.numel() != 1
+                or status.get_device() != query.get_device()):
+            _lib.require_cuda(status)
             raise ValueError("status must be one int32 on the query's device")
-        return status
-    return _status_word(device)
+        return status.data_ptr()
+    word = _STATUS.get(query.device)
+    if word is None:
+        # made under capture it would live in that graph's memory
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("make one call before capturing the first, or pass status=")
+        word = _status_word(query.device)
+    return word.data_ptr()
 
 
-def _check_rows(name: str, t: torch.Tensor, like: torch.Tensor, shape: tuple) -> None:
-    if t.device != like.device or t.dtype != like.dtype:
+def _refuse(name: str, t: torch.Tensor, device: int, dtype: torch.dtype, shape: tuple) -> None:
+    _lib.require_cuda(t)
+    if t.get_device() != device or t.dtype is not dtype:
         raise ValueError(f"{name} must have the query's device and dtype")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
-    if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name} needs a contiguous head width")
+    raise ValueError(f"{name} needs a contiguous head width")
 
 
-def _check_out(out: torch.Tensor, query: torch.Tensor, *inputs: torch.Tensor) -> None:
-    _check_rows("out", out, query, tuple(query.shape))
+def _rows(name: str, t: torch.Tensor, device: int, dtype: torch.dtype, shape: tuple) -> tuple:
+    """Strides of t, rows of the query's device and dtype and the given shape
+    with a contiguous last dimension."""
+    stride = t.stride()
+    if (t.get_device() != device or t.dtype is not dtype or t.shape != shape
+            or (stride[-1] != 1 and shape[-1] > 1)):
+        _refuse(name, t, device, dtype, shape)
+    return stride
+
+
+def _out_rows(out: torch.Tensor, device: int, dtype: torch.dtype, shape: tuple,
+              *inputs: torch.Tensor | None) -> tuple:
+    stride = _rows("out", out, device, dtype, shape)
     need = 1
-    for size, stride in sorted(zip(out.shape, out.stride()), key=lambda p: p[1]):
-        if size > 1 and stride < need:
+    for size, step in sorted(zip(shape, stride), key=lambda p: p[1]):
+        if size > 1 and step < need:
             raise ValueError("out must not overlap itself")
-        need = max(need, stride * size)
-    if out.numel() and any(out.data_ptr() == t.data_ptr() for t in (query, *inputs)):
+        need = max(need, step * size)
+    at = out.data_ptr()
+    if out.numel() and any(t is not None and t.data_ptr() == at for t in inputs):
         raise ValueError("out must not be one of the inputs")
+    return stride
 
 
-def _check_heads(query: torch.Tensor, kv_heads: int) -> None:
-    if query.dtype not in _lib.DTYPE_CODES:
+def _check_heads(query: torch.Tensor, heads: int, kv_heads: int, width: int) -> int:
+    """Type code of a query whose heads and width are supported."""
+    code = _lib.DTYPE_CODES.get(query.dtype)
+    if code is None:
         raise ValueError("attention takes bf16 or fp32 queries")
-    heads, width = query.shape[1:]
     if not 1 <= width <= 256:
         raise ValueError("head widths from 1 to 256 are supported")
-    if not kv_heads or heads % kv_heads:
+    if not kv_heads or not heads or heads % kv_heads:
         raise ValueError("query heads must be a multiple of the key/value heads")
+    return code
 
 
 def _check_scale(scale: float | None, width: int) -> float:
@@ -91,34 +115,38 @@ def prompt_attention(
     inputs.  The call neither synchronises nor reads ``offsets`` on the host,
     so it can be captured into a CUDA graph.
     """
-    _lib.require_cuda(query, key, value, offsets, out, status)
+    device = query.get_device()
+    if device < 0:
+        _lib.require_cuda(query)
+    if device != _lib.current_device():
+        with torch.cuda.device(device):
+            return prompt_attention(query, key, value, offsets, scale=scale, out=out,
+                                    status=status)
     if query.dim() != 3 or key.dim() != 3:
         raise ValueError("query must be [tokens, heads, D], key and value [tokens, kv_heads, D]")
-    tokens, heads, width = query.shape
+    shape = query.shape
+    tokens, heads, width = shape
     kv_heads = key.shape[1]
-    _check_heads(query, kv_heads)
-    _check_rows("query", query, query, tuple(query.shape))
-    _check_rows("key", key, query, (tokens, kv_heads, width))
-    _check_rows("value", value, query, (tokens, kv_heads, width))
-    if (offsets.dtype != torch.int32 or offsets.dim() != 1 or not offsets.numel()
-            or not offsets.is_contiguous() or offsets.device != query.device):
+    code, dtype = _check_heads(query, heads, kv_heads, width), query.dtype
+    q = _rows("query", query, device, dtype, shape)
+    k = _rows("key", key, device, dtype, (tokens, kv_heads, width))
+    v = _rows("value", value, device, dtype, (tokens, kv_heads, width))
+    if (offsets.dtype is not torch.int32 or offsets.dim() != 1 or not offsets.numel()
+            or not offsets.is_contiguous() or offsets.get_device() != device):
+        _lib.require_cuda(offsets)
         raise ValueError("offsets must be a contiguous int32 [sequences + 1] on the query's device")
+    scale = _check_scale(scale, width)
     fresh = out is None
     if fresh:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        o = (heads * width, width)
     else:
-        _check_out(out, query, key, value)
-    if not out.numel():
+        o = _out_rows(out, device, dtype, shape, query, key, value)
+    if not tokens:
         return out
-    scale = _check_scale(scale, width)
-    word = _status_for(query.device, status)
-    with _lib.on_device(query):
-        code = _lib.lib().grs_prompt_attention(
-            _lib.DTYPE_CODES[query.dtype], query.data_ptr(), query.stride(0), query.stride(1),
-            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-            value.stride(1), offsets.data_ptr(), offsets.numel() - 1, out.data_ptr(),
-            out.stride(0), out.stride(1), tokens, heads, kv_heads, width,
-            scale, int(fresh),
-            word.data_ptr(), _lib.stream_of(query))
-    _lib.check(code, "prompt attention")
+    word = _status_for(query, status)
+    _lib.check(_lib.lib().grs_prompt_attention(
+        code, query.data_ptr(), q[0], q[1], key.data_ptr(), k[0], k[1], value.data_ptr(), v[0],
+        v[1], offsets.data_ptr(), offsets.numel() - 1, out.data_ptr(), o[0], o[1], tokens, heads,
+        kv_heads, width, scale, int(fresh), word, _lib.stream_on(device)), "prompt attention")
     return out

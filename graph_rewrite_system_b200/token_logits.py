@@ -13,26 +13,39 @@ import torch
 from . import _lib
 
 
-def _knob(name: str, value, rows: int, device: torch.device):
-    """(device pointer or None, scalar) of a penalty given per row or for all."""
+def _ints(name: str, t: torch.Tensor | None, rows: int, device: int) -> int | None:
+    """Address of an optional int32 [rows]."""
+    if t is None:
+        return None
+    if (t.dtype is not torch.int32 or t.shape != (rows,) or not t.is_contiguous()
+            or t.get_device() != device):
+        _lib.require_cuda(t)
+        raise ValueError(f"{name} must be contiguous int32 [rows] on the logits' device")
+    return t.data_ptr()
+
+
+def _knob(name: str, value, rows: int, device: int):
+    """(address or None, scalar) of a penalty given per row or for all."""
     if isinstance(value, torch.Tensor):
-        _lib.require_cuda(value)
-        if (value.dtype != torch.float32 or tuple(value.shape) != (rows,)
-                or not value.is_contiguous() or value.device != device):
+        if (value.dtype is not torch.float32 or value.shape != (rows,)
+                or not value.is_contiguous() or value.get_device() != device):
+            _lib.require_cuda(value)
             raise ValueError(f"{name} must be a number or contiguous fp32 [rows]")
         return value.data_ptr(), 0.0
     return None, float(value)
 
 
-def _row_stride(name: str, t: torch.Tensor, rows: int, columns: int, device) -> int:
+def _table(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int, columns: int,
+           device: int) -> int:
     """Row stride of a [columns], [1, columns] or [rows, columns] tensor."""
-    if t.dim() == 1:
-        t = t.unsqueeze(0)
-    if t.dim() != 2 or t.shape[0] not in (1, rows) or t.shape[1] != columns:
-        raise ValueError(f"{name} must be [{columns}] or [{rows}, {columns}]")
-    if t.device != device or (columns > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} needs contiguous rows on the logits' device")
-    return t.stride(0) if t.shape[0] > 1 else 0
+    shape, stride = t.shape, t.stride()
+    if (t.dtype is not dtype or t.get_device() != device or not 1 <= len(shape) <= 2
+            or shape[-1] != columns or (len(shape) == 2 and shape[0] not in (1, rows))
+            or (columns > 1 and stride[-1] != 1)):
+        _lib.require_cuda(t)
+        raise ValueError(f"{name} must be {dtype} [{columns}] or [{rows}, {columns}] with "
+                         "contiguous rows on the logits' device")
+    return stride[0] if len(shape) == 2 and shape[0] > 1 else 0
 
 
 def adjust_logits(
@@ -64,57 +77,66 @@ def adjust_logits(
     nothing is all ``fill``.  repetition (> 0), presence and frequency are
     numbers or fp32 [rows].  Computed in fp32 and rounded once.
     """
-    _lib.require_cuda(logits, tokens, lengths, prompt_lengths, bias, allowed, out)
-    if logits.dtype not in _lib.DTYPE_CODES or logits.dim() != 2:
+    device = logits.get_device()
+    if device < 0:
+        _lib.require_cuda(logits)
+    if device != _lib.current_device():
+        with torch.cuda.device(device):
+            return adjust_logits(logits, tokens=tokens, lengths=lengths,
+                                 prompt_lengths=prompt_lengths, repetition=repetition,
+                                 presence=presence, frequency=frequency, bias=bias,
+                                 allowed=allowed, fill=fill, out=out)
+    dtype = logits.dtype
+    code = _lib.DTYPE_CODES.get(dtype)
+    if code is None or logits.dim() != 2:
         raise ValueError("logits must be bf16 or fp32 [rows, vocab]")
     rows, vocab = logits.shape
-    device = logits.device
-    if vocab > 1 and logits.stride(1) != 1:
+    row, step = logits.stride()
+    if vocab > 1 and step != 1:
         raise ValueError("logits need contiguous rows")
-    history = 0
+    history = tokens_row = wide = 0
+    token_ptr = None
     if tokens is not None:
         if (tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 2
-                or tokens.shape[0] != rows or tokens.device != device
+                or tokens.shape[0] != rows or tokens.get_device() != device
                 or (tokens.shape[1] > 1 and tokens.stride(1) != 1)):
+            _lib.require_cuda(tokens)
             raise ValueError("tokens must be int32 or int64 [rows, history], contiguous rows")
-        history = tokens.shape[1]
+        history, tokens_row = tokens.shape[1], tokens.stride(0)
+        wide, token_ptr = int(tokens.dtype is torch.int64), tokens.data_ptr()
     elif lengths is not None or prompt_lengths is not None:
         raise ValueError("lengths and prompt_lengths come with tokens")
-    for name, t in (("lengths", lengths), ("prompt_lengths", prompt_lengths)):
-        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (rows,)
-                              or not t.is_contiguous() or t.device != device):
-            raise ValueError(f"{name} must be contiguous int32 [rows]")
+    lengths_ptr = _ints("lengths", lengths, rows, device)
+    prompts_ptr = _ints("prompt_lengths", prompt_lengths, rows, device)
     rep_ptr, rep = _knob("repetition", repetition, rows, device)
     pres_ptr, pres = _knob("presence", presence, rows, device)
     freq_ptr, freq = _knob("frequency", frequency, rows, device)
     if rep_ptr is None and not rep > 0:
         raise ValueError("repetition must be positive")
-    bias_sb = allowed_sb = 0
+    bias_ptr = allowed_ptr = None
+    bias_row = allowed_row = 0
     if bias is not None:
-        if bias.dtype != torch.float32:
-            raise ValueError("bias must be fp32")
-        bias_sb = _row_stride("bias", bias, rows, vocab, device)
+        bias_row = _table("bias", bias, torch.float32, rows, vocab, device)
+        bias_ptr = bias.data_ptr()
     if allowed is not None:
-        if allowed.dtype != torch.int32:
-            raise ValueError("allowed must be int32 words")
-        allowed_sb = _row_stride("allowed", allowed, rows, -(-vocab // 32), device)
+        allowed_row = _table("allowed", allowed, torch.int32, rows, (vocab + 31) // 32, device)
+        allowed_ptr = allowed.data_ptr()
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-    elif (out.shape != logits.shape or out.dtype != logits.dtype or out.device != device
-          or (vocab > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < vocab)):
-        raise ValueError("out must have the logits' shape, dtype and device, contiguous rows")
-    elif out.data_ptr() == logits.data_ptr() and rows > 1 and out.stride(0) != logits.stride(0):
-        raise ValueError("out must be the logits themselves or not overlap them")
-    if not logits.numel():
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        out_row = vocab
+    else:
+        if (out.shape != logits.shape or out.dtype is not dtype or out.get_device() != device
+                or (vocab > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < vocab)):
+            _lib.require_cuda(out)
+            raise ValueError("out must have the logits' shape, dtype and device, contiguous rows")
+        out_row = out.stride(0)
+        if rows > 1 and out_row != row and out.data_ptr() == logits.data_ptr():
+            raise ValueError("out must be the logits themselves or not overlap them")
+    if not rows or not vocab:
         return out
-    with _lib.on_device(logits):
-        code = _lib.lib().grs_adjust_logits(
-            _lib.DTYPE_CODES[logits.dtype], logits.data_ptr(), logits.stride(0), out.data_ptr(),
-            out.stride(0), rows, vocab, _lib.ptr(tokens),
-            int(tokens is not None and tokens.dtype == torch.int64),
-            0 if tokens is None else tokens.stride(0), history, _lib.ptr(lengths),
-            _lib.ptr(prompt_lengths), rep_ptr, pres_ptr, freq_ptr, rep, pres, freq,
-            _lib.ptr(bias), bias_sb, _lib.ptr(allowed), allowed_sb, float(fill),
-            _lib.stream_of(logits))
-    _lib.check(code, "adjust_logits")
+    _lib.check(_lib.lib().grs_adjust_logits(
+        code, logits.data_ptr(), row, out.data_ptr(), out_row, rows, vocab, token_ptr, wide,
+        tokens_row, history, lengths_ptr, prompts_ptr, rep_ptr, pres_ptr, freq_ptr, rep, pres,
+        freq, bias_ptr, bias_row, allowed_ptr, allowed_row, float(fill),
+        _lib.stream_on(device)), "adjust_logits")
     return out

@@ -621,10 +621,11 @@ GRS_API int grs_prompt_attention(int dtype, const void* query, int64_t q_st, int
  * grs_prompt_attention.  Beams with no key are written as zeros.  Page ids
  * outside [0, num_pages) set GRS_ERR_BAD_PAGE in `status` and their tokens
  * are skipped; lengths outside [0, max_blocks * page_size] set GRS_ERR_LENGTH
- * and are clamped.  The workspace (fp32 partial sums of the prefix slices)
- * is the call's own until it has run. */
+ * and are clamped.  The workspace (fp32 partial sums; page_tokens is
+ * max_blocks * page_size; 16-byte aligned) is the call's own until it has run. */
 GRS_API int64_t grs_shared_prefix_workspace_bytes(int batch, int heads, int kv_heads,
-                                                  int head_width, int num_prefix);
+                                                  int head_width, int num_prefix,
+                                                  int64_t page_tokens);
 GRS_API int grs_shared_prefix_attention(
     int dtype, const void* query, int64_t q_sb, int64_t q_sh, const void* prefix_key,
     int64_t pk_st, int64_t pk_sh, const void* prefix_value, int64_t pv_st, int64_t pv_sh,

@@ -15,7 +15,8 @@ def lifted(monkeypatch):
         raise AssertionError("a launch was reached")
 
     monkeypatch.setattr(_lib, "require_cuda", lambda *t: None)
-    monkeypatch.setattr(_lib, "on_device", nothing)
+    monkeypatch.setattr(_lib, "current_device", lambda: -1)
+    monkeypatch.setattr(_lib, "lib", nothing)
 
 
 def _z(*shape, dtype=torch.bfloat16):
@@ -155,7 +156,7 @@ def test_c_abi_refusals():
     for change in (dict(work=None), dict(bytes=8), dict(work=260)):
         assert lib.grs_shared_prefix_attention(*{**prefix, **change}.values()) == work, change
     assert lib.grs_shared_prefix_attention(*{**prefix, "batch": 0}.values()) == 0
-    assert lib.grs_shared_prefix_workspace_bytes(2, 4, 2, 32, 0) == 0
+    assert lib.grs_shared_prefix_workspace_bytes(2, 4, 2, 32, 0, 32) == 0
     logits = dict(dtype=1, x=256, x_sb=9, out=256, o_sb=9, rows=1, vocab=9, tokens=256, i64=0,
                   t_sb=3, history=3, lengths=None, prompts=None, rep=None, pres=None, freq=None,
                   r=1.0, p=0.0, f=0.0, bias=None, b_sb=0, allowed=None, a_sb=0, fill=0.0,
