@@ -56,7 +56,7 @@ __device__ __forceinline__ void causal_range(const int32_t* __restrict__ offsets
 // sequence, a neighbour sequence, a later token); rows whose tiled result is
 // not finite are computed again here.
 template <typename T, int ND>
-__device__ void causal_row_again(const GroupedArgs<T>& a, int p, int head, int begin, int end) {
+__device__ __noinline__ void causal_row_again(const GroupedArgs<T>& a, int p, int head, int begin, int end) {
   const int lane = threadIdx.x & 31;
   const T* q = a.q + (int64_t)p * a.q_sp + (int64_t)head * a.q_sh;
   const T* kh = a.k + (int64_t)(head / a.group) * a.k_sh;
@@ -70,6 +70,7 @@ __device__ void causal_row_again(const GroupedArgs<T>& a, int p, int head, int b
     if (t < end) {
       const T* k = kh + (int64_t)t * a.k_st;
       float dot = 0.f;
+#pragma unroll 1
       for (int d = 0; d < a.D; ++d) dot = fmaf(to_float(q[d]), to_float(k[d]), dot);
       s = dot * a.scale_log2;
     }
@@ -82,6 +83,7 @@ __device__ void causal_row_again(const GroupedArgs<T>& a, int p, int head, int b
     for (int i = 0; i < ND; ++i) acc[i] *= keep;
     m = top;
     const int n = min(32, end - t0);
+#pragma unroll 1
     for (int j = 0; j < n; ++j) {
       const float wj = __shfl_sync(0xffffffffu, w, j);
       const T* v = vh + (int64_t)(t0 + j) * a.v_st;

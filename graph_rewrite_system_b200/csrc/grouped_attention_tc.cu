@@ -40,6 +40,7 @@ namespace grs {
 
 constexpr int GTC_THREADS = 384, GTC_KEYS = 128;
 constexpr int GTC_O = 256;                  // first TMEM column of the outputs
+constexpr int GTC_WINDOW = 260;             // offsets held for a tile's rows
 
 template <int DP>
 struct GtcShape {
@@ -65,11 +66,39 @@ __device__ __forceinline__ uint32_t gtc_pack(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// mbar_wait with its polling loop out of line: the kernel waits in many places
+// and its code should stay near the size of the instruction caches (the first
+// form, with everything unrolled in line, ran its once-per-tile parts at a
+// quarter of their issue rate)
+__device__ __noinline__ bool gtc_wait_more(uint64_t* bar, uint32_t parity) {
+  return sm100::mbar_wait(bar, parity);
+}
+__device__ __forceinline__ bool gtc_wait(uint64_t* bar, uint32_t parity) {
+  return sm100::mbar_try_wait(bar, parity) || gtc_wait_more(bar, parity);
+}
+
+// How many of the ascending offsets are <= p, by one warp
+__device__ __forceinline__ int offsets_up_to(const int32_t* __restrict__ offsets, int count,
+                                             int p) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = count;
+  while (hi - lo > 32) {
+    const int step = (hi - lo + 31) / 32;
+    const int at = lo + lane * step;
+    const int n = __popc(__ballot_sync(0xffffffffu, at < hi && __ldg(offsets + at) <= p));
+    if (n == 0) return lo;
+    hi = min(hi, lo + n * step);
+    lo += (n - 1) * step + 1;
+  }
+  const bool in = lo + lane < hi && __ldg(offsets + lo + lane) <= p;
+  return lo + __popc(__ballot_sync(0xffffffffu, in));
+}
+
 template <int DP, int MODE>
 __global__ void __launch_bounds__(GTC_THREADS, 1)
 grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                  const __grid_constant__ CUtensorMap tm_v, GroupedArgs<__nv_bfloat16> a, int pps,
-                  int negate) {
+                  const __grid_constant__ CUtensorMap tm_v,
+                  const __grid_constant__ GroupedArgs<__nv_bfloat16> a, int pps) {
   using namespace sm100;
   using S = GtcShape<DP>;
   constexpr bool kCausal = MODE == GTC_CAUSAL, kSplit = MODE == GTC_SPLIT;
@@ -79,8 +108,9 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   __shared__ __align__(8) uint64_t last_full, last_clean;   // the causal tile's last V block
   __shared__ uint32_t tmem_slot;
   __shared__ int failed, drain_failed;
-  // per slot: first and last key of any row, last first and first last key
-  __shared__ int lo_key[2], hi_key[2], in_lo[2], in_hi[2];
+  // per softmax warp: first and last key of any row, last first and first last key
+  __shared__ int4 spans[8];
+  __shared__ int window[kCausal ? GTC_WINDOW : 1];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(gtc_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* ring = smem + 2 * S::kTile;
@@ -98,8 +128,10 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     slice = blockIdx.z;
   }
   const int p_tile = tile * (kSplit ? pps : 2 * pps);    // first position
+  // r / group for r < 128: exact for groups below 512
+  const int per_group = (65536 + a.group - 1) / a.group;
 
-  if (tid == 0) {
+  if (tid == 8 * 32) {
     mbar_init(&q_full, 1);
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(&kv_full[s], 1);
@@ -108,28 +140,56 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 4);
-      lo_key[s] = INT_MAX;
-      hi_key[s] = 0;
-      in_lo[s] = 0;
-      in_hi[s] = INT_MAX;
     }
     mbar_init(&drain_bar, 1);
     mbar_init(&last_full, 1);
     mbar_init(&last_clean, 1);
     failed = drain_failed = 0;
     mbar_init_fence();
+    // the queries need no key range: their loads go out at once
+    const int q_slots = kSplit ? 1 : 2;
+    mbar_arrive_expect_tx(&q_full, q_slots * S::kBoxes * pps * a.group * S::kRow);
+    for (int s = 0; s < q_slots; ++s)
+      for (int b = 0; b < S::kBoxes; ++b)
+        tma_load_3d(smem + s * S::kTile + b * S::kBox, &tm_q, b * 64, h * a.group,
+                    p_tile + s * pps, &q_full);
   }
   // the kernel that joins the slices may start as SMs fall free
   if (!kCausal) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
+  // The offsets that can begin or end a sequence of this tile: all of them, or
+  // a window from the sequence of the first position on (found by a 32-way
+  // search: one round of loads per factor of 32, where a binary search per row
+  // would wait for one load per factor of 2).
+  int window_at = 0, window_n = 0;
+  if (kCausal && warp < 8) {
+    const int count = a.sequences + 1;
+    if (count > GTC_WINDOW)
+      window_at = max(0, offsets_up_to(a.offsets, count, p_tile) - 1);
+    window_n = min(GTC_WINDOW, count - window_at);
+    for (int i = tid; i < window_n; i += 256) window[i] = __ldg(a.offsets + window_at + i);
+  }
   __syncthreads();
   int begin = 0, end = 0, position = -1;
   if (tid < 256) {
     const int slot = tid >> 7, r = tid & 127;
-    const int p = p_tile + (kSplit ? 0 : slot * pps) + r / a.group;
+    const int p = p_tile + (kSplit ? 0 : slot * pps) + ((r * per_group) >> 16);
     if (r < pps * a.group && p < a.positions) position = p;
     if (kCausal) {
-      if (position >= 0) causal_range(a.offsets, a.sequences, position, begin, end);
+      if (position >= 0) {
+        int from = 0, to = window_n;       // first window entry past p
+        while (from < to) {
+          const int mid = (from + to) >> 1;
+          if (window[mid] <= position) from = mid + 1; else to = mid;
+        }
+        if (from == window_n && window_at + window_n <= a.sequences) {
+          // sequences without tokens filled the window
+          causal_range(a.offsets, a.sequences, position, begin, end);
+        } else if (from > 0 && from < window_n) {
+          begin = min(max(window[from - 1], 0), position);
+          end = position + 1;
+        }
+      }
     } else {
       begin = slice * a.slice_keys;
       end = max(begin, min(a.keys, begin + a.slice_keys));
@@ -140,17 +200,27 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       if (!kSplit && p_tile + slot * pps >= a.positions) end = begin;
     }
-    if (end > begin) {
-      atomicMin(&lo_key[slot], begin);
-      atomicMax(&hi_key[slot], end);
-      atomicMax(&in_lo[slot], begin);
-      atomicMin(&in_hi[slot], end);
-    }
+    const bool any = end > begin;
+    const int4 span = make_int4(__reduce_min_sync(0xffffffffu, any ? begin : INT_MAX),
+                                __reduce_max_sync(0xffffffffu, any ? end : 0),
+                                __reduce_max_sync(0xffffffffu, any ? begin : 0),
+                                __reduce_min_sync(0xffffffffu, any ? end : INT_MAX));
+    if (lane == 0) spans[warp] = span;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  int lo_key[2], hi_key[2], in_lo[2], in_hi[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int4 w0 = spans[4 * s], w1 = spans[4 * s + 1], w2 = spans[4 * s + 2],
+               w3 = spans[4 * s + 3];
+    lo_key[s] = min(min(w0.x, w1.x), min(w2.x, w3.x));
+    hi_key[s] = max(max(w0.y, w1.y), max(w2.y, w3.y));
+    in_lo[s] = max(max(w0.z, w1.z), max(w2.z, w3.z));
+    in_hi[s] = min(min(w0.w, w1.w), min(w2.w, w3.w));
+  }
   // block ranges [first[s], last[s]) of 128 keys from origin[s]
   int origin[2], first[2], last[2];
 #pragma unroll
@@ -170,134 +240,143 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const int end_row = kCausal && (any0 || any1)
                           ? max(hi_key[0], hi_key[1]) - origin[0] - (hi - 1) * GTC_KEYS
                           : GTC_KEYS;
-  const bool clear = end_row < GTC_KEYS;
+  const bool clear = end_row % 16 != 0;
   volatile int* gave_up = &failed;
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
     if (warp == 8) {
-      if (lane == 0 && (any0 || any1)) {   // TMA producer
-        const int q_slots = kSplit ? 1 : 2;
-        mbar_arrive_expect_tx(&q_full, q_slots * S::kBoxes * pps * a.group * S::kRow);
-        for (int s = 0; s < q_slots; ++s)
-          for (int b = 0; b < S::kBoxes; ++b)
-            tma_load_3d(smem + s * S::kTile + b * S::kBox, &tm_q, b * 64, h * a.group,
-                        p_tile + s * pps, &q_full);
+      if (lane == 0) {                   // TMA producer
+        // order of the ring: per block and stream V(j), K(j + 1)
         int g = 0;
-        int armed[S::kStages] = {};
+        unsigned armed = 0;              // stages with a load, their last phase in `phase`
+        unsigned phase = 0;
         bool last_armed = false;
-        const auto load = [&](const CUtensorMap* map, int key, bool is_last = false) {
+#pragma unroll 1
+        for (int n = 0; n < 2 * (kSplit ? 2 : 1) * (hi - lo + 1); ++n) {
+          // pair: (block, K or V); split: (block, slot, K or V)
+          const int s = kSplit ? (n >> 1) & 1 : 0, is_k = n & 1;
+          const int j = lo - 1 + (kSplit ? n >> 2 : n >> 1) + is_k;
+          const int end_j = kSplit ? (s ? last[1] : last[0]) : hi;
+          if (j < lo || j >= end_j) continue;
           const int st = g % S::kStages, r = g / S::kStages;
-          if (*gave_up) return;
-          if (r > 0 && !mbar_wait(&kv_empty[st], (r - 1) & 1)) {
+          if (*gave_up) break;
+          if (r > 0 && !gtc_wait(&kv_empty[st], (r - 1) & 1)) {
             failed = 1;
-            return;
+            break;
           }
+          const bool is_last = kCausal && clear && !is_k && j == hi - 1;
           uint64_t* bar = is_last ? &last_full : &kv_full[st];
           mbar_arrive_expect_tx(bar, S::kTile);
+          const int key = (kSplit && s ? origin[1] : origin[0]) + j * GTC_KEYS;
+#pragma unroll
           for (int b = 0; b < S::kBoxes; ++b)
-            tma_load_3d(ring + st * S::kTile + b * S::kBox, map, b * 64, h, key, bar);
-          if (is_last) last_armed = true; else armed[st] = r + 1;
-          ++g;
-        };
-        if (!kSplit) {
-          for (int j = lo - 1; j < hi; ++j) {
-            if (j >= lo) load(&tm_v, origin[0] + j * GTC_KEYS, clear && j == hi - 1);
-            if (j + 1 < hi) load(&tm_k, origin[0] + (j + 1) * GTC_KEYS);
+            tma_load_3d(ring + st * S::kTile + b * S::kBox, is_k ? &tm_k : &tm_v, b * 64, h, key,
+                        bar);
+          if (is_last) {
+            last_armed = true;
+          } else {
+            armed |= 1u << st;
+            phase = (phase & ~(1u << st)) | (unsigned)(r & 1) << st;
           }
-        } else {
-          for (int j = -1; j < hi; ++j)
-            for (int s = 0; s < 2; ++s) {
-              if (j >= 0 && j < last[s]) load(&tm_v, origin[s] + j * GTC_KEYS);
-              if (j + 1 < last[s]) load(&tm_k, origin[s] + (j + 1) * GTC_KEYS);
-            }
+          ++g;
         }
         // every load in flight lands before the CTA exits
-        if (!mbar_wait(&q_full, 0)) drain_failed = 1;
-        if (last_armed && !mbar_wait(&last_full, 0)) drain_failed = 1;
+        if (!gtc_wait(&q_full, 0)) drain_failed = 1;
+        if (last_armed && !gtc_wait(&last_full, 0)) drain_failed = 1;
+#pragma unroll 1
         for (int s = 0; s < S::kStages; ++s)
-          if (armed[s] > 0 && !mbar_wait(&kv_full[s], (armed[s] - 1) & 1)) drain_failed = 1;
+          if (((armed >> s) & 1) && !gtc_wait(&kv_full[s], (phase >> s) & 1)) drain_failed = 1;
       }
-    } else if (warp == 9) {
-      if (lane == 0) {                     // MMA issuer
-        constexpr uint32_t i_qk = idesc_bf16_f32(128, GTC_KEYS);
-        constexpr uint32_t i_pv = idesc_bf16_f32(128, DP) | IDESC_B_MN;
-        constexpr int kPerBox = S::kRow / 32;             // 16-element steps of a box
-        int g = 0;
-        bool ok = any0 || any1;
-        if (ok && !mbar_wait(&q_full, 0)) ok = false;
-        const auto arrived = [&](int at) {
-          if (ok && !mbar_wait(&kv_full[at % S::kStages], (at / S::kStages) & 1)) ok = false;
-          tc_fence_after();
-        };
-        const auto scores = [&](int s, int at) {
-          const uint64_t qd = smem_desc(smem + (kSplit ? 0 : s) * S::kTile, S::kRow, 16, 8 * S::kRow);
-          const uint64_t kd = smem_desc(ring + (at % S::kStages) * S::kTile, S::kRow, 16,
-                                        8 * S::kRow);
-  #pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk) {
-            const uint32_t off = ((kk / kPerBox) * S::kBox + (kk % kPerBox) * 32) >> 4;
-            mma_bf16(tmem + s * GTC_KEYS, qd + off, kd + off, i_qk, kk > 0);
+    } else if (warp == 9) {              // MMA issuer
+      // The whole warp walks the loop and one elected lane issues, so that
+      // addresses and descriptors stay in uniform registers (2.21 -> 1.82 ms on
+      // 16384 tokens against a loop inside `if (lane == 0)`); what a block
+      // needs is computed before the wait for its weights.
+      uint32_t elected;
+      asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
+                   : "=r"(elected));
+      const bool lead = elected != 0;
+      constexpr uint32_t i_pv = idesc_bf16_f32(128, DP) | IDESC_B_MN;
+      constexpr int kPerBox = S::kRow / 32;             // 16-element steps of a box
+      constexpr int kSteps = GTC_KEYS / 16;
+      // products of a slot's last block stop at its last key, in steps of 16
+      const int tail0 = (hi_key[0] - origin[0] - (last[0] - 1) * GTC_KEYS + 15) / 16;
+      const int tail1 = (hi_key[1] - origin[1] - (last[1] - 1) * GTC_KEYS + 15) / 16;
+      const uint64_t q_desc = smem_desc(smem, S::kRow, 16, 8 * S::kRow);
+      const uint64_t k_desc = smem_desc(ring, S::kRow, 16, 8 * S::kRow);
+      const uint64_t v_desc = smem_desc(ring, S::kRow, S::kBox, 8 * S::kRow);
+      int v_st = 0, k_st = 0, next = 0;                 // ring stages and phase bits
+      uint32_t v_ph = 0, k_ph = 0, ph = 0;
+      bool ok = any0 || any1;
+      if (ok && !mbar_wait(&q_full, 0)) ok = false;
+#pragma unroll 1
+      for (int n = 0; n < 2 * (hi - lo + 1) && ok; ++n) {
+        const int s = n & 1, j = lo - 1 + (n >> 1);     // P V of block j, Q K of block j + 1
+        const int first_s = s ? first[1] : first[0], last_s = s ? last[1] : last[0];
+        const bool v_here = j >= (kSplit ? first_s : lo) && j < (kSplit ? last_s : hi);
+        const bool k_here = j + 1 < (kSplit ? last_s : hi);
+        const bool v_mine = j >= first_s && j < last_s;
+        const bool k_mine = j + 1 >= first_s && j + 1 < last_s;
+        const int tail = s ? tail1 : tail0, i = j - first_s;
+        if (kSplit || s == 0) {          // the pair's second slot takes the same blocks
+          if (v_here) {
+            v_st = next;
+            v_ph = ph;
+            if (++next == S::kStages) next = 0, ph ^= 1;
           }
-          mma_commit(&s_full[s]);
-        };
-        const auto values = [&](int s, int at, int i) {
-          if (ok && !mbar_wait(&p_full[s], i & 1)) ok = false;
-          tc_fence_after();
-          if (!ok) return;
-          const uint64_t vd = smem_desc(ring + (at % S::kStages) * S::kTile, S::kRow, S::kBox,
-                                        8 * S::kRow);
-  #pragma unroll
-          for (int kk = 0; kk < GTC_KEYS / 16; ++kk)
-            mma_bf16_tmem_a(tmem + GTC_O + s * DP, tmem + s * GTC_KEYS + kk * 8,
-                            vd + kk * ((16 * S::kRow) >> 4), i_pv, i > 0 || kk > 0);
-          if (i == last[s] - first[s] - 1) mma_commit(&s_full[s]);
-        };
-        if (!kSplit) {
-          for (int j = lo - 1; j < hi && ok; ++j) {
-            const int gv = j >= lo ? g++ : -1, gk = j + 1 < hi ? g++ : -1;
-            if (gv >= 0) {
-              if (clear && j == hi - 1) {
-                if (!mbar_wait(&last_clean, 0)) ok = false;
-                tc_fence_after();
-              } else {
-                arrived(gv);
-              }
-            }
-  #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              if (j >= first[s] && j < last[s]) values(s, gv, j - first[s]);
-              if (s == 1 && gv >= 0 && ok) mma_commit(&kv_empty[gv % S::kStages]);
-              if (s == 0 && gk >= 0) arrived(gk);
-              if (ok && j + 1 >= first[s] && j + 1 < last[s]) scores(s, gk);
-            }
-            if (gk >= 0 && ok) mma_commit(&kv_empty[gk % S::kStages]);
+          if (k_here) {
+            k_st = next;
+            k_ph = ph;
+            if (++next == S::kStages) next = 0, ph ^= 1;
           }
-        } else {
-          for (int j = -1; j < hi && ok; ++j)
-  #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              if (j >= 0 && j < last[s]) {
-                const int gv = g++;
-                arrived(gv);
-                values(s, gv, j);
-                if (ok) mma_commit(&kv_empty[gv % S::kStages]);
-              }
-              if (j + 1 < last[s]) {
-                const int gk = g++;
-                arrived(gk);
-                if (ok) {
-                  scores(s, gk);
-                  mma_commit(&kv_empty[gk % S::kStages]);
-                }
-              }
-            }
+          if (v_here)
+            ok = kCausal && clear && j == hi - 1 ? mbar_wait(&last_clean, 0)
+                                                 : mbar_wait(&kv_full[v_st], v_ph);
+          if (ok && k_here) ok = mbar_wait(&kv_full[k_st], k_ph);
         }
-        if (!ok && (any0 || any1)) failed = 1;
-        // no MMA may still use TMEM or shared memory when they are given back
-        mma_commit(&drain_bar);
-        if (!mbar_wait(&drain_bar, 0)) drain_failed = 1;
+        const int steps = j == last_s - 1 ? tail : kSteps;
+        const uint64_t vd = v_desc + v_st * (S::kTile >> 4);
+        const uint64_t qd = q_desc + (kSplit ? 0 : s) * (S::kTile >> 4);
+        const uint64_t kd = k_desc + k_st * (S::kTile >> 4);
+        const uint32_t t_s = tmem + s * GTC_KEYS, t_o = tmem + GTC_O + s * DP;
+        const uint32_t i_qk = idesc_bf16_f32(128, j + 2 == last_s ? tail * 16 : GTC_KEYS);
+        if (ok && v_mine) ok = mbar_wait(&p_full[s], i & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lead) {
+          if (v_mine) {
+            if (steps == kSteps) {
+#pragma unroll
+              for (int kk = 0; kk < kSteps; ++kk)
+                mma_bf16_tmem_a(t_o, t_s + kk * 8, vd + kk * ((16 * S::kRow) >> 4), i_pv,
+                                i > 0 || kk > 0);
+            } else {
+#pragma unroll 1
+              for (int kk = 0; kk < steps; ++kk)
+                mma_bf16_tmem_a(t_o, t_s + kk * 8, vd + kk * ((16 * S::kRow) >> 4), i_pv,
+                                i > 0 || kk > 0);
+            }
+            if (j == last_s - 1) mma_commit(&s_full[s]);
+          }
+          if (k_mine) {
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+              const uint32_t off = ((kk / kPerBox) * S::kBox + (kk % kPerBox) * 32) >> 4;
+              mma_bf16(t_s, qd + off, kd + off, i_qk, kk > 0);
+            }
+            mma_commit(&s_full[s]);
+          }
+          if (kSplit || s == 1) {
+            if (v_here) mma_commit(&kv_empty[v_st]);
+            if (k_here) mma_commit(&kv_empty[k_st]);
+          }
+        }
       }
+      if (!ok && (any0 || any1)) failed = 1;
+      // no MMA may still use TMEM or shared memory when they are given back
+      if (lead) mma_commit(&drain_bar);
+      if (!mbar_wait(&drain_bar, 0)) drain_failed = 1;
     } else if (kCausal && warp == 10 && clear) {
       const int at = 1 + 2 * (hi - 1 - lo);   // its place in the ring
       // (the stream may still be a whole tile's work away from its last block)
@@ -307,7 +386,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         uint8_t* block = ring + (at % S::kStages) * S::kTile;
         constexpr int kPieces = S::kRow / 16;
         for (int b = 0; b < S::kBoxes; ++b)
-          for (int i = end_row * kPieces + lane; i < GTC_KEYS * kPieces; i += 32)
+          for (int i = end_row * kPieces + lane; i < (end_row + 15) / 16 * 16 * kPieces; i += 32)
             *reinterpret_cast<uint4*>(block + b * S::kBox + i * 16) = make_uint4(0, 0, 0, 0);
         fence_async_shared();
         __syncwarp();
@@ -323,7 +402,8 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + slot * GTC_KEYS, t_o = tmem + lanes + GTC_O + slot * DP;
     const float c = a.scale_log2, slack = 8.f / c;
-    const int all_from = in_lo[slot], all_to = in_hi[slot];
+    const int all_from = slot == 0 ? in_lo[0] : in_lo[1];
+    const int all_to = slot == 0 ? in_hi[0] : in_hi[1];
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int i = 0; i < blocks; ++i) {
@@ -337,20 +417,23 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       for (int q = 0; q < 4; ++q) tmem_load32_async(t_s + 32 * q, raw[q]);
 #pragma unroll
       for (int q = 0; q < 4; ++q) tmem_loaded32(raw[q]);
-      if (negate) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int j = 0; j < 32; ++j) raw[q][j] ^= 0x80000000u;
-      }
       const int key0 = key_first + i * GTC_KEYS;
+      unsigned live = 0xf;                 // runs of 32 keys that some row of the warp sees
       if (key0 < all_from || key0 + GTC_KEYS > all_to) {
         const int from = begin - key0, to = end - key0;
+        const int least = __reduce_min_sync(0xffffffffu, to > from ? from : INT_MAX);
+        const int most = __reduce_max_sync(0xffffffffu, to > from ? to : 0);
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < 4; ++q) {
+          if (32 * q >= most || 32 * q + 32 <= least) live &= ~(1u << q);
+          // bit j: key 32 q + j is seen
+          const int f = min(max(from - 32 * q, 0), 32), e = min(max(to - 32 * q, 0), 32);
+          const uint32_t seen_bits =
+              (e == 32 ? 0xffffffffu : (1u << e) - 1u) & (f == 32 ? 0u : 0xffffffffu << f);
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (32 * q + j < from || 32 * q + j >= to) raw[q][j] = 0xff800000u;
+            if (!(seen_bits & (1u << j))) raw[q][j] = 0xff800000u;
+        }
       }
       float top = -INFINITY;
       {
@@ -371,7 +454,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           const float keep = grown ? gtc_exp2((m - top) * c) : 1.f;
           if (grown) m = top;
           l *= keep;
-#pragma unroll
+#pragma unroll 1
           for (int q = 0; q < DP / 32; ++q) {
             uint32_t o[32];
             tmem_load32_async(t_o + 32 * q, o);
@@ -389,10 +472,15 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       for (int half = 0; half < 2; ++half) {
         uint32_t packed[32];
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t* s = raw[2 * half + q];
+          if (!((live >> (2 * half + q)) & 1)) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) packed[16 * q + j] = 0;
+            continue;
+          }
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const uint32_t* s = raw[2 * half + q];
             float2 x = __ffma2_rn(make_float2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])),
                                   c2, b2);
             x.x = gtc_exp2(x.x);
@@ -400,6 +488,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             sum = __fadd2_rn(sum, x);
             packed[16 * q + j / 2] = gtc_pack(x.x, x.y);
           }
+        }
         tmem_store32(t_s + 32 * half, packed);
       }
       l += sum.x + sum.y;
@@ -425,6 +514,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         return reinterpret_cast<uint4*>(stage + row * (DP * 2) + ((at ^ x) << 4));
       };
       bool odd = seen && !(fabsf(l) <= FLT_MAX);
+      float2 nil = make_float2(0.f, 0.f);     // stays 0 while every output is finite
 #pragma unroll 1
       for (int q = 0; q < DP / 32; ++q) {
         uint32_t o[32];
@@ -432,50 +522,47 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           tmem_load32_async(t_o + 32 * q, o);
           tmem_loaded32(o);
         }
-        float big = 0.f;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float x = seen ? __uint_as_float(o[j]) * inv : 0.f;
-          big = fmaxf(big, x == x ? fabsf(x) : INFINITY);
-          o[j] = __float_as_uint(x);
-        }
-        odd |= big == INFINITY;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          uint4 w;
-          w.x = gtc_pack(__uint_as_float(o[8 * k]), __uint_as_float(o[8 * k + 1]));
-          w.y = gtc_pack(__uint_as_float(o[8 * k + 2]), __uint_as_float(o[8 * k + 3]));
-          w.z = gtc_pack(__uint_as_float(o[8 * k + 4]), __uint_as_float(o[8 * k + 5]));
-          w.w = gtc_pack(__uint_as_float(o[8 * k + 6]), __uint_as_float(o[8 * k + 7]));
-          *piece(r, 4 * q + k) = w;
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float2 x = __fmul2_rn(make_float2(__uint_as_float(o[8 * k + 2 * j]),
+                                              __uint_as_float(o[8 * k + 2 * j + 1])),
+                                  make_float2(inv, inv));
+            nil = __ffma2_rn(x, make_float2(0.f, 0.f), nil);
+            w[j] = seen ? gtc_pack(x.x, x.y) : 0u;
+          }
+          *piece(r, 4 * q + k) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
+      odd |= seen && !(nil.x + nil.y == 0.f);
       __syncwarp();
-      const int row0 = (warp & 3) * 32;
       const bool mine = position >= 0 && (seen || a.clear_rest);
       const unsigned write = __ballot_sync(0xffffffffu, mine && ok);
       unsigned again = __ballot_sync(0xffffffffu, odd && seen && ok);
-#pragma unroll 1
+      const int head = h * a.group + r - ((r * per_group) >> 16) * a.group;
+      const int64_t to = (int64_t)position * a.o_sp + (int64_t)head * a.o_sh;
+      const int row0 = (warp & 3) * 32, at = lane % kPieces;
+#pragma unroll 4
       for (int i = 0; i < 32; i += 32 / kPieces) {
-        const int rr = i + lane / kPieces, at = lane % kPieces;
-        if (!((write >> rr) & 1) || at * 8 >= a.D) continue;
-        const int row = row0 + rr;
-        const int p = p_tile + slot * pps + row / a.group, head = h * a.group + row % a.group;
-        *reinterpret_cast<uint4*>(a.out + (int64_t)p * a.o_sp + (int64_t)head * a.o_sh + at * 8) =
-            *piece(row, at);
+        const int rr = i + lane / kPieces;
+        const int64_t off = __shfl_sync(0xffffffffu, to, rr);
+        if (((write >> rr) & 1) && at * 8 < a.D)
+          *reinterpret_cast<uint4*>(a.out + off + at * 8) = *piece(row0 + rr, at);
       }
       __syncwarp();
       while (again) {
-        const int rr = __ffs(again) - 1, row = row0 + rr;
+        const int rr = __ffs(again) - 1;
         again &= again - 1;
         causal_row_again<__nv_bfloat16, DP / 32>(
-            a, p_tile + slot * pps + row / a.group, h * a.group + row % a.group,
+            a, __shfl_sync(0xffffffffu, position, rr), __shfl_sync(0xffffffffu, head, rr),
             __shfl_sync(0xffffffffu, begin, rr), __shfl_sync(0xffffffffu, end, rr));
       }
     } else {
       const int part = kSplit ? 2 * slice + slot : slice;
       const int64_t at = ((int64_t)part * a.positions + position) * a.heads +
-                         (int64_t)h * a.group + r % a.group;
+                         (int64_t)h * a.group + r - ((r * per_group) >> 16) * a.group;
 #pragma unroll 1
       for (int q = 0; q < DP / 32; ++q) {
         uint32_t o[32];
@@ -558,8 +645,7 @@ int gtc_launch(const GroupedArgs<__nv_bfloat16>& args, cudaStream_t stream) {
   const int pps = 128 / a.group;                        // positions of a slot
   const int cols = S::kRow / 2;
   // a zero scale weighs every key alike; masked scores must stay -inf
-  const int negate = a.scale_log2 < 0.f;
-  a.scale_log2 = std::max(std::fabs(a.scale_log2), 1e-30f);
+  a.scale_log2 = std::max(a.scale_log2, 1e-30f);
   CUtensorMap q, k, v;
   if (!gtc_map(&q, a.q, a.positions, a.heads, a.D, a.q_sp, a.q_sh, cols, a.group, pps) ||
       !gtc_map(&k, a.k, a.keys, a.kv_heads, a.D, a.k_st, a.k_sh, cols, 1, GTC_KEYS) ||
@@ -576,8 +662,7 @@ int gtc_launch(const GroupedArgs<__nv_bfloat16>& args, cudaStream_t stream) {
   if (cudaFuncSetAttribute(grouped_tc_kernel<DP, MODE>,
                            cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
     return GRS_ERR_CUDA;
-  grouped_tc_kernel<DP, MODE><<<grid, GTC_THREADS, S::kSmem, counted(stream)>>>(q, k, v, a, pps,
-                                                                               negate);
+  grouped_tc_kernel<DP, MODE><<<grid, GTC_THREADS, S::kSmem, counted(stream)>>>(q, k, v, a, pps);
   GRS_CUDA_CHECK_LAUNCH();
   return GRS_OK;
 }
@@ -592,7 +677,7 @@ int gtc_width(const GroupedArgs<__nv_bfloat16>& a, cudaStream_t stream) {
 }  // namespace
 
 bool grouped_tc_takes(const GroupedArgs<__nv_bfloat16>& a) {
-  return a.D <= 128 && a.group <= 128 &&
+  return a.D <= 128 && a.group <= 128 && a.scale_log2 >= 0.f &&
          gtc_rows_ok(a.q, a.positions, a.q_sp, a.heads, a.q_sh, a.D) &&
          gtc_rows_ok(a.k, a.keys, a.k_st, a.kv_heads, a.k_sh, a.D) &&
          gtc_rows_ok(a.v, a.keys, a.v_st, a.kv_heads, a.v_sh, a.D) &&
