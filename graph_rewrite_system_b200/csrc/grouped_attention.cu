@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(GA_THREADS) grouped_rows_kernel(GroupedArgs<T>
         if (row < total && row_end[r] > row_begin[r])
           causal_row_again<T, (DP + 31) / 32>(a, (int)(row / a.group),
                                               h * a.group + (int)(row % a.group), row_begin[r],
-                                              row_end[r]);
+                                              row_end[r], 0, a.D);
       }
     }
   }

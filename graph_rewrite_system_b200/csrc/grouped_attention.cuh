@@ -54,9 +54,11 @@ __device__ __forceinline__ void causal_range(const int32_t* __restrict__ offsets
 // sees.  The tiled kernels multiply masked keys by a weight of zero, which is
 // nothing unless such a key's value is infinite or NaN (rows behind the last
 // sequence, a neighbour sequence, a later token); rows whose tiled result is
-// not finite are computed again here.
+// not finite are computed again here, columns [column0, column1) of at most
+// 32 ND.
 template <typename T, int ND>
-__device__ __noinline__ void causal_row_again(const GroupedArgs<T>& a, int p, int head, int begin, int end) {
+__device__ __noinline__ void causal_row_again(const GroupedArgs<T>& a, int p, int head, int begin, int end,
+                                              int column0, int column1) {
   const int lane = threadIdx.x & 31;
   const T* q = a.q + (int64_t)p * a.q_sp + (int64_t)head * a.q_sh;
   const T* kh = a.k + (int64_t)(head / a.group) * a.k_sh;
@@ -89,8 +91,8 @@ __device__ __noinline__ void causal_row_again(const GroupedArgs<T>& a, int p, in
       const T* v = vh + (int64_t)(t0 + j) * a.v_st;
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
-        const int d = lane + 32 * i;
-        if (d < a.D) acc[i] = fmaf(wj, to_float(v[d]), acc[i]);
+        const int d = column0 + lane + 32 * i;
+        if (d < column1) acc[i] = fmaf(wj, to_float(v[d]), acc[i]);
       }
     }
     // a NaN weight makes every later sum NaN: the row is decided
@@ -100,8 +102,8 @@ __device__ __noinline__ void causal_row_again(const GroupedArgs<T>& a, int p, in
   T* o = a.out + (int64_t)p * a.o_sp + (int64_t)head * a.o_sh;
 #pragma unroll
   for (int i = 0; i < ND; ++i) {
-    const int d = lane + 32 * i;
-    if (d < a.D) o[d] = from_float<T>(acc[i] * inv);
+    const int d = column0 + lane + 32 * i;
+    if (d < column1) o[d] = from_float<T>(acc[i] * inv);
   }
 }
 

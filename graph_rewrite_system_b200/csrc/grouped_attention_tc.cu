@@ -4,20 +4,22 @@
 // One CTA per SM works on two "slots" of 128 rows that take turns on the
 // tensor cores, so that one slot's softmax runs under the other slot's
 // products.  Per 128-key block and slot: S = Q K^T (tcgen05.mma, fp32 in
-// TMEM); four softmax warps read S, one row per thread, and write the weights
-// back over S as bf16; O += P V takes the weights from TMEM.  The running
-// maximum is lazy: O and the sum are rescaled only when the maximum has grown
-// by more than 2^8 in weight, which fp32 sums and bf16 weights (same relative
-// rounding at any exponent) do not notice.  The commit that hands a slot its
-// next scores also covers the slot's previous P V, so the softmax warps may
-// rescale O in place without a further barrier.
+// TMEM); eight softmax warps read S and write the weights back over S as bf16;
+// O += P V takes the weights from TMEM.  Two threads share a row, 64 keys
+// each, and exchange the row's maximum: a slot's turn is a chain of latencies
+// (scores out, maximum, exponentials, weights in, products), and four softmax
+// warps per scheduler hide them where two with 128 keys a thread did not.  The
+// running maximum is lazy: O and the sum are rescaled only when the maximum
+// has grown by more than 2^8 in weight, which fp32 sums and bf16 weights (same
+// relative rounding at any exponent) do not notice.  The commit that hands a
+// slot its next scores also covers the slot's previous P V, so the softmax
+// warps may rescale O in place without a further barrier.
 //
-//   warps 0-3   softmax and epilogue of slot 0      warp 8  TMA loads
-//   warps 4-7   softmax and epilogue of slot 1      warp 9  MMA issue
-//   warp 10     zeroes the value rows behind a causal tile's last key
-// The launch's 384 x 168 registers are split 216 to a softmax thread, which
-// holds a row's 128 scores, and 72 to the other warpgroup (256 x 216 + 128 x
-// 72 = 64512 = 384 x 168).
+//   warps 0-7   softmax and epilogue of slot 0      warp 16  TMA loads
+//   warps 8-15  softmax and epilogue of slot 1      warps 17, 19  MMA issue
+//   warp 18     zeroes the value rows behind a causal tile's last key
+// The launch's 640 x 96 registers are split 104 to a softmax thread and 64 to
+// the other warpgroup (512 x 104 + 128 x 64 = 61440 = 640 x 96).
 //
 // Causal and wide-batch slices give the slots neighbouring row tiles over one
 // K/V stream (each K/V block is loaded once for 256 rows); a batch of at most
@@ -28,6 +30,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -38,8 +41,9 @@
 
 namespace grs {
 
-constexpr int GTC_THREADS = 384, GTC_KEYS = 128;
+constexpr int GTC_THREADS = 640, GTC_KEYS = 128;
 constexpr int GTC_O = 256;                  // first TMEM column of the outputs
+constexpr int GTC_EMULATE = 4;              // one pair in four takes gtc_exp2_pair
 constexpr int GTC_WINDOW = 260;             // offsets held for a tile's rows
 
 template <int DP>
@@ -50,8 +54,8 @@ struct GtcShape {
   static constexpr int kTile = kBoxes * kBox;           // Q tile, K or V block
   static constexpr int kStages = DP == 128 ? 5 : DP == 64 ? 6 : 13;
   // above half an SM's shared memory: the 512 TMEM columns are one CTA's
-  static constexpr int kSmem = (2 + kStages) * kTile + 1024;
-  static_assert(kSmem > 116 * 1024 && kSmem <= 227 * 1024, "one CTA per SM");
+  static constexpr int kTiles = (2 + kStages) * kTile;
+  static_assert(kTiles > 114 * 1024 && kTiles <= 224 * 1024, "one CTA per SM");
 };
 
 constexpr int GTC_CAUSAL = 0, GTC_PAIR = 1, GTC_SPLIT = 2;
@@ -60,6 +64,27 @@ __device__ __forceinline__ float gtc_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^x of a pair on the multiply-add pipes: x = n + f with n = floor(x) taken by
+// adding 1.5 * 2^23 rounded down, 2^f on [0, 1) by the cubic of least largest
+// relative error (8.6e-5 = 2^-13.5, a thirtieth of the weights' rounding to
+// bf16) among those that are 1 at 0, n added to the exponent bits.  x is cut
+// at -127, where that gives exactly 0, so masked scores (-inf) weigh nothing.
+__device__ __forceinline__ float2 gtc_exp2_pair(float2 x) {
+  const auto both = [](float v) { return make_float2(v, v); };
+  x = make_float2(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
+  const float2 t = __fadd2_rd(x, both(12582912.f));
+  const float2 f = __ffma2_rn(__fadd2_rn(t, both(-12582912.f)), both(-1.f), x);
+  float2 p = __ffma2_rn(both(0.07706641f), f, both(0.22764569f));
+  p = __ffma2_rn(p, f, both(0.69511663f));
+  p = __ffma2_rn(p, f, both(1.f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+__device__ __forceinline__ float gtc_max3(float x, float y, float z) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+  return m;
 }
 __device__ __forceinline__ uint32_t gtc_pack(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -104,13 +129,17 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   constexpr bool kCausal = MODE == GTC_CAUSAL, kSplit = MODE == GTC_SPLIT;
   extern __shared__ uint8_t gtc_smem_raw[];
   __shared__ __align__(8) uint64_t q_full, kv_full[S::kStages], kv_empty[S::kStages];
-  __shared__ __align__(8) uint64_t s_full[2], p_full[2], drain_bar;
+  __shared__ __align__(8) uint64_t s_full[2][2], p_full[2][2], drain_bar;
+  __shared__ __align__(8) uint64_t turn[2];                 // slot s has issued a block
+  __shared__ __align__(8) uint64_t pair_bar[8];             // the two warps of 32 rows
   __shared__ __align__(8) uint64_t last_full, last_clean;   // the causal tile's last V block
   __shared__ uint32_t tmem_slot;
   __shared__ int failed, drain_failed;
   // per softmax warp: first and last key of any row, last first and first last key
-  __shared__ int4 spans[8];
-  __shared__ int window[kCausal ? GTC_WINDOW : 1];
+  __shared__ int4 spans[16];
+  // the window of offsets; then per slot the maxima [parity][half][row] in
+  // bf16; then its sums [half][row] in fp32
+  __shared__ int scratch[512];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(gtc_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* ring = smem + 2 * S::kTile;
@@ -131,17 +160,22 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   // r / group for r < 128: exact for groups below 512
   const int per_group = (65536 + a.group - 1) / a.group;
 
-  if (tid == 8 * 32) {
+  if (tid == 16 * 32) {
     mbar_init(&q_full, 1);
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&kv_empty[s], kSplit ? 1 : 2);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
+      for (int half = 0; half < 2; ++half) {
+        mbar_init(&s_full[s][half], 1);
+        mbar_init(&p_full[s][half], 4);
+      }
     }
-    mbar_init(&drain_bar, 1);
+    mbar_init(&drain_bar, 2);
+    for (int s = 0; s < 8; ++s) mbar_init(&pair_bar[s], 2);
+    mbar_init(&turn[0], 1);
+    mbar_init(&turn[1], 1);
     mbar_init(&last_full, 1);
     mbar_init(&last_clean, 1);
     failed = drain_failed = 0;
@@ -156,23 +190,23 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   }
   // the kernel that joins the slices may start as SMs fall free
   if (!kCausal) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  if (warp == 9) tmem_alloc(&tmem_slot, 512);
+  if (warp == 17) tmem_alloc(&tmem_slot, 512);
   // The offsets that can begin or end a sequence of this tile: all of them, or
   // a window from the sequence of the first position on (found by a 32-way
   // search: one round of loads per factor of 32, where a binary search per row
   // would wait for one load per factor of 2).
   int window_at = 0, window_n = 0;
-  if (kCausal && warp < 8) {
+  if (kCausal && warp < 16) {
     const int count = a.sequences + 1;
     if (count > GTC_WINDOW)
       window_at = max(0, offsets_up_to(a.offsets, count, p_tile) - 1);
     window_n = min(GTC_WINDOW, count - window_at);
-    for (int i = tid; i < window_n; i += 256) window[i] = __ldg(a.offsets + window_at + i);
+    for (int i = tid; i < window_n; i += 512) scratch[i] = __ldg(a.offsets + window_at + i);
   }
   __syncthreads();
   int begin = 0, end = 0, position = -1;
-  if (tid < 256) {
-    const int slot = tid >> 7, r = tid & 127;
+  if (tid < 512) {
+    const int slot = tid >> 8, r = tid & 127;
     const int p = p_tile + (kSplit ? 0 : slot * pps) + ((r * per_group) >> 16);
     if (r < pps * a.group && p < a.positions) position = p;
     if (kCausal) {
@@ -180,13 +214,13 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         int from = 0, to = window_n;       // first window entry past p
         while (from < to) {
           const int mid = (from + to) >> 1;
-          if (window[mid] <= position) from = mid + 1; else to = mid;
+          if (scratch[mid] <= position) from = mid + 1; else to = mid;
         }
         if (from == window_n && window_at + window_n <= a.sequences) {
           // sequences without tokens filled the window
           causal_range(a.offsets, a.sequences, position, begin, end);
         } else if (from > 0 && from < window_n) {
-          begin = min(max(window[from - 1], 0), position);
+          begin = min(max(scratch[from - 1], 0), position);
           end = position + 1;
         }
       }
@@ -214,8 +248,8 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   int lo_key[2], hi_key[2], in_lo[2], in_hi[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const int4 w0 = spans[4 * s], w1 = spans[4 * s + 1], w2 = spans[4 * s + 2],
-               w3 = spans[4 * s + 3];
+    const int4 w0 = spans[8 * s], w1 = spans[8 * s + 1], w2 = spans[8 * s + 2],
+               w3 = spans[8 * s + 3];
     lo_key[s] = min(min(w0.x, w1.x), min(w2.x, w3.x));
     hi_key[s] = max(max(w0.y, w1.y), max(w2.y, w3.y));
     in_lo[s] = max(max(w0.z, w1.z), max(w2.z, w3.z));
@@ -243,9 +277,9 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const bool clear = end_row % 16 != 0;
   volatile int* gave_up = &failed;
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
-    if (warp == 8) {
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
+    if (warp == 16) {
       if (lane == 0) {                   // TMA producer
         // order of the ring: per block and stream V(j), K(j + 1)
         int g = 0;
@@ -288,96 +322,127 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         for (int s = 0; s < S::kStages; ++s)
           if (((armed >> s) & 1) && !gtc_wait(&kv_full[s], (phase >> s) & 1)) drain_failed = 1;
       }
-    } else if (warp == 9) {              // MMA issuer
-      // The whole warp walks the loop and one elected lane issues, so that
-      // addresses and descriptors stay in uniform registers (2.21 -> 1.82 ms on
-      // 16384 tokens against a loop inside `if (lane == 0)`); what a block
-      // needs is computed before the wait for its weights.
+    } else if (warp != 18) {             // MMA issuer of one slot
+      // A warp per slot: what it computes between two blocks runs under the
+      // other slot's products.  The two issue in turn, which keeps the slots half
+      // a period apart (without the turns they fall into step, both in their
+      // softmax, then both waiting for products: 1.87 against 1.73 ms on 16384
+      // tokens).  The whole warp walks the loop and one elected lane issues, so
+      // that addresses and descriptors can stay in uniform registers.  Per block
+      // the slot issues P V of its first 64 keys and the next scores for 64 keys,
+      // then the same for the other 64: each half of the softmax warps waits for
+      // its own half only.
+      const int s = warp == 17 ? 0 : 1;
       uint32_t elected;
       asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
                    : "=r"(elected));
       const bool lead = elected != 0;
       constexpr uint32_t i_pv = idesc_bf16_f32(128, DP) | IDESC_B_MN;
       constexpr int kPerBox = S::kRow / 32;             // 16-element steps of a box
-      constexpr int kSteps = GTC_KEYS / 16;
-      // products of a slot's last block stop at its last key, in steps of 16
-      const int tail0 = (hi_key[0] - origin[0] - (last[0] - 1) * GTC_KEYS + 15) / 16;
-      const int tail1 = (hi_key[1] - origin[1] - (last[1] - 1) * GTC_KEYS + 15) / 16;
-      const uint64_t q_desc = smem_desc(smem, S::kRow, 16, 8 * S::kRow);
+      const int first_s = s ? first[1] : first[0], last_s = s ? last[1] : last[0];
+      // products of the slot's last block stop at its last key, in steps of 16
+      const int tail = ((s ? hi_key[1] : hi_key[0]) - (s ? origin[1] : origin[0]) -
+                        (last_s - 1) * GTC_KEYS + 15) / 16;
+      const uint64_t q_desc = smem_desc(smem + (kSplit ? 0 : s) * S::kTile, S::kRow, 16,
+                                        8 * S::kRow);
       const uint64_t k_desc = smem_desc(ring, S::kRow, 16, 8 * S::kRow);
       const uint64_t v_desc = smem_desc(ring, S::kRow, S::kBox, 8 * S::kRow);
-      int v_st = 0, k_st = 0, next = 0;                 // ring stages and phase bits
-      uint32_t v_ph = 0, k_ph = 0, ph = 0;
+      const uint32_t t_s = tmem + s * GTC_KEYS, t_o = tmem + GTC_O + s * DP;
+      int next = 0;                                     // ring stage and phase bit
+      uint32_t ph = 0;
       bool ok = any0 || any1;
-      if (ok && !mbar_wait(&q_full, 0)) ok = false;
+      if (ok) ok = mbar_wait(&q_full, 0);
+      const auto advance = [&] {
+        if (++next == S::kStages) next = 0, ph ^= 1;
+      };
+      // the other slot of a split fetches its own blocks in between
+      const int last_o = s ? last[0] : last[1];
+      const auto skip = [&](int j) {
+        if (j >= 0 && j < last_o) advance();
+        if (j + 1 < last_o) advance();
+      };
 #pragma unroll 1
-      for (int n = 0; n < 2 * (hi - lo + 1) && ok; ++n) {
-        const int s = n & 1, j = lo - 1 + (n >> 1);     // P V of block j, Q K of block j + 1
-        const int first_s = s ? first[1] : first[0], last_s = s ? last[1] : last[0];
-        const bool v_here = j >= (kSplit ? first_s : lo) && j < (kSplit ? last_s : hi);
-        const bool k_here = j + 1 < (kSplit ? last_s : hi);
+      for (int j = lo - 1; j < hi && ok; ++j) {         // P V of block j, Q K of block j + 1
         const bool v_mine = j >= first_s && j < last_s;
         const bool k_mine = j + 1 >= first_s && j + 1 < last_s;
-        const int tail = s ? tail1 : tail0, i = j - first_s;
-        if (kSplit || s == 0) {          // the pair's second slot takes the same blocks
-          if (v_here) {
-            v_st = next;
-            v_ph = ph;
-            if (++next == S::kStages) next = 0, ph ^= 1;
-          }
-          if (k_here) {
-            k_st = next;
-            k_ph = ph;
-            if (++next == S::kStages) next = 0, ph ^= 1;
-          }
-          if (v_here)
-            ok = kCausal && clear && j == hi - 1 ? mbar_wait(&last_clean, 0)
-                                                 : mbar_wait(&kv_full[v_st], v_ph);
-          if (ok && k_here) ok = mbar_wait(&kv_full[k_st], k_ph);
+        const bool v_here = kSplit ? v_mine : j >= lo;
+        const bool k_here = kSplit ? k_mine : j + 1 < hi;
+        if (kSplit && s == 1) skip(j);
+        int v_st = 0, k_st = 0;
+        if (v_here) {
+          v_st = next;
+          ok = kCausal && clear && j == hi - 1 ? mbar_wait(&last_clean, 0)
+                                               : mbar_wait(&kv_full[v_st], ph);
+          advance();
         }
-        const int steps = j == last_s - 1 ? tail : kSteps;
+        if (k_here) {
+          k_st = next;
+          if (ok) ok = mbar_wait(&kv_full[k_st], ph);
+          advance();
+        }
+        if (kSplit && s == 0) skip(j);
+        const int i = j - first_s;
+        const bool v_last = j == last_s - 1, k_last = j + 2 == last_s;
         const uint64_t vd = v_desc + v_st * (S::kTile >> 4);
-        const uint64_t qd = q_desc + (kSplit ? 0 : s) * (S::kTile >> 4);
         const uint64_t kd = k_desc + k_st * (S::kTile >> 4);
-        const uint32_t t_s = tmem + s * GTC_KEYS, t_o = tmem + GTC_O + s * DP;
-        const uint32_t i_qk = idesc_bf16_f32(128, j + 2 == last_s ? tail * 16 : GTC_KEYS);
-        if (ok && v_mine) ok = mbar_wait(&p_full[s], i & 1);
-        if (!ok) break;
-        tc_fence_after();
-        if (lead) {
-          if (v_mine) {
-            if (steps == kSteps) {
 #pragma unroll
-              for (int kk = 0; kk < kSteps; ++kk)
-                mma_bf16_tmem_a(t_o, t_s + kk * 8, vd + kk * ((16 * S::kRow) >> 4), i_pv,
-                                i > 0 || kk > 0);
-            } else {
+        for (int half = 0; half < 2; ++half) {
+          if (ok && v_mine) ok = mbar_wait(&p_full[s][half], i & 1);
+          if (ok && half == 0) {         // this slot's turn of block j
+            const int turns = j - lo + 1;
+            if (s == 1)
+              ok = mbar_wait(&turn[0], turns & 1);
+            else if (turns > 0)
+              ok = mbar_wait(&turn[1], (turns - 1) & 1);
+          }
+          if (!ok) break;
+          tc_fence_after();
+          if (lead) {
+            if (v_mine) {
+              const uint64_t vh = vd + half * ((64 * S::kRow) >> 4);
+              const uint32_t t_p = t_s + 64 * half;
+              if (!v_last) {
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                  mma_bf16_tmem_a(t_o, t_p + kk * 8, vh + kk * ((16 * S::kRow) >> 4), i_pv,
+                                  i > 0 || half > 0 || kk > 0);
+              } else {
 #pragma unroll 1
-              for (int kk = 0; kk < steps; ++kk)
-                mma_bf16_tmem_a(t_o, t_s + kk * 8, vd + kk * ((16 * S::kRow) >> 4), i_pv,
-                                i > 0 || kk > 0);
+                for (int kk = 0; kk < min(tail - 4 * half, 4); ++kk)
+                  mma_bf16_tmem_a(t_o, t_p + kk * 8, vh + kk * ((16 * S::kRow) >> 4), i_pv,
+                                  i > 0 || half > 0 || kk > 0);
+                if (half == 1) {
+                  mma_commit(&s_full[s][0]);
+                  mma_commit(&s_full[s][1]);
+                }
+              }
             }
-            if (j == last_s - 1) mma_commit(&s_full[s]);
-          }
-          if (k_mine) {
+            if (k_mine) {
+              const uint64_t kh = kd + half * ((64 * S::kRow) >> 4);
+              const uint32_t i_qk =
+                  idesc_bf16_f32(128, k_last ? max(1, min(tail - 4 * half, 4)) * 16 : 64);
 #pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) {
-              const uint32_t off = ((kk / kPerBox) * S::kBox + (kk % kPerBox) * 32) >> 4;
-              mma_bf16(t_s, qd + off, kd + off, i_qk, kk > 0);
+              for (int kk = 0; kk < DP / 16; ++kk) {
+                const uint32_t off = ((kk / kPerBox) * S::kBox + (kk % kPerBox) * 32) >> 4;
+                mma_bf16(t_s + 64 * half, q_desc + off, kh + off, i_qk, kk > 0);
+              }
+              mma_commit(&s_full[s][half]);
             }
-            mma_commit(&s_full[s]);
           }
-          if (kSplit || s == 1) {
-            if (v_here) mma_commit(&kv_empty[v_st]);
-            if (k_here) mma_commit(&kv_empty[k_st]);
-          }
+        }
+        if (!ok) break;
+        if (lead) {
+          mbar_arrive(&turn[s]);
+          // a stage is free when both slots of a pair are done with it
+          if (v_mine) mma_commit(&kv_empty[v_st]); else if (v_here) mbar_arrive(&kv_empty[v_st]);
+          if (k_mine) mma_commit(&kv_empty[k_st]); else if (k_here) mbar_arrive(&kv_empty[k_st]);
         }
       }
       if (!ok && (any0 || any1)) failed = 1;
       // no MMA may still use TMEM or shared memory when they are given back
       if (lead) mma_commit(&drain_bar);
       if (!mbar_wait(&drain_bar, 0)) drain_failed = 1;
-    } else if (kCausal && warp == 10 && clear) {
+    } else if (kCausal && warp == 18 && clear) {
       const int at = 1 + 2 * (hi - 1 - lo);   // its place in the ring
       // (the stream may still be a whole tile's work away from its last block)
       bool ok = false;
@@ -393,39 +458,42 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (lane == 0) mbar_arrive(&last_clean);
       }
     }
-  } else {                               // softmax and epilogue, one row per thread
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
-    const int slot = warp >> 2;
+  } else {                               // softmax and epilogue, two threads per row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n");
+    const int slot = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, r = tid & 127;
     const int blocks = slot == 0 ? last[0] - first[0] : last[1] - first[1];
-    const int key_first = slot == 0 ? origin[0] + first[0] * GTC_KEYS
-                                    : origin[1] + first[1] * GTC_KEYS;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lanes + slot * GTC_KEYS, t_o = tmem + lanes + GTC_O + slot * DP;
-    const float c = a.scale_log2, slack = 8.f / c;
+    const int key_first = (slot == 0 ? origin[0] + first[0] * GTC_KEYS
+                                     : origin[1] + first[1] * GTC_KEYS) + 64 * half;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t t_s = tmem + lanes + slot * GTC_KEYS;
+    const float c = a.scale_log2, slack = 32.f / c;
     const int all_from = slot == 0 ? in_lo[0] : in_lo[1];
     const int all_to = slot == 0 ? in_hi[0] : in_hi[1];
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int i = 0; i < blocks; ++i) {
-      if (!mbar_wait_warp(&s_full[slot], i & 1)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      uint32_t raw[4][32];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tmem_load32_async(t_s + 32 * q, raw[q]);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tmem_loaded32(raw[q]);
+    // this thread's half of the output columns, in runs of kCols
+    constexpr int kCols = DP == 32 ? 16 : 32, kRuns = DP / 2 / kCols;
+    const uint32_t t_o = tmem + lanes + GTC_O + slot * DP + half * (DP / 2);
+    __nv_bfloat16* tops = reinterpret_cast<__nv_bfloat16*>(scratch + slot * 256);
+    float* sums = reinterpret_cast<float*>(scratch + slot * 256);
+    uint64_t* pair = &pair_bar[slot * 4 + quarter];
+    const auto tell = [&] {                // own value is in shared memory
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pair);
+    };
+    const float2 c2 = make_float2(c, c);
+    uint32_t raw[2][32];
+    // this thread's 64 scores, masked; returns their maximum
+    const auto scores = [&](int i, bool& dead) {
+      tmem_load32_async(t_s + 64 * half, raw[0]);
+      tmem_load32_async(t_s + 64 * half + 32, raw[1]);
+      tmem_loaded32(raw[0]);
+      tmem_loaded32(raw[1]);
       const int key0 = key_first + i * GTC_KEYS;
-      unsigned live = 0xf;                 // runs of 32 keys that some row of the warp sees
-      if (key0 < all_from || key0 + GTC_KEYS > all_to) {
+      dead = false;                        // no row of the warp sees any of its 64 keys
+      if (key0 < all_from || key0 + 64 > all_to) {
         const int from = begin - key0, to = end - key0;
-        const int least = __reduce_min_sync(0xffffffffu, to > from ? from : INT_MAX);
-        const int most = __reduce_max_sync(0xffffffffu, to > from ? to : 0);
+        dead = !__any_sync(0xffffffffu, max(from, 0) < min(to, 64));
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (32 * q >= most || 32 * q + 32 <= least) live &= ~(1u << q);
+        for (int q = 0; q < 2; ++q) {
           // bit j: key 32 q + j is seen
           const int f = min(max(from - 32 * q, 0), 32), e = min(max(to - 32 * q, 0), 32);
           const uint32_t seen_bits =
@@ -435,95 +503,168 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             if (!(seen_bits & (1u << j))) raw[q][j] = 0xff800000u;
         }
       }
-      float top = -INFINITY;
-      {
-        float t4[4];
+      float t4[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          t4[q] = __uint_as_float(raw[q][0]);
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t* v = &raw[q >> 1][16 * (q & 1)];
+        t4[q] = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
 #pragma unroll
-          for (int j = 1; j < 32; ++j) t4[q] = fmaxf(t4[q], __uint_as_float(raw[q][j]));
-        }
-        top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+        for (int j = 2; j < 16; j += 2)
+          t4[q] = gtc_max3(t4[q], __uint_as_float(v[j]), __uint_as_float(v[j + 1]));
       }
+      return gtc_max3(fmaxf(t4[0], t4[1]), t4[2], t4[3]);
+    };
+    // weights exp2(c s - base) of the scores in raw, packed into raw[0]; returns
+    // their sum.  Groups of 16 scores pass through three stages (scale,
+    // exponential, sum and pack) one behind the other: in the order of the
+    // formula every pair waits for its own exponential.
+    const auto weights = [&](float base) {
+      const float2 b2 = make_float2(-base, -base);
+      float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+      const auto exps = [&](int g) {
+        uint32_t* v = &raw[g >> 1][16 * (g & 1)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float2 x = __ffma2_rn(
+              make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), c2, b2);
+          v[2 * j] = __float_as_uint(x.x);
+          v[2 * j + 1] = __float_as_uint(x.y);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float2 x = make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+          if (j % GTC_EMULATE == 1)
+            x = gtc_exp2_pair(x);
+          else
+            x = make_float2(gtc_exp2(x.x), gtc_exp2(x.y));
+          v[2 * j] = __float_as_uint(x.x);
+          v[2 * j + 1] = __float_as_uint(x.y);
+        }
+      };
+      const auto pack = [&](int g) {
+        uint32_t* v = &raw[g >> 1][16 * (g & 1)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float2 x = make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+          if (j & 1) sum1 = __fadd2_rn(sum1, x); else sum0 = __fadd2_rn(sum0, x);
+          raw[0][8 * g + j] = gtc_pack(x.x, x.y);
+        }
+      };
+      exps(0);
+#pragma unroll
+      for (int g = 1; g < 4; ++g) {
+        exps(g);
+        pack(g - 1);
+      }
+      pack(3);
+      sum0 = __fadd2_rn(sum0, sum1);
+      return sum0.x + sum0.y;
+    };
+    float m = -INFINITY, l = 0.f;
+    int met = 0;                           // phases of the pair's barrier
+    bool ok = true;
+    const auto meet = [&] {
+      ok = mbar_wait_warp(pair, met & 1);
+      ++met;
+    };
+#pragma unroll 1
+    for (int i = 0; i < blocks; ++i) {
+      if (!(ok = mbar_wait_warp(&s_full[slot][half], i & 1))) break;
+      tc_fence_after();
+      bool dead;
+      // The reference maximum need not be exact, only the same for both threads
+      // of a row: it passes between them in bf16, rounded up.  (Two copies: the
+      // partner may be one block behind, not two.)
+      const __nv_bfloat16 mine16 = __float2bfloat16_ru(scores(i, dead));
+      __nv_bfloat16* at = tops + (i & 1) * 256 + r;
+      at[half * 128] = mine16;
+      tell();
+      // The weights are taken against the maximum so far; the partner's part of
+      // this block's maximum is read behind them.  Only where the maximum has
+      // grown by more than 2^32 in weight (and in a row's first block) are the
+      // scores read again and the sums rescaled.
+      float part = 0.f;
+      const float before = m;
+      if (i > 0 && !dead) part = weights(m == -INFINITY ? 0.f : m * c);
+      meet();
+      if (!ok) break;
+      const float top =
+          fmaxf(__bfloat162float(mine16), __bfloat162float(at[(half ^ 1) * 128]));
+      const bool grown = top > m + slack;
       if (i == 0) {
         m = top;
-      } else {
-        const bool grown = top > m + slack;
-        if (__any_sync(0xffffffffu, grown)) {
-          const float keep = grown ? gtc_exp2((m - top) * c) : 1.f;
-          if (grown) m = top;
-          l *= keep;
+        if (!dead) part = weights(m == -INFINITY ? 0.f : m * c);
+      } else if (__any_sync(0xffffffffu, grown)) {
+        // Both threads of the row are here with their scores of this block, so
+        // every product into O is done, and none starts before both are through.
+        if (grown) m = top;
+        const float keep = grown ? gtc_exp2((before - m) * c) : 1.f;
+        l *= keep;
 #pragma unroll 1
-          for (int q = 0; q < DP / 32; ++q) {
-            uint32_t o[32];
-            tmem_load32_async(t_o + 32 * q, o);
-            tmem_loaded32(o);
+        for (int q = 0; q < DP / 2; q += 16) {
+          uint32_t o[16];
+          tmem_load16_async(t_o + q, o);
+          tmem_loaded16(o);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-            tmem_store32(t_o + 32 * q, o);
-          }
+          for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+          tmem_store16(t_o + q, o);
         }
+        tmem_stored();
+        scores(i, dead);
+        if (!dead) part = weights(m == -INFINITY ? 0.f : m * c);
+        tc_fence_before();
+        tell();
+        meet();
+        if (!ok) break;
+        tc_fence_after();
       }
-      const float base = m == -INFINITY ? 0.f : m * c;
-      const float2 c2 = make_float2(c, c), b2 = make_float2(-base, -base);
-      float2 sum = make_float2(0.f, 0.f);
+      if (dead) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t packed[32];
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint32_t* s = raw[2 * half + q];
-          if (!((live >> (2 * half + q)) & 1)) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) packed[16 * q + j] = 0;
-            continue;
-          }
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float2 x = __ffma2_rn(make_float2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])),
-                                  c2, b2);
-            x.x = gtc_exp2(x.x);
-            x.y = gtc_exp2(x.y);
-            sum = __fadd2_rn(sum, x);
-            packed[16 * q + j / 2] = gtc_pack(x.x, x.y);
-          }
-        }
-        tmem_store32(t_s + 32 * half, packed);
+        for (int j = 0; j < 32; ++j) raw[0][j] = 0;
       }
-      l += sum.x + sum.y;
+      l += part;
+      tmem_store32(t_s + 64 * half, raw[0]);   // over the thread's own scores
       tmem_stored();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[slot]);
+      if (lane == 0) mbar_arrive(&p_full[slot][half]);
     }
-    if (ok && blocks > 0 && !mbar_wait_warp(&s_full[slot], blocks & 1)) ok = false;
-    if (!ok) failed = 1;
+    if (ok && blocks > 0) ok = mbar_wait_warp(&s_full[slot][half], blocks & 1);
     tc_fence_after();
-
-    const int r = tid & 127;
+    // every warp of the slot has stored its last weights, so the maxima are read
+    sums[half * 128 + r] = l;
+    tell();
+    if (ok) meet();
+    if (!ok) failed = 1;
+    l += sums[(half ^ 1) * 128 + r];
     const bool seen = end > begin && position >= 0;
     const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int head = h * a.group + r - ((r * per_group) >> 16) * a.group;
     if constexpr (kCausal) {
       // the output row goes through the slot's Q tile (its products are done)
       // so that whole rows leave in 16-byte pieces of neighbouring lanes
-      constexpr int kPieces = DP / 8;
+      constexpr int kPieces = DP / 16;     // of this half
       uint8_t* stage = smem + slot * S::kTile;
       const auto piece = [&](int row, int at) {
-        const int x = kPieces >= 8 ? row & 7 : (row >> 1) & 3;
-        return reinterpret_cast<uint4*>(stage + row * (DP * 2) + ((at ^ x) << 4));
+        const int x = DP >= 64 ? row & 7 : (row >> 1) & 3;
+        return reinterpret_cast<uint4*>(stage + row * (DP * 2) + (((half * kPieces + at) ^ x) << 4));
       };
       bool odd = seen && !(fabsf(l) <= FLT_MAX);
-      float2 nil = make_float2(0.f, 0.f);     // stays 0 while every output is finite
+      float2 nil = make_float2(0.f, 0.f);  // stays 0 while every output is finite
 #pragma unroll 1
-      for (int q = 0; q < DP / 32; ++q) {
-        uint32_t o[32];
+      for (int q = 0; q < kRuns; ++q) {
+        uint32_t o[kCols];
         if (blocks > 0) {
-          tmem_load32_async(t_o + 32 * q, o);
-          tmem_loaded32(o);
+          if constexpr (kCols == 32) {
+            tmem_load32_async(t_o + 32 * q, o);
+            tmem_loaded32(o);
+          } else {
+            tmem_load16_async(t_o, o);
+            tmem_loaded16(o);
+          }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kCols / 8; ++k) {
           uint32_t w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -533,7 +674,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             nil = __ffma2_rn(x, make_float2(0.f, 0.f), nil);
             w[j] = seen ? gtc_pack(x.x, x.y) : 0u;
           }
-          *piece(r, 4 * q + k) = make_uint4(w[0], w[1], w[2], w[3]);
+          *piece(r, kCols / 8 * q + k) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
       odd |= seen && !(nil.x + nil.y == 0.f);
@@ -541,52 +682,52 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const bool mine = position >= 0 && (seen || a.clear_rest);
       const unsigned write = __ballot_sync(0xffffffffu, mine && ok);
       unsigned again = __ballot_sync(0xffffffffu, odd && seen && ok);
-      const int head = h * a.group + r - ((r * per_group) >> 16) * a.group;
       const int64_t to = (int64_t)position * a.o_sp + (int64_t)head * a.o_sh;
-      const int row0 = (warp & 3) * 32, at = lane % kPieces;
+      const int at = lane % kPieces, column = half * (DP / 2) + at * 8;
 #pragma unroll 4
       for (int i = 0; i < 32; i += 32 / kPieces) {
         const int rr = i + lane / kPieces;
         const int64_t off = __shfl_sync(0xffffffffu, to, rr);
-        if (((write >> rr) & 1) && at * 8 < a.D)
-          *reinterpret_cast<uint4*>(a.out + off + at * 8) = *piece(row0 + rr, at);
+        if (((write >> rr) & 1) && column < a.D)
+          *reinterpret_cast<uint4*>(a.out + off + column) = *piece(quarter * 32 + rr, at);
       }
       __syncwarp();
       while (again) {
         const int rr = __ffs(again) - 1;
         again &= again - 1;
-        causal_row_again<__nv_bfloat16, DP / 32>(
+        causal_row_again<__nv_bfloat16, (DP + 63) / 64>(
             a, __shfl_sync(0xffffffffu, position, rr), __shfl_sync(0xffffffffu, head, rr),
-            __shfl_sync(0xffffffffu, begin, rr), __shfl_sync(0xffffffffu, end, rr));
+            __shfl_sync(0xffffffffu, begin, rr), __shfl_sync(0xffffffffu, end, rr),
+            half * (DP / 2), min(a.D, (half + 1) * (DP / 2)));
       }
     } else {
       const int part = kSplit ? 2 * slice + slot : slice;
-      const int64_t at = ((int64_t)part * a.positions + position) * a.heads +
-                         (int64_t)h * a.group + r - ((r * per_group) >> 16) * a.group;
+      const int64_t at = ((int64_t)part * a.positions + position) * a.heads + head;
 #pragma unroll 1
-      for (int q = 0; q < DP / 32; ++q) {
-        uint32_t o[32];
+      for (int q = 0; q < DP / 2; q += 16) {
+        uint32_t o[16];
         if (blocks > 0) {
-          tmem_load32_async(t_o + 32 * q, o);
-          tmem_loaded32(o);
+          tmem_load16_async(t_o + q, o);
+          tmem_loaded16(o);
         }
         if (position < 0 || !ok) continue;
+        const int column = half * (DP / 2) + q;
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          if (32 * q + j >= a.D) break;
+        for (int j = 0; j < 16; j += 4) {
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
           if (blocks > 0)
             x = make_float4(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv,
                             __uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
-          *reinterpret_cast<float4*>(a.part + at * a.D + 32 * q + j) = x;
+          if (column + j < a.D) *reinterpret_cast<float4*>(a.part + at * a.D + column + j) = x;
         }
       }
-      if (position >= 0 && ok) a.part_lse[at] = l == 0.f ? -INFINITY : m * c + log2f(l);
+      if (position >= 0 && ok && half == 0)
+        a.part_lse[at] = l == 0.f ? -INFINITY : m * c + log2f(l);
     }
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -659,10 +800,23 @@ int gtc_launch(const GroupedArgs<__nv_bfloat16>& args, cudaStream_t stream) {
   const dim3 grid = MODE == GTC_CAUSAL
                         ? dim3((unsigned)(tiles * a.kv_heads))
                         : dim3((unsigned)tiles, a.kv_heads, a.slices);
-  if (cudaFuncSetAttribute(grouped_tc_kernel<DP, MODE>,
-                           cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
-    return GRS_ERR_CUDA;
-  grouped_tc_kernel<DP, MODE><<<grid, GTC_THREADS, S::kSmem, counted(stream)>>>(q, k, v, a, pps);
+  // the tiles start at the first 1024-byte boundary behind the static variables
+  static std::atomic<int> smem_of[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GRS_ERR_CUDA;
+  int smem = smem_of[dev].load(std::memory_order_acquire);
+  if (smem == 0) {
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, grouped_tc_kernel<DP, MODE>) != cudaSuccess)
+      return GRS_ERR_CUDA;
+    const int fixed = (int)fa.sharedSizeBytes;
+    smem = (fixed + 1023) / 1024 * 1024 - fixed + S::kTiles;
+    if (cudaFuncSetAttribute(grouped_tc_kernel<DP, MODE>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return GRS_ERR_CUDA;
+    smem_of[dev].store(smem, std::memory_order_release);
+  }
+  grouped_tc_kernel<DP, MODE><<<grid, GTC_THREADS, smem, counted(stream)>>>(q, k, v, a, pps);
   GRS_CUDA_CHECK_LAUNCH();
   return GRS_OK;
 }
