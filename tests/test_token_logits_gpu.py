@@ -172,6 +172,17 @@ def test_captured(cuda_device):
     _check(outs[0], logits, kw)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_histories_past_the_packed_counters(cuda_device, dtype):
+    """2^14 tokens and more count in whole words; one token fills them all."""
+    for history in (16383, 16384, 40000):
+        logits, kw = _case(9, 2, 30001, history, dtype)
+        kw["tokens"][1] = 5
+        kw["lengths"][:] = history
+        kw["prompt_lengths"][:] = 0
+        _check(_call(cuda_device, logits, kw), logits, kw)
+
+
 def test_many_rows(cuda_device):
     logits, kw = _case(8, 70000, 3, 2, FP32)
     got = _call(cuda_device, logits, kw)
