@@ -56,6 +56,8 @@ struct GtcShape {
   // above half an SM's shared memory: the 512 TMEM columns are one CTA's
   static constexpr int kTiles = (2 + kStages) * kTile;
   static_assert(kTiles > 114 * 1024 && kTiles <= 224 * 1024, "one CTA per SM");
+  // whether the partial sums of 16 warps pass through one Q tile
+  static constexpr bool kStageFree = kTile >= 16 * 2048;
 };
 
 constexpr int GTC_CAUSAL = 0, GTC_PAIR = 1, GTC_SPLIT = 2;
@@ -701,8 +703,17 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             half * (DP / 2), min(a.D, (half + 1) * (DP / 2)));
       }
     } else {
+      // 16 columns of the warp's 32 rows at a time pass through 2 KB of shared
+      // memory: written from the rows' own threads, a warp's store would touch
+      // 32 rows with 16 bytes each, and 6.6 of 15 us of a three-block slice went
+      // into that.  The Q tile is free in a pair (the slot's scores are done); a
+      // split leaves the second one unused.
       const int part = kSplit ? 2 * slice + slot : slice;
       const int64_t at = ((int64_t)part * a.positions + position) * a.heads + head;
+      uint8_t* stage = S::kStageFree ? smem + (kSplit ? S::kTile + warp * 2048
+                                                      : slot * S::kTile + (warp & 7) * 2048)
+                                     : ring + S::kStages * S::kTile + warp * 2048;
+      const unsigned write = __ballot_sync(0xffffffffu, position >= 0 && ok);
 #pragma unroll 1
       for (int q = 0; q < DP / 2; q += 16) {
         uint32_t o[16];
@@ -710,16 +721,26 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           tmem_load16_async(t_o + q, o);
           tmem_loaded16(o);
         }
-        if (position < 0 || !ok) continue;
-        const int column = half * (DP / 2) + q;
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
+        for (int j = 0; j < 4; ++j) {
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
           if (blocks > 0)
-            x = make_float4(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv,
-                            __uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
-          if (column + j < a.D) *reinterpret_cast<float4*>(a.part + at * a.D + column + j) = x;
+            x = make_float4(__uint_as_float(o[4 * j]) * inv, __uint_as_float(o[4 * j + 1]) * inv,
+                            __uint_as_float(o[4 * j + 2]) * inv,
+                            __uint_as_float(o[4 * j + 3]) * inv);
+          *reinterpret_cast<float4*>(stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = x;
         }
+        __syncwarp();
+        const int column = half * (DP / 2) + q + 4 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          const int rr = i + (lane >> 2);
+          const int64_t to = __shfl_sync(0xffffffffu, at, rr) * a.D + column;
+          if (((write >> rr) & 1) && column < a.D)
+            *reinterpret_cast<float4*>(a.part + to) = *reinterpret_cast<const float4*>(
+                stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+        }
+        __syncwarp();
       }
       if (position >= 0 && ok && half == 0)
         a.part_lse[at] = l == 0.f ? -INFINITY : m * c + log2f(l);
@@ -810,7 +831,8 @@ int gtc_launch(const GroupedArgs<__nv_bfloat16>& args, cudaStream_t stream) {
     if (cudaFuncGetAttributes(&fa, grouped_tc_kernel<DP, MODE>) != cudaSuccess)
       return GRS_ERR_CUDA;
     const int fixed = (int)fa.sharedSizeBytes;
-    smem = (fixed + 1023) / 1024 * 1024 - fixed + S::kTiles;
+    smem = (fixed + 1023) / 1024 * 1024 - fixed + S::kTiles +
+           (MODE != GTC_CAUSAL && !S::kStageFree ? 16 * 2048 : 0);
     if (cudaFuncSetAttribute(grouped_tc_kernel<DP, MODE>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return GRS_ERR_CUDA;

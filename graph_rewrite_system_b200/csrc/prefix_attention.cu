@@ -22,7 +22,7 @@ struct PagesArgs {
   const int32_t* bt; int64_t bt_s; int max_blocks; const int32_t* lengths; int num_pages, page;
   const T* ck; const T* cv; int64_t ck_sb, ck_sh; const uint8_t* cvalid;
   const float* part; const float* part_lse; int slices;   // parts of the prefix
-  float* page_part; float* page_lse;                      // the same arrays, for page slices
+  float* page_part; float* page_lse;   // the same arrays, for page slices joined by a later kernel
   T* out; int64_t o_sb, o_sh;
   int batch, heads, kv_heads, group, D;
   float scale_log2;
@@ -140,11 +140,14 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
 // quad takes the pieces t, t + 4, ... of a key row for its K fragments (the
 // query fragments are loaded in the same order), and for V the lane's column
 // index picks the piece and the eight elements of a piece go to eight
-// different n-tiles; two keys' pieces are interleaved by byte permutes.  The
-// weights leave the score product in the layout of the value product's A
-// operand.  The warps' sums meet in shared memory and are joined there with
+// different tiles; two keys' pieces are interleaved by byte permutes.  Groups
+// of more than 8 heads take the heads as the 16 rows of both products (the
+// weights leave the first in the layout of the second's A operand); groups of
+// up to 8 (kFew) take keys, then value columns as rows and the heads as the 8
+// columns, with two 8 x 8 transposes of the weights in between: half the
+// instructions, accumulators and query registers.  The warps' sums meet in shared memory and are joined there with
 // the prefix slices; only that join waits for the prefix kernel.
-constexpr int PG_HEADS = 16;
+constexpr int PG_HEADS = 16, PG_BESIDE = 148;
 
 __device__ __forceinline__ void pg_mma(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -171,8 +174,51 @@ struct PgShape {
   static constexpr int kStride = DP + 4;                  // row of the joined sums (floats)
 };
 
-template <int DP>
-__global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16> a, int rows) {
+__device__ __forceinline__ uint32_t pg_transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// x += the parts first, first + step, ... of one (beam, head), four columns a
+// lane, by their weights against `base`; returns the weights' sum.  The weights
+// of 32 parts are taken at once, a lane each, so that the rows' loads depend on
+// nothing and go out together.
+__device__ __forceinline__ float pg_add_parts(const PagesArgs<__nv_bfloat16>& a, int parts,
+                                              int first, int step, int64_t at, float base,
+                                              float4& x) {
+  const int lane = threadIdx.x & 31, d = 4 * lane;
+  const int64_t stride = (int64_t)a.batch * a.heads;
+  float norm = 0.f;
+  for (int p0 = first; p0 < parts; p0 += 32 * step) {
+    const int mine = p0 + lane * step;
+    const float w = mine < parts ? pg_exp2(a.part_lse[mine * stride + at] - base) : 0.f;
+    norm += warp_sum(w);
+    const int n = min(32, (parts - p0 + step - 1) / step);
+    for (int i0 = 0; i0 < n; i0 += 8) {
+      float4 y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i0 + i < n && d < a.D)
+          y[i] = *reinterpret_cast<const float4*>(
+              a.part + ((p0 + (i0 + i) * step) * stride + at) * a.D + d);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, min(i0 + i, 31));
+        x.x = fmaf(wi, y[i].x, x.x);
+        x.y = fmaf(wi, y[i].y, x.y);
+        x.z = fmaf(wi, y[i].z, x.z);
+        x.w = fmaf(wi, y[i].w, x.w);
+      }
+    }
+  }
+  return norm;
+}
+
+template <int DP, bool kFew>
+__global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16> a) {
   using S = PgShape<DP>;
   using T = __nv_bfloat16;
   extern __shared__ float pg_smem[];
@@ -184,23 +230,31 @@ __global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16>
   const int head0 = h * a.group + blockIdx.x % chunks * PG_HEADS;
   const int n_heads = min(PG_HEADS, (h + 1) * a.group - head0);
 
-  // query fragments: rows g and g + 8, pieces t, t + 4, ...
-  uint32_t qa[2 * S::kKey][4];
+  constexpr int rows = kFew ? 8 : PG_HEADS;
+  // query fragments: heads g and g + 8 (or g alone), pieces t, t + 4, ...
+  uint32_t qa[2 * S::kKey][kFew ? 2 : 4];
 #pragma unroll
   for (int i = 0; i < S::kKey; ++i) {
     uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
     const int d = 8 * (t + 4 * i);
     const T* q = a.q + (int64_t)b * a.q_sb + (int64_t)(head0 + g) * a.q_sh + d;
     if (d < a.D && g < n_heads) lo = *reinterpret_cast<const uint4*>(q);
-    if (d < a.D && g + 8 < n_heads) hi = *reinterpret_cast<const uint4*>(q + 8 * a.q_sh);
-    qa[2 * i][0] = lo.x;
-    qa[2 * i][1] = hi.x;
-    qa[2 * i][2] = lo.y;
-    qa[2 * i][3] = hi.y;
-    qa[2 * i + 1][0] = lo.z;
-    qa[2 * i + 1][1] = hi.z;
-    qa[2 * i + 1][2] = lo.w;
-    qa[2 * i + 1][3] = hi.w;
+    if constexpr (kFew) {
+      qa[2 * i][0] = lo.x;
+      qa[2 * i][1] = lo.y;
+      qa[2 * i + 1][0] = lo.z;
+      qa[2 * i + 1][1] = lo.w;
+    } else {
+      if (d < a.D && g + 8 < n_heads) hi = *reinterpret_cast<const uint4*>(q + 8 * a.q_sh);
+      qa[2 * i][0] = lo.x;
+      qa[2 * i][1] = hi.x;
+      qa[2 * i][2] = lo.y;
+      qa[2 * i][3] = hi.y;
+      qa[2 * i + 1][0] = lo.z;
+      qa[2 * i + 1][1] = hi.z;
+      qa[2 * i + 1][2] = lo.w;
+      qa[2 * i + 1][3] = hi.w;
+    }
   }
 
   const int room = a.max_blocks * a.page;
@@ -229,9 +283,12 @@ __global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16>
            (int64_t)h * a.kc_sh;
   };
 
-  float acc[DP / 8][4];
+  // kFew: columns (d, d + 1) x heads (2t, 2t + 1), d = piece (g + 8 j) + 2 i;
+  // else: heads (g, g + 8) x columns of the pieces 2t and 2t + 1
+  constexpr int kTiles = kFew ? DP / 16 : DP / 8;
+  float acc[kTiles][4];
 #pragma unroll
-  for (int i = 0; i < DP / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+  for (int i = 0; i < kTiles; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   const T* next = place(run_lo + warp);
   for (int run = run_lo + warp; run < run_hi; run += warps) {
@@ -279,67 +336,124 @@ __global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16>
           }
         }
       }
-      float s[2][4];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      if constexpr (kFew) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};   // keys (g, g + 8) x heads (2t, 2t + 1)
 #pragma unroll
         for (int i = 0; i < S::kKey; ++i) {
-          pg_mma(s[n], qa[2 * i], kr[n][i].x, kr[n][i].y);
-          pg_mma(s[n], qa[2 * i + 1], kr[n][i].z, kr[n][i].w);
+          const uint32_t k0[4] = {kr[0][i].x, kr[1][i].x, kr[0][i].y, kr[1][i].y};
+          const uint32_t k1[4] = {kr[0][i].z, kr[1][i].z, kr[0][i].w, kr[1][i].w};
+          pg_mma(s, k0, qa[2 * i][0], qa[2 * i][1]);
+          pg_mma(s, k1, qa[2 * i + 1][0], qa[2 * i + 1][1]);
         }
-      }
-      float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
+        bool grown = false;
+        float top[2];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const bool ok = (valid >> (16 * half + 8 * n + 2 * t + (c & 1))) & 1;
-          s[n][c] = ok ? s[n][c] * a.scale_log2 : -INFINITY;
-          top[c >> 1] = fmaxf(top[c >> 1], s[n][c]);
+          const bool ok = (valid >> (16 * half + g + 8 * (c >> 1))) & 1;
+          s[c] = ok ? s[c] * a.scale_log2 : -INFINITY;
         }
-      float base[2];
-      bool grown = false;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-        grown |= top[r] > m[r];
-      }
-      if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float now = fmaxf(m[r], top[r]);
-          const float keep = now == -INFINITY ? 1.f : pg_exp2(m[r] - now);
-          m[r] = now;
-          l[r] *= keep;
+          top[r] = fmaxf(s[r], s[r + 2]);
 #pragma unroll
-          for (int i = 0; i < DP / 8; ++i) {
-            acc[i][2 * r] *= keep;
-            acc[i][2 * r + 1] *= keep;
+          for (int o = 4; o < 32; o <<= 1)
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], o));
+          grown |= top[r] > m[r];
+        }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float now = fmaxf(m[r], top[r]);
+            const float keep = now == -INFINITY ? 1.f : pg_exp2(m[r] - now);
+            m[r] = now;
+            l[r] *= keep;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+              acc[i][r] *= keep;
+              acc[i][r + 2] *= keep;
+            }
           }
         }
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) base[r] = m[r] == -INFINITY ? 0.f : m[r];
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          s[n][c] = pg_exp2(s[n][c] - base[c >> 1]);
-          l[c >> 1] += s[n][c];
+          s[c] = pg_exp2(s[c] - (m[c & 1] == -INFINITY ? 0.f : m[c & 1]));
+          l[c & 1] += s[c];
         }
-      const uint32_t pa[4] = {pg_pack(s[0][0], s[0][1]), pg_pack(s[0][2], s[0][3]),
-                              pg_pack(s[1][0], s[1][1]), pg_pack(s[1][2], s[1][3])};
+        const uint32_t p0 = pg_transpose(pg_pack(s[0], s[1]));
+        const uint32_t p1 = pg_transpose(pg_pack(s[2], s[3]));
 #pragma unroll
-      for (int i = 0; i < S::kRuns; ++i)
+        for (int i = 0; i < S::kRuns; ++i)
 #pragma unroll
-        for (int e = 0; e < S::kPiece; ++e) {
-          const unsigned pick = (e & 1) ? 0x7632u : 0x5410u;
-          pg_mma(acc[i * S::kPiece + e], pa,
-                 __byte_perm(vr[0][i][e >> 1], vr[1][i][e >> 1], pick),
-                 __byte_perm(vr[2][i][e >> 1], vr[3][i][e >> 1], pick));
+          for (int e = 0; e < S::kPiece / 2; ++e) {
+            const uint32_t va[4] = {__byte_perm(vr[0][i][e], vr[1][i][e], 0x5410u),
+                                    __byte_perm(vr[0][i][e], vr[1][i][e], 0x7632u),
+                                    __byte_perm(vr[2][i][e], vr[3][i][e], 0x5410u),
+                                    __byte_perm(vr[2][i][e], vr[3][i][e], 0x7632u)};
+            pg_mma(acc[i * (S::kPiece / 2) + e], va, p0, p1);
+          }
+      } else {
+        float s[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+          for (int i = 0; i < S::kKey; ++i) {
+            pg_mma(s[n], qa[2 * i], kr[n][i].x, kr[n][i].y);
+            pg_mma(s[n], qa[2 * i + 1], kr[n][i].z, kr[n][i].w);
+          }
         }
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const bool ok = (valid >> (16 * half + 8 * n + 2 * t + (c & 1))) & 1;
+            s[n][c] = ok ? s[n][c] * a.scale_log2 : -INFINITY;
+            top[c >> 1] = fmaxf(top[c >> 1], s[n][c]);
+          }
+        float base[2];
+        bool grown = false;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+          grown |= top[r] > m[r];
+        }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float now = fmaxf(m[r], top[r]);
+            const float keep = now == -INFINITY ? 1.f : pg_exp2(m[r] - now);
+            m[r] = now;
+            l[r] *= keep;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+              acc[i][2 * r] *= keep;
+              acc[i][2 * r + 1] *= keep;
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) base[r] = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            s[n][c] = pg_exp2(s[n][c] - base[c >> 1]);
+            l[c >> 1] += s[n][c];
+          }
+        const uint32_t pa[4] = {pg_pack(s[0][0], s[0][1]), pg_pack(s[0][2], s[0][3]),
+                                pg_pack(s[1][0], s[1][1]), pg_pack(s[1][2], s[1][3])};
+#pragma unroll
+        for (int i = 0; i < S::kRuns; ++i)
+#pragma unroll
+          for (int e = 0; e < S::kPiece; ++e) {
+            const unsigned pick = (e & 1) ? 0x7632u : 0x5410u;
+            pg_mma(acc[i * S::kPiece + e], pa,
+                   __byte_perm(vr[0][i][e >> 1], vr[1][i][e >> 1], pick),
+                   __byte_perm(vr[2][i][e >> 1], vr[3][i][e >> 1], pick));
+          }
+      }
     }
   }
 
@@ -347,67 +461,65 @@ __global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16>
   float* sums = pg_smem;                                   // [warps][rows][kStride]
   float* tops = sums + warps * rows * S::kStride;
   float* totals = tops + warps * rows;
+  if constexpr (kFew) {
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    const int head = g + 8 * r;
-    if (head >= rows) continue;
-    float* row = sums + (warp * rows + head) * S::kStride;
+    for (int r = 0; r < 2; ++r) {
 #pragma unroll
-    for (int i = 0; i < S::kRuns; ++i)
+      for (int o = 4; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+      const int head = 2 * t + r;
+      float* row = sums + (warp * rows + head) * S::kStride;
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int i = 0; i < S::kRuns; ++i)
 #pragma unroll
-        for (int e = 0; e < S::kPiece; e += 4)
-          *reinterpret_cast<float4*>(row + S::kPiece * (2 * t + c + 8 * i) + e) = make_float4(
-              acc[i * S::kPiece + e][2 * r + c], acc[i * S::kPiece + e + 1][2 * r + c],
-              acc[i * S::kPiece + e + 2][2 * r + c], acc[i * S::kPiece + e + 3][2 * r + c]);
-    if (t == 0) {
-      tops[warp * rows + head] = m[r];
-      totals[warp * rows + head] = l[r];
+        for (int e = 0; e < S::kPiece; e += 4) {
+          const int at = i * (S::kPiece / 2) + e / 2;
+          *reinterpret_cast<float4*>(row + S::kPiece * (g + 8 * i) + e) =
+              make_float4(acc[at][r], acc[at][r + 2], acc[at + 1][r], acc[at + 1][r + 2]);
+        }
+      if (g == 0) {
+        tops[warp * rows + head] = m[r];
+        totals[warp * rows + head] = l[r];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      const int head = g + 8 * r;
+      float* row = sums + (warp * rows + head) * S::kStride;
+#pragma unroll
+      for (int i = 0; i < S::kRuns; ++i)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < S::kPiece; e += 4)
+            *reinterpret_cast<float4*>(row + S::kPiece * (2 * t + c + 8 * i) + e) = make_float4(
+                acc[i * S::kPiece + e][2 * r + c], acc[i * S::kPiece + e + 1][2 * r + c],
+                acc[i * S::kPiece + e + 2][2 * r + c], acc[i * S::kPiece + e + 3][2 * r + c]);
+      if (t == 0) {
+        tops[warp * rows + head] = m[r];
+        totals[warp * rows + head] = l[r];
+      }
     }
   }
   __syncthreads();
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");   // the prefix slices are written
+  // The prefix slices are written.  Where a later kernel joins, one CTA waits
+  // for all, so that this kernel ends behind the prefix kernel, and the others
+  // leave their SMs to the CTAs still to come.
+  const bool last = a.page_part == nullptr;
+  if (last || (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1))
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
 
-  // a warp per head joins the warps' sums with the prefix slices, lane = 4 columns
-  const bool last = gridDim.y == 1;
+  // The warps' sums and the prefix slices are joined by a warp per head, or by
+  // several that take turns on the parts; lane = 4 columns.
   const int64_t stride = (int64_t)a.batch * a.heads;
-  for (int head = warp; head < n_heads; head += warps) {
+  const int parts = last ? a.slices : 0, teams = max(1, warps / n_heads);
+  const int team = teams > 1 ? warp / n_heads : 0, d = 4 * lane;
+  float4* shared_x = reinterpret_cast<float4*>(totals + warps * rows);   // [warps][32]
+  float* shared_norm = reinterpret_cast<float*>(shared_x + warps * 32);
+  const auto finish = [&](int head, float4 x, float norm, float base) {
     const int64_t at = (int64_t)b * a.heads + head0 + head;
-    const int parts = last ? a.slices : 0;
-    float top = -INFINITY;
-    for (int i = lane; i < warps; i += 32) top = fmaxf(top, tops[i * rows + head]);
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[i * stride + at]);
-    top = warp_max(top);
-    const float base = top == -INFINITY ? 0.f : top;
-    float norm = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int d = 4 * lane;
-    for (int i = 0; i < warps; ++i) {
-      const float w = pg_exp2(tops[i * rows + head] - base);
-      norm = fmaf(w, totals[i * rows + head], norm);
-      if (d < DP) {
-        const float4 y = *reinterpret_cast<const float4*>(sums + (i * rows + head) * S::kStride + d);
-        x.x = fmaf(w, y.x, x.x);
-        x.y = fmaf(w, y.y, x.y);
-        x.z = fmaf(w, y.z, x.z);
-        x.w = fmaf(w, y.w, x.w);
-      }
-    }
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) {
-      const float w = pg_exp2(a.part_lse[i * stride + at] - base);
-      norm += w;
-      if (d < a.D) {
-        const float4 y = *reinterpret_cast<const float4*>(a.part + (i * stride + at) * a.D + d);
-        x.x = fmaf(w, y.x, x.x);
-        x.y = fmaf(w, y.y, x.y);
-        x.z = fmaf(w, y.z, x.z);
-        x.w = fmaf(w, y.w, x.w);
-      }
-    }
     const float inv = norm == 0.f ? 0.f : 1.f / norm;
     x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
     if (last) {
@@ -419,36 +531,80 @@ __global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16>
       if (d < a.D) *reinterpret_cast<float4*>(a.page_part + to * a.D + d) = x;
       if (lane == 0) a.page_lse[to] = norm == 0.f ? -INFINITY : base + log2f(norm);
     }
+  };
+  for (int head = teams > 1 ? warp % n_heads : warp; head < n_heads && team < teams;
+       head += teams > 1 ? n_heads : warps) {
+    const int64_t at = (int64_t)b * a.heads + head0 + head;
+    float top = -INFINITY;
+    for (int i = lane; i < warps; i += 32) top = fmaxf(top, tops[i * rows + head]);
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[i * stride + at]);
+    top = warp_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    float norm = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = team; i < warps; i += teams) {
+      const float w = pg_exp2(tops[i * rows + head] - base);
+      norm = fmaf(w, totals[i * rows + head], norm);
+      if (d < DP) {
+        const float4 y = *reinterpret_cast<const float4*>(sums + (i * rows + head) * S::kStride + d);
+        x.x = fmaf(w, y.x, x.x);
+        x.y = fmaf(w, y.y, x.y);
+        x.z = fmaf(w, y.z, x.z);
+        x.w = fmaf(w, y.w, x.w);
+      }
+    }
+    norm += pg_add_parts(a, parts, team, teams, at, base, x);
+    if (teams == 1) {
+      finish(head, x, norm, base);
+    } else {
+      shared_x[warp * 32 + lane] = x;
+      if (lane == 0) shared_norm[2 * warp] = norm, shared_norm[2 * warp + 1] = base;
+    }
+  }
+  if (teams > 1) {
+    __syncthreads();
+    if (warp < n_heads) {
+      float4 x = shared_x[warp * 32 + lane];
+      float norm = shared_norm[2 * warp];
+      for (int i = 1; i < teams; ++i) {
+        const float4 y = shared_x[(warp + i * n_heads) * 32 + lane];
+        x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        norm += shared_norm[2 * (warp + i * n_heads)];
+      }
+      finish(warp, x, norm, shared_norm[2 * warp + 1]);
+    }
   }
 }
 
-// The join alone, for pages that are cut into slices too: a warp per (beam,
-// head) over all parts.
-__global__ void __launch_bounds__(128) join_parts_kernel(PagesArgs<__nv_bfloat16> a, int parts) {
-  const int lane = threadIdx.x & 31;
+// The join alone: `team` (1 or 4) of a CTA's four warps per (beam, head).
+__global__ void __launch_bounds__(128) join_parts_kernel(PagesArgs<__nv_bfloat16> a, int parts,
+                                                         int team) {
+  __shared__ float4 xs[4][32];
+  __shared__ float norms[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t stride = (int64_t)a.batch * a.heads;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (at >= stride) return;
+  const int64_t at = team == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + warp;
+  if (at >= stride) return;                // whole CTAs, or warps that meet nobody
   float top = -INFINITY;
   for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[i * stride + at]);
   top = warp_max(top);
-  const float base = top == -INFINITY ? 0.f : top;
-  float norm = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int d = 4 * lane;
-#pragma unroll 8
-  for (int i = 0; i < parts; ++i) {
-    const float w = pg_exp2(a.part_lse[i * stride + at] - base);
-    norm += w;
-    if (d < a.D) {
-      const float4 y = *reinterpret_cast<const float4*>(a.part + (i * stride + at) * a.D + d);
-      x.x = fmaf(w, y.x, x.x);
-      x.y = fmaf(w, y.y, x.y);
-      x.z = fmaf(w, y.z, x.z);
-      x.w = fmaf(w, y.w, x.w);
+  float norm = pg_add_parts(a, parts, team == 4 ? warp : 0, team, at,
+                            top == -INFINITY ? 0.f : top, x);
+  if (team == 4) {
+    xs[warp][lane] = x;
+    if (lane == 0) norms[warp] = norm;
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      const float4 y = xs[i][lane];
+      x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+      norm += norms[i];
     }
   }
   const float inv = norm == 0.f ? 0.f : 1.f / norm;
+  const int d = 4 * lane;
   if (d < a.D)
     *reinterpret_cast<uint2*>(a.out + at / a.heads * a.o_sb + at % a.heads * a.o_sh + d) =
         make_uint2(pg_pack(x.x * inv, x.y * inv), pg_pack(x.z * inv, x.w * inv));
@@ -500,12 +656,21 @@ static PrefixPlan tc_plan(int batch, int heads, int kv_heads, int D, int keys) {
 }
 
 // Slices of each beam's pages: enough CTAs of a long table to fill 148 SMs
-// four times when there are few beams, none for less than 256 tokens.
-static int pages_slices(int batch, int heads, int kv_heads, int64_t room) {
+// four times when there are few beams, none for less than 256 tokens.  They are
+// joined by a kernel of its own when they are cut, or when there are more CTAs
+// than fit beside the prefix kernel: CTAs that wait for it to join would keep
+// the SMs it leaves free from the rest.
+struct PagesPlan {
+  int slices;
+  bool separate;
+};
+static PagesPlan pages_plan(int batch, int heads, int kv_heads, int num_prefix, int64_t room) {
   const int group = heads / kv_heads;
   const int64_t tasks = (int64_t)batch * kv_heads * ((group + PG_HEADS - 1) / PG_HEADS);
   const int64_t want = (4 * 148 + tasks - 1) / tasks;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), room / 256));
+  const int slices =
+      (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), room / 256));
+  return {slices, slices > 1 || (num_prefix > 0 && room > 0 && tasks > PG_BESIDE)};
 }
 
 static bool aligned(const void* p, int64_t bytes) {
@@ -520,7 +685,7 @@ static bool pages_mma_takes(const PagesArgs<__nv_bfloat16>& p) {
          p.ck_sh % 8 == 0 && aligned(p.out, 8) && p.o_sb % 4 == 0 && p.o_sh % 4 == 0;
 }
 
-template <int DP>
+template <int DP, bool kFew>
 static int pages_mma_run(const PagesArgs<__nv_bfloat16>& p, int page_slices, bool after_prefix,
                          cudaStream_t stream) {
   const int64_t tasks = (int64_t)p.batch * p.kv_heads * ((p.group + PG_HEADS - 1) / PG_HEADS);
@@ -528,10 +693,11 @@ static int pages_mma_run(const PagesArgs<__nv_bfloat16>& p, int page_slices, boo
   // warps of a CTA: a run of 32 tokens each, more when there are few CTAs
   const int64_t runs = ((int64_t)p.max_blocks * p.page + 1 + 31) / 32;
   const int warps = runs <= 2 && tasks * page_slices >= 4 * 148 ? 2 : tasks * page_slices >= 2 * 148 ? 4 : 8;
-  const int rows = p.group <= 8 ? 8 : PG_HEADS;
-  const int smem = warps * rows * (PgShape<DP>::kStride + 2) * 4;
-  if (cudaFuncSetAttribute(pages_mma_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           8 * PG_HEADS * (PgShape<DP>::kStride + 2) * 4) != cudaSuccess)
+  constexpr int kRow = ((kFew ? 8 : PG_HEADS) * (PgShape<DP>::kStride + 2) + 32 * 4 + 2) * 4;
+  const int smem = warps * kRow;
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(pages_mma_kernel<DP, kFew>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           8 * kRow) != cudaSuccess)
     return GRS_ERR_CUDA;
   // starts under the prefix kernel's tail; its join waits for the slices
   cudaLaunchAttribute attr;
@@ -544,12 +710,14 @@ static int pages_mma_run(const PagesArgs<__nv_bfloat16>& p, int page_slices, boo
   config.stream = counted(stream);
   config.attrs = &attr;
   config.numAttrs = after_prefix ? 1 : 0;
-  if (cudaLaunchKernelEx(&config, pages_mma_kernel<DP>, p, rows) != cudaSuccess)
+  if (cudaLaunchKernelEx(&config, pages_mma_kernel<DP, kFew>, p) != cudaSuccess)
     return GRS_ERR_CUDA;
-  if (page_slices > 1) {
+  if (p.page_part) {
+    const int parts = p.slices + page_slices, team = parts > 8 ? 4 : 1;
     const int64_t n = (int64_t)p.batch * p.heads;
-    join_parts_kernel<<<(unsigned)((n + 3) / 4), 128, 0, counted(stream)>>>(p, p.slices +
-                                                                                  page_slices);
+    if (n > INT_MAX) return GRS_ERR_SHAPE;
+    join_parts_kernel<<<(unsigned)((n + 4 / team - 1) / (4 / team)), 128, 0, counted(stream)>>>(
+        p, parts, team);
   }
   GRS_CUDA_CHECK_LAUNCH();
   return GRS_OK;
@@ -557,9 +725,13 @@ static int pages_mma_run(const PagesArgs<__nv_bfloat16>& p, int page_slices, boo
 
 static int pages_mma_launch(const PagesArgs<__nv_bfloat16>& p, int page_slices, bool after_prefix,
                             cudaStream_t stream) {
-  if (p.D <= 32) return pages_mma_run<32>(p, page_slices, after_prefix, stream);
-  if (p.D <= 64) return pages_mma_run<64>(p, page_slices, after_prefix, stream);
-  return pages_mma_run<128>(p, page_slices, after_prefix, stream);
+  const auto run = [&](auto few) {
+    constexpr bool kFew = decltype(few)::value;
+    if (p.D <= 32) return pages_mma_run<32, kFew>(p, page_slices, after_prefix, stream);
+    if (p.D <= 64) return pages_mma_run<64, kFew>(p, page_slices, after_prefix, stream);
+    return pages_mma_run<128, kFew>(p, page_slices, after_prefix, stream);
+  };
+  return p.group <= 8 ? run(std::true_type{}) : run(std::false_type{});
 }
 
 template <typename T>
@@ -596,8 +768,8 @@ extern "C" int64_t grs_shared_prefix_workspace_bytes(int batch, int heads, int k
   const int parts = std::max(
       grs::rows_plan(batch, heads / kv_heads, kv_heads, num_prefix).parts,
       grs::tc_plan(batch, heads, kv_heads, head_width, num_prefix).parts);
-  const int pages = grs::pages_slices(batch, heads, kv_heads, page_tokens);
-  return (int64_t)(parts + (pages > 1 ? pages : 0)) * batch * heads * (head_width + 1) * 4;
+  const grs::PagesPlan pages = grs::pages_plan(batch, heads, kv_heads, num_prefix, page_tokens);
+  return (int64_t)(parts + (pages.separate ? pages.slices : 0)) * batch * heads * (head_width + 1) * 4;
 }
 
 extern "C" int grs_shared_prefix_attention(
@@ -640,8 +812,8 @@ extern "C" int grs_shared_prefix_attention(
     const PrefixPlan plan = tensor_cores ? tc_plan(batch, heads, kv_heads, head_width, num_prefix)
                                          : rows_plan(batch, group, kv_heads, num_prefix);
     float* part = static_cast<float*>(workspace);
-    const int page_slices = pages_slices(batch, heads, kv_heads, room);
-    const int64_t parts = plan.parts + (page_slices > 1 ? page_slices : 0);
+    const PagesPlan pages = pages_plan(batch, heads, kv_heads, num_prefix, room);
+    const int64_t parts = plan.parts + (pages.separate ? pages.slices : 0);
     float* lse = part + parts * batch * heads * head_width;
     g.part = part; g.part_lse = lse; g.slices = plan.slices; g.slice_keys = plan.keys;
     g.status = status;
@@ -653,11 +825,12 @@ extern "C" int grs_shared_prefix_attention(
     p.lengths = max_blocks ? lengths : nullptr; p.num_pages = num_pages; p.page = page_size;
     p.ck = static_cast<const T*>(current_key); p.cv = static_cast<const T*>(current_value);
     p.ck_sb = ck_sb; p.ck_sh = ck_sh; p.cvalid = current_valid;
-    p.part = p.page_part = part; p.part_lse = p.page_lse = lse; p.slices = plan.parts;
+    p.part = part; p.part_lse = lse;
+    if (pages.separate) p.page_part = part, p.page_lse = lse; p.slices = plan.parts;
     p.out = static_cast<T*>(output); p.o_sb = o_sb; p.o_sh = o_sh;
     p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.group = group; p.D = head_width;
     p.scale_log2 = scale_log2; p.status = status;
-    return shared_prefix<T>(p, g, tensor_cores, page_slices, s);
+    return shared_prefix<T>(p, g, tensor_cores, pages.slices, s);
   };
   if (dtype == GRS_DTYPE_F32) return go(float{});
   if (dtype == GRS_DTYPE_BF16) return go(__nv_bfloat16{});
