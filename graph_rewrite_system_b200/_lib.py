@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 from pathlib import Path
 import re
+import struct
 
 import torch
 
@@ -153,6 +154,13 @@ class pinned_stream:
 
     def __exit__(self, *exc):
         _PINNED_STREAM.pop()
+
+
+def words_of(name: str) -> struct.Struct:
+    """Packs the arguments of entry point `name` into the table that its
+    ``_words`` form takes (0 for a null pointer)."""
+    codes = {c_f32: "d", ctypes.c_double: "d"}
+    return struct.Struct("=" + "".join(codes.get(t, "q") for t in _SIGNATURES[name][1]))
 
 
 def current_device() -> int:

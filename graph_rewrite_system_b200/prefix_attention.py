@@ -12,10 +12,19 @@ tensors raise.
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _lib
 from .prompt_attention import _check_heads, _check_scale, _out_rows, _rows, _status_for
+
+_WORDS = _lib.words_of("grs_shared_prefix_attention").pack
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(*sizes: int) -> int:
+    return _lib.lib().grs_shared_prefix_workspace_bytes(*sizes)
 
 
 def shared_prefix_attention(
@@ -73,7 +82,7 @@ def shared_prefix_attention(
 
     columns = pages = page = table_row = 0
     c = (0, 0, 0)
-    table = past = None
+    keys = values = table = past = 0
     if key_cache is None or value_cache is None or block_table is None or lengths is None:
         if not (key_cache is value_cache is block_table is lengths):
             raise ValueError("caches, block table and lengths must be supplied together")
@@ -99,16 +108,18 @@ def shared_prefix_attention(
         if columns * page >= 1 << 30:
             raise ValueError("a block table row holds at most 2^30 tokens")
         columns = columns if page else 0
+        keys, values = key_cache.data_ptr(), value_cache.data_ptr()
         table, past = block_table.data_ptr(), lengths.data_ptr()
 
     cur = (0, 0)
-    valid = None
+    cur_key = cur_value = valid = 0
     if (current_key is None) != (current_value is None):
         raise ValueError("current key/value must be supplied together")
     if current_key is not None:
         cur = _rows("current_key", current_key, device, dtype, (batch, kv_heads, width))
         if cur != _rows("current_value", current_value, device, dtype, (batch, kv_heads, width)):
             raise ValueError("current key/value must share a layout")
+        cur_key, cur_value = current_key.data_ptr(), current_value.data_ptr()
     if current_valid is not None:
         if current_key is None:
             raise ValueError("current_valid comes with the current key/value")
@@ -128,18 +139,16 @@ def shared_prefix_attention(
     if not batch:
         return out
     word = _status_for(query, status)
-    lib, stream = _lib.lib(), _lib.stream_on(device)
-    work = None
-    need = lib.grs_shared_prefix_workspace_bytes(batch, heads, kv_heads, width, num_prefix,
-                                                 columns * page)
+    stream = _lib.stream_on(device)
+    work, need = 0, _workspace_bytes(batch, heads, kv_heads, width, num_prefix, columns * page)
     if need:
         scratch = _lib.scratch(query, need, stream)
         work = scratch.data_ptr()
-    _lib.check(lib.grs_shared_prefix_attention(
+    code = _lib.lib().grs_shared_prefix_attention_words(_WORDS(
         code, query.data_ptr(), q[0], q[1], prefix_key.data_ptr(), pk[0], pk[1],
-        prefix_value.data_ptr(), pv[0], pv[1], num_prefix, _lib.ptr(key_cache),
-        _lib.ptr(value_cache), c[0], c[1], c[2], table, table_row, columns, past, pages, page,
-        _lib.ptr(current_key), _lib.ptr(current_value), cur[0], cur[1], valid, out.data_ptr(),
-        o[0], o[1], batch, heads, kv_heads, width, scale, work, need, word, stream),
-        "shared-prefix attention")
+        prefix_value.data_ptr(), pv[0], pv[1], num_prefix, keys, values, c[0], c[1], c[2], table,
+        table_row, columns, past, pages, page, cur_key, cur_value, cur[0], cur[1], valid,
+        out.data_ptr(), o[0], o[1], batch, heads, kv_heads, width, scale, work, need, word, stream))
+    if code:
+        _lib.check(code, "shared-prefix attention")
     return out

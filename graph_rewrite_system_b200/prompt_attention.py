@@ -19,6 +19,8 @@ import torch
 from . import _lib
 from .paged_attention import _STATUS, _status_word
 
+_WORDS = _lib.words_of("grs_prompt_attention").pack
+
 
 def _status_for(query: torch.Tensor, status: torch.Tensor | None) -> int:
     """Address of the caller's status word, or of the device's
@@ -145,8 +147,10 @@ def prompt_attention(
     if not tokens:
         return out
     word = _status_for(query, status)
-    _lib.check(_lib.lib().grs_prompt_attention(
+    status = _lib.lib().grs_prompt_attention_words(_WORDS(
         code, query.data_ptr(), q[0], q[1], key.data_ptr(), k[0], k[1], value.data_ptr(), v[0],
         v[1], offsets.data_ptr(), offsets.numel() - 1, out.data_ptr(), o[0], o[1], tokens, heads,
-        kv_heads, width, scale, int(fresh), word, _lib.stream_on(device)), "prompt attention")
+        kv_heads, width, scale, int(fresh), word, _lib.stream_on(device)))
+    if status:
+        _lib.check(status, "prompt attention")
     return out

@@ -12,11 +12,13 @@ import torch
 
 from . import _lib
 
+_WORDS = _lib.words_of("grs_adjust_logits").pack
 
-def _ints(name: str, t: torch.Tensor | None, rows: int, device: int) -> int | None:
-    """Address of an optional int32 [rows]."""
+
+def _ints(name: str, t: torch.Tensor | None, rows: int, device: int) -> int:
+    """Address of an optional int32 [rows], or 0."""
     if t is None:
-        return None
+        return 0
     if (t.dtype is not torch.int32 or t.shape != (rows,) or not t.is_contiguous()
             or t.get_device() != device):
         _lib.require_cuda(t)
@@ -25,14 +27,14 @@ def _ints(name: str, t: torch.Tensor | None, rows: int, device: int) -> int | No
 
 
 def _knob(name: str, value, rows: int, device: int):
-    """(address or None, scalar) of a penalty given per row or for all."""
+    """(address or 0, scalar) of a penalty given per row or for all."""
     if isinstance(value, torch.Tensor):
         if (value.dtype is not torch.float32 or value.shape != (rows,)
                 or not value.is_contiguous() or value.get_device() != device):
             _lib.require_cuda(value)
             raise ValueError(f"{name} must be a number or contiguous fp32 [rows]")
         return value.data_ptr(), 0.0
-    return None, float(value)
+    return 0, float(value)
 
 
 def _table(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int, columns: int,
@@ -95,7 +97,7 @@ def adjust_logits(
     if vocab > 1 and step != 1:
         raise ValueError("logits need contiguous rows")
     history = tokens_row = wide = 0
-    token_ptr = None
+    token_ptr = 0
     if tokens is not None:
         if (tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 2
                 or tokens.shape[0] != rows or tokens.get_device() != device
@@ -111,9 +113,9 @@ def adjust_logits(
     rep_ptr, rep = _knob("repetition", repetition, rows, device)
     pres_ptr, pres = _knob("presence", presence, rows, device)
     freq_ptr, freq = _knob("frequency", frequency, rows, device)
-    if rep_ptr is None and not rep > 0:
+    if not rep_ptr and not rep > 0:
         raise ValueError("repetition must be positive")
-    bias_ptr = allowed_ptr = None
+    bias_ptr = allowed_ptr = 0
     bias_row = allowed_row = 0
     if bias is not None:
         bias_row = _table("bias", bias, torch.float32, rows, vocab, device)
@@ -134,9 +136,11 @@ def adjust_logits(
             raise ValueError("out must be the logits themselves or not overlap them")
     if not rows or not vocab:
         return out
-    _lib.check(_lib.lib().grs_adjust_logits(
+    status = _lib.lib().grs_adjust_logits_words(_WORDS(
         code, logits.data_ptr(), row, out.data_ptr(), out_row, rows, vocab, token_ptr, wide,
         tokens_row, history, lengths_ptr, prompts_ptr, rep_ptr, pres_ptr, freq_ptr, rep, pres,
         freq, bias_ptr, bias_row, allowed_ptr, allowed_row, float(fill),
-        _lib.stream_on(device)), "adjust_logits")
+        _lib.stream_on(device)))
+    if status:
+        _lib.check(status, "adjust_logits")
     return out

@@ -656,6 +656,15 @@ GRS_API int grs_adjust_logits(int dtype, const void* logits, int64_t l_sb, void*
                               const float* bias, int64_t bias_sb, const int32_t* allowed,
                               int64_t a_sb, float fill, void* stream);
 
+/* The three calls above with their arguments in a host table of 64-bit words,
+ * one per argument in the same order (pointers and integers as such, floats as
+ * the bits of a double; read before the call returns): a foreign-function
+ * interface that converts argument by argument spends longer on 20 to 40 of
+ * them than the launch takes. */
+GRS_API int grs_prompt_attention_words(const int64_t* words);
+GRS_API int grs_shared_prefix_attention_words(const int64_t* words);
+GRS_API int grs_adjust_logits_words(const int64_t* words);
+
 #ifdef __cplusplus
 }
 #endif

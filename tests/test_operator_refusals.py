@@ -165,3 +165,15 @@ def test_c_abi_refusals():
                    dict(history=1 << 30), dict(tokens=None), dict(x=None), dict(out=None)):
         assert lib.grs_adjust_logits(*{**logits, **change}.values()) == shape, change
     assert lib.grs_adjust_logits(*{**logits, "rows": 0}.values()) == 0
+    # the table forms: the same answers, floats and null pointers included
+    for name, args, change in (("prompt_attention", prompt, dict(tokens=0)),
+                               ("prompt_attention", prompt, dict(scale=float("inf"))),
+                               ("shared_prefix_attention", prefix, dict(work=None)),
+                               ("shared_prefix_attention", prefix, dict(scale=float("nan"))),
+                               ("adjust_logits", logits, dict(rows=0)),
+                               ("adjust_logits", logits, dict(out=None))):
+        values = [v or 0 for v in {**args, **change}.values()]
+        table = _lib.words_of(f"grs_{name}").pack(*values)
+        expected = getattr(lib, f"grs_{name}")(*{**args, **change}.values())
+        assert getattr(lib, f"grs_{name}_words")(table) == expected, (name, change)
+        assert getattr(lib, f"grs_{name}_words")(None) == shape
