@@ -1,14 +1,17 @@
 // Grouped attention on the fp32 pipes: fp32 inputs, and bf16 inputs that the
 // tensor-core kernel does not take (widths that are no multiple of 8 or above
-// 128, groups above 128, unaligned rows).
+// 128, groups above 128, unaligned rows, negative scales).
 //
-// One CTA of 128 threads takes 64 rows of one K/V head and walks 64-key tiles.
-// Q, K and V stand in shared memory in fp32, Q and K transposed, so that a
-// thread's 8 x 4 scores read three 16-byte vectors per dimension for 32
-// multiply-adds; the weights go through shared memory (transposed) to the
-// 8 x DP/16 outputs of the same half warp, four vectors per key for 64
-// multiply-adds at DP = 128.  Running maximum and sum, scores and outputs are
-// fp32.
+// One CTA takes 128 rows of one K/V head (64 at widths above 128) and walks
+// 64-key tiles; a thread holds 8 rows x 4 keys of the scores and 8 rows x DP/16
+// columns of the output.  Both products read 16-byte vectors from shared memory
+// (12 for 128 multiply-adds, 16 for 256 at DP = 128) into packed fp32x2
+// multiply-adds: the scores sum even and odd dimensions apart, so both factors
+// are pairs as they lie.  The next K tile is fetched (cp.async) under the value
+// product and the next V tile under the scores, in one buffer each.  The
+// weights pass through shared memory between the 16 threads of a row.  Running
+// maximum and sum, scores, weights and outputs are fp32.  Bound by the
+// multiply-adds.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -17,172 +20,224 @@
 
 namespace grs {
 
-constexpr int GA_ROWS = 64, GA_KEYS = 64, GA_THREADS = 128;
-constexpr int GA_QS = GA_ROWS + 4, GA_KS = GA_KEYS + 4;   // transposed row strides (floats)
+constexpr int GA_KEYS = 64, GA_PS = GA_KEYS + 4;
 
 template <int DP>
-constexpr int ga_smem() {
-  return (DP * GA_QS + DP * GA_KS + GA_KEYS * DP + GA_KEYS * GA_QS) * 4;
+struct GaShape {
+  static constexpr int kRows = DP <= 128 ? 128 : 64;
+  static constexpr int kThreads = 2 * kRows;           // 16 threads for 8 rows
+  static constexpr int kRowStep = kRows / 8;           // thread rows: rg + kRowStep i
+  static constexpr int kQS = DP + 4;                   // padded row strides (floats)
+  static constexpr int kSmem = (kRows * kQS + GA_KEYS * kQS + GA_KEYS * DP + kRows * GA_PS) * 4;
+};
+
+__device__ __forceinline__ void ga_copy16(float* dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(
+                   (unsigned)__cvta_generic_to_shared(dst)),
+               "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void ga_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void ga_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
 }
 
-template <typename T, int DP, bool kCausal>
-__global__ void __launch_bounds__(GA_THREADS) grouped_rows_kernel(GroupedArgs<T> a) {
-  extern __shared__ float ga_smem_raw[];
-  float* qt = ga_smem_raw;                  // [DP][GA_QS]
-  float* kt = qt + DP * GA_QS;              // [DP][GA_KS]
-  float* vs = kt + DP * GA_KS;              // [GA_KEYS][DP]
-  float* pt = vs + GA_KEYS * DP;            // [GA_KEYS][GA_QS]
-  __shared__ int row_begin[GA_ROWS], row_end[GA_ROWS], span[2];
-  constexpr int NV = DP / 16;               // output columns of a thread
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int rg = tid >> 4, cg = tid & 15;   // 8 rows from 8 rg; keys and columns of cg
+// rows [t0, t0 + 64) of a K or V head into shared memory, zeros past `end` and
+// past the width
+template <typename T, int DP, int kStride, bool kAsync>
+__device__ __forceinline__ void ga_load(float* dst, const T* src, int64_t st, int D, int t0,
+                                        int end) {
+  constexpr int kThreads = GaShape<DP>::kThreads;
+  if constexpr (kAsync) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < GA_KEYS * DP / 4; i += kThreads) {
+      const int t = i / (DP / 4), d = i % (DP / 4) * 4;
+      const bool in = t0 + t < end && d < D;
+      ga_copy16(dst + t * kStride + d, in ? src + (int64_t)(t0 + t) * st + d : src, in);
+    }
+  } else {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < GA_KEYS * DP; i += kThreads) {
+      const int t = i / DP, d = i % DP;
+      dst[t * kStride + d] =
+          t0 + t < end && d < D ? to_float(src[(int64_t)(t0 + t) * st + d]) : 0.f;
+    }
+  }
+  ga_commit();
+}
+
+template <typename T, int DP, bool kCausal, bool kAsync>
+__global__ void __launch_bounds__(GaShape<DP>::kThreads, DP == 32 ? 2 : 1)
+grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
+  using S = GaShape<DP>;
+  extern __shared__ __align__(16) float ga_smem_raw[];
+  float* qs = ga_smem_raw;                  // [kRows][kQS], scaled
+  float* ks = qs + S::kRows * S::kQS;       // [GA_KEYS][kQS]
+  float* vs = ks + GA_KEYS * S::kQS;        // [GA_KEYS][DP]
+  float* ps = vs + GA_KEYS * DP;            // [kRows][GA_PS]
+  // per row its keys; first and last key of any row, last first and first last
+  __shared__ int row_begin[S::kRows], row_end[S::kRows], span[4];
+  constexpr int kPairs = DP / 32;           // output column pairs of a thread
+  const int tid = threadIdx.x;
+  const int rg = tid >> 4, cg = tid & 15;
   const int h = blockIdx.y;
   const int64_t total = (int64_t)a.positions * a.group;
   // late rows of a causal tile see the most keys: they start first
-  const int64_t row0 = (int64_t)(kCausal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * GA_ROWS;
+  const int64_t row0 = (int64_t)(kCausal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * S::kRows;
 
-  if (tid < GA_ROWS) {
+  if (tid == 0) {
+    span[0] = span[3] = INT_MAX;
+    span[1] = span[2] = 0;
+  }
+  __syncthreads();
+  if (tid < S::kRows) {
     const int64_t r = row0 + tid;
     int begin = 0, end = 0;
     if (r < total) {
       if (kCausal) {
         causal_range(a.offsets, a.sequences, (int)(r / a.group), begin, end);
       } else {
-        begin = blockIdx.z * a.slice_keys;
+        begin = min(a.keys, (int)blockIdx.z * a.slice_keys);
         end = min(a.keys, begin + a.slice_keys);
       }
     }
     row_begin[tid] = begin;
     row_end[tid] = end;
+    if (end > begin) {
+      atomicMin(&span[0], begin);
+      atomicMax(&span[1], end);
+      atomicMax(&span[2], begin);
+      atomicMin(&span[3], end);
+    }
   }
-  if (tid == 0) { span[0] = INT_MAX; span[1] = 0; }
   __syncthreads();
-  if (tid < GA_ROWS && row_end[tid] > row_begin[tid]) {
-    atomicMin(&span[0], row_begin[tid]);
-    atomicMax(&span[1], row_end[tid]);
+  const int first = span[0], last = span[1], all_from = span[2], all_to = span[3];
+  const T* kh = a.k + (int64_t)h * a.k_sh;
+  const T* vh = a.v + (int64_t)h * a.v_sh;
+  if (first < last) {
+    ga_load<T, DP, S::kQS, kAsync>(ks, kh, a.k_st, a.D, first, last);
+    ga_load<T, DP, DP, kAsync>(vs, vh, a.v_st, a.D, first, last);
   }
-  for (int i = tid; i < GA_ROWS * DP; i += GA_THREADS) {
+#pragma unroll 8
+  for (int i = tid; i < S::kRows * DP; i += S::kThreads) {
     const int r = i / DP, d = i % DP;
     const int64_t row = row0 + r;
     float x = 0.f;
-    if (row < total && d < a.D)
-      x = to_float(a.q[(row / a.group) * a.q_sp +
-                       ((int64_t)h * a.group + row % a.group) * a.q_sh + d]);
-    qt[d * GA_QS + r] = x * a.scale_log2;
+    if (row < total && d < a.D) {
+      const int p = (int)(row / a.group), head = h * a.group + (int)(row - (int64_t)p * a.group);
+      x = to_float(a.q[(int64_t)p * a.q_sp + (int64_t)head * a.q_sh + d]);
+    }
+    qs[r * S::kQS + d] = x * a.scale_log2;
   }
-  __syncthreads();
-  const int first = span[0], last = span[1];
 
-  float acc[8][NV], m[8], l[8];
+  float2 acc[8][kPairs];
+  float m[8], l[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) acc[i][j] = 0.f;
-  }
-  int rb[8], re[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    rb[i] = row_begin[8 * rg + i];
-    re[i] = row_end[8 * rg + i];
+    for (int j = 0; j < kPairs; ++j) acc[i][j] = make_float2(0.f, 0.f);
   }
 
   for (int t0 = first; t0 < last; t0 += GA_KEYS) {
-    // keys along the lanes: the transposed writes hit every bank once
-    for (int i = tid; i < GA_KEYS * DP; i += GA_THREADS) {
-      const int t = i % GA_KEYS, d = i / GA_KEYS;
-      float x = 0.f;
-      if (t0 + t < last && d < a.D)
-        x = to_float(a.k[(int64_t)(t0 + t) * a.k_st + (int64_t)h * a.k_sh + d]);
-      kt[d * GA_KS + t] = x;
-    }
-    for (int i = tid; i < GA_KEYS * DP; i += GA_THREADS) {
-      const int t = i / DP, d = i % DP;
-      float x = 0.f;
-      if (t0 + t < last && d < a.D)
-        x = to_float(a.v[(int64_t)(t0 + t) * a.v_st + (int64_t)h * a.v_sh + d]);
-      vs[i] = x;
-    }
+    ga_wait<1>();                           // K is here; V may be on its way
     __syncthreads();
     float s[8][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-#pragma unroll 4
-    for (int d = 0; d < DP; ++d) {
-      const float4 q0 = *reinterpret_cast<const float4*>(qt + d * GA_QS + 8 * rg);
-      const float4 q1 = *reinterpret_cast<const float4*>(qt + d * GA_QS + 8 * rg + 4);
-      const float4 k4 = *reinterpret_cast<const float4*>(kt + d * GA_KS + 4 * cg);
-      const float qv[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
-      const float kv[4] = {k4.x, k4.y, k4.z, k4.w};
+    {
+      float2 s2[8][4];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = fmaf(qv[i], kv[j], s[i][j]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = t0 + 4 * cg + j;
-        if (t < rb[i] || t >= re[i]) s[i][j] = -INFINITY;
-        top = fmaxf(top, s[i][j]);
-      }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      top = fmaxf(top, m[i]);
-      const float base = top == -INFINITY ? 0.f : top;
-      const float keep = exp2f(m[i] - base);
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[i][j] = exp2f(s[i][j] - base);
-        sum += s[i][j];
-      }
-      l[i] = l[i] * keep + sum;             // this thread's share of the row's sum
-      m[i] = top;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) acc[i][j] *= keep;
-    }
-    // the weights of 8 rows pass between the 16 threads of the half warp
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float* p = pt + (4 * cg + j) * GA_QS + 8 * rg;
-      *reinterpret_cast<float4*>(p) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
-      *reinterpret_cast<float4*>(p + 4) = make_float4(s[4][j], s[5][j], s[6][j], s[7][j]);
-    }
-    __syncwarp();
+        for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 2
-    for (int t = 0; t < GA_KEYS; ++t) {
-      const float4 p0 = *reinterpret_cast<const float4*>(pt + t * GA_QS + 8 * rg);
-      const float4 p1 = *reinterpret_cast<const float4*>(pt + t * GA_QS + 8 * rg + 4);
-      const float pv[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
-      float vv[NV];
-      if constexpr (NV == 2) {
-        const float2 v2 = *reinterpret_cast<const float2*>(vs + t * DP + 2 * cg);
-        vv[0] = v2.x;
-        vv[1] = v2.y;
-      } else {
+      for (int d = 0; d < DP; d += 4) {
+        float4 k4[4];
 #pragma unroll
-        for (int j = 0; j < NV / 4; ++j) {
-          const float4 v4 = *reinterpret_cast<const float4*>(vs + t * DP + 64 * j + 4 * cg);
-          vv[4 * j] = v4.x;
-          vv[4 * j + 1] = v4.y;
-          vv[4 * j + 2] = v4.z;
-          vv[4 * j + 3] = v4.w;
+        for (int j = 0; j < 4; ++j)
+          k4[j] = *reinterpret_cast<const float4*>(ks + (cg + 16 * j) * S::kQS + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 q4 = *reinterpret_cast<const float4*>(qs + (rg + S::kRowStep * i) * S::kQS + d);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s2[i][j] = __ffma2_rn(make_float2(q4.x, q4.y), make_float2(k4[j].x, k4[j].y), s2[i][j]);
+            s2[i][j] = __ffma2_rn(make_float2(q4.z, q4.w), make_float2(k4[j].z, k4[j].w), s2[i][j]);
+          }
         }
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < NV; ++j) acc[i][j] = fmaf(pv[i], vv[j], acc[i][j]);
+        for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
     }
+    __syncthreads();                        // K is read
+    ga_load<T, DP, S::kQS, kAsync>(ks, kh, a.k_st, a.D, t0 + GA_KEYS, last);
+    if (t0 < all_from || t0 + GA_KEYS > all_to) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int from = row_begin[rg + S::kRowStep * i] - t0, to = row_end[rg + S::kRowStep * i] - t0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (cg + 16 * j < from || cg + 16 * j >= to) s[i][j] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float top = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top = fmaxf(top, m[i]);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float keep = exp2f(m[i] - base);
+      m[i] = top;
+      float sum = 0.f;
+      float* p = ps + (rg + S::kRowStep * i) * GA_PS + cg;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float w = exp2f(s[i][j] - base);
+        sum += w;
+        p[16 * j] = w;
+      }
+      l[i] = l[i] * keep + sum;             // this thread's share of the row's sum
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j)
+        acc[i][j] = __fmul2_rn(acc[i][j], make_float2(keep, keep));
+    }
+    ga_wait<1>();                           // V is here
     __syncthreads();
+#pragma unroll 1
+    for (int t = 0; t < GA_KEYS; t += 4) {
+      float4 p4[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        p4[i] = *reinterpret_cast<const float4*>(ps + (rg + S::kRowStep * i) * GA_PS + t);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float2 v2[kPairs];
+        if constexpr (DP == 32) {
+          v2[0] = *reinterpret_cast<const float2*>(vs + (t + k) * DP + 2 * cg);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kPairs / 2; ++j) {
+            const float4 v4 = *reinterpret_cast<const float4*>(vs + (t + k) * DP + 64 * j + 4 * cg);
+            v2[2 * j] = make_float2(v4.x, v4.y);
+            v2[2 * j + 1] = make_float2(v4.z, v4.w);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float w = k == 0 ? p4[i].x : k == 1 ? p4[i].y : k == 2 ? p4[i].z : p4[i].w;
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j) acc[i][j] = __ffma2_rn(make_float2(w, w), v2[j], acc[i][j]);
+        }
+      }
+    }
+    __syncthreads();                        // V is read
+    ga_load<T, DP, DP, kAsync>(vs, vh, a.v_st, a.D, t0 + GA_KEYS, last);
   }
+  ga_wait<0>();
 
   unsigned again = 0;                       // rows (of 8) whose result is not finite
 #pragma unroll
@@ -190,19 +245,21 @@ __global__ void __launch_bounds__(GA_THREADS) grouped_rows_kernel(GroupedArgs<T>
     float sum = l[i];
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const int64_t row = row0 + 8 * rg + i;
+    const int r = rg + S::kRowStep * i;
+    const int64_t row = row0 + r;
     if (row >= total) continue;
-    const int p = (int)(row / a.group), head = h * a.group + (int)(row % a.group);
+    const int p = (int)(row / a.group), head = h * a.group + (int)(row - (int64_t)p * a.group);
+    const bool seen = row_end[r] > row_begin[r];
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     bool odd = !(fabsf(sum) <= FLT_MAX);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int d = NV == 2 ? 2 * cg + j : 64 * (j / 4) + 4 * cg + (j & 3);
-      const float x = acc[i][j] * inv;
+    for (int j = 0; j < 2 * kPairs; ++j) {
+      const int d = DP == 32 ? 2 * cg + j : 64 * (j / 4) + 4 * cg + (j & 3);
+      const float x = (j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x) * inv;
       if (d >= a.D) continue;
       if (kCausal) {
-        if (re[i] > rb[i] || a.clear_rest)
-          a.out[(int64_t)p * a.o_sp + (int64_t)head * a.o_sh + d] = from_float<T>(x);
+        if (seen || a.clear_rest)
+          a.out[(int64_t)p * a.o_sp + (int64_t)head * a.o_sh + d] = from_float<T>(seen ? x : 0.f);
         odd |= !(fabsf(x) <= FLT_MAX);
       } else {
         a.part[(((int64_t)blockIdx.z * a.positions + p) * a.heads + head) * a.D + d] = x;
@@ -211,55 +268,70 @@ __global__ void __launch_bounds__(GA_THREADS) grouped_rows_kernel(GroupedArgs<T>
     if (!kCausal && cg == 0)
       a.part_lse[((int64_t)blockIdx.z * a.positions + p) * a.heads + head] =
           sum == 0.f ? -INFINITY : m[i] + log2f(sum);
-    if (odd) again |= 1u << i;
+    if (odd && seen) again |= 1u << i;
   }
   if constexpr (kCausal) {
-    // the whole warp holds rows 16 (warp) .. + 15; the writes above come first
+    // the writes of the half warp's rows come first
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) again |= __shfl_xor_sync(0xffffffffu, again, o);
     __syncwarp();
+#pragma unroll 1
     for (int half = 0; half < 2; ++half) {
       unsigned todo = __shfl_sync(0xffffffffu, again, 16 * half);
       while (todo) {
         const int i = __ffs(todo) - 1;
         todo &= todo - 1;
-        const int r = (tid >> 5) * 16 + 8 * half + i;
+        const int r = (tid >> 5) * 2 + half + S::kRowStep * i;
         const int64_t row = row0 + r;
-        if (row < total && row_end[r] > row_begin[r])
-          causal_row_again<T, (DP + 31) / 32>(a, (int)(row / a.group),
-                                              h * a.group + (int)(row % a.group), row_begin[r],
-                                              row_end[r], 0, a.D);
+        const int p = (int)(row / a.group);
+        causal_row_again<T, (DP + 31) / 32>(a, p, h * a.group + (int)(row - (int64_t)p * a.group),
+                                            row_begin[r], row_end[r], 0, a.D);
       }
     }
   }
 }
 
-template <typename T, int DP, bool kCausal>
+template <typename T, int DP, bool kCausal, bool kAsync>
 static int rows_launch(const GroupedArgs<T>& a, cudaStream_t stream) {
-  const int64_t tiles = ((int64_t)a.positions * a.group + GA_ROWS - 1) / GA_ROWS;
+  using S = GaShape<DP>;
+  static_assert(S::kSmem + 4 * (2 * S::kRows + 4) <= 227 * 1024, "shared memory of a CTA");
+  const int64_t tiles = ((int64_t)a.positions * a.group + S::kRows - 1) / S::kRows;
   if (tiles > INT_MAX || a.kv_heads > 65535 || (!kCausal && a.slices > 65535))
     return GRS_ERR_SHAPE;
-  if (cudaFuncSetAttribute(grouped_rows_kernel<T, DP, kCausal>,
-                           cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           ga_smem<DP>()) != cudaSuccess)
+  if (cudaFuncSetAttribute(grouped_rows_kernel<T, DP, kCausal, kAsync>,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
     return GRS_ERR_CUDA;
   const dim3 grid((unsigned)tiles, a.kv_heads, kCausal ? 1 : a.slices);
-  grouped_rows_kernel<T, DP, kCausal><<<grid, GA_THREADS, ga_smem<DP>(), counted(stream)>>>(a);
+  grouped_rows_kernel<T, DP, kCausal, kAsync>
+      <<<grid, S::kThreads, S::kSmem, counted(stream)>>>(a);
   GRS_CUDA_CHECK_LAUNCH();
   return GRS_OK;
 }
 
+// 16-byte copies need rows of whole 16 bytes at 16-byte addresses
+static bool rows_aligned(const GroupedArgs<float>& a) {
+  return (reinterpret_cast<uintptr_t>(a.k) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.v) & 15) == 0 &&
+         a.D % 4 == 0 && a.k_st % 4 == 0 && a.k_sh % 4 == 0 && a.v_st % 4 == 0 && a.v_sh % 4 == 0;
+}
+static bool rows_aligned(const GroupedArgs<__nv_bfloat16>&) { return false; }
+
+template <typename T, int DP>
+static int rows_forms(const GroupedArgs<T>& a, cudaStream_t stream) {
+  const bool causal = a.offsets != nullptr;
+  if constexpr (sizeof(T) == 4)
+    if (rows_aligned(a))
+      return causal ? rows_launch<T, DP, true, true>(a, stream)
+                    : rows_launch<T, DP, false, true>(a, stream);
+  return causal ? rows_launch<T, DP, true, false>(a, stream)
+                : rows_launch<T, DP, false, false>(a, stream);
+}
+
 template <typename T>
 int grouped_rows_launch(const GroupedArgs<T>& a, cudaStream_t stream) {
-  const bool causal = a.offsets != nullptr;
-#define GRS_GA_WIDTH(DP)                                       \
-  if (a.D <= DP)                                               \
-    return causal ? rows_launch<T, DP, true>(a, stream) : rows_launch<T, DP, false>(a, stream)
-  GRS_GA_WIDTH(32);
-  GRS_GA_WIDTH(64);
-  GRS_GA_WIDTH(128);
-  GRS_GA_WIDTH(256);
-#undef GRS_GA_WIDTH
+  if (a.D <= 32) return rows_forms<T, 32>(a, stream);
+  if (a.D <= 64) return rows_forms<T, 64>(a, stream);
+  if (a.D <= 128) return rows_forms<T, 128>(a, stream);
+  if (a.D <= 256) return rows_forms<T, 256>(a, stream);
   return GRS_ERR_SHAPE;
 }
 

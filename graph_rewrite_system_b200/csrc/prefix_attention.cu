@@ -29,54 +29,74 @@ struct PagesArgs {
   int32_t* status;
 };
 
-// One warp per (beam, head): online softmax over 32-key steps, a lane per key
-// for the scores and a lane per dimension for the values, then the join with
-// the prefix slices.
-template <typename T, int DP>
+// One CTA of four warps per (beam, head), every warp taking each fourth run of
+// 32 tokens: a lane per key for the scores (the key row in vectors of kVec
+// elements against the query in shared memory, all requested before the first
+// is used), a lane per column for the values, eight keys' rows in flight.  The
+// warps take turns on the prefix slices too and meet in shared memory.
+template <typename T, int DP, int kVec>
 __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
   constexpr int ND = (DP + 31) / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (int64_t)a.batch * a.heads) return;
-  const int b = (int)(row / a.heads), head = (int)(row % a.heads), h = head / a.group;
-  const T* q = a.q + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh;
+  __shared__ __align__(16) float q[DP];
+  __shared__ float sums[4][DP], tops[4], totals[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads, h = head / a.group;
+  for (int d = threadIdx.x; d < DP; d += 128)
+    q[d] = d < a.D ? to_float(a.q[(int64_t)b * a.q_sb + (int64_t)head * a.q_sh + d]) * a.scale_log2
+                   : 0.f;
 
   const int room = a.max_blocks * a.page;
   int past = a.lengths ? a.lengths[b] : 0;
   if (past < 0 || past > room) {
-    if (lane == 0) set_status(a.status, GRS_ERR_LENGTH);
+    if (threadIdx.x == 0) set_status(a.status, GRS_ERR_LENGTH);
     past = min(max(past, 0), room);
   }
   const bool cur = a.ck != nullptr && (a.cvalid == nullptr || a.cvalid[b] != 0);
   const int total = past + (cur ? 1 : 0);
-  // element offset of token t's row, or -1 when its page is not in the cache
-  const auto place = [&](int t) -> int64_t {
-    const int page = a.bt[(int64_t)b * a.bt_s + t / a.page];
-    if (page < 0 || page >= a.num_pages) {
-      set_status(a.status, GRS_ERR_BAD_PAGE);
-      return -1;
-    }
-    return (int64_t)page * a.kc_sp + (int64_t)(t % a.page) * a.kc_st + (int64_t)h * a.kc_sh;
-  };
+  const T* cur_k = cur ? a.ck + (int64_t)b * a.ck_sb + (int64_t)h * a.ck_sh : nullptr;
+  __syncthreads();
 
   float m = -INFINITY, l = 0.f, acc[ND];
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i] = 0.f;
-  for (int t0 = 0; t0 < total; t0 += 32) {
+  for (int t0 = 32 * warp; t0 < total; t0 += 128) {
     const int t = t0 + lane;
-    int64_t at = -1;
+    int64_t at = 0;
     const T* k = nullptr;
     if (t < past) {
-      at = place(t);
-      if (at >= 0) k = a.kc + at;
+      const int page = __ldg(a.bt + (int64_t)b * a.bt_s + t / a.page);
+      if (page >= 0 && page < a.num_pages) {
+        at = (int64_t)page * a.kc_sp + (int64_t)(t % a.page) * a.kc_st + (int64_t)h * a.kc_sh;
+        k = a.kc + at;
+      } else {
+        set_status(a.status, GRS_ERR_BAD_PAGE);
+      }
     } else if (t < total) {
-      k = a.ck + (int64_t)b * a.ck_sb + (int64_t)h * a.ck_sh;
+      k = cur_k;
     }
+    const unsigned valid = __ballot_sync(0xffffffffu, k != nullptr);
     float s = -INFINITY;
     if (k) {
-      float dot = 0.f;
-      for (int d = 0; d < a.D; ++d) dot = fmaf(to_float(q[d]), to_float(k[d]), dot);
-      s = dot * a.scale_log2;
+      float dot[4] = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (kVec > 1) {
+#pragma unroll
+        for (int d = 0; d < DP; d += kVec) {
+          if (d >= a.D) break;
+          const uint4 w = __ldg(reinterpret_cast<const uint4*>(k + d));
+          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            const float x = kVec == 4 ? __uint_as_float(words[j])
+                                      : __uint_as_float(j & 1 ? words[j / 2] & 0xffff0000u
+                                                              : words[j / 2] << 16);
+            dot[j & 3] = fmaf(q[d + j], x, dot[j & 3]);
+          }
+        }
+      } else {
+#pragma unroll 8
+        for (int d = 0; d < a.D; ++d) dot[0] = fmaf(q[d], to_float(k[d]), dot[0]);
+      }
+      s = (dot[0] + dot[1]) + (dot[2] + dot[3]);
     }
     const float top = fmaxf(m, warp_max(s));
     const float base = top == -INFINITY ? 0.f : top;
@@ -86,49 +106,95 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
 #pragma unroll
     for (int i = 0; i < ND; ++i) acc[i] *= keep;
     m = top;
-    const int n = min(32, total - t0);
-    for (int j = 0; j < n; ++j) {
-      const float wj = __shfl_sync(0xffffffffu, w, j);
-      const int64_t vat = __shfl_sync(0xffffffffu, at, j);
-      const bool is_cur = t0 + j >= past;
-      if (vat < 0 && !is_cur) continue;
-      const T* v = is_cur ? a.cv + (int64_t)b * a.ck_sb + (int64_t)h * a.ck_sh : a.vc + vat;
 #pragma unroll
-      for (int i = 0; i < ND; ++i) {
-        const int d = lane + 32 * i;
-        if (d < a.D) acc[i] = fmaf(wj, to_float(v[d]), acc[i]);
+    for (int j0 = 0; j0 < 32; j0 += 8) {
+      if (((valid >> j0) & 0xffu) == 0) continue;
+      float x[8][ND];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t vat = __shfl_sync(0xffffffffu, at, j0 + j);
+        const T* v = t0 + j0 + j >= past
+                         ? a.cv + (int64_t)b * a.ck_sb + (int64_t)h * a.ck_sh : a.vc + vat;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          const int d = lane + 32 * i;
+          x[j][i] = ((valid >> (j0 + j)) & 1) && d < a.D ? to_float(v[d]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float wj = __shfl_sync(0xffffffffu, w, j0 + j);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) acc[i] = fmaf(wj, x[j][i], acc[i]);
       }
     }
   }
 
-  // join: weights exp2(lse_i - max lse); the pages' sum enters unnormalised
-  float top = m;
-  for (int i = lane; i < a.slices; i += 32)
-    top = fmaxf(top, a.part_lse[((int64_t)i * a.batch + b) * a.heads + head]);
+  // join: weights exp2(lse_i - max lse); the pages' sums enter unnormalised
+  const int64_t stride = (int64_t)a.batch * a.heads, row = blockIdx.x;
+  if (lane == 0) tops[warp] = m;
+  __syncthreads();
+  float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  for (int i = lane; i < a.slices; i += 32) top = fmaxf(top, a.part_lse[i * stride + row]);
   top = warp_max(top);
   const float base = top == -INFINITY ? 0.f : top;
   const float own = exp2f(m - base);
   float norm = l * own;
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i] *= own;
-#pragma unroll 4
-  for (int i = 0; i < a.slices; ++i) {
-    const int64_t at = ((int64_t)i * a.batch + b) * a.heads + head;
-    const float w = exp2f(a.part_lse[at] - base);
-    norm += w;
+  for (int p0 = warp; p0 < a.slices; p0 += 16) {
+    float w[4], x[4][ND];
 #pragma unroll
-    for (int j = 0; j < ND; ++j) {
-      const int d = lane + 32 * j;
-      if (d < a.D) acc[j] = fmaf(w, a.part[at * a.D + d], acc[j]);
+    for (int j = 0; j < 4; ++j) {
+      const int i = p0 + 4 * j;
+      w[j] = i < a.slices ? a.part_lse[i * stride + row] : -INFINITY;
+#pragma unroll
+      for (int n = 0; n < ND; ++n) {
+        const int d = lane + 32 * n;
+        x[j][n] = i < a.slices && d < a.D ? a.part[(i * stride + row) * a.D + d] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float e = exp2f(w[j] - base);
+      norm += e;
+#pragma unroll
+      for (int n = 0; n < ND; ++n) acc[n] = fmaf(e, x[j][n], acc[n]);
     }
   }
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+    if (lane + 32 * i < DP) sums[warp][lane + 32 * i] = acc[i];
+  if (lane == 0) totals[warp] = norm;
+  __syncthreads();
+  norm = (totals[0] + totals[1]) + (totals[2] + totals[3]);
   const float inv = norm == 0.f ? 0.f : 1.f / norm;
   T* o = a.out + (int64_t)b * a.o_sb + (int64_t)head * a.o_sh;
-#pragma unroll
-  for (int i = 0; i < ND; ++i) {
-    const int d = lane + 32 * i;
-    if (d < a.D) o[d] = from_float<T>(acc[i] * inv);
-  }
+  for (int d = threadIdx.x; d < a.D; d += 128)
+    o[d] = from_float<T>(((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) * inv);
+}
+
+template <typename T>
+static int pages_rows_launch(const PagesArgs<T>& p, cudaStream_t stream) {
+  const int64_t rows = (int64_t)p.batch * p.heads;
+  if (rows > INT_MAX) return GRS_ERR_SHAPE;
+  constexpr int kVec = 16 / sizeof(T);
+  const auto whole = [](const void* at) { return (reinterpret_cast<uintptr_t>(at) & 15) == 0; };
+  const bool vec = p.D % kVec == 0 && whole(p.kc) && whole(p.ck) && p.kc_sp % kVec == 0 &&
+                   p.kc_st % kVec == 0 && p.kc_sh % kVec == 0 && p.ck_sb % kVec == 0 &&
+                   p.ck_sh % kVec == 0;
+  const unsigned grid = (unsigned)rows;
+  const auto go = [&](auto width) {
+    constexpr int DP = decltype(width)::value;
+    if (vec) pages_rows_kernel<T, DP, kVec><<<grid, 128, 0, counted(stream)>>>(p);
+    else pages_rows_kernel<T, DP, 1><<<grid, 128, 0, counted(stream)>>>(p);
+  };
+  if (p.D <= 32) go(std::integral_constant<int, 32>{});
+  else if (p.D <= 64) go(std::integral_constant<int, 64>{});
+  else if (p.D <= 128) go(std::integral_constant<int, 128>{});
+  else go(std::integral_constant<int, 256>{});
+  GRS_CUDA_CHECK_LAUNCH();
+  return GRS_OK;
 }
 
 // ---- bf16 pages on the tensor cores -------------------------------------------
@@ -616,13 +682,14 @@ struct PrefixPlan {
   int slices, parts, keys;
 };
 
-// fp32 rows: enough CTAs for two waves of 148 SMs, none shorter than 256 keys.
-static PrefixPlan rows_plan(int batch, int group, int kv_heads, int keys) {
+// fp32 rows: enough CTAs for two waves of 148 SMs, none shorter than 64 keys.
+static PrefixPlan rows_plan(int batch, int group, int kv_heads, int D, int keys) {
   if (keys <= 0) return {0, 0, 0};
-  const int64_t tiles = ((int64_t)batch * group + 63) / 64 * kv_heads;
-  const int64_t want =
-      std::max<int64_t>(1, std::min<int64_t>((2 * 148 + tiles - 1) / tiles, (keys + 255) / 256));
-  const int each = (int)(((keys + want - 1) / want + 127) / 128 * 128);
+  const int64_t rows = D <= 128 ? 128 : 64;
+  const int64_t tiles = ((int64_t)batch * group + rows - 1) / rows * kv_heads;
+  const int64_t want = std::max<int64_t>(
+      1, std::min<int64_t>(std::min<int64_t>((2 * 148 + tiles - 1) / tiles, 64), (keys + 63) / 64));
+  const int each = (int)(((keys + want - 1) / want + 63) / 64 * 64);
   const int slices = (keys + each - 1) / each;
   return {slices, slices, each};
 }
@@ -748,14 +815,7 @@ static int shared_prefix(const PagesArgs<T>& p, const GroupedArgs<T>& prefix, bo
   }
   if constexpr (std::is_same<T, __nv_bfloat16>::value)
     if (pages_mma_takes(p)) return pages_mma_launch(p, page_slices, prefix.slices > 0, stream);
-  const int64_t rows = (int64_t)p.batch * p.heads;
-  const unsigned grid = (unsigned)((rows + 3) / 4);
-  if (p.D <= 32) pages_rows_kernel<T, 32><<<grid, 128, 0, counted(stream)>>>(p);
-  else if (p.D <= 64) pages_rows_kernel<T, 64><<<grid, 128, 0, counted(stream)>>>(p);
-  else if (p.D <= 128) pages_rows_kernel<T, 128><<<grid, 128, 0, counted(stream)>>>(p);
-  else pages_rows_kernel<T, 256><<<grid, 128, 0, counted(stream)>>>(p);
-  GRS_CUDA_CHECK_LAUNCH();
-  return GRS_OK;
+  return pages_rows_launch<T>(p, stream);
 }
 
 }  // namespace grs
@@ -766,7 +826,7 @@ extern "C" int64_t grs_shared_prefix_workspace_bytes(int batch, int heads, int k
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
   // any of the kernels may take the call, by the alignment of its tensors
   const int parts = std::max(
-      grs::rows_plan(batch, heads / kv_heads, kv_heads, num_prefix).parts,
+      grs::rows_plan(batch, heads / kv_heads, kv_heads, head_width, num_prefix).parts,
       grs::tc_plan(batch, heads, kv_heads, head_width, num_prefix).parts);
   const grs::PagesPlan pages = grs::pages_plan(batch, heads, kv_heads, num_prefix, page_tokens);
   return (int64_t)(parts + (pages.separate ? pages.slices : 0)) * batch * heads * (head_width + 1) * 4;
@@ -810,7 +870,7 @@ extern "C" int grs_shared_prefix_attention(
     bool tensor_cores = false;
     if constexpr (std::is_same<T, __nv_bfloat16>::value) tensor_cores = grouped_tc_takes(g);
     const PrefixPlan plan = tensor_cores ? tc_plan(batch, heads, kv_heads, head_width, num_prefix)
-                                         : rows_plan(batch, group, kv_heads, num_prefix);
+                                         : rows_plan(batch, group, kv_heads, head_width, num_prefix);
     float* part = static_cast<float*>(workspace);
     const PagesPlan pages = pages_plan(batch, heads, kv_heads, num_prefix, room);
     const int64_t parts = plan.parts + (pages.separate ? pages.slices : 0);
