@@ -20,6 +20,9 @@
 //   warp 18     zeroes the value rows behind a causal tile's last key
 // The launch's 640 x 96 registers are split 104 to a softmax thread and 64 to
 // the other warpgroup (512 x 104 + 128 x 64 = 61440 = 640 x 96).
+// Short prompts take CTAs of one slot, two to an SM (384 x 80 registers: 256 x
+// 104 + 128 x 32 = 30720): most of a short tile's time is its start and end,
+// which then run under the other CTA's blocks.
 //
 // Causal and wide-batch slices give the slots neighbouring row tiles over one
 // K/V stream (each K/V block is loaded once for 256 rows); a batch of at most
@@ -41,26 +44,33 @@
 
 namespace grs {
 
-constexpr int GTC_THREADS = 640, GTC_KEYS = 128;
-constexpr int GTC_O = 256;                  // first TMEM column of the outputs
+constexpr int GTC_KEYS = 128;
 constexpr int GTC_EMULATE = 4;              // one pair in four takes gtc_exp2_pair
 constexpr int GTC_WINDOW = 260;             // offsets held for a tile's rows
 
-template <int DP>
+template <int DP, int kSlots>
 struct GtcShape {
   static constexpr int kRow = DP >= 64 ? 128 : 64;      // bytes of a staged row
   static constexpr int kBoxes = DP * 2 / kRow;          // TMA boxes side by side
   static constexpr int kBox = 128 * kRow;
   static constexpr int kTile = kBoxes * kBox;           // Q tile, K or V block
-  static constexpr int kStages = DP == 128 ? 5 : DP == 64 ? 6 : 13;
-  // above half an SM's shared memory: the 512 TMEM columns are one CTA's
-  static constexpr int kTiles = (2 + kStages) * kTile;
-  static_assert(kTiles > 114 * 1024 && kTiles <= 224 * 1024, "one CTA per SM");
+  static constexpr int kStages = kSlots == 2 ? (DP == 128 ? 5 : DP == 64 ? 6 : 13)
+                                             : (DP == 128 ? 2 : DP == 64 ? 5 : 10);
+  static constexpr int kTiles = (kSlots + kStages) * kTile;
+  // two slots: above half an SM's shared memory, as their 512 TMEM columns are
+  // all there are; one slot: two CTAs per SM
+  static_assert(kSlots == 2 ? kTiles > 114 * 1024 && kTiles <= 224 * 1024 : kTiles <= 96 * 1024,
+                "CTAs per SM");
   // whether the partial sums of 16 warps pass through one Q tile
   static constexpr bool kStageFree = kTile >= 16 * 2048;
+  static constexpr int kSoft = 256 * kSlots;            // softmax threads
+  static constexpr int kThreads = kSoft + 128;
+  static constexpr int kColumns = 256 * kSlots;         // TMEM
+  static constexpr int kO = 128 * kSlots;               // first column of the outputs
 };
 
-constexpr int GTC_CAUSAL = 0, GTC_PAIR = 1, GTC_SPLIT = 2;
+constexpr int GTC_CAUSAL = 0, GTC_PAIR = 1, GTC_SPLIT = 2, GTC_SINGLE = 3;
+constexpr int gtc_slots(int mode) { return mode == GTC_SINGLE ? 1 : 2; }
 
 __device__ __forceinline__ float gtc_exp2(float x) {
   float y;
@@ -111,10 +121,10 @@ __device__ __forceinline__ int offsets_up_to(const int32_t* __restrict__ offsets
   int lo = 0, hi = count;
   while (hi - lo > 32) {
     const int step = (hi - lo + 31) / 32;
-    const int at = lo + lane * step;
+    const int64_t at = lo + (int64_t)lane * step;
     const int n = __popc(__ballot_sync(0xffffffffu, at < hi && __ldg(offsets + at) <= p));
     if (n == 0) return lo;
-    hi = min(hi, lo + n * step);
+    hi = (int)min((int64_t)hi, lo + (int64_t)n * step);
     lo += (n - 1) * step + 1;
   }
   const bool in = lo + lane < hi && __ldg(offsets + lo + lane) <= p;
@@ -122,13 +132,15 @@ __device__ __forceinline__ int offsets_up_to(const int32_t* __restrict__ offsets
 }
 
 template <int DP, int MODE>
-__global__ void __launch_bounds__(GTC_THREADS, 1)
+__global__ void __launch_bounds__(GtcShape<DP, gtc_slots(MODE)>::kThreads, 3 - gtc_slots(MODE))
 grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v,
                   const __grid_constant__ GroupedArgs<__nv_bfloat16> a, int pps) {
   using namespace sm100;
-  using S = GtcShape<DP>;
-  constexpr bool kCausal = MODE == GTC_CAUSAL, kSplit = MODE == GTC_SPLIT;
+  constexpr int kSlots = gtc_slots(MODE);
+  using S = GtcShape<DP, kSlots>;
+  constexpr bool kCausal = MODE == GTC_CAUSAL || MODE == GTC_SINGLE, kSplit = MODE == GTC_SPLIT;
+  constexpr int kAux = S::kSoft / 32;      // first warp that is not softmax
   extern __shared__ uint8_t gtc_smem_raw[];
   __shared__ __align__(8) uint64_t q_full, kv_full[S::kStages], kv_empty[S::kStages];
   __shared__ __align__(8) uint64_t s_full[2][2], p_full[2][2], drain_bar;
@@ -141,10 +153,10 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   __shared__ int4 spans[16];
   // the window of offsets; then per slot the maxima [parity][half][row] in
   // bf16; then its sums [half][row] in fp32
-  __shared__ int scratch[512];
+  __shared__ int scratch[GTC_WINDOW > 256 * kSlots ? GTC_WINDOW : 256 * kSlots];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(gtc_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* ring = smem + 2 * S::kTile;
+  uint8_t* ring = smem + kSlots * S::kTile;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // late causal tiles see the most keys: they start first
@@ -158,15 +170,15 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     h = blockIdx.y;
     slice = blockIdx.z;
   }
-  const int p_tile = tile * (kSplit ? pps : 2 * pps);    // first position
+  const int p_tile = tile * (kSplit ? pps : kSlots * pps);    // first position
   // r / group for r < 128: exact for groups below 512
   const int per_group = (65536 + a.group - 1) / a.group;
 
-  if (tid == 16 * 32) {
+  if (tid == S::kSoft) {
     mbar_init(&q_full, 1);
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], kSplit ? 1 : 2);
+      mbar_init(&kv_empty[s], kSplit ? 1 : kSlots);
     }
     for (int s = 0; s < 2; ++s) {
       for (int half = 0; half < 2; ++half) {
@@ -174,7 +186,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         mbar_init(&p_full[s][half], 4);
       }
     }
-    mbar_init(&drain_bar, 2);
+    mbar_init(&drain_bar, kSlots);
     for (int s = 0; s < 8; ++s) mbar_init(&pair_bar[s], 2);
     mbar_init(&turn[0], 1);
     mbar_init(&turn[1], 1);
@@ -183,7 +195,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     failed = drain_failed = 0;
     mbar_init_fence();
     // the queries need no key range: their loads go out at once
-    const int q_slots = kSplit ? 1 : 2;
+    const int q_slots = kSplit ? 1 : kSlots;
     mbar_arrive_expect_tx(&q_full, q_slots * S::kBoxes * pps * a.group * S::kRow);
     for (int s = 0; s < q_slots; ++s)
       for (int b = 0; b < S::kBoxes; ++b)
@@ -192,22 +204,22 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   }
   // the kernel that joins the slices may start as SMs fall free
   if (!kCausal) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  if (warp == 17) tmem_alloc(&tmem_slot, 512);
+  if (warp == kAux + 1) tmem_alloc(&tmem_slot, S::kColumns);
   // The offsets that can begin or end a sequence of this tile: all of them, or
-  // a window from the sequence of the first position on (found by a 32-way
-  // search: one round of loads per factor of 32, where a binary search per row
-  // would wait for one load per factor of 2).
+  // a window from the sequence of the first position on (found by a search of
+  // one round of loads per factor of 32, where a binary search per row would
+  // wait for one load per factor of 2).
   int window_at = 0, window_n = 0;
-  if (kCausal && warp < 16) {
+  if (kCausal && warp < kAux) {
     const int count = a.sequences + 1;
     if (count > GTC_WINDOW)
       window_at = max(0, offsets_up_to(a.offsets, count, p_tile) - 1);
     window_n = min(GTC_WINDOW, count - window_at);
-    for (int i = tid; i < window_n; i += 512) scratch[i] = __ldg(a.offsets + window_at + i);
+    for (int i = tid; i < window_n; i += S::kSoft) scratch[i] = __ldg(a.offsets + window_at + i);
   }
   __syncthreads();
   int begin = 0, end = 0, position = -1;
-  if (tid < 512) {
+  if (tid < S::kSoft) {
     const int slot = tid >> 8, r = tid & 127;
     const int p = p_tile + (kSplit ? 0 : slot * pps) + ((r * per_group) >> 16);
     if (r < pps * a.group && p < a.positions) position = p;
@@ -250,6 +262,11 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   int lo_key[2], hi_key[2], in_lo[2], in_hi[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
+    if (s >= kSlots) {
+      lo_key[s] = in_hi[s] = INT_MAX;
+      hi_key[s] = in_lo[s] = 0;
+      continue;
+    }
     const int4 w0 = spans[8 * s], w1 = spans[8 * s + 1], w2 = spans[8 * s + 2],
                w3 = spans[8 * s + 3];
     lo_key[s] = min(min(w0.x, w1.x), min(w2.x, w3.x));
@@ -279,9 +296,12 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const bool clear = end_row % 16 != 0;
   volatile int* gave_up = &failed;
 
-  if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
-    if (warp == 16) {
+  if (warp >= kAux) {
+    if (kSlots == 2)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
+    else
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 32;\n");
+    if (warp == kAux) {
       if (lane == 0) {                   // TMA producer
         // order of the ring: per block and stream V(j), K(j + 1)
         int g = 0;
@@ -324,7 +344,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         for (int s = 0; s < S::kStages; ++s)
           if (((armed >> s) & 1) && !gtc_wait(&kv_full[s], (phase >> s) & 1)) drain_failed = 1;
       }
-    } else if (warp != 18) {             // MMA issuer of one slot
+    } else if (warp == kAux + 1 || (kSlots == 2 && warp == kAux + 3)) {   // MMA issuer of a slot
       // A warp per slot: what it computes between two blocks runs under the
       // other slot's products.  The two issue in turn, which keeps the slots half
       // a period apart (without the turns they fall into step, both in their
@@ -334,7 +354,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       // the slot issues P V of its first 64 keys and the next scores for 64 keys,
       // then the same for the other 64: each half of the softmax warps waits for
       // its own half only.
-      const int s = warp == 17 ? 0 : 1;
+      const int s = warp == kAux + 1 ? 0 : 1;
       uint32_t elected;
       asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
                    : "=r"(elected));
@@ -349,7 +369,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                                         8 * S::kRow);
       const uint64_t k_desc = smem_desc(ring, S::kRow, 16, 8 * S::kRow);
       const uint64_t v_desc = smem_desc(ring, S::kRow, S::kBox, 8 * S::kRow);
-      const uint32_t t_s = tmem + s * GTC_KEYS, t_o = tmem + GTC_O + s * DP;
+      const uint32_t t_s = tmem + s * GTC_KEYS, t_o = tmem + S::kO + s * DP;
       int next = 0;                                     // ring stage and phase bit
       uint32_t ph = 0;
       bool ok = any0 || any1;
@@ -390,7 +410,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           if (ok && v_mine) ok = mbar_wait(&p_full[s][half], i & 1);
-          if (ok && half == 0) {         // this slot's turn of block j
+          if (kSlots == 2 && ok && half == 0) {   // this slot's turn of block j
             const int turns = j - lo + 1;
             if (s == 1)
               ok = mbar_wait(&turn[0], turns & 1);
@@ -444,7 +464,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       // no MMA may still use TMEM or shared memory when they are given back
       if (lead) mma_commit(&drain_bar);
       if (!mbar_wait(&drain_bar, 0)) drain_failed = 1;
-    } else if (kCausal && warp == 18 && clear) {
+    } else if (kCausal && warp == kAux + 2 && clear) {
       const int at = 1 + 2 * (hi - 1 - lo);   // its place in the ring
       // (the stream may still be a whole tile's work away from its last block)
       bool ok = false;
@@ -473,7 +493,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int all_to = slot == 0 ? in_hi[0] : in_hi[1];
     // this thread's half of the output columns, in runs of kCols
     constexpr int kCols = DP == 32 ? 16 : 32, kRuns = DP / 2 / kCols;
-    const uint32_t t_o = tmem + lanes + GTC_O + slot * DP + half * (DP / 2);
+    const uint32_t t_o = tmem + lanes + S::kO + slot * DP + half * (DP / 2);
     __nv_bfloat16* tops = reinterpret_cast<__nv_bfloat16*>(scratch + slot * 256);
     float* sums = reinterpret_cast<float*>(scratch + slot * 256);
     uint64_t* pair = &pair_bar[slot * 4 + quarter];
@@ -748,9 +768,9 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 17) {
+  if (warp == kAux + 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, S::kColumns);
   }
   if (tid == 0 && (failed || drain_failed)) set_status(a.status, GRS_ERR_TIMEOUT);
 }
@@ -802,7 +822,8 @@ bool gtc_rows_ok(const void* base, int64_t rows, int64_t st, int64_t heads, int6
 
 template <int DP, int MODE>
 int gtc_launch(const GroupedArgs<__nv_bfloat16>& args, cudaStream_t stream) {
-  using S = GtcShape<DP>;
+  constexpr int kSlots = gtc_slots(MODE);
+  using S = GtcShape<DP, kSlots>;
   GroupedArgs<__nv_bfloat16> a = args;
   const int pps = 128 / a.group;                        // positions of a slot
   const int cols = S::kRow / 2;
@@ -813,14 +834,13 @@ int gtc_launch(const GroupedArgs<__nv_bfloat16>& args, cudaStream_t stream) {
       !gtc_map(&k, a.k, a.keys, a.kv_heads, a.D, a.k_st, a.k_sh, cols, 1, GTC_KEYS) ||
       !gtc_map(&v, a.v, a.keys, a.kv_heads, a.D, a.v_st, a.v_sh, cols, 1, GTC_KEYS))
     return GRS_ERR_SHAPE;
-  const int64_t tiles = ((int64_t)a.positions + pps * (MODE == GTC_SPLIT ? 1 : 2) - 1) /
-                        (pps * (MODE == GTC_SPLIT ? 1 : 2));
-  if (tiles * a.kv_heads > INT_MAX || (MODE != GTC_CAUSAL && (a.kv_heads > 65535 ||
-                                                              a.slices > 65535)))
+  constexpr bool kCausal = MODE == GTC_CAUSAL || MODE == GTC_SINGLE;
+  const int step = pps * (MODE == GTC_SPLIT ? 1 : kSlots);
+  const int64_t tiles = ((int64_t)a.positions + step - 1) / step;
+  if (tiles * a.kv_heads > INT_MAX || (!kCausal && (a.kv_heads > 65535 || a.slices > 65535)))
     return GRS_ERR_SHAPE;
-  const dim3 grid = MODE == GTC_CAUSAL
-                        ? dim3((unsigned)(tiles * a.kv_heads))
-                        : dim3((unsigned)tiles, a.kv_heads, a.slices);
+  const dim3 grid = kCausal ? dim3((unsigned)(tiles * a.kv_heads))
+                            : dim3((unsigned)tiles, a.kv_heads, a.slices);
   // the tiles start at the first 1024-byte boundary behind the static variables
   static std::atomic<int> smem_of[64];
   int dev = 0;
@@ -832,13 +852,13 @@ int gtc_launch(const GroupedArgs<__nv_bfloat16>& args, cudaStream_t stream) {
       return GRS_ERR_CUDA;
     const int fixed = (int)fa.sharedSizeBytes;
     smem = (fixed + 1023) / 1024 * 1024 - fixed + S::kTiles +
-           (MODE != GTC_CAUSAL && !S::kStageFree ? 16 * 2048 : 0);
+           (!kCausal && !S::kStageFree ? 16 * 2048 : 0);
     if (cudaFuncSetAttribute(grouped_tc_kernel<DP, MODE>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return GRS_ERR_CUDA;
     smem_of[dev].store(smem, std::memory_order_release);
   }
-  grouped_tc_kernel<DP, MODE><<<grid, GTC_THREADS, smem, counted(stream)>>>(q, k, v, a, pps);
+  grouped_tc_kernel<DP, MODE><<<grid, S::kThreads, smem, counted(stream)>>>(q, k, v, a, pps);
   GRS_CUDA_CHECK_LAUNCH();
   return GRS_OK;
 }
@@ -861,7 +881,16 @@ bool grouped_tc_takes(const GroupedArgs<__nv_bfloat16>& a) {
 }
 
 int grouped_tc_launch(const GroupedArgs<__nv_bfloat16>& a, cudaStream_t stream) {
-  if (a.offsets) return gtc_width<GTC_CAUSAL>(a, stream);
+  if (a.offsets) {
+    // One slot per CTA where pairs would leave SMs without work (one prompt of
+    // 512 tokens, 32/8 heads: 18.8 -> 13.3 us) or hold mostly different
+    // sequences (500 prompts of up to 64: 60 -> 55 us); pairs read K and V half as
+    // often (8 x 1024 tokens: 106 against 119 us).
+    const int pps = 128 / a.group;
+    const int64_t pairs = ((int64_t)a.positions + 2 * pps - 1) / (2 * pps) * a.kv_heads;
+    return pairs < 148 || (int64_t)a.positions < 128ll * a.sequences
+               ? gtc_width<GTC_SINGLE>(a, stream) : gtc_width<GTC_CAUSAL>(a, stream);
+  }
   return grouped_tc_split(a.positions, a.group) ? gtc_width<GTC_SPLIT>(a, stream)
                                                 : gtc_width<GTC_PAIR>(a, stream);
 }

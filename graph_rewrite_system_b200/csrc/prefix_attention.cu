@@ -213,7 +213,7 @@ static int pages_rows_launch(const PagesArgs<T>& p, cudaStream_t stream) {
 // columns, with two 8 x 8 transposes of the weights in between: half the
 // instructions, accumulators and query registers.  The warps' sums meet in shared memory and are joined there with
 // the prefix slices; only that join waits for the prefix kernel.
-constexpr int PG_HEADS = 16, PG_BESIDE = 148;
+constexpr int PG_HEADS = 16;
 
 __device__ __forceinline__ void pg_mma(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -296,6 +296,7 @@ __global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16>
   const int head0 = h * a.group + blockIdx.x % chunks * PG_HEADS;
   const int n_heads = min(PG_HEADS, (h + 1) * a.group - head0);
 
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   constexpr int rows = kFew ? 8 : PG_HEADS;
   // query fragments: heads g and g + 8 (or g alone), pieces t, t + 4, ...
   uint32_t qa[2 * S::kKey][kFew ? 2 : 4];
@@ -645,6 +646,7 @@ __global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16>
 // The join alone: `team` (1 or 4) of a CTA's four warps per (beam, head).
 __global__ void __launch_bounds__(128) join_parts_kernel(PagesArgs<__nv_bfloat16> a, int parts,
                                                          int team) {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");   // launched under the pages kernel
   __shared__ float4 xs[4][32];
   __shared__ float norms[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -696,7 +698,8 @@ static PrefixPlan rows_plan(int batch, int group, int kv_heads, int D, int keys)
 
 // Tensor cores: the count whose waves of 148 CTAs take the fewest 128-key
 // blocks, each wave paying about four blocks for its start and end and every
-// part the write and read of its fp32 sums (a block takes about 1.1 us).
+// part the write and read of its fp32 sums, mostly in L2 (a block takes about
+// 1.1 us).
 static PrefixPlan tc_plan(int batch, int heads, int kv_heads, int D, int keys) {
   if (keys <= 0) return {0, 0, 0};
   const int group = heads / kv_heads;
@@ -705,7 +708,7 @@ static PrefixPlan tc_plan(int batch, int heads, int kv_heads, int D, int keys) {
   const int64_t tiles = ((int64_t)batch + pps - 1) / pps * kv_heads;
   // slots of a split slice take turns on half the blocks each
   const int blocks = (keys + 127) / 128, per = split ? 2 : 1;
-  const double join = 8.0 * batch * heads * D / 6.5e12 / 1.1e-6 + 0.02;
+  const double join = 3.0 * batch * heads * D / 6.5e12 / 1.1e-6 + 0.02;
   double best = 1e30;
   int slices = 1;
   for (int z = 1; z <= std::min(64, (blocks + per - 1) / per); ++z) {
@@ -724,9 +727,11 @@ static PrefixPlan tc_plan(int batch, int heads, int kv_heads, int D, int keys) {
 
 // Slices of each beam's pages: enough CTAs of a long table to fill 148 SMs
 // four times when there are few beams, none for less than 256 tokens.  They are
-// joined by a kernel of its own when they are cut, or when there are more CTAs
-// than fit beside the prefix kernel: CTAs that wait for it to join would keep
-// the SMs it leaves free from the rest.
+// joined by a kernel of its own when they are cut, or when there are so many
+// CTAs that those which wait for the prefix kernel to join it would keep the
+// rest from the SMs it leaves free (512 beams x 8 K/V heads over 16384 keys: 179
+// -> 168 us; 200 x 8 over 2048 keys: 39 against 41 us, so not there).
+constexpr int PG_BESIDE = 2048;
 struct PagesPlan {
   int slices;
   bool separate;
@@ -783,8 +788,13 @@ static int pages_mma_run(const PagesArgs<__nv_bfloat16>& p, int page_slices, boo
     const int parts = p.slices + page_slices, team = parts > 8 ? 4 : 1;
     const int64_t n = (int64_t)p.batch * p.heads;
     if (n > INT_MAX) return GRS_ERR_SHAPE;
-    join_parts_kernel<<<(unsigned)((n + 4 / team - 1) / (4 / team)), 128, 0, counted(stream)>>>(
-        p, parts, team);
+    config.gridDim = dim3((unsigned)((n + 4 / team - 1) / (4 / team)));
+    config.blockDim = dim3(128);
+    config.dynamicSmemBytes = 0;
+    config.stream = counted(stream);
+    config.numAttrs = 1;
+    if (cudaLaunchKernelEx(&config, join_parts_kernel, p, parts, team) != cudaSuccess)
+      return GRS_ERR_CUDA;
   }
   GRS_CUDA_CHECK_LAUNCH();
   return GRS_OK;
