@@ -600,6 +600,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const __nv_bfloat16 mine16 = __float2bfloat16_ru(scores(i, dead));
       __nv_bfloat16* at = tops + (i & 1) * 256 + r;
       at[half * 128] = mine16;
+      tc_fence_before();
       tell();
       // The weights are taken against the maximum so far; the partner's part of
       // this block's maximum is read behind them.  Only where the maximum has
@@ -619,6 +620,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       } else if (__any_sync(0xffffffffu, grown)) {
         // Both threads of the row are here with their scores of this block, so
         // every product into O is done, and none starts before both are through.
+        tc_fence_after();
         if (grown) m = top;
         const float keep = grown ? gtc_exp2((before - m) * c) : 1.f;
         l *= keep;
@@ -651,7 +653,10 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[slot][half]);
     }
-    if (ok && blocks > 0) ok = mbar_wait_warp(&s_full[slot][half], blocks & 1);
+    // the slot's last products are done; without any, its queries have landed
+    // (the outputs are staged over them)
+    if (ok) ok = blocks > 0 ? mbar_wait_warp(&s_full[slot][half], blocks & 1)
+                            : mbar_wait_warp(&q_full, 0);
     tc_fence_after();
     // every warp of the slot has stored its last weights, so the maxima are read
     sums[half * 128 + r] = l;

@@ -121,6 +121,27 @@ def test_rows_behind_the_last_sequence(cuda_device, dtype):
     _check(out, clean, offsets)
 
 
+@pytest.mark.parametrize("width", [32, 64, 128])
+@pytest.mark.parametrize("sequences", [0, 1, 40])
+def test_long_tails(cuda_device, width, sequences):
+    """Whole tiles behind the last sequence, holding NaN, many times over: the
+    rows are zero in a new output and untouched in a given one."""
+    from graph_rewrite_system_b200.prompt_attention import prompt_attention
+
+    offsets = _offsets([70] * sequences)
+    base = torch.cat(_inputs(16, offsets[-1] + 3000, 8, 2, width, BF16), 1).to(cuda_device)
+    base[offsets[-1]:] = float("nan")
+    q, k, v = base.split([8, 2, 2], 1)
+    off = torch.tensor(offsets, dtype=torch.int32, device=cuda_device)
+    first = prompt_attention(q, k, v, off)
+    out = torch.full_like(first, 3.0)
+    for _ in range(20):
+        assert torch.equal(prompt_attention(q, k, v, off), first)
+        prompt_attention(q, k, v, off, out=out)
+    assert not first[offsets[-1]:].any() and torch.isfinite(first).all()
+    assert (out[offsets[-1]:] == 3).all() and torch.equal(out[:offsets[-1]], first[:offsets[-1]])
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_bad_values_reach_only_rows_that_see_them(cuda_device, dtype, bad):
