@@ -3,9 +3,11 @@
 // 128, groups above 128, unaligned rows, negative scales).
 //
 // One CTA takes 128 rows of one K/V head (64 at widths above 128) and walks
-// 64-key tiles; a thread holds 8 rows x 4 keys of the scores and 8 rows x DP/16
-// columns of the output.  Both products read 16-byte vectors from shared memory
-// (12 for 128 multiply-adds, 16 for 256 at DP = 128) into packed fp32x2
+// 64-key tiles; a thread holds 4 rows x 4 keys of the scores and 4 rows x DP/16
+// columns of the output, so that 16 warps hide the latencies of shared memory
+// (8 rows a thread read less of it, but with 8 warps took 1.2 to 1.6 times as
+// long).  Both products read 16-byte vectors from shared memory (8 for 64
+// multiply-adds, 12 for 128 at DP = 128) into packed fp32x2
 // multiply-adds: the scores sum even and odd dimensions apart, so both factors
 // are pairs as they lie.  The next K tile is fetched (cp.async) under the value
 // product and the next V tile under the scores, in one buffer each.  The
@@ -21,12 +23,13 @@
 namespace grs {
 
 constexpr int GA_KEYS = 64, GA_PS = GA_KEYS + 4;
+constexpr int GA_I = 4;                                // rows of a thread
 
 template <int DP>
 struct GaShape {
   static constexpr int kRows = DP <= 128 ? 128 : 64;
-  static constexpr int kThreads = 2 * kRows;           // 16 threads for 8 rows
-  static constexpr int kRowStep = kRows / 8;           // thread rows: rg + kRowStep i
+  static constexpr int kThreads = 16 * kRows / GA_I;   // 16 threads for GA_I rows
+  static constexpr int kRowStep = kRows / GA_I;        // thread rows: rg + kRowStep i
   static constexpr int kQS = DP + 4;                   // padded row strides (floats)
   static constexpr int kSmem = (kRows * kQS + GA_KEYS * kQS + GA_KEYS * DP + kRows * GA_PS) * 4;
 };
@@ -68,7 +71,7 @@ __device__ __forceinline__ void ga_load(float* dst, const T* src, int64_t st, in
 }
 
 template <typename T, int DP, bool kCausal, bool kAsync>
-__global__ void __launch_bounds__(GaShape<DP>::kThreads, DP == 32 ? 2 : 1)
+__global__ void __launch_bounds__(GaShape<DP>::kThreads, 1)
 grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
   using S = GaShape<DP>;
   extern __shared__ __align__(16) float ga_smem_raw[];
@@ -131,10 +134,10 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
     qs[r * S::kQS + d] = x * a.scale_log2;
   }
 
-  float2 acc[8][kPairs];
-  float m[8], l[8];
+  float2 acc[GA_I][kPairs];
+  float m[GA_I], l[GA_I];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < GA_I; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
@@ -144,11 +147,11 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
   for (int t0 = first; t0 < last; t0 += GA_KEYS) {
     ga_wait<1>();                           // K is here; V may be on its way
     __syncthreads();
-    float s[8][4];
+    float s[GA_I][4];
     {
-      float2 s2[8][4];
+      float2 s2[GA_I][4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < GA_I; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 2
@@ -158,7 +161,7 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
         for (int j = 0; j < 4; ++j)
           k4[j] = *reinterpret_cast<const float4*>(ks + (cg + 16 * j) * S::kQS + d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < GA_I; ++i) {
           const float4 q4 = *reinterpret_cast<const float4*>(qs + (rg + S::kRowStep * i) * S::kQS + d);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -168,7 +171,7 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < GA_I; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
     }
@@ -176,7 +179,7 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
     ga_load<T, DP, S::kQS, kAsync>(ks, kh, a.k_st, a.D, t0 + GA_KEYS, last);
     if (t0 < all_from || t0 + GA_KEYS > all_to) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < GA_I; ++i) {
         const int from = row_begin[rg + S::kRowStep * i] - t0, to = row_end[rg + S::kRowStep * i] - t0;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -184,7 +187,7 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < GA_I; ++i) {
       float top = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -209,9 +212,9 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
     __syncthreads();
 #pragma unroll 1
     for (int t = 0; t < GA_KEYS; t += 4) {
-      float4 p4[8];
+      float4 p4[GA_I];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < GA_I; ++i)
         p4[i] = *reinterpret_cast<const float4*>(ps + (rg + S::kRowStep * i) * GA_PS + t);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -227,7 +230,7 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
           }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < GA_I; ++i) {
           const float w = k == 0 ? p4[i].x : k == 1 ? p4[i].y : k == 2 ? p4[i].z : p4[i].w;
 #pragma unroll
           for (int j = 0; j < kPairs; ++j) acc[i][j] = __ffma2_rn(make_float2(w, w), v2[j], acc[i][j]);
@@ -239,9 +242,9 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
   }
   ga_wait<0>();
 
-  unsigned again = 0;                       // rows (of 8) whose result is not finite
+  unsigned again = 0;                       // rows (of GA_I) whose result is not finite
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < GA_I; ++i) {
     float sum = l[i];
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
