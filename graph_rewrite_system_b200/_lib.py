@@ -163,6 +163,12 @@ def words_of(name: str) -> struct.Struct:
     return struct.Struct("=" + "".join(codes.get(t, "q") for t in _SIGNATURES[name][1]))
 
 
+def words_entry(name: str):
+    """The ``_words`` form of entry point `name`, called with its packed table
+    and nothing in between."""
+    return getattr(lib().handle, name + "_words")
+
+
 def current_device() -> int:
     """Index of the current device (the library launches on it)."""
     return torch._C._cuda_getDevice()

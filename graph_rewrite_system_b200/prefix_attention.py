@@ -17,9 +17,11 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from .prompt_attention import _check_heads, _check_scale, _out_rows, _rows, _status_for
+from .prompt_attention import (_STATUS_AT, _check_heads, _check_scale, _out_rows, _rows,
+                               _status_for)
 
-_WORDS = _lib.words_of("grs_shared_prefix_attention").pack
+_pack = _lib.words_of("grs_shared_prefix_attention").pack
+_entry = None
 
 
 @lru_cache(maxsize=4096)
@@ -61,6 +63,7 @@ def shared_prefix_attention(
     ``check_decode_status`` reads).  ``out`` must not overlap the inputs.  The
     call does not synchronise and can be captured into a CUDA graph.
     """
+    global _entry
     device = query.get_device()
     if device < 0:
         _lib.require_cuda(query)
@@ -138,13 +141,17 @@ def shared_prefix_attention(
                       value_cache, current_key, current_value)
     if not batch:
         return out
-    word = _status_for(query, status)
+    word = None if status is not None else _STATUS_AT.get(device)
+    if word is None:
+        word = _status_for(query, device, status)
+    if _entry is None:
+        _entry = _lib.words_entry("grs_shared_prefix_attention")
     stream = _lib.stream_on(device)
     work, need = 0, _workspace_bytes(batch, heads, kv_heads, width, num_prefix, columns * page)
     if need:
         scratch = _lib.scratch(query, need, stream)
         work = scratch.data_ptr()
-    code = _lib.lib().grs_shared_prefix_attention_words(_WORDS(
+    code = _entry(_pack(
         code, query.data_ptr(), q[0], q[1], prefix_key.data_ptr(), pk[0], pk[1],
         prefix_value.data_ptr(), pv[0], pv[1], num_prefix, keys, values, c[0], c[1], c[2], table,
         table_row, columns, past, pages, page, cur_key, cur_value, cur[0], cur[1], valid,

@@ -19,15 +19,17 @@ import torch
 from . import _lib
 from .paged_attention import _STATUS, _status_word
 
-_WORDS = _lib.words_of("grs_prompt_attention").pack
+_pack = _lib.words_of("grs_prompt_attention").pack
+_entry = None
+_STATUS_AT: dict[int, int] = {}          # device index -> address of its status word
 
 
-def _status_for(query: torch.Tensor, status: torch.Tensor | None) -> int:
+def _status_for(query: torch.Tensor, device: int, status: torch.Tensor | None) -> int:
     """Address of the caller's status word, or of the device's
     (``check_decode_status``)."""
     if status is not None:
         if (status.dtype is not torch.int32 or status.numel() != 1
-                or status.get_device() != query.get_device()):
+                or status.get_device() != device):
             _lib.require_cuda(status)
             raise ValueError("status must be one int32 on the query's device")
         return status.data_ptr()
@@ -37,7 +39,8 @@ def _status_for(query: torch.Tensor, status: torch.Tensor | None) -> int:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("make one call before capturing the first, or pass status=")
         word = _status_word(query.device)
-    return word.data_ptr()
+    _STATUS_AT[device] = word.data_ptr()     # the word lives as long as the process
+    return _STATUS_AT[device]
 
 
 def _refuse(name: str, t: torch.Tensor, device: int, dtype: torch.dtype, shape: tuple) -> None:
@@ -117,6 +120,7 @@ def prompt_attention(
     inputs.  The call neither synchronises nor reads ``offsets`` on the host,
     so it can be captured into a CUDA graph.
     """
+    global _entry
     device = query.get_device()
     if device < 0:
         _lib.require_cuda(query)
@@ -146,11 +150,15 @@ def prompt_attention(
         o = _out_rows(out, device, dtype, shape, query, key, value)
     if not tokens:
         return out
-    word = _status_for(query, status)
-    status = _lib.lib().grs_prompt_attention_words(_WORDS(
+    word = None if status is not None else _STATUS_AT.get(device)
+    if word is None:
+        word = _status_for(query, device, status)
+    if _entry is None:
+        _entry = _lib.words_entry("grs_prompt_attention")
+    code = _entry(_pack(
         code, query.data_ptr(), q[0], q[1], key.data_ptr(), k[0], k[1], value.data_ptr(), v[0],
         v[1], offsets.data_ptr(), offsets.numel() - 1, out.data_ptr(), o[0], o[1], tokens, heads,
-        kv_heads, width, scale, int(fresh), word, _lib.stream_on(device)))
-    if status:
-        _lib.check(status, "prompt attention")
+        kv_heads, width, scale, fresh, word, _lib.stream_on(device)))
+    if code:
+        _lib.check(code, "prompt attention")
     return out

@@ -12,7 +12,8 @@ import torch
 
 from . import _lib
 
-_WORDS = _lib.words_of("grs_adjust_logits").pack
+_pack = _lib.words_of("grs_adjust_logits").pack
+_entry = None
 
 
 def _ints(name: str, t: torch.Tensor | None, rows: int, device: int) -> int:
@@ -79,6 +80,7 @@ def adjust_logits(
     nothing is all ``fill``.  repetition (> 0), presence and frequency are
     numbers or fp32 [rows].  Computed in fp32 and rounded once.
     """
+    global _entry
     device = logits.get_device()
     if device < 0:
         _lib.require_cuda(logits)
@@ -136,7 +138,9 @@ def adjust_logits(
             raise ValueError("out must be the logits themselves or not overlap them")
     if not rows or not vocab:
         return out
-    status = _lib.lib().grs_adjust_logits_words(_WORDS(
+    if _entry is None:
+        _entry = _lib.words_entry("grs_adjust_logits")
+    status = _entry(_pack(
         code, logits.data_ptr(), row, out.data_ptr(), out_row, rows, vocab, token_ptr, wide,
         tokens_row, history, lengths_ptr, prompts_ptr, rep_ptr, pres_ptr, freq_ptr, rep, pres,
         freq, bias_ptr, bias_row, allowed_ptr, allowed_row, float(fill),

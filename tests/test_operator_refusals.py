@@ -17,6 +17,7 @@ def lifted(monkeypatch):
     monkeypatch.setattr(_lib, "require_cuda", lambda *t: None)
     monkeypatch.setattr(_lib, "current_device", lambda: -1)
     monkeypatch.setattr(_lib, "lib", nothing)
+    monkeypatch.setattr(_lib, "stream_on", nothing)
 
 
 def _z(*shape, dtype=torch.bfloat16):
