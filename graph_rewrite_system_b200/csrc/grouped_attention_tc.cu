@@ -45,7 +45,6 @@
 namespace grs {
 
 constexpr int GTC_KEYS = 128;
-constexpr int GTC_EMULATE = 4;              // one pair in four takes gtc_exp2_pair
 constexpr int GTC_WINDOW = 260;             // offsets held for a tile's rows
 
 template <int DP, int kSlots>
@@ -76,22 +75,6 @@ __device__ __forceinline__ float gtc_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
-}
-// 2^x of a pair on the multiply-add pipes: x = n + f with n = floor(x) taken by
-// adding 1.5 * 2^23 rounded down, 2^f on [0, 1) by the cubic of least largest
-// relative error (8.6e-5 = 2^-13.5, a thirtieth of the weights' rounding to
-// bf16) among those that are 1 at 0, n added to the exponent bits.  x is cut
-// at -127, where that gives exactly 0, so masked scores (-inf) weigh nothing.
-__device__ __forceinline__ float2 gtc_exp2_pair(float2 x) {
-  const auto both = [](float v) { return make_float2(v, v); };
-  x = make_float2(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
-  const float2 t = __fadd2_rd(x, both(12582912.f));
-  const float2 f = __ffma2_rn(__fadd2_rn(t, both(-12582912.f)), both(-1.f), x);
-  float2 p = __ffma2_rn(both(0.07706641f), f, both(0.22764569f));
-  p = __ffma2_rn(p, f, both(0.69511663f));
-  p = __ffma2_rn(p, f, both(1.f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 __device__ __forceinline__ float gtc_max3(float x, float y, float z) {
   float m;
@@ -554,13 +537,8 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          float2 x = make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-          if (j % GTC_EMULATE == 1)
-            x = gtc_exp2_pair(x);
-          else
-            x = make_float2(gtc_exp2(x.x), gtc_exp2(x.y));
-          v[2 * j] = __float_as_uint(x.x);
-          v[2 * j + 1] = __float_as_uint(x.y);
+          v[2 * j] = __float_as_uint(gtc_exp2(__uint_as_float(v[2 * j])));
+          v[2 * j + 1] = __float_as_uint(gtc_exp2(__uint_as_float(v[2 * j + 1])));
         }
       };
       const auto pack = [&](int g) {

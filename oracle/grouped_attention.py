@@ -81,8 +81,7 @@ def attention_bound(out, spread, reach, dtype, width, keys):
     (bf16 products are exact, fp32 ones round) are off by (width + 4) 2^-24
     times the row's sum of |q k scale|, in a natural exponent; the running
     maximum subtracts exactly up to one more such term.  Exponential: 2^-21
-    relative in fp32; the bf16 kernels round the weights to bf16 (2^-8) and may
-    take 2^-13 for an exponential that is rounded so.  Sums over `keys` weights
+    relative; the bf16 kernels round the weights to bf16 (2^-8).  Sums over `keys` weights
     in fp32: keys 2^-24 in the numerator and in the denominator, on partial
     sums no larger than the absolute sums.  The output rounds once (2^-8 or
     2^-24)."""
@@ -90,7 +89,7 @@ def attention_bound(out, spread, reach, dtype, width, keys):
     weight = 2 * (width + 5) * 2.0 ** -24 * reach[..., None] + 2 * 2.0 ** -21 \
         + 2 * (keys + 8) * 2.0 ** -24
     if dtype == torch.bfloat16:
-        weight = weight + 2.0 ** -8 + 2 * 2.0 ** -13
+        weight = weight + 2.0 ** -8
     return 1.01 * (weight * spread + half * out.abs()) + 1e-30
 
 
