@@ -185,6 +185,20 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tma_load_3d(smem + s * S::kTile + b * S::kBox, &tm_q, b * 64, h * a.group,
                     p_tile + s * pps, &q_full);
   }
+  // So does the first K block of a causal tile whose first position lies in a
+  // sequence: it begins with that sequence, whatever the other rows see.
+  bool k_sent = false;
+  if (kCausal && warp == kAux) {
+    const int n = offsets_up_to(a.offsets, a.sequences + 1, p_tile);
+    k_sent = n > 0 && n <= a.sequences;
+    if (k_sent && lane == 0) {
+      const int key = min(max(__ldg(a.offsets + n - 1), 0), p_tile);
+      mbar_arrive_expect_tx(&kv_full[0], S::kTile);
+      for (int b = 0; b < S::kBoxes; ++b)
+        tma_load_3d(ring + b * S::kBox, &tm_k, b * 64, h, key, &kv_full[0]);
+    }
+    __syncwarp();
+  }
   // the kernel that joins the slices may start as SMs fall free
   if (!kCausal) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   if (warp == kAux + 1) tmem_alloc(&tmem_slot, S::kColumns);
@@ -287,8 +301,8 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     if (warp == kAux) {
       if (lane == 0) {                   // TMA producer
         // order of the ring: per block and stream V(j), K(j + 1)
-        int g = 0;
-        unsigned armed = 0;              // stages with a load, their last phase in `phase`
+        int g = k_sent ? 1 : 0;
+        unsigned armed = k_sent ? 1 : 0; // stages with a load, their last phase in `phase`
         unsigned phase = 0;
         bool last_armed = false;
 #pragma unroll 1
@@ -297,7 +311,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           const int s = kSplit ? (n >> 1) & 1 : 0, is_k = n & 1;
           const int j = lo - 1 + (kSplit ? n >> 2 : n >> 1) + is_k;
           const int end_j = kSplit ? (s ? last[1] : last[0]) : hi;
-          if (j < lo || j >= end_j) continue;
+          if (j < lo || j >= end_j || (k_sent && j == lo && is_k)) continue;
           const int st = g % S::kStages, r = g / S::kStages;
           if (*gave_up) break;
           if (r > 0 && !gtc_wait(&kv_empty[st], (r - 1) & 1)) {
