@@ -709,16 +709,20 @@ static PrefixPlan tc_plan(int batch, int heads, int kv_heads, int D, int keys) {
   // slots of a split slice take turns on half the blocks each
   const int blocks = (keys + 127) / 128, per = split ? 2 : 1;
   const double join = 3.0 * batch * heads * D / 6.5e12 / 1.1e-6 + 0.02;
+  const int most = std::min(64, (blocks + per - 1) / per);
+  const int64_t least_waves = (tiles + 147) / 148;
   double best = 1e30;
   int slices = 1;
-  for (int z = 1; z <= std::min(64, (blocks + per - 1) / per); ++z) {
-    const int64_t waves = (tiles * z + 147) / 148;
-    const int64_t each = ((blocks + z - 1) / z + per - 1) / per;
-    const double cost = (double)waves * (each + 4) + join * z * per;
+  for (int64_t waves = least_waves; waves < least_waves + 8; ++waves) {
+    // as many slices as these waves hold, then as few as give the same length
+    int z = (int)std::min<int64_t>(148 * waves / tiles, most);
+    const int each = ((blocks + z - 1) / z + per - 1) / per;
+    const double cost = (double)waves * (each + 4) + join * per * ((blocks + each * per - 1) / (each * per));
     if (cost < best) {
       best = cost;
-      slices = z;
+      slices = (blocks + each * per - 1) / (each * per);
     }
+    if (z == most) break;
   }
   const int each = (blocks + slices - 1) / slices;
   slices = (blocks + each - 1) / each;

@@ -78,8 +78,12 @@ def shared_prefix_attention(
     shape = query.shape
     batch, heads, width = shape
     num_prefix, kv_heads, _ = prefix_key.shape
+    if batch >= 1 << 30 or num_prefix >= 1 << 30:
+        raise ValueError("at most 2^30 beams and prefix keys")
     code, dtype = _check_heads(query, heads, kv_heads, width), query.dtype
-    q = _rows("query", query, device, dtype, shape)
+    q = query.stride()
+    if q[2] != 1 and width > 1:
+        raise ValueError("query needs a contiguous head width")
     pk = _rows("prefix_key", prefix_key, device, dtype, (num_prefix, kv_heads, width))
     pv = _rows("prefix_value", prefix_value, device, dtype, (num_prefix, kv_heads, width))
 
@@ -108,7 +112,7 @@ def shared_prefix_attention(
                 or not lengths.is_contiguous() or lengths.get_device() != device):
             _lib.require_cuda(lengths)
             raise ValueError("lengths must be contiguous int32 [batch] on the query's device")
-        if columns * page >= 1 << 30:
+        if columns * page >= 1 << 30 or pages >= 1 << 31 or columns >= 1 << 30 or page >= 1 << 30:
             raise ValueError("a block table row holds at most 2^30 tokens")
         columns = columns if page else 0
         keys, values = key_cache.data_ptr(), value_cache.data_ptr()

@@ -133,8 +133,12 @@ def prompt_attention(
     shape = query.shape
     tokens, heads, width = shape
     kv_heads = key.shape[1]
+    if tokens >= 1 << 30:
+        raise ValueError("at most 2^30 tokens")
     code, dtype = _check_heads(query, heads, kv_heads, width), query.dtype
-    q = _rows("query", query, device, dtype, shape)
+    q = query.stride()
+    if q[2] != 1 and width > 1:
+        raise ValueError("query needs a contiguous head width")
     k = _rows("key", key, device, dtype, (tokens, kv_heads, width))
     v = _rows("value", value, device, dtype, (tokens, kv_heads, width))
     if (offsets.dtype is not torch.int32 or offsets.dim() != 1 or not offsets.numel()

@@ -66,7 +66,8 @@ def adjust_logits(
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Adjusted copy of logits [rows, vocab] (bf16 or fp32, contiguous rows),
-    or ``out`` (``out=logits`` adjusts in place).
+    or ``out`` (``out=logits`` adjusts in place; otherwise it must not overlap
+    them).
 
     For every token v of row b, in this order: if v is among the first
     ``lengths[b]`` (default: all) of ``tokens[b]`` (int32 or int64 [rows,
@@ -95,6 +96,8 @@ def adjust_logits(
     if code is None or logits.dim() != 2:
         raise ValueError("logits must be bf16 or fp32 [rows, vocab]")
     rows, vocab = logits.shape
+    if rows >= 1 << 30 or vocab >= 1 << 30:
+        raise ValueError("at most 2^30 rows and columns")
     row, step = logits.stride()
     if vocab > 1 and step != 1:
         raise ValueError("logits need contiguous rows")
@@ -107,6 +110,8 @@ def adjust_logits(
             _lib.require_cuda(tokens)
             raise ValueError("tokens must be int32 or int64 [rows, history], contiguous rows")
         history, tokens_row = tokens.shape[1], tokens.stride(0)
+        if history >= 1 << 30:
+            raise ValueError("histories hold at most 2^30 tokens")
         wide, token_ptr = int(tokens.dtype is torch.int64), tokens.data_ptr()
     elif lengths is not None or prompt_lengths is not None:
         raise ValueError("lengths and prompt_lengths come with tokens")

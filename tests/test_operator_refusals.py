@@ -33,6 +33,8 @@ PROMPT = dict(query=_z(6, 4, 32), key=_z(6, 2, 32), value=_z(6, 2, 32), offsets=
 
 @pytest.mark.parametrize("change", [
     dict(query=_z(6, 4, 32, dtype=torch.float16)), dict(query=_z(6, 4, 32, dtype=torch.float32)),
+    dict(query=_z(1, 4, 32).expand(1 << 30, 4, 32), key=_z(1, 2, 32).expand(1 << 30, 2, 32),
+         value=_z(1, 2, 32).expand(1 << 30, 2, 32)),
     dict(query=_z(6, 3, 32)), dict(query=_z(6, 4, 1, 32)), dict(query=_z(6, 4, 300),
                                                                 key=_z(6, 2, 300),
                                                                 value=_z(6, 2, 300)),
@@ -86,6 +88,8 @@ PREFIX = dict(query=_z(3, 4, 32), prefix_key=_z(9, 2, 32), prefix_value=_z(9, 2,
     dict(current_valid=torch.ones(3)), dict(current_valid=torch.ones(2, dtype=torch.bool)),
     dict(scale=float("nan")), dict(out=_z(3, 4, 33)), dict(out=PREFIX["query"]), dict(out=_z(3, 1, 32).expand(3, 4, 32)),
     dict(block_table=torch.zeros(3, 1, dtype=torch.int32).expand(3, 1 << 27)),
+    dict(prefix_key=_z(1, 2, 32).expand(1 << 30, 2, 32),
+         prefix_value=_z(1, 2, 32).expand(1 << 30, 2, 32)),
 ])
 def test_prefix_refusals(lifted, change):
     from graph_rewrite_system_b200.prefix_attention import shared_prefix_attention
@@ -100,6 +104,7 @@ LOGITS = dict(logits=torch.zeros(3, 70), tokens=torch.zeros(3, 5, dtype=torch.in
 @pytest.mark.parametrize("change", [
     dict(logits=torch.zeros(3, 70, dtype=torch.float16)), dict(logits=torch.zeros(70)),
     dict(logits=torch.zeros(70, 3).T), dict(tokens=torch.zeros(3, 5)),
+    dict(tokens=torch.zeros(3, 1, dtype=torch.int32).expand(3, 1 << 30)),
     dict(tokens=torch.zeros(2, 5, dtype=torch.int32)),
     dict(tokens=torch.zeros(5, 3, dtype=torch.int32).T),
     dict(lengths=torch.zeros(3, dtype=torch.int64)),

@@ -49,6 +49,8 @@ LENGTHS = {
     "one": [1], "pair": [1, 1], "tile": [128], "tile+1": [129], "two tiles": [256],
     "odd": [37], "empties": [0, 5, 0, 0, 1, 130, 0], "mixed": [127, 1, 300, 64, 2],
     "many": [3, 17, 1, 9, 0, 31, 33, 2, 64, 5] * 6, "long": [700],
+    "hundreds empty": [5] + [0] * 700 + [70, 0, 3], "all empty between": ([0] * 300 + [9]) * 3,
+    "thousands": [1, 0, 2] * 900,
 }
 
 
