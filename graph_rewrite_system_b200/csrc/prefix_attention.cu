@@ -1,11 +1,12 @@
 // One query per beam against a prefix that every beam shares and against the
 // beam's own pages: grs_shared_prefix_attention.
 //
-// The prefix is attention of beams * group rows per K/V head to the same keys,
-// so its K/V are read once per tile of rows instead of once per beam; it is cut
-// into slices when the tiles alone would leave SMs idle.  Each slice leaves its
-// normalised fp32 sum and log2 weight in the workspace; the pages kernel adds
-// the beam's own keys, joins all parts by their weights and writes the output.
+// A long prefix is attention of beams * group rows per K/V head to the same
+// keys, so its K/V are read once per tile of rows instead of once per beam; it
+// is cut into slices when the tiles alone would leave SMs idle.  Each slice
+// leaves its normalised fp32 sum and log2 weight in the workspace; the pages
+// kernel adds the beam's own keys, joins all parts by their weights and writes
+// the output.  A short prefix is read by the pages kernel itself.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -18,6 +19,8 @@ namespace grs {
 template <typename T>
 struct PagesArgs {
   const T* q; int64_t q_sb, q_sh;
+  // a short prefix that the pages' kernels read themselves, or 0 rows
+  const T* pk; const T* pv; int64_t pk_st, pk_sh, pv_st, pv_sh; int prefix;
   const T* kc; const T* vc; int64_t kc_sp, kc_st, kc_sh;
   const int32_t* bt; int64_t bt_s; int max_blocks; const int32_t* lengths; int num_pages, page;
   const T* ck; const T* cv; int64_t ck_sb, ck_sh; const uint8_t* cvalid;
@@ -34,6 +37,32 @@ struct PagesArgs {
 // elements against the query in shared memory, all requested before the first
 // is used), a lane per column for the values, eight keys' rows in flight.  The
 // warps take turns on the prefix slices too and meet in shared memory.
+// The key and value rows of a beam's token t (K/V head h): prefix rows, then
+// the first `past` tokens of its pages, then its current token; null where the
+// page is not in the cache.
+template <typename T>
+__device__ __forceinline__ void pages_token(const PagesArgs<T>& a, int b, int h, int t, int past,
+                                            const T*& k, const T*& v) {
+  if (t < a.prefix) {
+    k = a.pk + (int64_t)t * a.pk_st + (int64_t)h * a.pk_sh;
+    v = a.pv + (int64_t)t * a.pv_st + (int64_t)h * a.pv_sh;
+    return;
+  }
+  t -= a.prefix;
+  int64_t at = (int64_t)b * a.ck_sb + (int64_t)h * a.ck_sh;
+  if (t < past) {
+    const int page = __ldg(a.bt + (int64_t)b * a.bt_s + t / a.page);
+    if (page < 0 || page >= a.num_pages) {
+      set_status(a.status, GRS_ERR_BAD_PAGE);
+      k = v = nullptr;
+      return;
+    }
+    at = (int64_t)page * a.kc_sp + (int64_t)(t % a.page) * a.kc_st + (int64_t)h * a.kc_sh;
+  }
+  k = (t < past ? a.kc : a.ck) + at;
+  v = (t < past ? a.vc : a.cv) + at;
+}
+
 template <typename T, int DP, int kVec>
 __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
   constexpr int ND = (DP + 31) / 32;
@@ -52,8 +81,7 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
     past = min(max(past, 0), room);
   }
   const bool cur = a.ck != nullptr && (a.cvalid == nullptr || a.cvalid[b] != 0);
-  const int total = past + (cur ? 1 : 0);
-  const T* cur_k = cur ? a.ck + (int64_t)b * a.ck_sb + (int64_t)h * a.ck_sh : nullptr;
+  const int total = a.prefix + past + (cur ? 1 : 0);
   __syncthreads();
 
   float m = -INFINITY, l = 0.f, acc[ND];
@@ -61,19 +89,8 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
   for (int i = 0; i < ND; ++i) acc[i] = 0.f;
   for (int t0 = 32 * warp; t0 < total; t0 += 128) {
     const int t = t0 + lane;
-    int64_t at = 0;
-    const T* k = nullptr;
-    if (t < past) {
-      const int page = __ldg(a.bt + (int64_t)b * a.bt_s + t / a.page);
-      if (page >= 0 && page < a.num_pages) {
-        at = (int64_t)page * a.kc_sp + (int64_t)(t % a.page) * a.kc_st + (int64_t)h * a.kc_sh;
-        k = a.kc + at;
-      } else {
-        set_status(a.status, GRS_ERR_BAD_PAGE);
-      }
-    } else if (t < total) {
-      k = cur_k;
-    }
+    const T *k = nullptr, *v = nullptr;
+    if (t < total) pages_token(a, b, h, t, past, k, v);
     const unsigned valid = __ballot_sync(0xffffffffu, k != nullptr);
     float s = -INFINITY;
     if (k) {
@@ -112,13 +129,12 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
       float x[8][ND];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int64_t vat = __shfl_sync(0xffffffffu, at, j0 + j);
-        const T* v = t0 + j0 + j >= past
-                         ? a.cv + (int64_t)b * a.ck_sb + (int64_t)h * a.ck_sh : a.vc + vat;
+        const T* vj = reinterpret_cast<const T*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), j0 + j));
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
           const int d = lane + 32 * i;
-          x[j][i] = ((valid >> (j0 + j)) & 1) && d < a.D ? to_float(v[d]) : 0.f;
+          x[j][i] = ((valid >> (j0 + j)) & 1) && d < a.D ? to_float(vj[d]) : 0.f;
         }
       }
 #pragma unroll
@@ -180,7 +196,8 @@ static int pages_rows_launch(const PagesArgs<T>& p, cudaStream_t stream) {
   if (rows > INT_MAX) return GRS_ERR_SHAPE;
   constexpr int kVec = 16 / sizeof(T);
   const auto whole = [](const void* at) { return (reinterpret_cast<uintptr_t>(at) & 15) == 0; };
-  const bool vec = p.D % kVec == 0 && whole(p.kc) && whole(p.ck) && p.kc_sp % kVec == 0 &&
+  const bool vec = p.D % kVec == 0 && (p.prefix == 0 || (whole(p.pk) && p.pk_st % kVec == 0 &&
+                                                         p.pk_sh % kVec == 0)) && whole(p.kc) && whole(p.ck) && p.kc_sp % kVec == 0 &&
                    p.kc_st % kVec == 0 && p.kc_sh % kVec == 0 && p.ck_sb % kVec == 0 &&
                    p.ck_sh % kVec == 0;
   const unsigned grid = (unsigned)rows;
@@ -331,23 +348,14 @@ __global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16>
     past = min(max(past, 0), room);
   }
   const bool cur = a.ck != nullptr && (a.cvalid == nullptr || a.cvalid[b] != 0);
-  const int total = past + (cur ? 1 : 0);
+  const int total = a.prefix + past + (cur ? 1 : 0);
   const int runs = (total + 31) / 32;
   const int run_lo = (int)((int64_t)runs * blockIdx.y / gridDim.y);
   const int run_hi = (int)((int64_t)runs * (blockIdx.y + 1) / gridDim.y);
-  const T* cur_k = cur ? a.ck + (int64_t)b * a.ck_sb + (int64_t)h * a.ck_sh : nullptr;
-  const int64_t paged_v = a.vc - a.kc, cur_v = a.cv - a.ck;   // value row behind a key row
-  const auto place = [&](int run) -> const T* {               // key row of token 32 run + lane
+  const auto place = [&](int run, const T*& k, const T*& v) {   // rows of token 32 run + lane
     const int tok = run * 32 + lane;
-    if (run >= run_hi || tok >= total) return nullptr;
-    if (tok >= past) return cur_k;
-    const int page = __ldg(a.bt + (int64_t)b * a.bt_s + tok / a.page);
-    if (page < 0 || page >= a.num_pages) {
-      set_status(a.status, GRS_ERR_BAD_PAGE);
-      return nullptr;
-    }
-    return a.kc + (int64_t)page * a.kc_sp + (int64_t)(tok % a.page) * a.kc_st +
-           (int64_t)h * a.kc_sh;
+    k = v = nullptr;
+    if (run < run_hi && tok < total) pages_token(a, b, h, tok, past, k, v);
   };
 
   // kFew: columns (d, d + 1) x heads (2t, 2t + 1), d = piece (g + 8 j) + 2 i;
@@ -357,12 +365,13 @@ __global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16>
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  const T* next = place(run_lo + warp);
+  const T *next_k, *next_v;
+  place(run_lo + warp, next_k, next_v);
   for (int run = run_lo + warp; run < run_hi; run += warps) {
-    const T* mine = next;
-    next = place(run + warps);
-    const unsigned valid = __ballot_sync(0xffffffffu, mine != nullptr);
-    const unsigned long long at = reinterpret_cast<unsigned long long>(mine);
+    const unsigned valid = __ballot_sync(0xffffffffu, next_k != nullptr);
+    const unsigned long long k_at = reinterpret_cast<unsigned long long>(next_k);
+    const unsigned long long v_at = reinterpret_cast<unsigned long long>(next_v);
+    place(run + warps, next_k, next_v);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (((valid >> (16 * half)) & 0xffffu) == 0) continue;
@@ -370,7 +379,7 @@ __global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16>
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const T* k = reinterpret_cast<const T*>(
-            __shfl_sync(0xffffffffu, at, 16 * half + 8 * n + g));
+            __shfl_sync(0xffffffffu, k_at, 16 * half + 8 * n + g));
 #pragma unroll
         for (int i = 0; i < S::kKey; ++i) {
           const int d = 8 * (t + 4 * i);
@@ -383,21 +392,20 @@ __global__ void __launch_bounds__(256) pages_mma_kernel(PagesArgs<__nv_bfloat16>
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int j = 16 * half + 2 * t + (n & 1) + 8 * (n >> 1);
-        const T* k = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, at, j));
-        const T* v = k + (run * 32 + j >= past ? cur_v : paged_v);
+        const T* v = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, v_at, j));
 #pragma unroll
         for (int i = 0; i < S::kRuns; ++i) {
           const int d = S::kPiece * (g + 8 * i);
           if constexpr (S::kPiece == 8) {
             uint4 w = make_uint4(0, 0, 0, 0);
-            if (k && d < a.D) w = __ldg(reinterpret_cast<const uint4*>(v + d));
+            if (v && d < a.D) w = __ldg(reinterpret_cast<const uint4*>(v + d));
             vr[n][i][0] = w.x;
             vr[n][i][1] = w.y;
             vr[n][i][2] = w.z;
             vr[n][i][3] = w.w;
           } else {
             uint2 w = make_uint2(0, 0);
-            if (k && d < a.D) w = __ldg(reinterpret_cast<const uint2*>(v + d));
+            if (v && d < a.D) w = __ldg(reinterpret_cast<const uint2*>(v + d));
             vr[n][i][0] = w.x;
             vr[n][i][1] = w.y;
           }
@@ -729,6 +737,19 @@ static PrefixPlan tc_plan(int batch, int heads, int kv_heads, int D, int keys) {
   return {slices, slices * per, each * 128};
 }
 
+// Whether the pages' kernels read the prefix themselves, once per beam: while
+// that is little they need no second kernel, no workspace and no join (32/8
+// heads of 128: 16 beams over 128 keys 11.3 -> 6.4 us, 64 over 64 12.6 -> 7.6,
+// even at 64 over 256; 16 over 512 13.9 against 12.4 us, 64 over 512 28 against
+// 16; fp32, 8/8 heads of 64: 64 over 256 22 -> 20 us, 256 over 256 58 against
+// 32).
+constexpr int64_t PG_INLINE_BYTES = 64 << 20;   // of K and V in bf16, over all beams
+constexpr int PG_INLINE_KEYS = 256;
+static bool prefix_inline(int batch, int kv_heads, int D, int num_prefix) {
+  return num_prefix <= PG_INLINE_KEYS &&
+         (int64_t)batch * num_prefix * kv_heads * D * 4 <= PG_INLINE_BYTES;
+}
+
 // Slices of each beam's pages: enough CTAs of a long table to fill 148 SMs
 // four times when there are few beams, none for less than 256 tokens.  They are
 // joined by a kernel of its own when they are cut, or when there are so many
@@ -755,6 +776,9 @@ static bool aligned(const void* p, int64_t bytes) {
 
 // 16-byte pieces of query, cache and current rows, 8-byte pieces of the output
 static bool pages_mma_takes(const PagesArgs<__nv_bfloat16>& p) {
+  if (p.prefix > 0 && !(aligned(p.pk, 16) && aligned(p.pv, 16) && p.pk_st % 8 == 0 &&
+                        p.pk_sh % 8 == 0 && p.pv_st % 8 == 0 && p.pv_sh % 8 == 0))
+    return false;
   return p.D % 8 == 0 && p.D <= 128 && aligned(p.q, 16) && p.q_sb % 8 == 0 && p.q_sh % 8 == 0 &&
          aligned(p.kc, 16) && aligned(p.vc, 16) && p.kc_sp % 8 == 0 && p.kc_st % 8 == 0 &&
          p.kc_sh % 8 == 0 && aligned(p.ck, 16) && aligned(p.cv, 16) && p.ck_sb % 8 == 0 &&
@@ -767,7 +791,7 @@ static int pages_mma_run(const PagesArgs<__nv_bfloat16>& p, int page_slices, boo
   const int64_t tasks = (int64_t)p.batch * p.kv_heads * ((p.group + PG_HEADS - 1) / PG_HEADS);
   if (tasks > INT_MAX || page_slices > 65535) return GRS_ERR_SHAPE;
   // warps of a CTA: a run of 32 tokens each, more when there are few CTAs
-  const int64_t runs = ((int64_t)p.max_blocks * p.page + 1 + 31) / 32;
+  const int64_t runs = ((int64_t)p.prefix + (int64_t)p.max_blocks * p.page + 1 + 31) / 32;
   const int warps = runs <= 2 && tasks * page_slices >= 4 * 148 ? 2 : tasks * page_slices >= 2 * 148 ? 4 : 8;
   constexpr int kRow = ((kFew ? 8 : PG_HEADS) * (PgShape<DP>::kStride + 2) + 32 * 4 + 2) * 4;
   const int smem = warps * kRow;
@@ -838,6 +862,10 @@ extern "C" int64_t grs_shared_prefix_workspace_bytes(int batch, int heads, int k
                                                      int head_width, int num_prefix,
                                                      int64_t page_tokens) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  if (grs::prefix_inline(batch, kv_heads, head_width, num_prefix)) {
+    page_tokens += num_prefix;
+    num_prefix = 0;
+  }
   // any of the kernels may take the call, by the alignment of its tensors
   const int parts = std::max(
       grs::rows_plan(batch, heads / kv_heads, kv_heads, head_width, num_prefix).parts,
@@ -881,12 +909,15 @@ extern "C" int grs_shared_prefix_attention(
     g.v = static_cast<const T*>(prefix_value); g.v_st = pv_st; g.v_sh = pv_sh;
     g.positions = batch; g.keys = num_prefix; g.heads = heads; g.kv_heads = kv_heads;
     g.group = group; g.D = head_width; g.scale_log2 = scale_log2;
+    const bool inlined = prefix_inline(batch, kv_heads, head_width, num_prefix);
+    const int sliced = inlined ? 0 : num_prefix;
     bool tensor_cores = false;
     if constexpr (std::is_same<T, __nv_bfloat16>::value) tensor_cores = grouped_tc_takes(g);
-    const PrefixPlan plan = tensor_cores ? tc_plan(batch, heads, kv_heads, head_width, num_prefix)
-                                         : rows_plan(batch, group, kv_heads, head_width, num_prefix);
+    const PrefixPlan plan = tensor_cores ? tc_plan(batch, heads, kv_heads, head_width, sliced)
+                                         : rows_plan(batch, group, kv_heads, head_width, sliced);
     float* part = static_cast<float*>(workspace);
-    const PagesPlan pages = pages_plan(batch, heads, kv_heads, num_prefix, room);
+    const PagesPlan pages =
+        pages_plan(batch, heads, kv_heads, sliced, room + (inlined ? num_prefix : 0));
     const int64_t parts = plan.parts + (pages.separate ? pages.slices : 0);
     float* lse = part + parts * batch * heads * head_width;
     g.part = part; g.part_lse = lse; g.slices = plan.slices; g.slice_keys = plan.keys;
@@ -899,6 +930,11 @@ extern "C" int grs_shared_prefix_attention(
     p.lengths = max_blocks ? lengths : nullptr; p.num_pages = num_pages; p.page = page_size;
     p.ck = static_cast<const T*>(current_key); p.cv = static_cast<const T*>(current_value);
     p.ck_sb = ck_sb; p.ck_sh = ck_sh; p.cvalid = current_valid;
+    if (inlined) {
+      p.pk = g.k; p.pk_st = pk_st; p.pk_sh = pk_sh;
+      p.pv = g.v; p.pv_st = pv_st; p.pv_sh = pv_sh;
+      p.prefix = num_prefix;
+    }
     p.part = part; p.part_lse = lse;
     if (pages.separate) p.page_part = part, p.page_lse = lse; p.slices = plan.parts;
     p.out = static_cast<T*>(output); p.o_sb = o_sb; p.o_sh = o_sh;

@@ -62,7 +62,8 @@ def _clean(dev):
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 @pytest.mark.parametrize("batch,prefix,max_len", [
     (1, 0, 1), (1, 1, 0), (1, 129, 20), (5, 0, 40), (3, 0, 0), (9, 127, 1), (33, 128, 64),
-    (64, 700, 0), (40, 381, 65), (7, 5000, 300), (2, 33, 1000)])
+    (64, 700, 0), (40, 381, 65), (7, 5000, 300), (2, 33, 1000), (9, 256, 30), (9, 257, 30),
+    (1, 640, 5), (130, 384, 17), (33, 1025, 0), (2500, 64, 3), (600, 255, 9)])
 def test_sizes(cuda_device, batch, prefix, max_len, dtype):
     args = _case(batch + prefix, batch=batch, heads=8, kv_heads=2, width=64, prefix=prefix,
                  max_len=max_len, dtype=dtype)
@@ -73,16 +74,19 @@ def test_sizes(cuda_device, batch, prefix, max_len, dtype):
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 @pytest.mark.parametrize("heads,kv_heads", [(8, 8), (8, 1), (3, 1), (10, 2), (14, 2), (32, 2),
                                             (40, 1), (130, 1)])
-def test_head_groups(cuda_device, heads, kv_heads, dtype):
-    args = _case(heads, batch=19, heads=heads, kv_heads=kv_heads, width=32, prefix=200,
+@pytest.mark.parametrize("prefix", [200, 410])
+def test_head_groups(cuda_device, heads, kv_heads, dtype, prefix):
+    """A prefix that the pages' kernel reads itself, and a sliced one."""
+    args = _case(heads, batch=19, heads=heads, kv_heads=kv_heads, width=32, prefix=prefix,
                  max_len=40, page=8, dtype=dtype)
     _check(_call(cuda_device, args), args)
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 @pytest.mark.parametrize("width", [1, 8, 16, 24, 33, 40, 64, 80, 96, 128, 160, 256])
-def test_widths(cuda_device, width, dtype):
-    args = _case(width, batch=11, heads=4, kv_heads=2, width=width, prefix=150, max_len=50,
+@pytest.mark.parametrize("prefix", [150, 390])
+def test_widths(cuda_device, width, dtype, prefix):
+    args = _case(width, batch=11, heads=4, kv_heads=2, width=width, prefix=prefix, max_len=50,
                  dtype=dtype)
     _check(_call(cuda_device, args), args)
 
@@ -139,9 +143,10 @@ def test_bad_pages_and_lengths(cuda_device):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
-def test_bad_values_reach_only_their_beam(cuda_device, dtype):
+@pytest.mark.parametrize("prefix", [100, 500])
+def test_bad_values_reach_only_their_beam(cuda_device, dtype, prefix):
     """NaN in unused cache rows, in another beam's pages and query."""
-    args = _case(4, batch=6, heads=8, kv_heads=2, width=64, prefix=100, max_len=40, dtype=dtype,
+    args = _case(4, batch=6, heads=8, kv_heads=2, width=64, prefix=prefix, max_len=40, dtype=dtype,
                  lengths=torch.tensor([0, 17, 40, 33, 5, 31], dtype=torch.int32))
     args["block_table"] = torch.arange(18, dtype=torch.int32).view(6, 3)
     clean = {n: t.clone() for n, t in args.items()}
@@ -160,16 +165,18 @@ def test_bad_values_reach_only_their_beam(cuda_device, dtype):
     assert torch.isnan(got[2]).all() and torch.isnan(got[4]).all()
     keep = [0, 1, 3, 5]
     out, spread, reach = oracle.shared_prefix_attention(**clean)
-    bound = oracle.attention_bound(out, spread, reach, dtype, 64, 141)
+    bound = oracle.attention_bound(out, spread, reach, dtype, 64, prefix + 41)
     assert float(((got.double().cpu() - out).abs() / bound)[keep].max()) <= 1.0
 
 
-def test_layouts(cuda_device):
-    """A layer of a PagedKVCache, one projection's slices, unaligned rows."""
+@pytest.mark.parametrize("prefix", [90, 700])
+def test_layouts(cuda_device, prefix):
+    """A layer of a PagedKVCache, one projection's slices, unaligned rows, one
+    K/V head broadcast to two."""
     from graph_rewrite_system_b200.prefix_attention import shared_prefix_attention
 
     dev = cuda_device
-    args = _case(5, batch=10, heads=8, kv_heads=2, width=64, prefix=90, max_len=30)
+    args = _case(5, batch=10, heads=8, kv_heads=2, width=64, prefix=prefix, max_len=30)
     got = _call(dev, args)
     d = {n: t.to(dev) for n, t in args.items()}
     qkv = torch.cat([d["query"], d["current_key"], d["current_value"]], 1)
@@ -186,6 +193,10 @@ def test_layouts(cuda_device):
         room = torch.zeros(args[name].numel() + 1, dtype=BF16, device=dev)
         room[1:] = args[name].to(dev).reshape(-1)
         d[name] = room[1:].view(args[name].shape)
+    _check(shared_prefix_attention(**d), args)
+    for name in ("prefix_key", "prefix_value", "key_cache", "value_cache"):
+        args[name] = args[name][..., :1, :].expand(*args[name].shape)
+        d[name] = args[name][..., :1, :].to(dev).expand(*args[name].shape)
     _check(shared_prefix_attention(**d), args)
 
 
@@ -250,3 +261,23 @@ def test_equals_paged_attention(cuda_device):
                           current_value=d["current_value"], current_valid=d["current_valid"],
                           shared_key=d["prefix_key"], shared_value=d["prefix_value"]).squeeze(2)
     torch.testing.assert_close(got.float(), exp.float(), rtol=2e-2, atol=2e-2)
+
+
+def test_two_calls_at_once(cuda_device):
+    """Calls on two streams, each sliced with a workspace of its own."""
+    from graph_rewrite_system_b200.prefix_attention import shared_prefix_attention
+
+    cases = [_case(10 + i, batch=30, heads=8, kv_heads=2, width=64, prefix=3000 + 700 * i,
+                   max_len=60) for i in range(2)]
+    d = [{n: t.to(cuda_device) for n, t in c.items()} for c in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(10):
+        for s, x, o in zip(streams, d, outs):
+            with torch.cuda.stream(s):
+                o.append(shared_prefix_attention(**x))
+    torch.cuda.synchronize()
+    for c, o in zip(cases, outs):
+        _check(o[0], c)
+        assert all(torch.equal(y, o[0]) for y in o)
