@@ -10,7 +10,7 @@
 // (scores out, maximum, exponentials, weights in, products), and four softmax
 // warps per scheduler hide them where two with 128 keys a thread did not.  The
 // running maximum is lazy: O and the sum are rescaled only when the maximum
-// has grown by more than 2^8 in weight, which fp32 sums and bf16 weights (same
+// has grown by more than 2^32 in weight, which fp32 sums and bf16 weights (same
 // relative rounding at any exponent) do not notice.  The commit that hands a
 // slot its next scores also covers the slot's previous P V, so the softmax
 // warps may rescale O in place without a further barrier.
@@ -29,6 +29,12 @@
 // one row tile gives both slots the same rows and halves of the slice's keys.
 // Weights are rounded to bf16 for the value product; sums, statistics and
 // outputs are fp32 until the one rounding of the output.
+//
+// 16384 tokens of 32/8 heads of 128 take 1.65 ms, 1336 TFLOP/s or 0.80 of the
+// measured burst of the library's product; 2 x 8192 tokens 0.92 ms, of width 64
+// 0.77 ms (719 TFLOP/s: half the products' work per exponential).  On 2 x 8192
+// tokens the tensor pipe is active 64 % and the special-function pipe 65 % of
+// the time: what remains is the chain of a slot's turn.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

@@ -3,8 +3,9 @@
 ``paged_attention(shared_key=...)`` holds a prefix of a few hundred keys in the
 shared memory of every group of beams (head width 32, one K/V head per query
 head).  ``shared_prefix_attention`` is the form for long prefixes, grouped
-heads and wider heads: the prefix is read once for the whole batch on the
-tensor cores and joined with each beam's own pages and current token.
+heads and wider heads: a long prefix is read once for the whole batch (bf16 on
+the tensor cores) and joined with each beam's own pages and current token; a
+short one, up to 256 keys, is read with the beam's own keys in one launch.
 
 Inference only: no gradient is recorded.  The sm_100a kernels live in
 ``csrc/prefix_attention.cu`` and the grouped attention sources beside it; CPU

@@ -143,6 +143,26 @@ def test_bad_pages_and_lengths(cuda_device):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("prefix", [0, 40, 500])
+def test_no_pages(cuda_device, prefix, dtype):
+    """A cache without pages, and a table without columns: tokens that the
+    lengths claim are reported and skipped."""
+    args = _case(9, batch=4, heads=4, kv_heads=2, width=64, prefix=prefix, max_len=0, dtype=dtype)
+    for pages, columns, lengths, code in ((0, 2, [0, 0, 0, 0], 0), (0, 2, [0, 3, 0, 32], -2),
+                                          (0, 2, [0, 33, 0, 0], None), (5, 0, [0, 0, 0, 0], 0),
+                                          (5, 0, [0, 0, 1, 0], -7), (0, 0, [0, -1, 0, 0], -7)):
+        status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+        more = dict(args, key_cache=torch.zeros(pages, 16, 2, 64, dtype=dtype),
+                    value_cache=torch.zeros(pages, 16, 2, 64, dtype=dtype),
+                    block_table=torch.zeros(4, columns, dtype=torch.int32),
+                    lengths=torch.tensor(lengths, dtype=torch.int32))
+        got = _call(cuda_device, more, status=status)
+        _check(got, args)
+        # either report of a beam with both faults
+        assert int(status.item()) in ((code,) if code is not None else (-2, -7))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
 @pytest.mark.parametrize("prefix", [100, 500])
 def test_bad_values_reach_only_their_beam(cuda_device, dtype, prefix):
     """NaN in unused cache rows, in another beam's pages and query."""
@@ -216,6 +236,30 @@ def test_far_pages(cuda_device):
     args["block_table"] %= 3
     d["block_table"] = (args["block_table"] + pages - 3).to(cuda_device)
     _check(shared_prefix_attention(**d), args)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("prefix", [250, 2100])
+def test_far_prefix(cuda_device, prefix, dtype):
+    """Prefix rows, and with the short prefix the beams' too, whose last start
+    past 2^31 elements, all in one buffer."""
+    from graph_rewrite_system_b200.prefix_attention import shared_prefix_attention
+
+    step = (1 << 31) // (prefix - 2) // 64 * 64 + 128
+    if torch.cuda.mem_get_info()[0] < prefix * step * dtype.itemsize + (1 << 30):
+        pytest.skip("needs 10 GB")
+    batch = min(prefix, 250)
+    args = _case(7, batch=batch, heads=4, kv_heads=1, width=64, prefix=prefix, max_len=20,
+                 dtype=dtype)
+    buffer = torch.empty(prefix, step // 64, 64, dtype=dtype, device=cuda_device)
+    assert buffer[-1].data_ptr() - buffer.data_ptr() > (1 << 31) * dtype.itemsize
+    d, at = {n: t.to(cuda_device) for n, t in args.items()}, 0
+    for name in ("query", "prefix_key", "prefix_value", "current_key", "current_value"):
+        part = buffer[:args[name].shape[0], at:at + args[name].shape[1]]
+        d[name] = part.copy_(args[name])
+        at += args[name].shape[1]
+    out = buffer[:batch, at:at + 4]
+    _check(shared_prefix_attention(**d, out=out), args)
 
 
 def test_captured_and_on_another_stream(cuda_device):

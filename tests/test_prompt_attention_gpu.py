@@ -191,6 +191,27 @@ def test_layouts(cuda_device):
            (q, k[:, :1].expand(-1, 3, -1), k[:, :1].expand(-1, 3, -1)), offsets)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_far_rows(cuda_device, dtype):
+    """Tokens whose rows start past 2^31 elements: q, k, v and out in one
+    buffer."""
+    from graph_rewrite_system_b200.prompt_attention import prompt_attention
+
+    step = (1 << 20) + 64
+    offsets = _offsets([700, 1, 1340, 9])
+    tokens = offsets[-1]
+    if torch.cuda.mem_get_info()[0] < tokens * step * dtype.itemsize + (1 << 30):
+        pytest.skip("needs 10 GB")
+    buffer = torch.empty(tokens, step // 64, 64, dtype=dtype, device=cuda_device)
+    assert buffer[-1].data_ptr() - buffer.data_ptr() > (1 << 31) * dtype.itemsize
+    qkv = _inputs(12, tokens, 4, 2, 64, dtype)
+    q, k, v, out = buffer[:, :12].split([4, 2, 2, 4], 1)
+    for into, t in zip((q, k, v), qkv):
+        into.copy_(t)
+    off = torch.tensor(offsets, dtype=torch.int32, device=cuda_device)
+    _check(prompt_attention(q, k, v, off, out=out), qkv, offsets)
+
+
 @pytest.mark.parametrize("values", [[0, 0], [0], [5, 3, 90], [-7, 40, 400], [200, 100],
                                     [2 ** 31 - 1, -2 ** 31]])
 def test_any_offsets_are_safe(cuda_device, values):

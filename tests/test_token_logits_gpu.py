@@ -145,6 +145,28 @@ def test_in_place_and_strided(cuda_device, dtype):
     assert torch.equal(adjust_logits(logits.to(cuda_device), **d), got)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_far_and_shared_rows(cuda_device, dtype):
+    """Rows that start past 2^31 elements, adjusted in place; and one row of
+    logits, history and mask that every row shares by a stride of zero."""
+    from graph_rewrite_system_b200.token_logits import adjust_logits
+
+    logits, kw = _case(8, 3, 5003, 30, dtype, mask="row", bias="row")
+    d = {n: v.to(cuda_device) for n, v in kw.items()}
+    step = (1 << 30) + 16
+    if torch.cuda.mem_get_info()[0] < 3 * step * dtype.itemsize + (1 << 30):
+        pytest.skip("needs 14 GB")
+    rows = torch.empty(3, step, dtype=dtype, device=cuda_device)[:, 5:5008]
+    assert rows[2].data_ptr() - rows.data_ptr() > (1 << 31) * dtype.itemsize
+    rows.copy_(logits)
+    _check(adjust_logits(rows, **d, out=rows), logits, kw)
+    one = {n: v[1:2].expand(3, -1) if n in ("tokens", "allowed") else v for n, v in kw.items()}
+    d = {n: kw[n][1:2].to(cuda_device).expand(3, -1) if n in ("tokens", "allowed") else v
+         for n, v in d.items()}
+    got = adjust_logits(logits[:1].to(cuda_device).expand(3, -1), **d)
+    _check(got, logits[:1].expand(3, -1), one)
+
+
 def test_captured(cuda_device):
     from graph_rewrite_system_b200.token_logits import adjust_logits
 
