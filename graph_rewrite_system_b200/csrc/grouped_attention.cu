@@ -2,20 +2,24 @@
 // tensor-core kernel does not take (widths that are no multiple of 8 or above
 // 128, groups above 128, unaligned rows, negative scales).
 //
-// One CTA takes 128 rows of one K/V head (64 at widths above 128) and walks
+// One CTA takes 32 rows of one K/V head (64 at widths above 128) and walks
 // 64-key tiles; a thread holds 4 rows x 4 keys of the scores and 4 rows x DP/16
-// columns of the output, so that 16 warps hide the latencies of shared memory
-// (8 rows a thread read less of it, but with 8 warps took 1.2 to 1.6 times as
-// long).  Both products read 16-byte vectors from shared memory (8 for 64
-// multiply-adds, 12 for 128 at DP = 128) into packed fp32x2
-// multiply-adds: the scores sum even and odd dimensions apart, so both factors
-// are pairs as they lie.  The next K tile is fetched (cp.async) under the value
-// product and the next V tile under the scores, in one buffer each.  The
-// weights pass through shared memory between the 16 threads of a row.  Running
-// maximum and sum, scores, weights and outputs are fp32.  Bound by the
-// multiply-adds and the shared-memory reads that feed them: 2 x 2048 tokens of
-// 32/8 heads of 128 take 2.17 ms, 32 TFLOP/s of the 74 of the fp32 pipes; 8
-// heads of 32, 2704 tokens in four prompts, 112 us.
+// columns of the output.  Four CTAs share an SM (two at widths above 64): their
+// barriers fall at different times, and their tiles fill the SMs where one tile
+// of 128 rows and 512 threads left SMs idle (8 heads of 32, one prompt of 1001
+// tokens: 86 -> 45 us; 2 x 2048 tokens of 16/4 heads of 64: 675 -> 560 us; 16 rows
+// 53 and 710 us, 2 rows a thread 60 and 800 us).  Both products read 16-byte
+// vectors from shared memory (8 for 64 multiply-adds, 12 for 128 at DP = 128)
+// into packed fp32x2 multiply-adds: the scores sum even and odd dimensions apart,
+// so both factors are pairs as they lie.  Eight steps of either are unrolled, so
+// that loads run ahead of the multiply-adds (5 to 9 % over 2 and 1).  The next K
+// tile is fetched (cp.async) under the value product and the next V tile under
+// the scores, in one buffer each.  The weights pass through shared memory between
+// the 16 threads of a row.  Running maximum and sum, scores, weights and outputs
+// are fp32.  Bound by the shared-memory reads that feed the multiply-adds, and in
+// small calls by the chain of a tile: 2 x 2048 tokens of 32/8 heads of 128 take
+// 2.01 ms, 34 TFLOP/s of the 74 of the fp32 pipes; 8 heads of 32, 2704 tokens in
+// four prompts, 69 us.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -29,11 +33,12 @@ constexpr int GA_I = 4;                                // rows of a thread
 
 template <int DP>
 struct GaShape {
-  static constexpr int kRows = DP <= 128 ? 128 : 64;
+  static constexpr int kRows = grouped_rows_tile(DP);
   static constexpr int kThreads = 16 * kRows / GA_I;   // 16 threads for GA_I rows
   static constexpr int kRowStep = kRows / GA_I;        // thread rows: rg + kRowStep i
   static constexpr int kQS = DP + 4;                   // padded row strides (floats)
   static constexpr int kSmem = (kRows * kQS + GA_KEYS * kQS + GA_KEYS * DP + kRows * GA_PS) * 4;
+  static constexpr int kCtas = DP <= 64 ? 4 : DP <= 128 ? 2 : 1;   // of an SM
 };
 
 __device__ __forceinline__ void ga_copy16(float* dst, const void* src, bool in) {
@@ -50,10 +55,9 @@ __device__ __forceinline__ void ga_wait() {
 
 // rows [t0, t0 + 64) of a K or V head into shared memory, zeros past `end` and
 // past the width
-template <typename T, int DP, int kStride, bool kAsync>
+template <typename T, int DP, int kStride, int kThreads, bool kAsync>
 __device__ __forceinline__ void ga_load(float* dst, const T* src, int64_t st, int D, int t0,
                                         int end) {
-  constexpr int kThreads = GaShape<DP>::kThreads;
   if constexpr (kAsync) {
 #pragma unroll 4
     for (int i = threadIdx.x; i < GA_KEYS * DP / 4; i += kThreads) {
@@ -73,7 +77,7 @@ __device__ __forceinline__ void ga_load(float* dst, const T* src, int64_t st, in
 }
 
 template <typename T, int DP, bool kCausal, bool kAsync>
-__global__ void __launch_bounds__(GaShape<DP>::kThreads, 1)
+__global__ void __launch_bounds__(GaShape<DP>::kThreads, GaShape<DP>::kCtas)
 grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
   using S = GaShape<DP>;
   extern __shared__ __align__(16) float ga_smem_raw[];
@@ -83,6 +87,7 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
   float* ps = vs + GA_KEYS * DP;            // [kRows][GA_PS]
   // per row its keys; first and last key of any row, last first and first last
   __shared__ int row_begin[S::kRows], row_end[S::kRows], span[4];
+  __shared__ int row_position[S::kRows], row_head[S::kRows];   // -1: no row
   constexpr int kPairs = DP / 32;           // output column pairs of a thread
   const int tid = threadIdx.x;
   const int rg = tid >> 4, cg = tid & 15;
@@ -98,10 +103,12 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
   __syncthreads();
   if (tid < S::kRows) {
     const int64_t r = row0 + tid;
-    int begin = 0, end = 0;
+    int begin = 0, end = 0, p = -1, head = 0;
     if (r < total) {
+      p = (int)(r / a.group);
+      head = h * a.group + (int)(r - (int64_t)p * a.group);
       if (kCausal) {
-        causal_range(a.offsets, a.sequences, (int)(r / a.group), begin, end);
+        causal_range(a.offsets, a.sequences, p, begin, end);
       } else {
         begin = min(a.keys, (int)blockIdx.z * a.slice_keys);
         end = min(a.keys, begin + a.slice_keys);
@@ -109,6 +116,8 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
     }
     row_begin[tid] = begin;
     row_end[tid] = end;
+    row_position[tid] = p;
+    row_head[tid] = head;
     if (end > begin) {
       atomicMin(&span[0], begin);
       atomicMax(&span[1], end);
@@ -121,18 +130,15 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
   const T* kh = a.k + (int64_t)h * a.k_sh;
   const T* vh = a.v + (int64_t)h * a.v_sh;
   if (first < last) {
-    ga_load<T, DP, S::kQS, kAsync>(ks, kh, a.k_st, a.D, first, last);
-    ga_load<T, DP, DP, kAsync>(vs, vh, a.v_st, a.D, first, last);
+    ga_load<T, DP, S::kQS, S::kThreads, kAsync>(ks, kh, a.k_st, a.D, first, last);
+    ga_load<T, DP, DP, S::kThreads, kAsync>(vs, vh, a.v_st, a.D, first, last);
   }
 #pragma unroll 8
   for (int i = tid; i < S::kRows * DP; i += S::kThreads) {
-    const int r = i / DP, d = i % DP;
-    const int64_t row = row0 + r;
+    const int r = i / DP, d = i % DP, p = row_position[r];
     float x = 0.f;
-    if (row < total && d < a.D) {
-      const int p = (int)(row / a.group), head = h * a.group + (int)(row - (int64_t)p * a.group);
-      x = to_float(a.q[(int64_t)p * a.q_sp + (int64_t)head * a.q_sh + d]);
-    }
+    if (p >= 0 && d < a.D)
+      x = to_float(a.q[(int64_t)p * a.q_sp + (int64_t)row_head[r] * a.q_sh + d]);
     qs[r * S::kQS + d] = x * a.scale_log2;
   }
 
@@ -156,7 +162,7 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
       for (int i = 0; i < GA_I; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0.f, 0.f);
-#pragma unroll 2
+#pragma unroll 8
       for (int d = 0; d < DP; d += 4) {
         float4 k4[4];
 #pragma unroll
@@ -178,7 +184,7 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
         for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
     }
     __syncthreads();                        // K is read
-    ga_load<T, DP, S::kQS, kAsync>(ks, kh, a.k_st, a.D, t0 + GA_KEYS, last);
+    ga_load<T, DP, S::kQS, S::kThreads, kAsync>(ks, kh, a.k_st, a.D, t0 + GA_KEYS, last);
     if (t0 < all_from || t0 + GA_KEYS > all_to) {
 #pragma unroll
       for (int i = 0; i < GA_I; ++i) {
@@ -212,7 +218,7 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
     }
     ga_wait<1>();                           // V is here
     __syncthreads();
-#pragma unroll 1
+#pragma unroll 8
     for (int t = 0; t < GA_KEYS; t += 4) {
       float4 p4[GA_I];
 #pragma unroll
@@ -240,7 +246,7 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
       }
     }
     __syncthreads();                        // V is read
-    ga_load<T, DP, DP, kAsync>(vs, vh, a.v_st, a.D, t0 + GA_KEYS, last);
+    ga_load<T, DP, DP, S::kThreads, kAsync>(vs, vh, a.v_st, a.D, t0 + GA_KEYS, last);
   }
   ga_wait<0>();
 
@@ -250,10 +256,8 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
     float sum = l[i];
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const int r = rg + S::kRowStep * i;
-    const int64_t row = row0 + r;
-    if (row >= total) continue;
-    const int p = (int)(row / a.group), head = h * a.group + (int)(row - (int64_t)p * a.group);
+    const int r = rg + S::kRowStep * i, p = row_position[r], head = row_head[r];
+    if (p < 0) continue;
     const bool seen = row_end[r] > row_begin[r];
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     bool odd = !(fabsf(sum) <= FLT_MAX);
@@ -287,10 +291,8 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
         const int i = __ffs(todo) - 1;
         todo &= todo - 1;
         const int r = (tid >> 5) * 2 + half + S::kRowStep * i;
-        const int64_t row = row0 + r;
-        const int p = (int)(row / a.group);
-        causal_row_again<T, (DP + 31) / 32>(a, p, h * a.group + (int)(row - (int64_t)p * a.group),
-                                            row_begin[r], row_end[r], 0, a.D);
+        causal_row_again<T, (DP + 31) / 32>(a, row_position[r], row_head[r], row_begin[r],
+                                            row_end[r], 0, a.D);
       }
     }
   }
@@ -299,7 +301,7 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
 template <typename T, int DP, bool kCausal, bool kAsync>
 static int rows_launch(const GroupedArgs<T>& a, cudaStream_t stream) {
   using S = GaShape<DP>;
-  static_assert(S::kSmem + 4 * (2 * S::kRows + 4) <= 227 * 1024, "shared memory of a CTA");
+  static_assert(S::kSmem + 4 * (4 * S::kRows + 4) <= 227 * 1024, "shared memory of a CTA");
   const int64_t tiles = ((int64_t)a.positions * a.group + S::kRows - 1) / S::kRows;
   if (tiles > INT_MAX || a.kv_heads > 65535 || (!kCausal && a.slices > 65535))
     return GRS_ERR_SHAPE;

@@ -107,6 +107,9 @@ __device__ __noinline__ void causal_row_again(const GroupedArgs<T>& a, int p, in
   }
 }
 
+// Rows of a tile of the rows kernel, by head width
+constexpr int grouped_rows_tile(int width) { return width <= 128 ? 32 : 64; }
+
 // Launchers; both return a grs_status.  The rows kernel takes every width up
 // to 256, every group and any strides.
 template <typename T> int grouped_rows_launch(const GroupedArgs<T>& a, cudaStream_t stream);

@@ -699,16 +699,30 @@ struct PrefixPlan {
   int slices, parts, keys;
 };
 
-// fp32 rows: enough CTAs for two waves of 148 SMs, none shorter than 64 keys.
+// fp32 rows: the count that gives the SM with most CTAs the least work, a CTA
+// paying about one 64-key block for its start and end (64 beams of 32/8 heads of
+// 128 over 4000 keys: 192 / 320 / 448 / 576 / 832 CTAs took 224 / 209 / 204 / 174
+// / 190 us, 16 beams 144 / 256 / 336 / 512 CTAs 68 / 68 / 81 / 78 us).
 static PrefixPlan rows_plan(int batch, int group, int kv_heads, int D, int keys) {
   if (keys <= 0) return {0, 0, 0};
-  const int64_t rows = D <= 128 ? 128 : 64;
+  const int64_t rows = grouped_rows_tile(D);
   const int64_t tiles = ((int64_t)batch * group + rows - 1) / rows * kv_heads;
-  const int64_t want = std::max<int64_t>(
-      1, std::min<int64_t>(std::min<int64_t>((2 * 148 + tiles - 1) / tiles, 64), (keys + 63) / 64));
-  const int each = (int)(((keys + want - 1) / want + 63) / 64 * 64);
-  const int slices = (keys + each - 1) / each;
-  return {slices, slices, each};
+  const int blocks = (keys + 63) / 64, most = std::min(64, blocks);
+  const int64_t least = (tiles + 147) / 148;
+  int64_t best = INT64_MAX;
+  int slices = 1, each = blocks;
+  for (int64_t ctas = least; ctas < least + 8; ++ctas) {   // of an SM
+    // as many slices as this allows, then as few as give the same length
+    const int z = (int)std::min<int64_t>(148 * ctas / tiles, most);
+    const int length = (blocks + z - 1) / z;
+    if (ctas * (length + 1) < best) {
+      best = ctas * (length + 1);
+      each = length;
+      slices = (blocks + length - 1) / length;
+    }
+    if (z == most) break;
+  }
+  return {slices, slices, each * 64};
 }
 
 // Tensor cores: the count whose waves of 148 CTAs take the fewest 128-key
