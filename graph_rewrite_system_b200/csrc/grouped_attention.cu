@@ -93,6 +93,8 @@ grouped_rows_kernel(const __grid_constant__ GroupedArgs<T> a) {
   const int rg = tid >> 4, cg = tid & 15;
   const int h = blockIdx.y;
   const int64_t total = (int64_t)a.positions * a.group;
+  // the kernel that joins the slices may start as SMs fall free
+  if (!kCausal) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   // late rows of a causal tile see the most keys: they start first
   const int64_t row0 = (int64_t)(kCausal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * S::kRows;
 

@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
   }
 
   // join: weights exp2(lse_i - max lse); the pages' sums enter unnormalised
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");   // the prefix slices are written
   const int64_t stride = (int64_t)a.batch * a.heads, row = blockIdx.x;
   if (lane == 0) tops[warp] = m;
   __syncthreads();
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
 }
 
 template <typename T>
-static int pages_rows_launch(const PagesArgs<T>& p, cudaStream_t stream) {
+static int pages_rows_launch(const PagesArgs<T>& p, bool after_prefix, cudaStream_t stream) {
   const int64_t rows = (int64_t)p.batch * p.heads;
   if (rows > INT_MAX) return GRS_ERR_SHAPE;
   constexpr int kVec = 16 / sizeof(T);
@@ -204,16 +205,26 @@ static int pages_rows_launch(const PagesArgs<T>& p, cudaStream_t stream) {
   const bool vec = p.D % kVec == 0 && prefix_vec && whole(p.kc) && whole(p.ck) &&
                    p.kc_sp % kVec == 0 && p.kc_st % kVec == 0 && p.kc_sh % kVec == 0 &&
                    p.ck_sb % kVec == 0 && p.ck_sh % kVec == 0;
-  const unsigned grid = (unsigned)rows;
+  // starts under the prefix kernel's tail; its join waits for the slices
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)rows);
+  config.blockDim = dim3(128);
+  config.stream = counted(stream);
+  config.attrs = &attr;
+  config.numAttrs = after_prefix ? 1 : 0;
   const auto go = [&](auto width) {
     constexpr int DP = decltype(width)::value;
-    if (vec) pages_rows_kernel<T, DP, kVec><<<grid, 128, 0, counted(stream)>>>(p);
-    else pages_rows_kernel<T, DP, 1><<<grid, 128, 0, counted(stream)>>>(p);
+    return vec ? cudaLaunchKernelEx(&config, pages_rows_kernel<T, DP, kVec>, p)
+               : cudaLaunchKernelEx(&config, pages_rows_kernel<T, DP, 1>, p);
   };
-  if (p.D <= 32) go(std::integral_constant<int, 32>{});
-  else if (p.D <= 64) go(std::integral_constant<int, 64>{});
-  else if (p.D <= 128) go(std::integral_constant<int, 128>{});
-  else go(std::integral_constant<int, 256>{});
+  const cudaError_t status = p.D <= 32    ? go(std::integral_constant<int, 32>{})
+                             : p.D <= 64  ? go(std::integral_constant<int, 64>{})
+                             : p.D <= 128 ? go(std::integral_constant<int, 128>{})
+                                          : go(std::integral_constant<int, 256>{});
+  if (status != cudaSuccess) return GRS_ERR_CUDA;
   GRS_CUDA_CHECK_LAUNCH();
   return GRS_OK;
 }
@@ -762,13 +773,13 @@ static PrefixPlan tc_plan(int batch, int heads, int kv_heads, int D, int keys) {
 // that is little they need no second kernel, no workspace and no join (32/8
 // heads of 128: 16 beams over 128 keys 11.3 -> 6.4 us, 64 over 64 12.6 -> 7.6,
 // even at 64 over 256; 16 over 512 13.9 against 12.4 us, 64 over 512 28 against
-// 16; fp32, 8/8 heads of 64: 64 over 256 22 -> 20 us, 256 over 256 58 against
-// 32).
-constexpr int64_t PG_INLINE_BYTES = 64 << 20;   // of K and V in bf16, over all beams
+// 16; fp32, 8/8 heads of 64: 4 over 64 14.4 -> 6.8, 64 over 128 17.5 -> 13.7, 64
+// over 256 20 against 18, 256 over 128 35 against 24).
+constexpr int64_t PG_INLINE_BYTES = 64 << 20;   // of K and V, over all beams
 constexpr int PG_INLINE_KEYS = 256;
-static bool prefix_inline(int batch, int kv_heads, int D, int num_prefix) {
+static bool prefix_inline(int batch, int kv_heads, int D, int num_prefix, int item) {
   return num_prefix <= PG_INLINE_KEYS &&
-         (int64_t)batch * num_prefix * kv_heads * D * 4 <= PG_INLINE_BYTES;
+         (int64_t)batch * num_prefix * kv_heads * D * 2 * item < PG_INLINE_BYTES;
 }
 
 // Slices of each beam's pages: enough CTAs of a long table to fill 148 SMs
@@ -874,7 +885,7 @@ static int shared_prefix(const PagesArgs<T>& p, const GroupedArgs<T>& prefix, bo
   }
   if constexpr (std::is_same<T, __nv_bfloat16>::value)
     if (pages_mma_takes(p)) return pages_mma_launch(p, page_slices, prefix.slices > 0, stream);
-  return pages_rows_launch<T>(p, stream);
+  return pages_rows_launch<T>(p, prefix.slices > 0, stream);
 }
 
 }  // namespace grs
@@ -883,16 +894,19 @@ extern "C" int64_t grs_shared_prefix_workspace_bytes(int batch, int heads, int k
                                                      int head_width, int num_prefix,
                                                      int64_t page_tokens) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
-  if (grs::prefix_inline(batch, kv_heads, head_width, num_prefix)) {
-    page_tokens += num_prefix;
-    num_prefix = 0;
-  }
-  // any of the kernels may take the call, by the alignment of its tensors
-  const int parts = std::max(
-      grs::rows_plan(batch, heads / kv_heads, kv_heads, head_width, num_prefix).parts,
-      grs::tc_plan(batch, heads, kv_heads, head_width, num_prefix).parts);
-  const grs::PagesPlan pages = grs::pages_plan(batch, heads, kv_heads, num_prefix, page_tokens);
-  return (int64_t)(parts + (pages.separate ? pages.slices : 0)) * batch * heads * (head_width + 1) * 4;
+  // any of the kernels may take the call, by the type and alignment of its tensors
+  const auto parts = [&](int sliced, int64_t room) {
+    const grs::PagesPlan pages = grs::pages_plan(batch, heads, kv_heads, sliced, room);
+    return std::max(grs::rows_plan(batch, heads / kv_heads, kv_heads, head_width, sliced).parts,
+                    grs::tc_plan(batch, heads, kv_heads, head_width, sliced).parts) +
+           (pages.separate ? pages.slices : 0);
+  };
+  int most = 0;
+  if (grs::prefix_inline(batch, kv_heads, head_width, num_prefix, 2))
+    most = parts(0, page_tokens + num_prefix);
+  if (!grs::prefix_inline(batch, kv_heads, head_width, num_prefix, 4))
+    most = std::max(most, parts(num_prefix, page_tokens));
+  return (int64_t)most * batch * heads * (head_width + 1) * 4;
 }
 
 extern "C" int grs_shared_prefix_attention(
@@ -931,7 +945,8 @@ extern "C" int grs_shared_prefix_attention(
     g.v = static_cast<const T*>(prefix_value); g.v_st = pv_st; g.v_sh = pv_sh;
     g.positions = batch; g.keys = num_prefix; g.heads = heads; g.kv_heads = kv_heads;
     g.group = group; g.D = head_width; g.scale_log2 = scale_log2;
-    const bool inlined = prefix_inline(batch, kv_heads, head_width, num_prefix);
+    const bool inlined =
+        prefix_inline(batch, kv_heads, head_width, num_prefix, (int)sizeof(T));
     const int sliced = inlined ? 0 : num_prefix;
     bool tensor_cores = false;
     if constexpr (std::is_same<T, __nv_bfloat16>::value) tensor_cores = grouped_tc_takes(g);
