@@ -59,23 +59,33 @@ __device__ __forceinline__ void pages_token(const PagesArgs<T>& a, int b, int h,
 }
 
 // fp32 pages, and bf16 layouts that the tensor-core form does not take.  One CTA
-// of four warps per (beam, head), every warp taking each fourth run of 32
-// tokens: a lane per key for the scores (the key row in vectors of kVec elements
-// against the query in shared memory, all requested before the first is used), a
-// lane per column for the values, eight keys' rows in flight.  The warps take
-// turns on the prefix slices too and meet in shared memory.  Bound by latency:
-// 64 beams with pages of up to 64 tokens behind 381 keys, 8 heads of 32, take 18
-// us with the slices' kernel.
-template <typename T, int DP, int kVec>
+// of four warps per beam and kG heads of a K/V head, every warp taking each
+// fourth run of 32 tokens: a lane per key for the scores (the key row in vectors
+// of kVec elements against the queries in shared memory, up to 16 requested before
+// the first is used), a lane per column for the values, 8 to 32 keys' rows in
+// flight.  The warps take turns on the prefix slices too and meet in shared
+// memory.  Bound by the latency of a run's loads, in large calls by the L1's rate
+// for a lane per row: 200 beams of 500 tokens, 8/8 heads of 128, 154 us, 5.3 TB/s.
+template <typename T, int DP, int kVec, int kG>
 __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
   constexpr int ND = (DP + 31) / 32;
-  __shared__ __align__(16) float q[DP];
-  __shared__ float sums[4][DP], tops[4], totals[4];
+  constexpr int kSums = kG == 1 ? 4 : 1;    // running sums of a score
+  constexpr int kFlight = DP <= 64 ? 32 : DP <= 128 ? 16 : 8;   // keys' value rows in flight
+  constexpr unsigned kSome = 0xffffffffu >> (32 - kFlight);
+  __shared__ __align__(16) float q[kG][DP];
+  __shared__ float sums[4][kG][DP], tops[4][kG], totals[4][kG];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads, h = head / a.group;
-  for (int d = threadIdx.x; d < DP; d += 128)
-    q[d] = d < a.D ? to_float(a.q[(int64_t)b * a.q_sb + (int64_t)head * a.q_sh + d]) * a.scale_log2
-                   : 0.f;
+  const int chunks = (a.group + kG - 1) / kG;             // of a K/V head's group
+  const int chunk = blockIdx.x % chunks, at = blockIdx.x / chunks;
+  const int b = at / a.kv_heads, h = at % a.kv_heads;
+  const int head0 = h * a.group + chunk * kG, heads = min(kG, a.group - chunk * kG);
+#pragma unroll
+  for (int g = 0; g < kG; ++g)
+    for (int d = threadIdx.x; d < DP; d += 128)
+      q[g][d] = g < heads && d < a.D
+                    ? to_float(a.q[(int64_t)b * a.q_sb + (int64_t)(head0 + g) * a.q_sh + d]) *
+                          a.scale_log2
+                    : 0.f;
 
   const int room = a.max_blocks * a.page;
   int past = a.lengths ? a.lengths[b] : 0;
@@ -87,51 +97,84 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
   const int total = a.prefix + past + (cur ? 1 : 0);
   __syncthreads();
 
-  float m = -INFINITY, l = 0.f, acc[ND];
+  float m[kG], l[kG], acc[kG][ND];          // l: this lane's keys
 #pragma unroll
-  for (int i = 0; i < ND; ++i) acc[i] = 0.f;
+  for (int g = 0; g < kG; ++g) {
+    m[g] = -INFINITY;
+    l[g] = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) acc[g][i] = 0.f;
+  }
   for (int t0 = 32 * warp; t0 < total; t0 += 128) {
     const int t = t0 + lane;
     const T *k = nullptr, *v = nullptr;
     if (t < total) pages_token(a, b, h, t, past, k, v);
     const unsigned valid = __ballot_sync(0xffffffffu, k != nullptr);
-    float s = -INFINITY;
+    float w[kG];                            // scores, then weights
+#pragma unroll
+    for (int g = 0; g < kG; ++g) w[g] = -INFINITY;
     if (k) {
-      float dot[4] = {0.f, 0.f, 0.f, 0.f};
+      float dot[kG][kSums];
+#pragma unroll
+      for (int g = 0; g < kG; ++g)
+#pragma unroll
+        for (int j = 0; j < kSums; ++j) dot[g][j] = 0.f;
       if constexpr (kVec > 1) {
+        constexpr int kAhead = DP / kVec < 16 ? DP / kVec : 16;   // vectors in flight
 #pragma unroll
-        for (int d = 0; d < DP; d += kVec) {
-          if (d >= a.D) break;
-          const uint4 w = __ldg(reinterpret_cast<const uint4*>(k + d));
-          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+        for (int d0 = 0; d0 < DP; d0 += kAhead * kVec) {
+          uint4 y[kAhead];
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) {
-            const float x = kVec == 4 ? __uint_as_float(words[j])
-                                      : __uint_as_float(j & 1 ? words[j / 2] & 0xffff0000u
-                                                              : words[j / 2] << 16);
-            dot[j & 3] = fmaf(q[d + j], x, dot[j & 3]);
+          for (int n = 0; n < kAhead; ++n) {
+            y[n] = make_uint4(0, 0, 0, 0);
+            if (d0 + n * kVec < a.D) y[n] = __ldg(reinterpret_cast<const uint4*>(k + d0 + n * kVec));
+          }
+#pragma unroll
+          for (int n = 0; n < kAhead; ++n) {
+            const uint32_t words[4] = {y[n].x, y[n].y, y[n].z, y[n].w};
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+              const float x = kVec == 4 ? __uint_as_float(words[j])
+                                        : __uint_as_float(j & 1 ? words[j / 2] & 0xffff0000u
+                                                                : words[j / 2] << 16);
+              const int d = d0 + n * kVec + j;
+#pragma unroll
+              for (int g = 0; g < kG; ++g)
+                dot[g][d % kSums] = fmaf(q[g][d], x, dot[g][d % kSums]);
+            }
           }
         }
       } else {
 #pragma unroll 8
-        for (int d = 0; d < a.D; ++d) dot[0] = fmaf(q[d], to_float(k[d]), dot[0]);
+        for (int d = 0; d < a.D; ++d) {
+          const float x = to_float(k[d]);
+#pragma unroll
+          for (int g = 0; g < kG; ++g) dot[g][0] = fmaf(q[g][d], x, dot[g][0]);
+        }
       }
-      s = (dot[0] + dot[1]) + (dot[2] + dot[3]);
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        w[g] = dot[g][0];
+        if constexpr (kSums == 4) w[g] = (w[g] + dot[g][1]) + (dot[g][2] + dot[g][3]);
+      }
     }
-    const float top = fmaxf(m, warp_max(s));
-    const float base = top == -INFINITY ? 0.f : top;
-    const float w = exp2f(s - base);
-    const float keep = exp2f(m - base);
-    l = l * keep + warp_sum(w);
 #pragma unroll
-    for (int i = 0; i < ND; ++i) acc[i] *= keep;
-    m = top;
+    for (int g = 0; g < kG; ++g) {
+      const float top = fmaxf(m[g], warp_max(w[g]));
+      const float base = top == -INFINITY ? 0.f : top;
+      w[g] = exp2f(w[g] - base);
+      const float keep = exp2f(m[g] - base);
+      l[g] = l[g] * keep + w[g];
 #pragma unroll
-    for (int j0 = 0; j0 < 32; j0 += 8) {
-      if (((valid >> j0) & 0xffu) == 0) continue;
-      float x[8][ND];
+      for (int i = 0; i < ND; ++i) acc[g][i] *= keep;
+      m[g] = top;
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+    for (int j0 = 0; j0 < 32; j0 += kFlight) {
+      if (((valid >> j0) & kSome) == 0) continue;
+      float x[kFlight][ND];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
         const T* vj = reinterpret_cast<const T*>(
             __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), j0 + j));
 #pragma unroll
@@ -141,63 +184,87 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesArgs<T> a) {
         }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float wj = __shfl_sync(0xffffffffu, w, j0 + j);
+      for (int j = 0; j < kFlight; ++j)
 #pragma unroll
-        for (int i = 0; i < ND; ++i) acc[i] = fmaf(wj, x[j][i], acc[i]);
-      }
+        for (int g = 0; g < kG; ++g) {
+          const float wj = __shfl_sync(0xffffffffu, w[g], j0 + j);
+#pragma unroll
+          for (int i = 0; i < ND; ++i) acc[g][i] = fmaf(wj, x[j][i], acc[g][i]);
+        }
     }
   }
 
   // join: weights exp2(lse_i - max lse); the pages' sums enter unnormalised
   asm volatile("griddepcontrol.wait;\n" ::: "memory");   // the prefix slices are written
-  const int64_t stride = (int64_t)a.batch * a.heads, row = blockIdx.x;
-  if (lane == 0) tops[warp] = m;
+  const int64_t stride = (int64_t)a.batch * a.heads, row0 = (int64_t)b * a.heads + head0;
+#pragma unroll
+  for (int g = 0; g < kG; ++g)
+    if (lane == 0) tops[warp][g] = m[g];
   __syncthreads();
-  float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  for (int i = lane; i < a.slices; i += 32) top = fmaxf(top, a.part_lse[i * stride + row]);
-  top = warp_max(top);
-  const float base = top == -INFINITY ? 0.f : top;
-  const float own = exp2f(m - base);
-  float norm = l * own;
 #pragma unroll
-  for (int i = 0; i < ND; ++i) acc[i] *= own;
-  for (int p0 = warp; p0 < a.slices; p0 += 16) {
-    float w[4], x[4][ND];
+  for (int g = 0; g < kG; ++g) {
+    const int64_t row = row0 + g;
+    const int slices = g < heads ? a.slices : 0;
+    float top = fmaxf(fmaxf(tops[0][g], tops[1][g]), fmaxf(tops[2][g], tops[3][g]));
+    for (int i = lane; i < slices; i += 32) top = fmaxf(top, a.part_lse[i * stride + row]);
+    top = warp_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    const float own = exp2f(m[g] - base);
+    float norm = warp_sum(l[g]) * own;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = p0 + 4 * j;
-      w[j] = i < a.slices ? a.part_lse[i * stride + row] : -INFINITY;
+    for (int i = 0; i < ND; ++i) acc[g][i] *= own;
+    for (int p0 = warp; p0 < slices; p0 += 16) {
+      float w[4], x[4][ND];
 #pragma unroll
-      for (int n = 0; n < ND; ++n) {
-        const int d = lane + 32 * n;
-        x[j][n] = i < a.slices && d < a.D ? a.part[(i * stride + row) * a.D + d] : 0.f;
+      for (int j = 0; j < 4; ++j) {
+        const int i = p0 + 4 * j;
+        w[j] = i < slices ? a.part_lse[i * stride + row] : -INFINITY;
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          const int d = lane + 32 * n;
+          x[j][n] = i < slices && d < a.D ? a.part[(i * stride + row) * a.D + d] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = exp2f(w[j] - base);
+        norm += e;
+#pragma unroll
+        for (int n = 0; n < ND; ++n) acc[g][n] = fmaf(e, x[j][n], acc[g][n]);
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float e = exp2f(w[j] - base);
-      norm += e;
-#pragma unroll
-      for (int n = 0; n < ND; ++n) acc[n] = fmaf(e, x[j][n], acc[n]);
-    }
+    for (int i = 0; i < ND; ++i)
+      if (lane + 32 * i < DP) sums[warp][g][lane + 32 * i] = acc[g][i];
+    if (lane == 0) totals[warp][g] = norm;
   }
-#pragma unroll
-  for (int i = 0; i < ND; ++i)
-    if (lane + 32 * i < DP) sums[warp][lane + 32 * i] = acc[i];
-  if (lane == 0) totals[warp] = norm;
   __syncthreads();
-  norm = (totals[0] + totals[1]) + (totals[2] + totals[3]);
-  const float inv = norm == 0.f ? 0.f : 1.f / norm;
-  T* o = a.out + (int64_t)b * a.o_sb + (int64_t)head * a.o_sh;
-  for (int d = threadIdx.x; d < a.D; d += 128)
-    o[d] = from_float<T>(((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) * inv);
+#pragma unroll
+  for (int g = 0; g < kG; ++g) {
+    if (g >= heads) break;
+    const float norm = (totals[0][g] + totals[1][g]) + (totals[2][g] + totals[3][g]);
+    const float inv = norm == 0.f ? 0.f : 1.f / norm;
+    T* o = a.out + (int64_t)b * a.o_sb + (int64_t)(head0 + g) * a.o_sh;
+    for (int d = threadIdx.x; d < a.D; d += 128)
+      o[d] = from_float<T>(
+          ((sums[0][g][d] + sums[1][g][d]) + (sums[2][g][d] + sums[3][g][d])) * inv);
+  }
+}
+
+// Whether a CTA takes four heads of a group: their keys and values are read
+// once, unless single heads fit the SMs (fp32, 32/8 heads of 128: 200 beams of
+// 500 tokens 503 -> 207 us, 4.0 TB/s, 32 of 64 17 -> 10; 4 of 1000 44 against 50;
+// 16/8 heads, 200 of 500 269 -> 205, 4 of 1000 44 against 50).
+template <typename T>
+static bool pages_rows_few(const PagesArgs<T>& p) {
+  return p.group > 1 && (int64_t)p.batch * p.heads > 148;
 }
 
 template <typename T>
 static int pages_rows_launch(const PagesArgs<T>& p, bool after_prefix, cudaStream_t stream) {
-  const int64_t rows = (int64_t)p.batch * p.heads;
-  if (rows > INT_MAX) return GRS_ERR_SHAPE;
+  const bool few = pages_rows_few(p);
+  const int64_t ctas = (int64_t)p.batch * p.kv_heads * (few ? (p.group + 3) / 4 : p.group);
+  if (ctas > INT_MAX) return GRS_ERR_SHAPE;
   constexpr int kVec = 16 / sizeof(T);
   const auto whole = [](const void* at) { return (reinterpret_cast<uintptr_t>(at) & 15) == 0; };
   const bool prefix_vec =
@@ -210,15 +277,18 @@ static int pages_rows_launch(const PagesArgs<T>& p, bool after_prefix, cudaStrea
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)rows);
+  config.gridDim = dim3((unsigned)ctas);
   config.blockDim = dim3(128);
   config.stream = counted(stream);
   config.attrs = &attr;
   config.numAttrs = after_prefix ? 1 : 0;
   const auto go = [&](auto width) {
     constexpr int DP = decltype(width)::value;
-    return vec ? cudaLaunchKernelEx(&config, pages_rows_kernel<T, DP, kVec>, p)
-               : cudaLaunchKernelEx(&config, pages_rows_kernel<T, DP, 1>, p);
+    if (few)
+      return vec ? cudaLaunchKernelEx(&config, pages_rows_kernel<T, DP, kVec, 4>, p)
+                 : cudaLaunchKernelEx(&config, pages_rows_kernel<T, DP, 1, 4>, p);
+    return vec ? cudaLaunchKernelEx(&config, pages_rows_kernel<T, DP, kVec, 1>, p)
+               : cudaLaunchKernelEx(&config, pages_rows_kernel<T, DP, 1, 1>, p);
   };
   const cudaError_t status = p.D <= 32    ? go(std::integral_constant<int, 32>{})
                              : p.D <= 64  ? go(std::integral_constant<int, 64>{})
