@@ -151,7 +151,7 @@ def test_c_abi_refusals():
         assert lib.grs_prompt_attention(*{**prompt, **change}.values()) == shape, change
     assert lib.grs_prompt_attention(*{**prompt, "tokens": 0}.values()) == 0
     prefix = dict(dtype=0, q=256, q_sb=1, q_sh=1, pk=256, pk_st=1, pk_sh=1, pv=256, pv_st=1,
-                  pv_sh=1, n=5, kc=256, vc=256, kc_sp=1, kc_st=1, kc_sh=1, bt=256, bt_s=1,
+                  pv_sh=1, n=300, kc=256, vc=256, kc_sp=1, kc_st=1, kc_sh=1, bt=256, bt_s=1,
                   blocks=1, lengths=256, pages=1, page=16, ck=None, cv=None, ck_sb=0, ck_sh=0,
                   valid=None, out=256, o_sb=1, o_sh=1, batch=2, heads=4, kv=2, width=32, scale=1.0,
                   work=256, bytes=1 << 30, status=None, stream=None)
@@ -162,7 +162,10 @@ def test_c_abi_refusals():
     for change in (dict(work=None), dict(bytes=8), dict(work=260)):
         assert lib.grs_shared_prefix_attention(*{**prefix, **change}.values()) == work, change
     assert lib.grs_shared_prefix_attention(*{**prefix, "batch": 0}.values()) == 0
+    # short prefixes are read by the pages' kernel and need no workspace
     assert lib.grs_shared_prefix_workspace_bytes(2, 4, 2, 32, 0, 32) == 0
+    assert lib.grs_shared_prefix_workspace_bytes(2, 4, 2, 32, 5, 16) == 0
+    assert lib.grs_shared_prefix_workspace_bytes(2, 4, 2, 32, 300, 16) > 0
     logits = dict(dtype=1, x=256, x_sb=9, out=256, o_sb=9, rows=1, vocab=9, tokens=256, i64=0,
                   t_sb=3, history=3, lengths=None, prompts=None, rep=None, pres=None, freq=None,
                   r=1.0, p=0.0, f=0.0, bias=None, b_sb=0, allowed=None, a_sb=0, fill=0.0,
