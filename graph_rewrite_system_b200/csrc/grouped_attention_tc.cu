@@ -20,8 +20,8 @@
 //   warp 18     zeroes the value rows behind a causal tile's last key
 // The launch's 640 x 96 registers are split 104 to a softmax thread and 64 to
 // the other warpgroup (512 x 104 + 128 x 64 = 61440 = 640 x 96).
-// Short prompts take CTAs of one slot, two to an SM (384 x 80 registers: 256 x
-// 104 + 128 x 32 = 30720): most of a short tile's time is its start and end,
+// Short prompts take CTAs of one slot, two to an SM (384 x 80 registers, split 104
+// to a softmax thread and 32 to the others): most of a short tile's time is its start and end,
 // which then run under the other CTA's blocks.
 //
 // Causal and wide-batch slices give the slots neighbouring row tiles over one

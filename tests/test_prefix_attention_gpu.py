@@ -108,6 +108,15 @@ def test_wide_batches(cuda_device, batch, group, prefix):
     _check(_call(cuda_device, args), args)
 
 
+@pytest.mark.parametrize("width", [30, 32, 64, 100, 128, 256])
+@pytest.mark.parametrize("group,prefix", [(2, 300), (3, 0), (5, 40), (9, 500)])
+def test_fp32_groups_in_wide_batches(cuda_device, group, prefix, width):
+    """More heads than SMs: a CTA takes four heads of a group, or what is left."""
+    args = _case(group + width, batch=80, heads=2 * group, kv_heads=2, width=width,
+                 prefix=prefix, max_len=45, dtype=FP32)
+    _check(_call(cuda_device, args), args)
+
+
 def test_empty_rows_are_zero(cuda_device):
     args = _case(1, batch=6, heads=4, kv_heads=2, width=64, prefix=0, max_len=20,
                  lengths=torch.tensor([0, 3, 0, 20, 0, 1], dtype=torch.int32))
