@@ -52,6 +52,7 @@ namespace grs {
 
 constexpr int GTC_KEYS = 128;
 constexpr int GTC_WINDOW = 260;             // offsets held for a tile's rows
+constexpr float GTC_ABOVE = 16.f;           // the reference above the maximum, log2 weight
 
 template <int DP, int kSlots>
 struct GtcShape {
@@ -120,6 +121,28 @@ __device__ __forceinline__ int offsets_up_to(const int32_t* __restrict__ offsets
   return lo + __popc(__ballot_sync(0xffffffffu, in));
 }
 
+// The two warps of 32 rows exchange the rows' maxima in fp32, over their bf16
+// ones in shared memory: they meet before and behind it, three phases of `pair`
+// from phase `met` on.  Returns the larger maximum.  A wait that gives up sets
+// `failed`, which ends the stream of blocks.  Out of line like gtc_wait_more: in
+// line, prompts took 1.5 to 2 % longer.
+__device__ __noinline__ float gtc_exact_top(float mine, float* maxima, int half, uint64_t* pair,
+                                            int met, int* failed) {
+  bool ok = true;
+  const auto meet = [&](int phase) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) sm100::mbar_arrive(pair);
+    if (ok) ok = sm100::mbar_wait_warp(pair, phase & 1);
+  };
+  meet(met);
+  if (ok) maxima[half * 32] = mine;
+  meet(met + 1);
+  const float top = fmaxf(mine, maxima[(half ^ 1) * 32]);
+  meet(met + 2);
+  if (!ok) *failed = 1;
+  return top;
+}
+
 template <int DP, int MODE>
 __global__ void __launch_bounds__(GtcShape<DP, gtc_slots(MODE)>::kThreads, 3 - gtc_slots(MODE))
 grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -140,8 +163,8 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   __shared__ int failed, drain_failed;
   // per softmax warp: first and last key of any row, last first and first last key
   __shared__ int4 spans[16];
-  // the window of offsets; then per slot the maxima [parity][half][row] in
-  // bf16; then its sums [half][row] in fp32
+  // the window of offsets; then per slot and 32 rows, which two warps share, the
+  // maxima [parity][half][row] in bf16, or maxima or sums [half][row] in fp32
   __shared__ int scratch[GTC_WINDOW > 256 * kSlots ? GTC_WINDOW : 256 * kSlots];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(gtc_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -497,8 +520,9 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     // this thread's half of the output columns, in runs of kCols
     constexpr int kCols = DP == 32 ? 16 : 32, kRuns = DP / 2 / kCols;
     const uint32_t t_o = tmem + lanes + S::kO + slot * DP + half * (DP / 2);
-    __nv_bfloat16* tops = reinterpret_cast<__nv_bfloat16*>(scratch + slot * 256);
-    float* sums = reinterpret_cast<float*>(scratch + slot * 256);
+    int* shared32 = scratch + slot * 256 + quarter * 64;
+    __nv_bfloat16* tops = reinterpret_cast<__nv_bfloat16*>(shared32) + lane;
+    float* sums = reinterpret_cast<float*>(shared32) + lane;
     uint64_t* pair = &pair_bar[slot * 4 + quarter];
     const auto tell = [&] {                // own value is in shared memory
       __syncwarp();
@@ -587,17 +611,29 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       ok = mbar_wait_warp(pair, met & 1);
       ++met;
     };
+    // Where `top`, from bf16, can lie more than 2^16 in weight above the row's
+    // maximum (bf16 steps are up to 2^-7 of the value), the pair exchanges the
+    // maxima themselves: rows with scores beyond 2^14 in the exponent of 2 would
+    // lose every weight.  Both threads of a row know the same `top`, so both warps
+    // do this or neither.
+    const auto exact = [&](float& top, float mine) {
+      const bool far =
+          position >= 0 && top > -INFINITY && fabsf(top) * c > 128.f * GTC_ABOVE;
+      if (!__any_sync(0xffffffffu, far)) return;
+      top = gtc_exact_top(mine, sums, half, pair, met, &failed);
+      met += 3;
+    };
 #pragma unroll 1
     for (int i = 0; i < blocks; ++i) {
       if (!(ok = mbar_wait_warp(&s_full[slot][half], i & 1))) break;
       tc_fence_after();
       bool dead;
       // The reference maximum need not be exact, only the same for both threads
-      // of a row: it passes between them in bf16, rounded up.  (Two copies: the
-      // partner may be one block behind, not two.)
-      const __nv_bfloat16 mine16 = __float2bfloat16_ru(scores(i, dead));
-      __nv_bfloat16* at = tops + (i & 1) * 256 + r;
-      at[half * 128] = mine16;
+      // of a row and near enough to the maximum: it passes between them in bf16,
+      // rounded up.  (Two copies: the partner may be one block behind, not two.)
+      const float mine = scores(i, dead);
+      __nv_bfloat16* at = tops + (i & 1) * 64;
+      at[half * 32] = __float2bfloat16_ru(mine);
       tc_fence_before();
       tell();
       // The weights are taken against the maximum so far; the partner's part of
@@ -609,18 +645,22 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (i > 0 && !dead) part = weights(m == -INFINITY ? 0.f : m * c);
       meet();
       if (!ok) break;
-      const float top =
-          fmaxf(__bfloat162float(mine16), __bfloat162float(at[(half ^ 1) * 128]));
-      const bool grown = top > m + slack;
+      float top = fmaxf(__bfloat162float(__float2bfloat16_ru(mine)),
+                        __bfloat162float(at[(half ^ 1) * 32]));
+      bool grown = top > m + slack;
       if (i == 0) {
+        exact(top, mine);
         m = top;
         if (!dead) part = weights(m == -INFINITY ? 0.f : m * c);
       } else if (__any_sync(0xffffffffu, grown)) {
         // Both threads of the row are here with their scores of this block, so
         // every product into O is done, and none starts before both are through.
+        exact(top, mine);
         tc_fence_after();
+        grown = top > m + slack;
         if (grown) m = top;
-        const float keep = grown ? gtc_exp2((before - m) * c) : 1.f;
+        // the difference of what the weights are taken against, as it rounded there
+        const float keep = grown ? gtc_exp2(__fmul_rn(before, c) - __fmul_rn(m, c)) : 1.f;
         l *= keep;
 #pragma unroll 1
         for (int q = 0; q < DP / 2; q += 16) {
@@ -656,12 +696,12 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     if (ok) ok = blocks > 0 ? mbar_wait_warp(&s_full[slot][half], blocks & 1)
                             : mbar_wait_warp(&q_full, 0);
     tc_fence_after();
-    // every warp of the slot has stored its last weights, so the maxima are read
-    sums[half * 128 + r] = l;
+    // both warps have stored their last weights, so the maxima are read
+    sums[half * 32] = l;
     tell();
     if (ok) meet();
     if (!ok) failed = 1;
-    l += sums[(half ^ 1) * 128 + r];
+    l += sums[(half ^ 1) * 32];
     const bool seen = end > begin && position >= 0;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int head = h * a.group + r - ((r * per_group) >> 16) * a.group;
@@ -766,7 +806,7 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         __syncwarp();
       }
       if (position >= 0 && ok && half == 0)
-        a.part_lse[at] = l == 0.f ? -INFINITY : m * c + log2f(l);
+        a.part_lse[at] = l == 0.f ? -INFINITY : __fmul_rn(m, c) + log2f(l);
     }
     tc_fence_before();
   }
