@@ -492,9 +492,10 @@ grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (!mbar_wait(&drain_bar, 0)) drain_failed = 1;
     } else if (kCausal && warp == kAux + 2 && clear) {
       const int at = 1 + 2 * (hi - 1 - lo);   // its place in the ring
-      // (the stream may still be a whole tile's work away from its last block)
+      // (the stream may still be a whole tile's work away from its last block; the
+      // lanes may read the flag at different times, the warp leaves as one)
       bool ok = false;
-      while (!ok && !*gave_up) ok = mbar_wait_warp(&last_full, 0);
+      while (!ok && !__any_sync(0xffffffffu, *gave_up)) ok = mbar_wait_warp(&last_full, 0);
       if (ok) {
         uint8_t* block = ring + (at % S::kStages) * S::kTile;
         constexpr int kPieces = S::kRow / 16;
