@@ -10,6 +10,7 @@ import ctypes
 from pathlib import Path
 import re
 import struct
+import threading
 
 import torch
 
@@ -126,34 +127,42 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-_PINNED_STREAM: list[int] = []
+class _Pins(threading.local):
+    """Streams pinned by this thread, innermost last: raw handle, stream."""
+
+    def __init__(self):
+        self.stack: list[tuple[int, torch.cuda.Stream]] = []
+
+
+_PINS = _Pins()
 
 
 def current_stream() -> int:
     """Raw handle of the stream pinned by an enclosing ``pinned_stream()``
-    block, else of torch's current stream."""
-    if _PINNED_STREAM:
-        return _PINNED_STREAM[-1]
+    block of this thread, else of torch's current stream."""
+    if _PINS.stack:
+        return _PINS.stack[-1][0]
     return torch.cuda.current_stream().cuda_stream
 
 
 def stream_of(t: torch.Tensor) -> int:
-    if _PINNED_STREAM:
-        return _PINNED_STREAM[-1]
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """Raw handle of the stream that launches on t's device go to."""
+    return stream_on(t.get_device())
 
 
 class pinned_stream:
-    """Resolve torch's current stream once and launch every call inside the
-    block on it (a beam-search level makes ~60 launches; looking the stream
-    up per launch costs more host time than the launch itself)."""
+    """Resolve torch's current stream once and launch every call that this
+    thread makes inside the block, on that stream's device, on it (a beam-search
+    level makes ~60 launches; looking the stream up per launch costs more host
+    time than the launch itself)."""
 
     def __enter__(self):
-        _PINNED_STREAM.append(torch.cuda.current_stream().cuda_stream)
+        stream = torch.cuda.current_stream()
+        _PINS.stack.append((stream.cuda_stream, stream))
         return self
 
     def __exit__(self, *exc):
-        _PINNED_STREAM.pop()
+        _PINS.stack.pop()
 
 
 def words_of(name: str) -> struct.Struct:
@@ -174,22 +183,39 @@ def current_device() -> int:
     return torch._C._cuda_getDevice()
 
 
+def _pin_of(index: int) -> torch.cuda.Stream | None:
+    for _, stream in reversed(_PINS.stack):
+        if stream.device_index == index:
+            return stream
+    return None
+
+
 def stream_on(index: int) -> int:
-    """Raw handle of the pinned stream, else of torch's current stream of
-    device `index` (what ``stream_of`` gives, without building stream objects)."""
-    if _PINNED_STREAM:
-        return _PINNED_STREAM[-1]
+    """Raw handle of the stream pinned on device `index`, else of torch's
+    current stream there."""
+    if _PINS.stack:
+        pin = _pin_of(index)
+        if pin is not None:
+            return pin.cuda_stream
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def scratch(like: torch.Tensor, nbytes: int, stream: int) -> torch.Tensor:
-    """Uninitialised bytes on like's device for one call enqueued on `stream`:
-    when that is not torch's current stream, the allocator is told of the use."""
-    work = like.new_empty(nbytes, dtype=torch.uint8)
-    if _PINNED_STREAM and nbytes:
-        if stream != torch.cuda.current_stream(like.device).cuda_stream:
-            work.record_stream(torch.cuda.ExternalStream(stream, device=like.device))
-    return work
+def elsewhere(index: int):
+    """None when device `index` is current and its launches go to torch's
+    current stream; else the context that makes them so.  A call that allocates
+    enters it first: the allocator hands out memory that only the current stream
+    is done with."""
+    if _PINS.stack:
+        pin = _pin_of(index)
+        if pin is not None and (index != current_device() or pin.cuda_stream
+                                != torch._C._cuda_getCurrentRawStream(index)):
+            return torch.cuda.stream(pin)
+    return None if index == current_device() else torch.cuda.device(index)
+
+
+def scratch(like: torch.Tensor, nbytes: int) -> torch.Tensor:
+    """Uninitialised bytes on like's device for one call on the current stream."""
+    return like.new_empty(nbytes, dtype=torch.uint8)
 
 
 def require_cuda(*tensors: torch.Tensor | None) -> None:

@@ -68,8 +68,9 @@ def shared_prefix_attention(
     device = query.get_device()
     if device < 0:
         _lib.require_cuda(query)
-    if device != _lib.current_device():
-        with torch.cuda.device(device):
+    place = _lib.elsewhere(device)
+    if place is not None:
+        with place:
             return shared_prefix_attention(
                 query, prefix_key, prefix_value, key_cache, value_cache, block_table, lengths,
                 current_key=current_key, current_value=current_value,
@@ -151,16 +152,16 @@ def shared_prefix_attention(
         word = _status_for(query, device, status)
     if _entry is None:
         _entry = _lib.words_entry("grs_shared_prefix_attention")
-    stream = _lib.stream_on(device)
     work, need = 0, _workspace_bytes(batch, heads, kv_heads, width, num_prefix, columns * page)
     if need:
-        scratch = _lib.scratch(query, need, stream)
+        scratch = _lib.scratch(query, need)
         work = scratch.data_ptr()
     code = _entry(_pack(
         code, query.data_ptr(), q[0], q[1], prefix_key.data_ptr(), pk[0], pk[1],
         prefix_value.data_ptr(), pv[0], pv[1], num_prefix, keys, values, c[0], c[1], c[2], table,
         table_row, columns, past, pages, page, cur_key, cur_value, cur[0], cur[1], valid,
-        out.data_ptr(), o[0], o[1], batch, heads, kv_heads, width, scale, work, need, word, stream))
+        out.data_ptr(), o[0], o[1], batch, heads, kv_heads, width, scale, work, need, word,
+        _lib.stream_on(device)))
     if code:
         _lib.check(code, "shared-prefix attention")
     return out

@@ -124,8 +124,9 @@ def prompt_attention(
     device = query.get_device()
     if device < 0:
         _lib.require_cuda(query)
-    if device != _lib.current_device():
-        with torch.cuda.device(device):
+    place = _lib.elsewhere(device)
+    if place is not None:
+        with place:
             return prompt_attention(query, key, value, offsets, scale=scale, out=out,
                                     status=status)
     if query.dim() != 3 or key.dim() != 3:

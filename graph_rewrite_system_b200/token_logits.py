@@ -85,8 +85,9 @@ def adjust_logits(
     device = logits.get_device()
     if device < 0:
         _lib.require_cuda(logits)
-    if device != _lib.current_device():
-        with torch.cuda.device(device):
+    place = _lib.elsewhere(device)
+    if place is not None:
+        with place:
             return adjust_logits(logits, tokens=tokens, lengths=lengths,
                                  prompt_lengths=prompt_lengths, repetition=repetition,
                                  presence=presence, frequency=frequency, bias=bias,
