@@ -989,8 +989,10 @@ extern "C" int grs_shared_prefix_attention(
     int64_t o_sh, int batch, int heads, int kv_heads, int head_width, float scale, void* workspace,
     int64_t workspace_bytes, int32_t* status, void* stream) {
   using namespace grs;
-  if (batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_width <= 0 ||
-      head_width > 256 || !std::isfinite(scale) || num_prefix < 0 || max_blocks < 0 || num_pages < 0 ||
+  constexpr int kMost = 1 << 30;             // a tile's rows and a slice's keys add two places
+  if (batch < 0 || batch >= kMost || heads <= 0 || heads >= kMost || kv_heads <= 0 ||
+      heads % kv_heads || head_width <= 0 || head_width > 256 || !std::isfinite(scale) ||
+      num_prefix < 0 || num_prefix >= kMost || max_blocks < 0 || num_pages < 0 ||
       (max_blocks > 0 && (page_size <= 0 || !block_table || !lengths ||
                           (int64_t)max_blocks * page_size > INT_MAX / 2)) ||
       (max_blocks > 0 && num_pages > 0 && (!key_cache || !value_cache)) ||

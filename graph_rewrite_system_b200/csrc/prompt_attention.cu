@@ -39,8 +39,10 @@ extern "C" int grs_prompt_attention(int dtype, const void* query, int64_t q_st, 
                                     int64_t o_st, int64_t o_sh, int tokens, int heads,
                                     int kv_heads, int head_width, float scale, int clear_rest,
                                     int32_t* status, void* stream) {
-  if (tokens < 0 || sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads ||
-      head_width <= 0 || head_width > 256 ||
+  // below 2^30: the search among the offsets and a tile's positions add two places
+  constexpr int kMost = 1 << 30;
+  if (tokens < 0 || tokens >= kMost || sequences < 0 || sequences >= kMost || heads <= 0 ||
+      heads >= kMost || kv_heads <= 0 || heads % kv_heads || head_width <= 0 || head_width > 256 ||
       !std::isfinite(scale))
     return GRS_ERR_SHAPE;
   if (tokens == 0) return GRS_OK;

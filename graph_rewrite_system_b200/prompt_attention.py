@@ -85,6 +85,8 @@ def _check_heads(query: torch.Tensor, heads: int, kv_heads: int, width: int) -> 
         raise ValueError("head widths from 1 to 256 are supported")
     if not kv_heads or not heads or heads % kv_heads:
         raise ValueError("query heads must be a multiple of the key/value heads")
+    if heads >= 1 << 30:
+        raise ValueError("at most 2^30 heads")
     return code
 
 
@@ -146,6 +148,8 @@ def prompt_attention(
             or not offsets.is_contiguous() or offsets.get_device() != device):
         _lib.require_cuda(offsets)
         raise ValueError("offsets must be a contiguous int32 [sequences + 1] on the query's device")
+    if offsets.numel() > 1 << 30:
+        raise ValueError("at most 2^30 offsets")
     scale = _check_scale(scale, width)
     fresh = out is None
     if fresh:
