@@ -15,6 +15,8 @@
 
 namespace grs {
 
+constexpr float GA_LOG2E = 1.4426950408889634f;
+
 template <typename T>
 struct GroupedArgs {
   const T* q; int64_t q_sp, q_sh;          // [positions, heads, D], D contiguous

@@ -991,7 +991,7 @@ extern "C" int grs_shared_prefix_attention(
   using namespace grs;
   constexpr int kMost = 1 << 30;             // a tile's rows and a slice's keys add two places
   if (batch < 0 || batch >= kMost || heads <= 0 || heads >= kMost || kv_heads <= 0 ||
-      heads % kv_heads || head_width <= 0 || head_width > 256 || !std::isfinite(scale) ||
+      heads % kv_heads || head_width <= 0 || head_width > 256 || !std::isfinite(scale * GA_LOG2E) ||
       num_prefix < 0 || num_prefix >= kMost || max_blocks < 0 || num_pages < 0 ||
       (max_blocks > 0 && (page_size <= 0 || !block_table || !lengths ||
                           (int64_t)max_blocks * page_size > INT_MAX / 2)) ||
@@ -1007,7 +1007,7 @@ extern "C" int grs_shared_prefix_attention(
                    (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return GRS_ERR_WORKSPACE;
   const int group = heads / kv_heads;
-  const float scale_log2 = scale * 1.4426950408889634f;
+  const float scale_log2 = scale * GA_LOG2E;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const auto go = [&](auto zero) {
     using T = decltype(zero);

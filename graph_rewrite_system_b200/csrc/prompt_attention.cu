@@ -19,7 +19,7 @@ int prompt_attention(const void* query, int64_t q_st, int64_t q_sh, const void* 
   a.v = static_cast<const T*>(value); a.v_st = v_st; a.v_sh = v_sh;
   a.positions = a.keys = tokens;
   a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.D = head_width;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * GA_LOG2E;
   a.offsets = offsets; a.sequences = sequences;
   a.out = static_cast<T*>(out); a.o_sp = o_st; a.o_sh = o_sh;
   a.clear_rest = clear_rest;
@@ -43,7 +43,7 @@ extern "C" int grs_prompt_attention(int dtype, const void* query, int64_t q_st, 
   constexpr int kMost = 1 << 30;
   if (tokens < 0 || tokens >= kMost || sequences < 0 || sequences >= kMost || heads <= 0 ||
       heads >= kMost || kv_heads <= 0 || heads % kv_heads || head_width <= 0 || head_width > 256 ||
-      !std::isfinite(scale))
+      !std::isfinite(scale * grs::GA_LOG2E))
     return GRS_ERR_SHAPE;
   if (tokens == 0) return GRS_OK;
   if (!query || !key || !value || !offsets || !out) return GRS_ERR_SHAPE;

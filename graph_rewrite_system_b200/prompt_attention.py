@@ -22,6 +22,7 @@ from .paged_attention import _STATUS, _status_word
 _pack = _lib.words_of("grs_prompt_attention").pack
 _entry = None
 _STATUS_AT: dict[int, int] = {}          # device index -> address of its status word
+_LARGEST_SCALE = 3.4e38 / math.log2(math.e)
 
 
 def _status_for(query: torch.Tensor, device: int, status: torch.Tensor | None) -> int:
@@ -92,8 +93,8 @@ def _check_heads(query: torch.Tensor, heads: int, kv_heads: int, width: int) -> 
 
 def _check_scale(scale: float | None, width: int) -> float:
     scale = 1.0 / math.sqrt(width) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if not abs(scale) <= _LARGEST_SCALE:      # NaN too
+        raise ValueError("scale * log2(e) must be finite in fp32")
     return scale
 
 

@@ -65,3 +65,29 @@ def test_c_abi():
         assert lib.grs_prompt_attention(*{**prompt, **change}.values()) == -4, change
     for change in (dict(batch=far), dict(n=far), dict(heads=far, kv=1)):
         assert lib.grs_shared_prefix_attention(*{**prefix, **change}.values()) == -4, change
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38, 1e39, -1e300])
+def test_scales_beyond_fp32(lifted, scale):
+    """The kernels hold scale * log2(e) in fp32: infinite, it made every row NaN."""
+    from graph_rewrite_system_b200.prefix_attention import shared_prefix_attention
+    from graph_rewrite_system_b200.prompt_attention import prompt_attention
+
+    with pytest.raises(ValueError, match="scale"):
+        prompt_attention(_z(6, 4, 32), _z(6, 2, 32), _z(6, 2, 32),
+                         torch.tensor([0, 6], dtype=torch.int32), scale=scale, status=STATUS)
+    with pytest.raises(ValueError, match="scale"):
+        shared_prefix_attention(_z(6, 4, 32), _z(9, 2, 32), _z(9, 2, 32), scale=scale,
+                                status=STATUS)
+
+
+def test_c_abi_scales():
+    from graph_rewrite_system_b200 import _lib
+
+    for scale in (2.4e38, -3.4e38):
+        assert _lib.lib().grs_prompt_attention(
+            0, 256, 1, 1, 256, 1, 1, 256, 1, 1, 256, 1, 256, 1, 1, 1, 4, 2, 32, scale, 0, None,
+            None) == -4
+        assert _lib.lib().grs_shared_prefix_attention(
+            0, 256, 1, 1, 256, 1, 1, 256, 1, 1, 300, None, None, 0, 0, 0, None, 0, 0, None, 0, 0,
+            None, None, 0, 0, None, 256, 1, 1, 2, 4, 2, 32, scale, None, 0, None, None) == -4
