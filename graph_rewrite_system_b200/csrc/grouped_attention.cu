@@ -4,13 +4,13 @@
 //
 // One CTA takes 32 rows of one K/V head (64 at widths above 128) and walks
 // 64-key tiles; a thread holds 4 rows x 4 keys of the scores and 4 rows x DP/16
-// columns of the output.  Four CTAs share an SM (two at widths above 64): their
-// barriers fall at different times, and their tiles fill the SMs where one tile
-// of 128 rows and 512 threads left SMs idle (8 heads of 32, one prompt of 1001
-// tokens: 86 -> 45 us; 2 x 2048 tokens of 16/4 heads of 64: 675 -> 560 us; 16 rows
-// 53 and 710 us, 2 rows a thread 60 and 800 us).  Both products read 16-byte
-// vectors from shared memory (8 for 64 multiply-adds, 12 for 128 at DP = 128)
-// into packed fp32x2 multiply-adds: the scores sum even and odd dimensions apart,
+// columns of the output.  Four CTAs share an SM (two at widths above 64, one
+// above 128): their barriers fall at different times, and their tiles fill the
+// SMs where one tile of 128 rows and 512 threads left SMs idle (8 heads of 32, one
+// prompt of 1001 tokens: 86 -> 45 us; 2 x 2048 tokens of 16/4 heads of 64: 675 ->
+// 560 us; 16 rows 53 and 710 us, 2 rows a thread 60 and 800 us).  Both products
+// read 16-byte vectors from shared memory (8 for 64 multiply-adds, 12 for 128 at
+// DP = 128) into packed fp32x2 multiply-adds: the scores sum even and odd dimensions apart,
 // so both factors are pairs as they lie.  Eight steps of either are unrolled, so
 // that loads run ahead of the multiply-adds (5 to 9 % over 2 and 1).  The next K
 // tile is fetched (cp.async) under the value product and the next V tile under
@@ -19,7 +19,8 @@
 // are fp32.  Bound by the shared-memory reads that feed the multiply-adds, and in
 // small calls by the chain of a tile: 2 x 2048 tokens of 32/8 heads of 128 take
 // 2.01 ms, 34 TFLOP/s of the 74 of the fp32 pipes; 8 heads of 32, 2704 tokens in
-// four prompts, 69 us.
+// four prompts, 69 us.  bf16 rows are widened one element a load: 2 x 2048 tokens
+// of 32/8 heads take 3.8 ms at width 128 (18 TFLOP/s) and 7.6 ms at 256.
 #include <algorithm>
 #include <cfloat>
 #include <climits>

@@ -11,7 +11,9 @@
 // warps per scheduler hide them where two with 128 keys a thread did not.  The
 // running maximum is lazy: O and the sum are rescaled only when the maximum
 // has grown by more than 2^32 in weight, which fp32 sums and bf16 weights (same
-// relative rounding at any exponent) do not notice.  The commit that hands a
+// relative rounding at any exponent) do not notice.  A row's two threads exchange
+// it in bf16, rounded up, and in fp32 where that rounding could reach 2^16 in
+// weight (scores of 1e5: 159 instead of 94 us for 2 x 2048 tokens).  The commit that hands a
 // slot its next scores also covers the slot's previous P V, so the softmax
 // warps may rescale O in place without a further barrier.
 //
@@ -22,7 +24,8 @@
 // the other warpgroup (512 x 104 + 128 x 64 = 61440 = 640 x 96).
 // Short prompts take CTAs of one slot, two to an SM (384 x 80 registers, split 104
 // to a softmax thread and 32 to the others): most of a short tile's time is its start and end,
-// which then run under the other CTA's blocks.
+// which then run under the other CTA's blocks.  At those 80 registers a thread
+// spills 92 to 140 bytes.
 //
 // Causal and wide-batch slices give the slots neighbouring row tiles over one
 // K/V stream (each K/V block is loaded once for 256 rows); a batch of at most
@@ -30,8 +33,8 @@
 // Weights are rounded to bf16 for the value product; sums, statistics and
 // outputs are fp32 until the one rounding of the output.
 //
-// 16384 tokens of 32/8 heads of 128 take 1.65 ms, 1336 TFLOP/s or 0.80 of the
-// measured burst of the library's product; 2 x 8192 tokens 0.92 ms, of width 64
+// 16384 tokens of 32/8 heads of 128 take 1.65 to 1.68 ms by the card, up to 1336
+// TFLOP/s or 0.80 of the measured burst of the library's product; 2 x 8192 tokens 0.92 ms, of width 64
 // 0.77 ms (719 TFLOP/s: half the products' work per exponential).  On 2 x 8192
 // tokens the tensor pipe is active 64 % and the special-function pipe 65 % of
 // the time: what remains is the chain of a slot's turn.

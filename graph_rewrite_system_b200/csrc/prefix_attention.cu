@@ -783,7 +783,8 @@ struct PrefixPlan {
 // fp32 rows: the count that gives the SM with most CTAs the least work, a CTA
 // paying about one 64-key block for its start and end (64 beams of 32/8 heads of
 // 128 over 4000 keys: 192 / 320 / 448 / 576 / 832 CTAs took 224 / 209 / 204 / 174
-// / 190 us, 16 beams 144 / 256 / 336 / 512 CTAs 68 / 68 / 81 / 78 us).
+// / 190 us, 16 beams 144 / 256 / 336 / 512 CTAs 68 / 68 / 81 / 78 us).  Measured
+// up to width 128; above, where an SM holds one CTA, it is taken as it is.
 static PrefixPlan rows_plan(int batch, int group, int kv_heads, int D, int keys) {
   if (keys <= 0) return {0, 0, 0};
   const int64_t rows = grouped_rows_tile(D);
@@ -809,7 +810,7 @@ static PrefixPlan rows_plan(int batch, int group, int kv_heads, int D, int keys)
 // Tensor cores: the count whose waves of 148 CTAs take the fewest 128-key
 // blocks, each wave paying about four blocks for its start and end and every
 // part the write and read of its fp32 sums, mostly in L2 (a block takes about
-// 1.1 us).
+// 1.1 us; measured at width 128 and taken for the narrower ones too).
 static PrefixPlan tc_plan(int batch, int heads, int kv_heads, int D, int keys) {
   if (keys <= 0) return {0, 0, 0};
   const int group = heads / kv_heads;
@@ -853,8 +854,9 @@ static bool prefix_inline(int batch, int kv_heads, int D, int num_prefix, int it
 }
 
 // Slices of each beam's pages: enough CTAs of a long table to fill 148 SMs
-// four times when there are few beams, none for less than 256 tokens.  They are
-// joined by a kernel of its own when they are cut, or when there are so many
+// four times when there are few beams, none for less than 256 tokens (by the
+// table's width: the lengths are on the device, and slices past a beam's length
+// have no keys).  They are joined by a kernel of its own when they are cut, or when there are so many
 // CTAs that those which wait for the prefix kernel to join it would keep the
 // rest from the SMs it leaves free (512 beams x 8 K/V heads over 16384 keys: 179
 // -> 168 us; 200 x 8 over 2048 keys: 39 against 41 us, so not there).
@@ -1045,7 +1047,11 @@ extern "C" int grs_shared_prefix_attention(
       p.prefix = num_prefix;
     }
     p.part = part; p.part_lse = lse;
-    if (pages.separate) p.page_part = part, p.page_lse = lse; p.slices = plan.parts;
+    p.slices = plan.parts;
+    if (pages.separate) {
+      p.page_part = part;
+      p.page_lse = lse;
+    }
     p.out = static_cast<T*>(output); p.o_sb = o_sb; p.o_sh = o_sh;
     p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.group = group; p.D = head_width;
     p.scale_log2 = scale_log2; p.status = status;
