@@ -67,7 +67,7 @@ def adjust_logits(
 ) -> torch.Tensor:
     """Adjusted copy of logits [rows, vocab] (bf16 or fp32, contiguous rows),
     or ``out`` (``out=logits`` adjusts in place; otherwise it must not overlap
-    them).
+    them, and never the other inputs).
 
     For every token v of row b, in this order: if v is among the first
     ``lengths[b]`` (default: all) of ``tokens[b]`` (int32 or int64 [rows,
@@ -142,6 +142,8 @@ def adjust_logits(
         out_row = out.stride(0)
         if rows > 1 and out_row != row and out.data_ptr() == logits.data_ptr():
             raise ValueError("out must be the logits themselves or not overlap them")
+        if bias_ptr == out.data_ptr() and bias is not None and out.numel():
+            raise ValueError("out must not be the bias")
     if not rows or not vocab:
         return out
     if _entry is None:

@@ -91,3 +91,14 @@ def test_c_abi_scales():
         assert _lib.lib().grs_shared_prefix_attention(
             0, 256, 1, 1, 256, 1, 1, 256, 1, 1, 300, None, None, 0, 0, 0, None, 0, 0, None, 0, 0,
             None, None, 0, 0, None, 256, 1, 1, 2, 4, 2, 32, scale, None, 0, None, None) == -4
+
+
+def test_out_is_not_the_bias(lifted):
+    """A bias row that every row of logits adds would be overwritten by the first."""
+    from graph_rewrite_system_b200.token_logits import adjust_logits
+
+    logits = torch.zeros(3, 70)
+    room = torch.zeros(3, 70)
+    for bias in (room, room[0], room[:1]):
+        with pytest.raises(ValueError, match="bias"):
+            adjust_logits(logits, bias=bias, out=room)
