@@ -31,7 +31,7 @@ def test_sequences(lifted):
     """The search among the offsets adds two places: they stay below 2^30."""
     from graph_rewrite_system_b200.prompt_attention import prompt_attention
 
-    offsets = torch.empty((1 << 30) + 1, dtype=torch.int32)      # never touched
+    offsets = torch.empty((1 << 30) + 1, dtype=torch.int32, device="meta")
     with pytest.raises(ValueError, match="2\\^30"):
         prompt_attention(_z(6, 4, 32), _z(6, 2, 32), _z(6, 2, 32), offsets, status=STATUS)
 
