@@ -44,3 +44,12 @@ extern "C" int grs_shared_prefix_attention_words(const int64_t* words) {
 extern "C" int grs_adjust_logits_words(const int64_t* words) {
   return grs::call_words(&grs_adjust_logits, words);
 }
+extern "C" int grs_rotate_positions_words(const int64_t* words) {
+  return grs::call_words(&grs_rotate_positions, words);
+}
+extern "C" int grs_append_tokens_words(const int64_t* words) {
+  return grs::call_words(&grs_append_tokens, words);
+}
+extern "C" int grs_quantized_attention_words(const int64_t* words) {
+  return grs::call_words(&grs_quantized_attention, words);
+}

@@ -10,6 +10,8 @@
 // (paged_cache.py:99-105): that decrement is the page's last one in scan
 // order, found with an atomicMax over scan positions, and a single-CTA ordered
 // compaction appends the pages.
+#include <climits>
+
 #include "grs_common.cuh"
 
 namespace grs {
@@ -28,7 +30,7 @@ __device__ __forceinline__ int blocks_for(int length, int page) { return (length
 __global__ void cache_fork_kernel(int32_t* __restrict__ refcounts,
                                   const int32_t* __restrict__ free_list,
                                   const int32_t* __restrict__ free_count, int capacity,
-                                  const int32_t* __restrict__ ptable, int64_t pstride,
+                                  const int32_t* __restrict__ ptable, int64_t pstride, int pcols,
                                   const int32_t* __restrict__ plengths, int n, int page,
                                   int32_t* __restrict__ ctable, int64_t cstride,
                                   int32_t* __restrict__ clengths, int ccols,
@@ -41,6 +43,12 @@ __global__ void cache_fork_kernel(int32_t* __restrict__ refcounts,
   const int keep = offset == 0 ? nb : nb - 1;  // pages shared with the child
   const int32_t* prow = ptable + (int64_t)i * pstride;
   int32_t* crow = ctable + (int64_t)i * cstride;
+  if (len < 0 || nb > pcols) {
+    set_status(status, GRS_ERR_LENGTH);
+    for (int j = 0; j < ccols; ++j) crow[j] = 0;
+    clengths[i] = 0;
+    return;
+  }
   if (keep + 1 > ccols) { set_status(status, GRS_ERR_SHAPE); return; }
   // Error paths record a status and write page 0 so that no table ever holds
   // an out-of-range page id.
@@ -77,6 +85,12 @@ __global__ void cache_fork_kernel(int32_t* __restrict__ refcounts,
   crow[keep] = page_id;
   for (int j = keep + 1; j < ccols; ++j) crow[j] = 0;
   clengths[i] = len + 1;
+}
+
+// The pages that the fork of n children took, off the free count.
+__global__ void cache_taken_kernel(int32_t* free_count, int n) {
+  const int fc = *free_count;
+  *free_count = fc >= n ? fc - n : 0;
 }
 
 // Copy `rows` rows of `row_bytes` bytes from page src to page dst within one
@@ -420,6 +434,23 @@ extern "C" int grs_cache_init(int32_t* refcounts, int32_t* free_list, int32_t* f
   return GRS_OK;
 }
 
+extern "C" int grs_cache_fork(int32_t* refcounts, int32_t* free_list, int32_t* free_count,
+                              int capacity, const int32_t* parent_table, int64_t parent_stride,
+                              int parent_cols, const int32_t* parent_lengths, int n, int page_size,
+                              int32_t* child_table, int64_t child_stride, int32_t* child_lengths,
+                              int child_cols, int32_t* status, void* stream) {
+  cudaStream_t s = (cudaStream_t)stream;
+  if (n < 0 || capacity <= 0 || page_size <= 0 || child_cols <= 0) return GRS_ERR_SHAPE;
+  if (n == 0) return GRS_OK;
+  cache_fork_kernel<<<ceil_div(n, 128), 128, 0, grs::counted(s)>>>(
+      refcounts, free_list, free_count, capacity, parent_table, parent_stride, parent_cols,
+      parent_lengths, n, page_size, child_table, child_stride, child_lengths, child_cols, status);
+  GRS_CUDA_CHECK_LAUNCH();
+  cache_taken_kernel<<<1, 1, 0, grs::counted(s)>>>(free_count, n);
+  GRS_CUDA_CHECK_LAUNCH();
+  return GRS_OK;
+}
+
 extern "C" int grs_cache_append(int elem_bytes, int32_t* refcounts, int32_t* free_list,
                                 int32_t* free_count, int capacity, const int32_t* parent_table,
                                 int64_t parent_stride, const int32_t* parent_lengths, int n,
@@ -437,8 +468,8 @@ extern "C" int grs_cache_append(int elem_bytes, int32_t* refcounts, int32_t* fre
   if ((new_readout_keys == nullptr) != (new_readout_values == nullptr)) return GRS_ERR_SHAPE;
   if (n == 0) return GRS_OK;
   cache_fork_kernel<<<ceil_div(n, 128), 128, 0, grs::counted(s)>>>(refcounts, free_list, free_count, capacity,
-                                                      parent_table, parent_stride, parent_lengths,
-                                                      n, page_size, child_table, child_stride,
+                                                      parent_table, parent_stride, INT_MAX,
+                                                      parent_lengths, n, page_size, child_table, child_stride,
                                                       child_lengths, child_cols, status);
   GRS_CUDA_CHECK_LAUNCH();
   CacheArenas ar{keys, values, actions, readout_keys, readout_values, layers, capacity,

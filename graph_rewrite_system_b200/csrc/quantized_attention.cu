@@ -1,0 +1,695 @@
+// One query per sequence against 8-bit pages: grs_quantized_attention.
+//
+// softmax(scale q k) v with k and v an e4m3 code times the scale of its page and
+// head.  e4m3 is exact in f16, so the codes go into f16 tensor-core products as
+// they are and the scales join in fp32: the key scale multiplies the score, the
+// value scale's log2 is added to it before the exponential that weighs the values.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
+#include "e4m3.cuh"
+
+namespace grs {
+
+struct QuantArgs {
+  const void* q; int64_t q_sb, q_sh;
+  const uint8_t* kc; const uint8_t* vc; int64_t c_sp, c_st, c_sh;
+  const float* ks; const float* vs; int64_t s_sp;
+  const int32_t* bt; int64_t bt_s; int columns; const int32_t* lengths; int pages, page;
+  uint32_t magic; int shift;                // t / page = umulhi(t, magic) >> shift; magic 0: page 1
+  float* part; float* part_lse; int slices;
+  void* out; int64_t o_sb, o_sh;
+  int batch, heads, kv_heads, group, D;
+  float scale_log2;
+  int32_t* status;
+};
+
+constexpr float QA_LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ int quant_length(const QuantArgs& a, int b) {
+  const int room = a.columns * a.page, length = __ldg(a.lengths + b);
+  const int past = min(max(length, 0), room);
+  if (past != length && threadIdx.x == 0) set_status(a.status, GRS_ERR_LENGTH);
+  if (a.pages == 0 && past > 0) {           // no address to read from
+    if (threadIdx.x == 0) set_status(a.status, GRS_ERR_BAD_PAGE);
+    return 0;
+  }
+  return past;
+}
+
+// ---- any layout ---------------------------------------------------------------
+// One CTA of four warps per sequence and query head, every warp taking each fourth
+// run of 32 tokens: a lane per key for the scores, a lane per column for the
+// values, byte loads.  For widths that are no multiple of 8 and rows off 8 bytes.
+template <typename T>
+__global__ void __launch_bounds__(128) quant_rows_kernel(QuantArgs a) {
+  constexpr int ND = 8;
+  __shared__ float q[256], sums[4][256], tops[4], totals[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads, h = head / a.group;
+  const T* query = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)head * a.q_sh;
+  for (int d = threadIdx.x; d < a.D; d += 128) q[d] = to_float(query[d]) * a.scale_log2;
+  const int past = quant_length(a, b);
+  __syncthreads();
+  float m = -INFINITY, l = 0.f, acc[ND] = {};
+  for (int t0 = 32 * warp; t0 < past; t0 += 128) {
+    const int t = t0 + lane;
+    const uint8_t* v = nullptr;
+    float s = -INFINITY, vs = 0.f;
+    if (t < past) {
+      const int page = __ldg(a.bt + (int64_t)b * a.bt_s + t / a.page);
+      if (page < 0 || page >= a.pages) {
+        set_status(a.status, GRS_ERR_BAD_PAGE);
+      } else {
+        const int64_t at = (int64_t)page * a.c_sp + (int64_t)(t % a.page) * a.c_st + h * a.c_sh;
+        v = a.vc + at;
+        vs = a.vs[page * a.s_sp + h];
+        s = 0.f;
+        for (int d = 0; d < a.D; ++d) s = fmaf(q[d], from_e4m3(a.kc[at + d]), s);
+        s *= a.ks[page * a.s_sp + h];
+      }
+    }
+    const float top = fmaxf(m, warp_max(s)), base = top == -INFINITY ? 0.f : top;
+    const float p = exp2f(s - base), keep = exp2f(m - base);
+    l = l * keep + p;
+    m = top;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) acc[i] *= keep;
+    for (int j = 0; j < 32; ++j) {
+      const uint8_t* vj = reinterpret_cast<const uint8_t*>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), j));
+      const float w = __shfl_sync(0xffffffffu, p * vs, j);
+      if (!vj) continue;
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+        if (lane + 32 * i < a.D) acc[i] = fmaf(w, from_e4m3(vj[lane + 32 * i]), acc[i]);
+    }
+  }
+  l = warp_sum(l);
+  if (lane == 0) tops[warp] = m, totals[warp] = l;
+#pragma unroll
+  for (int i = 0; i < ND; ++i) sums[warp][lane + 32 * i] = acc[i];
+  __syncthreads();
+  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const float base = top == -INFINITY ? 0.f : top;
+  float w[4], norm = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = exp2f(tops[i] - base);
+    norm += w[i] * totals[i];
+  }
+  const float inv = norm == 0.f ? 0.f : 1.f / norm;
+  T* out = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)head * a.o_sh;
+  for (int d = threadIdx.x; d < a.D; d += 128)
+    out[d] = from_float<T>(((w[0] * sums[0][d] + w[1] * sums[1][d]) +
+                            (w[2] * sums[2][d] + w[3] * sums[3][d])) * inv);
+}
+
+// ---- tensor cores ---------------------------------------------------------------
+// A warp streams tiles of 16 tokens of one (sequence, K/V head) through a ring of
+// its own in shared memory: cp.async fetches the rows in 16-byte pieces wherever
+// their pages lie, three tiles ahead.  Keys, then value columns, are the 16 rows of
+// mma.m16n8k16, the group's query heads its columns.  The order in which a product
+// sums its inner dimension is free, so a lane takes whole pieces of a row, and a
+// lane's column index picks its piece of the value rows; two tokens' codes are
+// interleaved by byte permutes before they are widened.
+constexpr int QT_WARPS = 4;
+constexpr int QT_STAGES = 4;
+constexpr float QT_LIFT = 9.f;              // weights are at most 2^(9 + 6): f16 holds them to
+constexpr float QT_SLACK = 6.f;             // 2^-24, 2^-33 of the largest
+constexpr uint32_t QT_ABSENT = 0xffffffffu; // key scale of a token that is not there
+
+__device__ __forceinline__ void qt_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                       uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void qt_widen(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\n"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
+      : "=r"(lo), "=r"(hi) : "r"(codes));
+}
+__device__ __forceinline__ float qt_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t qt_pack(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// x - its f16 value, for the second part of an fp32 operand
+__device__ __forceinline__ float qt_rest(float x) { return x - __half2float(__float2half_rn(x)); }
+__device__ __forceinline__ uint32_t qt_transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+// log2 of a positive scale, exact for powers of two
+__device__ __forceinline__ float qt_log2(float s) {
+  const uint32_t bits = __float_as_uint(s);
+  const float part = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+  const float e = (float)((int)((bits >> 23) & 0xff) - 127);
+  return (bits & 0x7fffffu) ? e + __log2f(part) : e;
+}
+template <int kBytes>
+__device__ __forceinline__ void qt_fetch(uint32_t to, const void* from, bool there) {
+  const int n = there ? kBytes : 0;         // the rest is zeros
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;\n" ::"r"(to), "l"(from), "r"(n), "n"(kBytes) : "memory");
+}
+__device__ __forceinline__ void qt_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void qt_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(kPending) : "memory");
+}
+
+template <int DP>
+struct QtShape {
+  static constexpr int kRow = DP;                         // bytes of a staged row
+  static constexpr int kTile = 16 * kRow;
+  static constexpr int kStage = 2 * kTile + 128;          // K, V, the tokens' scales
+  static constexpr int kRing = QT_STAGES * kStage;
+  static constexpr int kKey = DP >= 64 ? DP / 64 : 1;     // key pieces of a lane
+  static constexpr int kKeyWords = DP >= 64 ? 4 : 2;      // of such a piece
+  static constexpr int kWords = DP / 32;                  // value words of a lane and token
+  static constexpr int kSum = DP + 4;                     // row of the joined sums (floats)
+  // Pieces of 16 bytes change places within their 128-byte line, by the row, so that
+  // the eight lanes of a read's phase meet all banks: for keys rows 0 and 1 (widths
+  // below 128 lie side by side already), for values rows 0, 2, 4 and 6.
+  static __device__ __forceinline__ int key_at(int row, int byte) {
+    const int flip = DP >= 128 ? (row & 1) << 6 : 0;
+    return row * kRow + (byte ^ flip);
+  }
+  static __device__ __forceinline__ int value_at(int row, int byte) {
+    const int flip = DP >= 64 ? (row & 6) << 4 : (row & 4) << 3;
+    return (row * kRow + byte) ^ flip;
+  }
+};
+
+template <typename T, int DP, int kTiles, int kPiece>
+__global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
+  using S = QtShape<DP>;
+  constexpr bool kSplit = std::is_same<T, float>::value;  // operands in two f16 parts
+  constexpr int kParts = kSplit ? 2 : 1, kHeads = 8 * kTiles;
+  constexpr int kSteps = S::kKey * S::kKeyWords;          // products of the scores
+  extern __shared__ __align__(128) uint8_t qt_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int chunks = (a.group + kHeads - 1) / kHeads;
+  const int b = blockIdx.x / (a.kv_heads * chunks), h = blockIdx.x / chunks % a.kv_heads;
+  const int head0 = h * a.group + blockIdx.x % chunks * kHeads;
+  const int n_heads = min(kHeads, (h + 1) * a.group - head0);
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+  const int past = quant_length(a, b), tiles = (past + 15) / 16;
+  const int lo = (int)((int64_t)tiles * blockIdx.y / gridDim.y);
+  const int hi = (int)((int64_t)tiles * (blockIdx.y + 1) / gridDim.y);
+  uint8_t* ring = qt_smem + warp * S::kRing;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const int32_t* table = a.bt + (int64_t)b * a.bt_s;
+  const uint8_t* const kh = a.kc + h * a.c_sh;
+  const uint8_t* const vh = a.vc + h * a.c_sh;
+
+  // lanes i and i + 16 hold the page of token i of the tile to be requested next
+  const auto column = [&](int token) {
+    return a.magic ? (int)(__umulhi((uint32_t)token, a.magic) >> a.shift) : token;
+  };
+  const auto page_of = [&](int tile) {
+    const int token = tile * 16 + (lane & 15);
+    return tile < hi && token < past ? __ldg(table + column(token)) : -1;
+  };
+  int page = page_of(lo + warp);
+  const auto request = [&](int tile, int stage) {
+    if (tile >= hi) {
+      qt_commit();
+      return;
+    }
+    const int token = tile * 16 + (lane & 15);
+    const bool there = token < past && page >= 0 && page < a.pages;
+    if (token < past && !there) set_status(a.status, GRS_ERR_BAD_PAGE);
+    const int64_t at =
+        there ? (int64_t)page * a.c_sp + (int64_t)(token - column(token) * a.page) * a.c_st : -1;
+    const uint32_t base = ring_at + stage * S::kStage;
+    constexpr int kLanes = DP / kPiece, kRows = 32 / kLanes;   // of a row; of a round
+    const int byte = lane % kLanes * kPiece;
+#pragma unroll
+    for (int i = 0; i < 16 / kRows; ++i) {
+      const int row = i * kRows + lane / kLanes;
+      const int64_t from = __shfl_sync(0xffffffffu, at, row);
+      const bool fetch = from >= 0 && byte < a.D;
+      qt_fetch<kPiece>(base + S::key_at(row, byte), fetch ? kh + from + byte : kh, fetch);
+      qt_fetch<kPiece>(base + S::kTile + S::value_at(row, byte), fetch ? vh + from + byte : vh,
+                       fetch);
+    }
+    // scales: the keys' by the first 16 lanes, the values' by the others
+    const uint32_t scale = base + 2 * S::kTile + 4 * lane;
+    if (there)
+      qt_fetch<4>(scale, (lane < 16 ? a.ks : a.vs) + page * a.s_sp + h, true);
+    else
+      asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(scale), "r"(lane < 16 ? QT_ABSENT : 0u) : "memory");
+    qt_commit();
+    page = page_of(tile + QT_WARPS);
+  };
+#pragma unroll
+  for (int i = 0; i < QT_STAGES - 1; ++i) request(lo + warp + i * QT_WARPS, i);
+
+  // Queries of head g, scaled by a power of two to at most 2^14: f16 then holds a
+  // bf16 element down to 2^-25 of the head's largest exactly, and two parts hold
+  // fp32 to 2^-22.
+  uint32_t qf[kTiles][kSteps][2][kParts];
+  float unit[kTiles][2];                    // of heads 2t, 2t + 1: log2(e) scale / 2^k
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    const bool on = 8 * n + g < n_heads;
+    const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb +
+                 (int64_t)(head0 + (on ? 8 * n + g : 0)) * a.q_sh;
+    float x[S::kKey][4 * S::kKeyWords], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < S::kKey; ++i)
+#pragma unroll
+      for (int e = 0; e < 4 * S::kKeyWords; ++e) {
+        const int d = (t + 4 * i) * 4 * S::kKeyWords + e;
+        x[i][e] = on && d < a.D ? to_float(q[d]) : 0.f;
+        const float y = fabsf(x[i][e]);
+        if (y <= 3.402823466e38f) top = fmaxf(top, y);
+      }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    int k = top > 0.f ? 13 + 127 - (int)(__float_as_uint(top) >> 23) : 0;
+    k = max(min(k, 120), -120);
+    const float lift = __uint_as_float((uint32_t)(k + 127) << 23);
+#pragma unroll
+    for (int i = 0; i < S::kKey; ++i)
+#pragma unroll
+      for (int e = 0; e < 4 * S::kKeyWords; e += 4)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float u = x[i][e + 2 * c] * lift, v = x[i][e + 2 * c + 1] * lift;
+          uint32_t (&to)[kParts] = qf[n][i * S::kKeyWords + e / 4][c];
+          to[0] = qt_pack(u, v);
+          if constexpr (kSplit) to[1] = qt_pack(qt_rest(u), qt_rest(v));
+        }
+    const float mine = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) unit[n][r] = __shfl_sync(0xffffffffu, mine, (2 * t + r) * 4);
+  }
+
+  // columns (d, d + 1) x heads (2t, 2t + 1)
+  float acc[kTiles][2 * S::kWords][4];
+  float m[kTiles][2], l[kTiles][2], w_top[kTiles][2];     // maxima of the scores and of the
+#pragma unroll                                            // scores with the value scale
+  for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+    for (int j = 0; j < 2 * S::kWords; ++j) acc[n][j][0] = acc[n][j][1] = acc[n][j][2] = acc[n][j][3] = 0.f;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) m[n][r] = w_top[n][r] = -INFINITY, l[n][r] = 0.f;
+  }
+  int stage = 0;
+  for (int tile = lo + warp; tile < hi; tile += QT_WARPS) {
+    qt_wait<QT_STAGES - 2>();
+    __syncwarp();
+    request(tile + (QT_STAGES - 1) * QT_WARPS, stage == 0 ? QT_STAGES - 1 : stage - 1);
+    const uint8_t* at = ring + stage * S::kStage;
+    stage = stage + 1 == QT_STAGES ? 0 : stage + 1;
+
+    float s[kTiles][4];                     // tokens (g, g + 8) x heads (2t, 2t + 1)
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < S::kKey; ++i) {
+      uint32_t k[2][4];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if constexpr (DP >= 64) {
+          const uint4 x = *reinterpret_cast<const uint4*>(at + S::key_at(g + 8 * r, 16 * (t + 4 * i)));
+          k[r][0] = x.x, k[r][1] = x.y, k[r][2] = x.z, k[r][3] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(at + S::key_at(g + 8 * r, 8 * t));
+          k[r][0] = x.x, k[r][1] = x.y;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < S::kKeyWords; ++e) {
+        uint32_t f[4];
+        qt_widen(k[0][e], f[0], f[2]);
+        qt_widen(k[1][e], f[1], f[3]);
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int p = 0; p < kParts; ++p) {
+            const auto& q = qf[n][i * S::kKeyWords + e];
+            qt_mma(s[n], f, q[0][p], q[1][p]);
+          }
+      }
+    }
+    const uint32_t* scales = reinterpret_cast<const uint32_t*>(at + 2 * S::kTile);
+    float z[kTiles][4];
+    bool grown = false;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint32_t key = scales[g + 8 * r];
+      const float value = qt_log2(__uint_as_float(scales[16 + g + 8 * r]));
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float& x = s[n][2 * r + c];
+          x = key == QT_ABSENT ? -INFINITY : x * unit[n][c] * __uint_as_float(key);
+          z[n][2 * r + c] = x + value;
+          grown |= x > m[n][c] + QT_SLACK || z[n][2 * r + c] > w_top[n][c] + QT_SLACK;
+        }
+    }
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = fmaxf(s[n][c], s[n][c + 2]), y = fmaxf(z[n][c], z[n][c + 2]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
+          }
+          x = fmaxf(x, m[n][c]);
+          y = fmaxf(y, w_top[n][c]);
+          if (x != -INFINITY) l[n][c] *= qt_exp2(m[n][c] - x);
+          const float keep = y == -INFINITY ? 1.f : qt_exp2(w_top[n][c] - y);
+#pragma unroll
+          for (int j = 0; j < 2 * S::kWords; ++j) {
+            acc[n][j][c] *= keep;
+            acc[n][j][c + 2] *= keep;
+          }
+          m[n][c] = x;
+          w_top[n][c] = y;
+        }
+    }
+    uint32_t p[kTiles][2][kParts];          // weights of tokens 2t, 2t + 1 (+ 8) of head g
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      float w[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float top = m[n][c & 1], high = w_top[n][c & 1];
+        l[n][c & 1] += qt_exp2(s[n][c] - (top == -INFINITY ? 0.f : top));
+        w[c] = qt_exp2(z[n][c] - (high == -INFINITY ? 0.f : high - QT_LIFT));
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        p[n][r][0] = qt_transpose(qt_pack(w[2 * r], w[2 * r + 1]));
+        if constexpr (kSplit)
+          p[n][r][1] = qt_transpose(qt_pack(qt_rest(w[2 * r]), qt_rest(w[2 * r + 1])));
+      }
+    }
+    // values of tokens 2t, 2t + 1, 2t + 8, 2t + 9
+    const uint8_t* values = at + S::kTile;
+#pragma unroll
+    for (int i = 0; i < (DP + 127) / 128; ++i) {
+      constexpr int kRead = S::kWords < 4 ? S::kWords : 4;   // words of a read
+      uint32_t v[4][kRead];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const uint8_t* x = values + S::value_at(2 * t + (n & 1) + 8 * (n >> 1),
+                                                128 * i + 4 * kRead * g);
+        if constexpr (kRead == 4) {
+          const uint4 y = *reinterpret_cast<const uint4*>(x);
+          v[n][0] = y.x, v[n][1] = y.y, v[n][2] = y.z, v[n][3] = y.w;
+        } else if constexpr (kRead == 2) {
+          const uint2 y = *reinterpret_cast<const uint2*>(x);
+          v[n][0] = y.x, v[n][1] = y.y;
+        } else {
+          v[n][0] = *reinterpret_cast<const uint32_t*>(x);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kRead; ++e)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const unsigned pick = c ? 0x7362u : 0x5140u;
+          uint32_t f[4];
+          qt_widen(__byte_perm(v[0][e], v[1][e], pick), f[0], f[1]);
+          qt_widen(__byte_perm(v[2][e], v[3][e], pick), f[2], f[3]);
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int k = 0; k < kParts; ++k)
+              qt_mma(acc[n][2 * (4 * i + e) + c], f, p[n][0][k], p[n][1][k]);
+        }
+    }
+  }
+
+  // the warps' sums meet in shared memory
+  qt_wait<0>();
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(qt_smem);        // [warps][kHeads][kSum]
+  float* tops = sums + QT_WARPS * kHeads * S::kSum;       // [warps][kHeads][3]
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[n][r] += __shfl_xor_sync(0xffffffffu, l[n][r], o);
+      const int head = 8 * n + 2 * t + r;
+      float* row = sums + (warp * kHeads + head) * S::kSum;
+      constexpr int kRead = S::kWords < 4 ? S::kWords : 4;
+#pragma unroll
+      for (int j = 0; j < S::kWords; ++j)
+        *reinterpret_cast<float4*>(row + 128 * (j / 4) + 4 * kRead * g + 4 * (j % 4)) = make_float4(
+            acc[n][2 * j][r], acc[n][2 * j][r + 2], acc[n][2 * j + 1][r], acc[n][2 * j + 1][r + 2]);
+      if (g == 0) {
+        float* top = tops + (warp * kHeads + head) * 3;
+        top[0] = m[n][r];
+        top[1] = l[n][r];
+        top[2] = w_top[n][r];
+      }
+    }
+  __syncthreads();
+  const int64_t stride = (int64_t)a.batch * a.heads;
+  for (int head = warp; head < n_heads; head += QT_WARPS) {
+    float top = -INFINITY, high = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < QT_WARPS; ++i) {
+      top = fmaxf(top, tops[(i * kHeads + head) * 3]);
+      high = fmaxf(high, tops[(i * kHeads + head) * 3 + 2]);
+    }
+    const float base = top == -INFINITY ? 0.f : top, w_base = high == -INFINITY ? 0.f : high;
+    float norm = 0.f, w[QT_WARPS];
+#pragma unroll
+    for (int i = 0; i < QT_WARPS; ++i) {
+      const float* x = tops + (i * kHeads + head) * 3;
+      norm = fmaf(exp2f(x[0] - base), x[1], norm);
+      w[i] = exp2f(x[2] - w_base);
+    }
+    // the references' difference in two halves: either alone may leave the range
+    const float half = exp2f(0.5f * (w_base - base - QT_LIFT));
+    const float inv = norm == 0.f ? 0.f : half / norm;
+    const int64_t row = (int64_t)b * a.heads + head0 + head;
+    for (int d = 4 * lane; d < a.D; d += 128) {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < QT_WARPS; ++i) {
+        const float4 y =
+            *reinterpret_cast<const float4*>(sums + (i * kHeads + head) * S::kSum + d);
+        x.x = fmaf(w[i], y.x, x.x);
+        x.y = fmaf(w[i], y.y, x.y);
+        x.z = fmaf(w[i], y.z, x.z);
+        x.w = fmaf(w[i], y.w, x.w);
+      }
+      const float o[4] = {x.x * inv * half, x.y * inv * half, x.z * inv * half, x.w * inv * half};
+      if (a.slices > 1) {
+        *reinterpret_cast<float4*>(a.part + (blockIdx.y * stride + row) * a.D + d) =
+            make_float4(o[0], o[1], o[2], o[3]);
+      } else {
+        T* to = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)(head0 + head) * a.o_sh + d;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = from_float<T>(o[i]);
+      }
+    }
+    if (a.slices > 1 && lane == 0)
+      a.part_lse[blockIdx.y * stride + row] = norm == 0.f ? -INFINITY : base + log2f(norm);
+  }
+}
+
+// A sequence's slices joined by their weights: a warp per (sequence, head).
+template <typename T>
+__global__ void __launch_bounds__(128) quant_join_kernel(QuantArgs a) {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int64_t stride = (int64_t)a.batch * a.heads;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= stride) return;
+  float top = -INFINITY;
+  for (int i = lane; i < a.slices; i += 32) top = fmaxf(top, a.part_lse[i * stride + row]);
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int d = 4 * lane; d < (a.D + 127) / 128 * 128; d += 128) {
+    float norm = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 < a.slices; p0 += 32) {
+      const float w = p0 + lane < a.slices ? exp2f(a.part_lse[(p0 + lane) * stride + row] - base) : 0.f;
+      norm += warp_sum(w);
+      const int n = min(32, a.slices - p0);
+      for (int i0 = 0; i0 < n; i0 += 8) {
+        float4 y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i0 + i < n && d < a.D)
+            y[i] = *reinterpret_cast<const float4*>(a.part + ((p0 + i0 + i) * stride + row) * a.D + d);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float wi = __shfl_sync(0xffffffffu, w, min(i0 + i, 31));
+          x.x = fmaf(wi, y[i].x, x.x);
+          x.y = fmaf(wi, y[i].y, x.y);
+          x.z = fmaf(wi, y[i].z, x.z);
+          x.w = fmaf(wi, y[i].w, x.w);
+        }
+      }
+    }
+    const float inv = norm == 0.f ? 0.f : 1.f / norm;
+    if (d < a.D) {
+      T* to = static_cast<T*>(a.out) + row / a.heads * a.o_sb + row % a.heads * a.o_sh + d;
+      const float o[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[i] = from_float<T>(o[i]);
+    }
+  }
+}
+
+// Whether a CTA takes 16 query heads of a group (two column tiles); above width 128
+// their accumulators and queries would not fit the registers.
+static bool quant_wide(int group, int D) { return group > 8 && D <= 128; }
+
+// Slices of each sequence: enough CTAs to fill the SMs several times, at least 256
+// tokens each (by the table's width: the lengths are on the device).
+static int quant_slices(int batch, int heads, int kv_heads, int D, int64_t room) {
+  const int group = heads / kv_heads, chunk = quant_wide(group, D) ? 16 : 8;
+  const int64_t tasks = (int64_t)batch * kv_heads * ((group + chunk - 1) / chunk);
+  const int64_t want = (4 * 3 * 148 + tasks - 1) / tasks;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, 128, room / 256}));
+}
+
+static bool quant_aligned(const QuantArgs& p, int bytes) {
+  const uint64_t bits = reinterpret_cast<uintptr_t>(p.kc) | reinterpret_cast<uintptr_t>(p.vc) |
+                        (uint64_t)p.c_sp | (uint64_t)p.c_st | (uint64_t)p.c_sh | (uint64_t)p.D;
+  return bits % bytes == 0;
+}
+
+template <typename T, int DP, int kTiles, int kPiece>
+static int quant_mma_run(const QuantArgs& p, cudaStream_t stream) {
+  using S = QtShape<DP>;
+  constexpr int kSums = QT_WARPS * 8 * kTiles * (S::kSum + 3) * 4;
+  constexpr int smem = std::max(QT_WARPS * S::kRing, kSums);
+  const int chunks = (p.group + 8 * kTiles - 1) / (8 * kTiles);
+  const int64_t tasks = (int64_t)p.batch * p.kv_heads * chunks;
+  const int64_t rows = (int64_t)p.batch * p.heads;
+  if (tasks > INT_MAX || rows > INT_MAX) return GRS_ERR_SHAPE;
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(quant_mma_kernel<T, DP, kTiles, kPiece>,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return GRS_ERR_CUDA;
+  quant_mma_kernel<T, DP, kTiles, kPiece>
+      <<<dim3((unsigned)tasks, p.slices), 32 * QT_WARPS, smem, counted(stream)>>>(p);
+  GRS_CUDA_CHECK_LAUNCH();
+  if (p.slices > 1) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)((rows + 3) / 4));
+    config.blockDim = dim3(128);
+    config.stream = counted(stream);
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    if (cudaLaunchKernelEx(&config, quant_join_kernel<T>, p) != cudaSuccess) return GRS_ERR_CUDA;
+    GRS_CUDA_CHECK_LAUNCH();
+  }
+  return GRS_OK;
+}
+
+template <typename T, int kTiles, int kPiece>
+static int quant_mma_width(const QuantArgs& p, cudaStream_t stream) {
+  if (p.D <= 32) return quant_mma_run<T, 32, kTiles, kPiece>(p, stream);
+  if (p.D <= 64) return quant_mma_run<T, 64, kTiles, kPiece>(p, stream);
+  if (kTiles == 2 || p.D <= 128) return quant_mma_run<T, 128, kTiles, kPiece>(p, stream);
+  return quant_mma_run<T, 256, 1, kPiece>(p, stream);
+}
+
+template <typename T>
+static int quant_launch(const QuantArgs& p, cudaStream_t stream) {
+  if (quant_aligned(p, 8)) {
+    const auto go = [&](auto tiles) -> int {
+      constexpr int kTiles = decltype(tiles)::value;
+      return quant_aligned(p, 16) ? quant_mma_width<T, kTiles, 16>(p, stream)
+                                  : quant_mma_width<T, kTiles, 8>(p, stream);
+    };
+    return quant_wide(p.group, p.D) ? go(std::integral_constant<int, 2>{})
+                                    : go(std::integral_constant<int, 1>{});
+  }
+  const int64_t rows = (int64_t)p.batch * p.heads;
+  if (rows > INT_MAX) return GRS_ERR_SHAPE;
+  quant_rows_kernel<T><<<(unsigned)rows, 128, 0, counted(stream)>>>(p);
+  GRS_CUDA_CHECK_LAUNCH();
+  return GRS_OK;
+}
+
+}  // namespace grs
+
+extern "C" int64_t grs_quantized_attention_workspace_bytes(int batch, int heads, int kv_heads,
+                                                           int head_width, int64_t page_tokens) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  const int slices = grs::quant_slices(batch, heads, kv_heads, head_width, page_tokens);
+  return slices > 1 ? (int64_t)slices * batch * heads * (head_width + 1) * 4 : 0;
+}
+
+extern "C" int grs_quantized_attention(
+    int dtype, const void* query, int64_t q_sb, int64_t q_sh, const void* key_cache,
+    const void* value_cache, int64_t c_sp, int64_t c_st, int64_t c_sh, const float* key_scale,
+    const float* value_scale, int64_t s_sp, const int32_t* block_table, int64_t bt_stride,
+    int max_blocks, const int32_t* lengths, int num_pages, int page_size, void* output,
+    int64_t o_sb, int64_t o_sh, int batch, int heads, int kv_heads, int head_width, float scale,
+    void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  using namespace grs;
+  constexpr int kMost = 1 << 30;
+  if ((dtype != GRS_DTYPE_F32 && dtype != GRS_DTYPE_BF16) || batch < 0 || batch >= kMost ||
+      heads <= 0 || heads >= kMost || kv_heads <= 0 || heads % kv_heads || head_width <= 0 ||
+      head_width > 256 || !std::isfinite(scale * QA_LOG2E) || max_blocks < 0 || num_pages < 0 ||
+      page_size <= 0 || page_size >= kMost || (int64_t)max_blocks * page_size >= kMost)
+    return GRS_ERR_SHAPE;
+  if (batch == 0) return GRS_OK;
+  if (!query || !output || !lengths || (max_blocks > 0 && !block_table) ||
+      (num_pages > 0 && (!key_cache || !value_cache || !key_scale || !value_scale)))
+    return GRS_ERR_SHAPE;
+  const int64_t room = (int64_t)max_blocks * page_size;
+  const int64_t need =
+      grs_quantized_attention_workspace_bytes(batch, heads, kv_heads, head_width, room);
+  if (need > 0 && (!workspace || workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return GRS_ERR_WORKSPACE;
+  QuantArgs p = {};
+  p.q = query; p.q_sb = q_sb; p.q_sh = q_sh;
+  p.kc = static_cast<const uint8_t*>(key_cache); p.vc = static_cast<const uint8_t*>(value_cache);
+  p.c_sp = c_sp; p.c_st = c_st; p.c_sh = c_sh;
+  p.ks = key_scale; p.vs = value_scale; p.s_sp = s_sp;
+  p.bt = block_table; p.bt_s = bt_stride; p.columns = max_blocks; p.lengths = lengths;
+  p.pages = num_pages; p.page = page_size;
+  if (page_size > 1) {                      // exact below 2^31 (round-up method)
+    while ((1ll << (p.shift + 1)) < page_size) ++p.shift;
+    p.magic = (uint32_t)(((1ull << (32 + p.shift)) + page_size - 1) / page_size);
+  }
+  p.slices = quant_slices(batch, heads, kv_heads, head_width, room);
+  p.part = static_cast<float*>(workspace);
+  p.part_lse = p.part + (int64_t)p.slices * batch * heads * head_width;
+  p.out = output; p.o_sb = o_sb; p.o_sh = o_sh;
+  p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads;
+  p.D = head_width; p.scale_log2 = scale * QA_LOG2E; p.status = status;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == GRS_DTYPE_F32 ? quant_launch<float>(p, s) : quant_launch<__nv_bfloat16>(p, s);
+}

@@ -28,7 +28,6 @@ import torch
 from . import _lib
 
 
-
 @dataclass(frozen=True)
 class PrefixHandle:
     """Logical ownership of one paged causal prefix (paged_cache.py:8-13)."""
@@ -37,31 +36,15 @@ class PrefixHandle:
     length: int
 
 
-class PagedKVCache:
-    """Fixed-size device KV/action pool with prefix sharing and COW tail pages."""
+class PagePool:
+    """Page ownership in device memory: reference counts, the LIFO free list and
+    the status word that its kernels record errors in."""
 
-    def __init__(self, *, layers: int, capacity: int, page_size: int, heads: int,
-                 head_width: int, model_width: int, device, dtype: torch.dtype,
-                 gather_backend: str = "vectorized"):
-        if min(layers, capacity, page_size, heads, head_width, model_width) <= 0:
-            raise ValueError("all cache dimensions must be positive")
-        if gather_backend not in {"loop", "vectorized"}:
-            raise ValueError("gather_backend must be 'loop' or 'vectorized'")
+    def __init__(self, capacity: int, page_size: int, device):
         device = torch.device(device)
         if device.type != "cuda":
-            raise RuntimeError("PagedKVCache lives in CUDA memory (no CPU fallback)")
-        if dtype not in (torch.bfloat16, torch.float32):
-            raise ValueError("PagedKVCache arenas are bf16 or fp32")
-        self.layers, self.capacity, self.page_size = layers, capacity, page_size
-        self.heads, self.head_width, self.model_width = heads, head_width, model_width
-        self.device, self.dtype, self.gather_backend = device, dtype, gather_backend
-        self.keys = torch.empty(layers, capacity, page_size, heads, head_width,
-                                device=device, dtype=dtype)
-        self.values = torch.empty_like(self.keys)
-        self.actions = torch.empty(capacity, page_size, model_width, device=device, dtype=dtype)
-        self.readout_keys = torch.empty(capacity, page_size, heads, head_width,
-                                        device=device, dtype=dtype)
-        self.readout_values = torch.empty_like(self.readout_keys)
+            raise RuntimeError(f"{type(self).__name__} lives in CUDA memory (no CPU fallback)")
+        self.capacity, self.page_size, self.device = capacity, page_size, device
         i32 = dict(device=device, dtype=torch.int32)
         self._refcounts = torch.empty(capacity, **i32)
         self._free = torch.empty(capacity, **i32)
@@ -70,14 +53,14 @@ class PagedKVCache:
         self._status = torch.zeros(1, **i32)
         _lib.check(_lib.lib().grs_cache_init(
             self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
-            self._last_pos.data_ptr(), capacity, self._stream()), "PagedKVCache")
+            self._last_pos.data_ptr(), capacity, self._stream()), type(self).__name__)
 
     def reset(self) -> None:
         """Return every page to the free list (the state of a new cache)."""
         self._status.zero_()
         _lib.check(_lib.lib().grs_cache_init(
             self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
-            self._last_pos.data_ptr(), self.capacity, self._stream()), "PagedKVCache")
+            self._last_pos.data_ptr(), self.capacity, self._stream()), type(self).__name__)
 
     def status_tensor(self) -> torch.Tensor:
         """The device status word (0 = ok) without synchronising."""
@@ -117,7 +100,87 @@ class PagedKVCache:
         code = int(self._status.item())
         if code:
             self._status.zero_()
-            _lib.check(code, "PagedKVCache")
+            _lib.check(code, type(self).__name__)
+
+    def release_device(self, table: torch.Tensor, lengths: torch.Tensor) -> None:
+        """Release handles given as device rows, in row order (no sync)."""
+        n = lengths.shape[0]
+        if n == 0:
+            return
+        table = table.to(torch.int32)
+        if table.stride(-1) != 1:
+            table = table.contiguous()
+        lengths = lengths.to(torch.int32).contiguous()
+        _lib.check(_lib.lib().grs_cache_release(
+            self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
+            self._last_pos.data_ptr(), self.capacity, table.data_ptr(), table.stride(0),
+            lengths.data_ptr(), n, table.shape[1], self.page_size, self._status.data_ptr(),
+            self._stream()), "release")
+
+    def alloc_pages(self, n: int) -> torch.Tensor:
+        """Allocate n pages (refcount 1, free-list order) for contents copied
+        in from another cache; returns their ids (device int32)."""
+        pages = torch.empty(n, device=self.device, dtype=torch.int32)
+        if n:
+            _lib.check(_lib.lib().grs_cache_alloc(
+                self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
+                self.capacity, n, pages.data_ptr(), self._status.data_ptr(), self._stream()),
+                "alloc_pages")
+        return pages
+
+    def _handle_rows(self, handles: list[PrefixHandle], min_cols: int = 1):
+        cols = max([len(h.blocks) for h in handles] + [min_cols])
+        rows = np.zeros((len(handles), cols), dtype=np.int32)
+        lengths = np.empty(len(handles), dtype=np.int32)
+        for i, h in enumerate(handles):
+            if (h.length + self.page_size - 1) // self.page_size != len(h.blocks):
+                raise RuntimeError("prefix handle length/block table mismatch")
+            if any(not 0 <= p < self.capacity for p in h.blocks):
+                raise ValueError("prefix handle names a page outside the cache")
+            rows[i, : len(h.blocks)] = h.blocks
+            lengths[i] = h.length
+        table = torch.from_numpy(rows).to(self.device, non_blocking=True)
+        length_tensor = torch.from_numpy(lengths).to(self.device, non_blocking=True)
+        return table, length_tensor
+
+    def release(self, handle: PrefixHandle) -> None:
+        if not handle.blocks:
+            return
+        table, lengths = self._handle_rows([handle])
+        self.release_device(table, lengths)
+        self.check_status()
+
+    def block_table(self, handles: list[PrefixHandle]) -> tuple[torch.Tensor, torch.Tensor]:
+        """Padded physical page ids (>= 1 column) and logical lengths (int32)."""
+        return self._handle_rows(handles, min_cols=1)
+
+
+class PagedKVCache(PagePool):
+    """Fixed-size device KV/action pool with prefix sharing and COW tail pages."""
+
+    def __init__(self, *, layers: int, capacity: int, page_size: int, heads: int,
+                 head_width: int, model_width: int, device, dtype: torch.dtype,
+                 gather_backend: str = "vectorized"):
+        if min(layers, capacity, page_size, heads, head_width, model_width) <= 0:
+            raise ValueError("all cache dimensions must be positive")
+        if gather_backend not in {"loop", "vectorized"}:
+            raise ValueError("gather_backend must be 'loop' or 'vectorized'")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise RuntimeError("PagedKVCache lives in CUDA memory (no CPU fallback)")
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("PagedKVCache arenas are bf16 or fp32")
+        super().__init__(capacity, page_size, device)
+        self.layers = layers
+        self.heads, self.head_width, self.model_width = heads, head_width, model_width
+        self.dtype, self.gather_backend = dtype, gather_backend
+        self.keys = torch.empty(layers, capacity, page_size, heads, head_width,
+                                device=device, dtype=dtype)
+        self.values = torch.empty_like(self.keys)
+        self.actions = torch.empty(capacity, page_size, model_width, device=device, dtype=dtype)
+        self.readout_keys = torch.empty(capacity, page_size, heads, head_width,
+                                        device=device, dtype=dtype)
+        self.readout_values = torch.empty_like(self.readout_keys)
 
     # ---- device-native API ------------------------------------------------
     def append_device(self, parent_table: torch.Tensor, parent_lengths: torch.Tensor,
@@ -169,21 +232,6 @@ class PagedKVCache:
         _lib.check(status, "append_batch")
         return child_table, child_lengths
 
-    def release_device(self, table: torch.Tensor, lengths: torch.Tensor) -> None:
-        """Release handles given as device rows, in row order (no sync)."""
-        n = lengths.shape[0]
-        if n == 0:
-            return
-        table = table.to(torch.int32)
-        if table.stride(-1) != 1:
-            table = table.contiguous()
-        lengths = lengths.to(torch.int32).contiguous()
-        _lib.check(_lib.lib().grs_cache_release(
-            self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
-            self._last_pos.data_ptr(), self.capacity, table.data_ptr(), table.stride(0),
-            lengths.data_ptr(), n, table.shape[1], self.page_size, self._status.data_ptr(),
-            self._stream()), "release")
-
     # ---- moving rows between caches (sharded beam search) -------------------
     def arenas(self) -> list[torch.Tensor]:
         """Every arena as a [capacity, page elements] view (page-major), per
@@ -199,40 +247,7 @@ class PagedKVCache:
         """Bytes one page holds across all arenas."""
         return sum(a.shape[1] * a.element_size() for a in self.arenas())
 
-    def alloc_pages(self, n: int) -> torch.Tensor:
-        """Allocate n pages (refcount 1, free-list order) for contents copied
-        in from another cache; returns their ids (device int32)."""
-        pages = torch.empty(n, device=self.device, dtype=torch.int32)
-        if n:
-            _lib.check(_lib.lib().grs_cache_alloc(
-                self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
-                self.capacity, n, pages.data_ptr(), self._status.data_ptr(), self._stream()),
-                "alloc_pages")
-        return pages
-
     # ---- reference API ----------------------------------------------------
-    def _handle_rows(self, handles: list[PrefixHandle], min_cols: int = 1):
-        cols = max([len(h.blocks) for h in handles] + [min_cols])
-        rows = np.zeros((len(handles), cols), dtype=np.int32)
-        lengths = np.empty(len(handles), dtype=np.int32)
-        for i, h in enumerate(handles):
-            if (h.length + self.page_size - 1) // self.page_size != len(h.blocks):
-                raise RuntimeError("prefix handle length/block table mismatch")
-            if any(not 0 <= p < self.capacity for p in h.blocks):
-                raise ValueError("prefix handle names a page outside the cache")
-            rows[i, : len(h.blocks)] = h.blocks
-            lengths[i] = h.length
-        table = torch.from_numpy(rows).to(self.device, non_blocking=True)
-        length_tensor = torch.from_numpy(lengths).to(self.device, non_blocking=True)
-        return table, length_tensor
-
-    def release(self, handle: PrefixHandle) -> None:
-        if not handle.blocks:
-            return
-        table, lengths = self._handle_rows([handle])
-        self.release_device(table, lengths)
-        self.check_status()
-
     def append_batch(self, parents: list[PrefixHandle], keys: torch.Tensor,
                      values: torch.Tensor, actions: torch.Tensor,
                      readout_keys: torch.Tensor | None = None,
@@ -256,10 +271,6 @@ class PagedKVCache:
             nb = (length + self.page_size - 1) // self.page_size
             out.append(PrefixHandle(tuple(int(p) for p in rows[i, :nb]), length))
         return out
-
-    def block_table(self, handles: list[PrefixHandle]) -> tuple[torch.Tensor, torch.Tensor]:
-        """Padded physical page ids (>= 1 column) and logical lengths (int32)."""
-        return self._handle_rows(handles, min_cols=1)
 
     def _token_indices(self, handles):
         n = len(handles)

@@ -1,0 +1,281 @@
+"""Keys and values of a token model in pages: as they are, or in 8 bits.
+
+``PagedKVCache`` appends one token to every layer of every beam at once, with
+the rollout's action states beside it.  ``append_tokens`` writes the keys and
+values of one layer as the model makes them - one token per sequence or whole
+packed prompts - and turns keys and queries by their positions on the way; pages
+may be bf16 or fp32 like the inputs, or e4m3 with a scale for each page and
+head.  ``TokenKVCache`` owns such pages for all layers: the rollout cache's free
+list, reference counts and forks.
+
+Inference only: no gradient is recorded.  The sm_100a kernels live in
+``csrc/token_cache.cu`` and ``csrc/paged_cache.cu``; CPU tensors raise.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .paged_cache import PagePool
+from .prefix_attention import shared_prefix_attention
+from .prompt_attention import _STATUS_AT, _rows, _status_for
+from .quantized_attention import (_E4M3, _cache, _lengths, _scales, _table, quantized_attention)
+from .rotary import _check_magnitude, _frequencies, _positions, _turned_out
+
+_pack = _lib.words_of("grs_append_tokens").pack
+_entry = None
+
+
+def append_tokens(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    *,
+    key_scale: torch.Tensor | None = None,
+    value_scale: torch.Tensor | None = None,
+    offsets: torch.Tensor | None = None,
+    source_table: torch.Tensor | None = None,
+    frequencies: torch.Tensor | None = None,
+    interleaved: bool = False,
+    magnitude: float = 1.0,
+    positions: torch.Tensor | None = None,
+    query: torch.Tensor | None = None,
+    query_out: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
+) -> torch.Tensor | None:
+    """Write key and value [T, Hkv, D] (bf16 or fp32, D <= 256 and contiguous)
+    behind the ``lengths[b]`` tokens that each sequence has in its pages; returns
+    the turned query [T, H, D], if one is given.
+
+    key_cache/value_cache [pages, page, Hkv, D] of one layout, block_table int32
+    [B, columns], lengths int32 [B] (before the call).  offsets int32 [B + 1],
+    ascending: sequence b has the tokens ``offsets[b]:offsets[b + 1]``, possibly
+    none; without offsets one each (T = B).  With ``frequencies`` keys and
+    queries are turned as by ``rotate_positions``, at the place in the sequence
+    or at ``positions`` (int32 or int64 [T]; behind a shared prefix, for
+    instance, ``lengths`` plus its length).
+
+    Caches have the inputs' dtype, or float8_e4m3fn with key_scale/value_scale
+    fp32 [pages, Hkv], which the call writes: a code stands for code * scale.
+    The scale of a page and head is the smallest power of two (from 2^-118 to
+    2^119) that holds the largest finite value of its new rows within 448 (for
+    turned keys the value before turning, times sqrt(2) * max(1, |magnitude|)
+    at most), or the page's old scale if rows are there and it is larger; rows
+    that are there move to a new scale.  Infinite values are held as NaN.  The
+    rows of a page behind the new ones are left as they were.
+
+    source_table (int32 [B, columns] or wider): the rows that a sequence has in
+    its first page to receive tokens are copied from the page that this table
+    names there - the parent's, after a fork - as are their scales.  No page may
+    receive tokens of two sequences, or receive tokens and be another's source.
+
+    Tokens whose pages lie outside the cache or whose place the table does not
+    hold are not written, which ``status`` records (default: the device word
+    that ``check_decode_status`` reads).  Query rows of no sequence are left as
+    they were in a given ``query_out`` and zero in a new one; ``query_out`` may
+    be the query itself.  The call does not synchronise and can be captured into
+    a CUDA graph.
+    """
+    global _entry
+    device = key.get_device()
+    if device < 0:
+        _lib.require_cuda(key)
+    place = _lib.elsewhere(device)
+    if place is not None:
+        with place:
+            return append_tokens(
+                key, value, key_cache, value_cache, block_table, lengths, key_scale=key_scale,
+                value_scale=value_scale, offsets=offsets, source_table=source_table,
+                frequencies=frequencies, interleaved=interleaved, magnitude=magnitude,
+                positions=positions, query=query, query_out=query_out, status=status)
+    shape, dtype = key.shape, key.dtype
+    code = _lib.DTYPE_CODES.get(dtype)
+    if code is None or len(shape) != 3:
+        raise ValueError("keys must be bf16 or fp32 [tokens, kv_heads, D]")
+    tokens, kv_heads, width = shape
+    if not 1 <= width <= 256:
+        raise ValueError("head widths from 1 to 256 are supported")
+    if tokens >= 1 << 30 or not 0 < kv_heads < 1 << 30:
+        raise ValueError("at most 2^30 tokens and heads, and one head at least")
+    k = _rows("key", key, device, dtype, shape)
+    v = _rows("value", value, device, dtype, shape)
+    if key_cache.dim() != 4:
+        raise ValueError("caches must be [pages, page, kv_heads, D]")
+    pages, page = key_cache.shape[:2]
+    cache_code, scale_row, key_at, value_at = code, 0, 0, 0
+    if key_cache.dtype is _E4M3:
+        if key_scale is None or value_scale is None:
+            raise ValueError("8-bit caches come with key and value scales")
+        cache_code = 2
+        c = _cache(key_cache, value_cache, device, _E4M3, kv_heads, width)
+        scale_row = _scales("key_scale", key_scale, device, pages, kv_heads)
+        if (scale_row != _scales("value_scale", value_scale, device, pages, kv_heads)
+                and pages > 1):
+            raise ValueError("key/value scales must share a layout")
+        if pages > 1 and scale_row < kv_heads:
+            raise ValueError("scales must not overlap themselves")
+        key_at, value_at = key_scale.data_ptr(), value_scale.data_ptr()
+        if key_at == value_at and pages:
+            raise ValueError("key and value scales must not be one tensor")
+    else:
+        if key_scale is not None or value_scale is not None:
+            raise ValueError("scales come with 8-bit caches")
+        c = _cache(key_cache, value_cache, device, dtype, kv_heads, width)
+    need = 1
+    for size, step in sorted(zip(key_cache.shape, c), key=lambda p: p[1]):
+        if size > 1 and step < need:
+            raise ValueError("a cache must not overlap itself")
+        need = max(need, step * size)
+    if key_cache.data_ptr() == value_cache.data_ptr() and key_cache.numel():
+        raise ValueError("key and value caches must not be one tensor")
+    rows = lengths.shape[0] if lengths.dim() else -1
+    past = _lengths(lengths, device, rows)
+    if rows >= 1 << 29:
+        raise ValueError("at most 2^29 sequences")
+    columns, row = _table("block_table", block_table, device, rows)
+    if columns * page >= 1 << 30:
+        raise ValueError("a block table row holds at most 2^30 tokens")
+    source = source_row = 0
+    if source_table is not None:
+        wide, source_row = _table("source_table", source_table, device, rows)
+        if wide < columns:
+            raise ValueError("source_table must have the block table's columns")
+        source = source_table.data_ptr()
+    begins = 0
+    if offsets is not None:
+        if (offsets.dtype is not torch.int32 or offsets.shape != (rows + 1,)
+                or not offsets.is_contiguous() or offsets.get_device() != device):
+            _lib.require_cuda(offsets)
+            raise ValueError("offsets must be contiguous int32 [sequences + 1] on the inputs' "
+                             "device")
+        begins = offsets.data_ptr()
+    elif tokens != rows:
+        raise ValueError("without offsets every sequence has one token")
+    pairs = turns = 0
+    if frequencies is not None:
+        pairs, turns = _frequencies(frequencies, device, width), frequencies.data_ptr()
+    elif query is not None or positions is not None:
+        raise ValueError("query and positions come with frequencies")
+    magnitude = _check_magnitude(magnitude)
+    places = wide = 0
+    if positions is not None:
+        wide, places = _positions(positions, device, tokens), positions.data_ptr()
+    heads = query_at = query_to = 0
+    q = qo = (0, 0)
+    fresh = query_out is None
+    if query is not None:
+        if query.dim() != 3:
+            raise ValueError("query must be [tokens, heads, D]")
+        heads = query.shape[1]
+        if not 0 < heads < 1 << 30 or heads % kv_heads:
+            raise ValueError("query heads must be a multiple of the key/value heads")
+        q = _rows("query", query, device, dtype, (tokens, heads, width))
+        query_out, qo = _turned_out("query_out", query_out, query, device, dtype, q, key, value)
+        query_at, query_to = query.data_ptr(), query_out.data_ptr()
+    elif not fresh:
+        raise ValueError("query_out comes with a query")
+    if not tokens:
+        return query_out
+    word = None if status is not None else _STATUS_AT.get(device)
+    if word is None:
+        word = _status_for(key, device, status)
+    if _entry is None:
+        _entry = _lib.words_entry("grs_append_tokens")
+    code = _entry(_pack(
+        code, cache_code, query_at, q[0], q[1], query_to, qo[0], qo[1], fresh, key.data_ptr(),
+        k[0], k[1], value.data_ptr(), v[0], v[1], key_cache.data_ptr(), value_cache.data_ptr(),
+        c[0], c[1], c[2], key_at, value_at, scale_row, block_table.data_ptr(), row, source,
+        source_row, columns, past, begins, places, wide, turns, pairs, bool(interleaved),
+        magnitude, tokens, rows, heads, kv_heads, width, pages, page, word,
+        _lib.stream_on(device)))
+    if code:
+        _lib.check(code, "append_tokens")
+    return query_out
+
+
+class TokenKVCache(PagePool):
+    """Pages of a token model's keys and values, one arena per layer.
+
+    ``keys`` and ``values`` [layers, capacity, page, heads, head_width] of
+    ``dtype`` (bf16, fp32 or float8_e4m3fn); ``key_scales`` and
+    ``value_scales`` fp32 [layers, capacity, heads] of 8-bit pages, else None.
+    Block tables and lengths are device tensors, as in ``PagedKVCache``'s
+    device-native API; nothing synchronises but ``check_status``.
+
+    A decode step of beams, parents gathered by the search::
+
+        table = cache.fork_device(parent_table, lengths)   # and release the parents after it
+        for layer in range(layers):
+            ...
+            query = cache.append(layer, key, value, table, lengths, source_table=parent_table,
+                                 query=query, frequencies=frequencies)
+            context = cache.attend(layer, query, table, lengths + 1)
+    """
+
+    def __init__(self, *, layers: int, capacity: int, page_size: int, heads: int,
+                 head_width: int, device, dtype: torch.dtype):
+        if min(layers, capacity, page_size, heads, head_width) <= 0:
+            raise ValueError("all cache dimensions must be positive")
+        if dtype not in (torch.bfloat16, torch.float32, _E4M3):
+            raise ValueError("TokenKVCache arenas are bf16, fp32 or float8_e4m3fn")
+        super().__init__(capacity, page_size, device)
+        self.layers, self.heads, self.head_width, self.dtype = layers, heads, head_width, dtype
+        self.keys = torch.empty(layers, capacity, page_size, heads, head_width,
+                                device=self.device, dtype=dtype)
+        self.values = torch.empty_like(self.keys)
+        self.key_scales = self.value_scales = None
+        if dtype is _E4M3:
+            self.key_scales = torch.ones(layers, capacity, heads, device=self.device)
+            self.value_scales = torch.ones_like(self.key_scales)
+
+    def _layer(self, layer: int) -> tuple:
+        scales = (None, None)
+        if self.key_scales is not None:
+            scales = self.key_scales[layer], self.value_scales[layer]
+        return self.keys[layer], self.values[layer], *scales
+
+    def fork_device(self, parent_table: torch.Tensor, parent_lengths: torch.Tensor,
+                    columns: int | None = None) -> torch.Tensor:
+        """The block table of one child per parent row, int32 [n, columns]
+        (default: one more than the parents'), before its next token: it shares
+        the parent's full pages and owns a page of the free list for the token.
+        parent_table int32 [n, cols], parent_lengths int32 [n].  The kept rows of
+        the parent's last page follow with ``append(source_table=parent_table)``
+        in every layer.  Errors land in the status word."""
+        n = parent_lengths.shape[0]
+        width, row = _table("parent_table", parent_table, self.device.index, n)
+        past = _lengths(parent_lengths, self.device.index, n)
+        columns = columns or width + 1
+        table = torch.empty(n, columns, device=self.device, dtype=torch.int32)
+        lengths = torch.empty(n, device=self.device, dtype=torch.int32)
+        if n:
+            _lib.check(_lib.lib().grs_cache_fork(
+                self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
+                self.capacity, parent_table.data_ptr(), row, width, past, n, self.page_size,
+                table.data_ptr(), columns, lengths.data_ptr(), columns, self._status.data_ptr(),
+                self._stream()), "fork")
+        return table
+
+    def append(self, layer: int, key: torch.Tensor, value: torch.Tensor,
+               block_table: torch.Tensor, lengths: torch.Tensor, **options):
+        """``append_tokens`` into one layer's pages (its keyword arguments)."""
+        keys, values, key_scale, value_scale = self._layer(layer)
+        return append_tokens(key, value, keys, values, block_table, lengths, key_scale=key_scale,
+                             value_scale=value_scale, status=self._status, **options)
+
+    def attend(self, layer: int, query: torch.Tensor, block_table: torch.Tensor,
+               lengths: torch.Tensor, *, scale: float | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of one query per row to its pages in one layer:
+        ``quantized_attention``, or ``shared_prefix_attention`` without a prefix
+        over pages of the query's type."""
+        keys, values, key_scale, value_scale = self._layer(layer)
+        if key_scale is not None:
+            return quantized_attention(query, keys, values, key_scale, value_scale, block_table,
+                                       lengths, scale=scale, out=out, status=self._status)
+        none = keys.new_empty(0, self.heads, self.head_width)
+        return shared_prefix_attention(query, none, none, keys, values, block_table, lengths,
+                                       scale=scale, out=out, status=self._status)

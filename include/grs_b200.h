@@ -38,7 +38,8 @@ typedef enum {
   GRS_ERR_ORDER = -11        /* ranked records out of order or inconsistent (sharded search) */
 } grs_status;
 
-enum { GRS_DTYPE_BF16 = 0, GRS_DTYPE_F32 = 1 };
+/* GRS_DTYPE_E4M3: pages of a cache only, with an fp32 scale per page and head */
+enum { GRS_DTYPE_BF16 = 0, GRS_DTYPE_F32 = 1, GRS_DTYPE_E4M3 = 2 };
 
 /* Library version string. */
 GRS_API const char* grs_version(void);
@@ -656,7 +657,82 @@ GRS_API int grs_adjust_logits(int dtype, const void* logits, int64_t l_sb, void*
                               const float* bias, int64_t bias_sb, const int32_t* allowed,
                               int64_t a_sb, float fill, void* stream);
 
-/* The three calls above with their arguments in a host table of 64-bit words,
+/* ---- rotary positions, token pages, attention over 8-bit pages -----------
+ * No reference counterpart (the reference embeds positions and keeps its cache
+ * in the model's type).
+ *
+ * Rotary positions of query [tokens, heads, D] and key [tokens, kv_heads, D]
+ * (kv_heads 0: none), D <= 256: pair i of the first 2 * pairs elements of a
+ * head - elements i and i + pairs, or 2 i and 2 i + 1 when interleaved - is
+ * turned by position * frequencies[i] radians (frequencies: device fp64
+ * [pairs]) and multiplied by magnitude; the rest is copied.  positions: device
+ * int32 or int64 [tokens], any value.  Angles are exact modulo whole turns at every position.
+ * The outputs may be the inputs themselves, with the same strides. */
+GRS_API int grs_rotate_positions(int dtype, const void* query, int64_t q_st, int64_t q_sh,
+                                 const void* key, int64_t k_st, int64_t k_sh,
+                                 const void* positions, int positions_are_i64,
+                                 const double* frequencies, int pairs, int interleaved,
+                                 double magnitude, void* query_out, int64_t qo_st, int64_t qo_sh,
+                                 void* key_out, int64_t ko_st, int64_t ko_sh, int tokens,
+                                 int heads, int kv_heads, int head_width, void* stream);
+
+/* New keys and values into pages (key/value cache [num_pages, page_size,
+ * kv_heads, D] of one layout; block_table int32 [sequences, max_blocks]).
+ * Packed tokens: sequence b has the tokens offsets[b] .. offsets[b+1] - 1
+ * (null: one each) and lengths[b] tokens in its pages; its token i is written
+ * as token lengths[b] + i.  Keys, and queries into query_out (query may be
+ * null; query_out may be query), are turned as by grs_rotate_positions, at that
+ * position or at positions[token] (pairs 0: not turned).  Query rows of no
+ * sequence are left as they were, or zeroed with clear_rest.
+ * cache_dtype: the inputs', or GRS_DTYPE_E4M3 with the scales [num_pages,
+ * kv_heads] (row stride s_sp): a code stands for code * scale.  The scale of a
+ * page and head is the smallest power of two, from 2^-118 to 2^119, that holds
+ * the largest finite value of its new rows (times sqrt(2) max(1, |magnitude|)
+ * for turned keys, before they are turned) in 448, or the old scale if rows are
+ * there and it is larger; those rows move to a new scale.  Infinities become NaN.
+ * source_table (or null): the rows that a sequence has in its first page to
+ * receive tokens are copied from that table's page.  No page receives tokens of
+ * two sequences, and none that receives tokens is another's source.
+ * Pages outside the cache set GRS_ERR_BAD_PAGE and lengths or tokens that the
+ * table cannot hold GRS_ERR_LENGTH in `status`; their tokens are not written. */
+GRS_API int grs_append_tokens(
+    int dtype, int cache_dtype, const void* query, int64_t q_st, int64_t q_sh, void* query_out,
+    int64_t qo_st, int64_t qo_sh, int clear_rest, const void* key, int64_t k_st, int64_t k_sh,
+    const void* value, int64_t v_st, int64_t v_sh, void* key_cache, void* value_cache,
+    int64_t c_sp, int64_t c_st, int64_t c_sh, float* key_scale, float* value_scale, int64_t s_sp,
+    const int32_t* block_table, int64_t bt_stride, const int32_t* source_table,
+    int64_t source_stride, int max_blocks, const int32_t* lengths, const int32_t* offsets,
+    const void* positions, int positions_are_i64, const double* frequencies, int pairs,
+    int interleaved, double magnitude, int tokens, int sequences, int heads, int kv_heads,
+    int head_width, int num_pages, int page_size, int32_t* status, void* stream);
+
+/* The fork of grs_cache_append alone: child i shares the full pages of its
+ * parent row and gets a page of its own, from the free list, for its next token
+ * (behind the parent's full pages).  Nothing is copied: grs_append_tokens takes
+ * the parent's table as its source_table. */
+GRS_API int grs_cache_fork(int32_t* refcounts, int32_t* free_list, int32_t* free_count,
+                           int capacity, const int32_t* parent_table, int64_t parent_stride,
+                           int parent_cols, const int32_t* parent_lengths, int n, int page_size,
+                           int32_t* child_table, int64_t child_stride, int32_t* child_lengths,
+                           int child_cols, int32_t* status, void* stream);
+
+/* One query per sequence, query/output [batch, heads, D] (bf16 or fp32), against
+ * the first lengths[b] tokens of its 8-bit pages, as grs_append_tokens writes
+ * them (scales: any positive finite values).  Heads group as in
+ * grs_prompt_attention; rows without keys are zeros; bad pages and lengths as in
+ * grs_shared_prefix_attention.  The workspace (16-byte aligned) is the call's own
+ * until it has run. */
+GRS_API int64_t grs_quantized_attention_workspace_bytes(int batch, int heads, int kv_heads,
+                                                        int head_width, int64_t page_tokens);
+GRS_API int grs_quantized_attention(
+    int dtype, const void* query, int64_t q_sb, int64_t q_sh, const void* key_cache,
+    const void* value_cache, int64_t c_sp, int64_t c_st, int64_t c_sh, const float* key_scale,
+    const float* value_scale, int64_t s_sp, const int32_t* block_table, int64_t bt_stride,
+    int max_blocks, const int32_t* lengths, int num_pages, int page_size, void* output,
+    int64_t o_sb, int64_t o_sh, int batch, int heads, int kv_heads, int head_width, float scale,
+    void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
+/* Calls with many arguments, with them in a host table of 64-bit words,
  * one per argument in the same order (pointers and integers as such, floats as
  * the bits of a double; read before the call returns): a foreign-function
  * interface that converts argument by argument spends longer on 20 to 40 of
@@ -664,6 +740,9 @@ GRS_API int grs_adjust_logits(int dtype, const void* logits, int64_t l_sb, void*
 GRS_API int grs_prompt_attention_words(const int64_t* words);
 GRS_API int grs_shared_prefix_attention_words(const int64_t* words);
 GRS_API int grs_adjust_logits_words(const int64_t* words);
+GRS_API int grs_rotate_positions_words(const int64_t* words);
+GRS_API int grs_append_tokens_words(const int64_t* words);
+GRS_API int grs_quantized_attention_words(const int64_t* words);
 
 #ifdef __cplusplus
 }
