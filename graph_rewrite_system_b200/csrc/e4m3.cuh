@@ -29,4 +29,56 @@ __device__ __forceinline__ float from_e4m3(uint8_t code) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3)));
 }
 
+
+// Two fp32 values to two codes, the first in the low byte.
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+// Two codes times `ratio`, a power of two up to 1, in f16: exact for results that f16
+// holds as normal numbers, and those that it does not are below 2^-14, which e4m3
+// rounds to zero all the same.
+__device__ __forceinline__ uint32_t e4m3x2_times(uint32_t codes, __half2 ratio) {
+  uint32_t x;
+  uint16_t y;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(x) : "h"((uint16_t)codes));
+  const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&x), ratio);
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;\n" : "=h"(y) : "r"(*reinterpret_cast<const uint32_t*>(&z)));
+  return y;
+}
+
+// Four codes times any ratio, in fp32.
+__device__ __forceinline__ uint32_t e4m3x4_times(uint32_t codes, float ratio) {
+  uint32_t out = 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    out |= (uint32_t)to_e4m3(from_e4m3((uint8_t)(codes >> i)) * ratio) << i;
+  return out;
+}
+// kVec values over a scale, stored as one word; `careful`: some may not be finite.
+template <int kVec>
+__device__ __forceinline__ void e4m3_store(uint8_t* at, const float (&y)[kVec], float inverse,
+                                           bool careful) {
+  float x[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) x[i] = y[i];
+  if (careful) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) x[i] = e4m3_checked(x[i]);
+  }
+  if constexpr (kVec == 1) {
+    *at = to_e4m3(x[0] * inverse);
+  } else {
+    uint32_t w[(kVec + 3) / 4] = {};
+#pragma unroll
+    for (int i = 0; i < kVec; i += 2)
+      w[i / 4] |= to_e4m3x2(x[i] * inverse, x[i + 1] * inverse) << 8 * (i % 4);
+    if constexpr (kVec == 2)
+      *reinterpret_cast<uint16_t*>(at) = (uint16_t)w[0];
+    else if constexpr (kVec == 4)
+      *reinterpret_cast<uint32_t*>(at) = w[0];
+    else
+      *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+  }
+}
+
 }  // namespace grs

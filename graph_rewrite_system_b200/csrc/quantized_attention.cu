@@ -18,8 +18,11 @@ struct QuantArgs {
   const uint8_t* kc; const uint8_t* vc; int64_t c_sp, c_st, c_sh;
   const float* ks; const float* vs; int64_t s_sp;
   const int32_t* bt; int64_t bt_s; int columns; const int32_t* lengths; int pages, page;
+  bool q_whole;                             // query rows in 16-byte pieces
   uint32_t magic; int shift;                // t / page = umulhi(t, magic) >> shift; magic 0: page 1
-  float* part; float* part_lse; int slices;
+  float* part; float* part_lse; int slices;             // partial sums
+  int ranges; int32_t* starts;              // of the stream form; first tiles of the sequences
+  bool o_whole;                             // output rows in pieces of four elements
   void* out; int64_t o_sb, o_sh;
   int batch, heads, kv_heads, group, D;
   float scale_log2;
@@ -110,13 +113,13 @@ __global__ void __launch_bounds__(128) quant_rows_kernel(QuantArgs a) {
 // ---- tensor cores ---------------------------------------------------------------
 // A warp streams tiles of 16 tokens of one (sequence, K/V head) through a ring of
 // its own in shared memory: cp.async fetches the rows in 16-byte pieces wherever
-// their pages lie, three tiles ahead.  Keys, then value columns, are the 16 rows of
+// their pages lie, two tiles ahead.  Keys, then value columns, are the 16 rows of
 // mma.m16n8k16, the group's query heads its columns.  The order in which a product
 // sums its inner dimension is free, so a lane takes whole pieces of a row, and a
 // lane's column index picks its piece of the value rows; two tokens' codes are
 // interleaved by byte permutes before they are widened.
 constexpr int QT_WARPS = 4;
-constexpr int QT_STAGES = 4;
+constexpr int QT_STAGES = 3;
 constexpr float QT_LIFT = 9.f;              // weights are at most 2^(9 + 6): f16 holds them to
 constexpr float QT_SLACK = 6.f;             // 2^-24, 2^-33 of the largest
 constexpr uint32_t QT_ABSENT = 0xffffffffu; // key scale of a token that is not there
@@ -194,131 +197,89 @@ struct QtShape {
   }
 };
 
-template <typename T, int DP, int kTiles, int kPiece>
-__global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
+// A warp's work on one sequence and kTiles * 8 query heads.
+template <typename T, int DP, int kTiles>
+struct QtState {
   using S = QtShape<DP>;
-  constexpr bool kSplit = std::is_same<T, float>::value;  // operands in two f16 parts
-  constexpr int kParts = kSplit ? 2 : 1, kHeads = 8 * kTiles;
-  constexpr int kSteps = S::kKey * S::kKeyWords;          // products of the scores
-  extern __shared__ __align__(128) uint8_t qt_smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int chunks = (a.group + kHeads - 1) / kHeads;
-  const int b = blockIdx.x / (a.kv_heads * chunks), h = blockIdx.x / chunks % a.kv_heads;
-  const int head0 = h * a.group + blockIdx.x % chunks * kHeads;
-  const int n_heads = min(kHeads, (h + 1) * a.group - head0);
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-
-  const int past = quant_length(a, b), tiles = (past + 15) / 16;
-  const int lo = (int)((int64_t)tiles * blockIdx.y / gridDim.y);
-  const int hi = (int)((int64_t)tiles * (blockIdx.y + 1) / gridDim.y);
-  uint8_t* ring = qt_smem + warp * S::kRing;
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  const int32_t* table = a.bt + (int64_t)b * a.bt_s;
-  const uint8_t* const kh = a.kc + h * a.c_sh;
-  const uint8_t* const vh = a.vc + h * a.c_sh;
-
-  // lanes i and i + 16 hold the page of token i of the tile to be requested next
-  const auto column = [&](int token) {
-    return a.magic ? (int)(__umulhi((uint32_t)token, a.magic) >> a.shift) : token;
-  };
-  const auto page_of = [&](int tile) {
-    const int token = tile * 16 + (lane & 15);
-    return tile < hi && token < past ? __ldg(table + column(token)) : -1;
-  };
-  int page = page_of(lo + warp);
-  const auto request = [&](int tile, int stage) {
-    if (tile >= hi) {
-      qt_commit();
-      return;
-    }
-    const int token = tile * 16 + (lane & 15);
-    const bool there = token < past && page >= 0 && page < a.pages;
-    if (token < past && !there) set_status(a.status, GRS_ERR_BAD_PAGE);
-    const int64_t at =
-        there ? (int64_t)page * a.c_sp + (int64_t)(token - column(token) * a.page) * a.c_st : -1;
-    const uint32_t base = ring_at + stage * S::kStage;
-    constexpr int kLanes = DP / kPiece, kRows = 32 / kLanes;   // of a row; of a round
-    const int byte = lane % kLanes * kPiece;
-#pragma unroll
-    for (int i = 0; i < 16 / kRows; ++i) {
-      const int row = i * kRows + lane / kLanes;
-      const int64_t from = __shfl_sync(0xffffffffu, at, row);
-      const bool fetch = from >= 0 && byte < a.D;
-      qt_fetch<kPiece>(base + S::key_at(row, byte), fetch ? kh + from + byte : kh, fetch);
-      qt_fetch<kPiece>(base + S::kTile + S::value_at(row, byte), fetch ? vh + from + byte : vh,
-                       fetch);
-    }
-    // scales: the keys' by the first 16 lanes, the values' by the others
-    const uint32_t scale = base + 2 * S::kTile + 4 * lane;
-    if (there)
-      qt_fetch<4>(scale, (lane < 16 ? a.ks : a.vs) + page * a.s_sp + h, true);
-    else
-      asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(scale), "r"(lane < 16 ? QT_ABSENT : 0u) : "memory");
-    qt_commit();
-    page = page_of(tile + QT_WARPS);
-  };
-#pragma unroll
-  for (int i = 0; i < QT_STAGES - 1; ++i) request(lo + warp + i * QT_WARPS, i);
-
-  // Queries of head g, scaled by a power of two to at most 2^14: f16 then holds a
-  // bf16 element down to 2^-25 of the head's largest exactly, and two parts hold
-  // fp32 to 2^-22.
+  static constexpr bool kSplit = std::is_same<T, float>::value;   // operands in two f16 parts
+  static constexpr int kParts = kSplit ? 2 : 1, kHeads = 8 * kTiles;
+  static constexpr int kSteps = S::kKey * S::kKeyWords;   // products of the scores
   uint32_t qf[kTiles][kSteps][2][kParts];
   float unit[kTiles][2];                    // of heads 2t, 2t + 1: log2(e) scale / 2^k
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
-    const bool on = 8 * n + g < n_heads;
-    const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb +
-                 (int64_t)(head0 + (on ? 8 * n + g : 0)) * a.q_sh;
-    float x[S::kKey][4 * S::kKeyWords], top = 0.f;
-#pragma unroll
-    for (int i = 0; i < S::kKey; ++i)
-#pragma unroll
-      for (int e = 0; e < 4 * S::kKeyWords; ++e) {
-        const int d = (t + 4 * i) * 4 * S::kKeyWords + e;
-        x[i][e] = on && d < a.D ? to_float(q[d]) : 0.f;
-        const float y = fabsf(x[i][e]);
-        if (y <= 3.402823466e38f) top = fmaxf(top, y);
-      }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    int k = top > 0.f ? 13 + 127 - (int)(__float_as_uint(top) >> 23) : 0;
-    k = max(min(k, 120), -120);
-    const float lift = __uint_as_float((uint32_t)(k + 127) << 23);
-#pragma unroll
-    for (int i = 0; i < S::kKey; ++i)
-#pragma unroll
-      for (int e = 0; e < 4 * S::kKeyWords; e += 4)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float u = x[i][e + 2 * c] * lift, v = x[i][e + 2 * c + 1] * lift;
-          uint32_t (&to)[kParts] = qf[n][i * S::kKeyWords + e / 4][c];
-          to[0] = qt_pack(u, v);
-          if constexpr (kSplit) to[1] = qt_pack(qt_rest(u), qt_rest(v));
+  float acc[kTiles][2 * S::kWords][4];      // columns (d, d + 1) x heads (2t, 2t + 1)
+  float m[kTiles][2], l[kTiles][2];         // maxima and sums of the scores' weights
+  float w_top[kTiles][2];                   // maxima of the scores with the value scale
+
+  __device__ __forceinline__ void begin(const QuantArgs& a, int b, int head0, int n_heads) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    // Queries of head g, scaled by a power of two to at most 2^14: f16 then holds a
+    // bf16 element down to 2^-25 of the head's largest exactly, and two parts hold
+    // fp32 to 2^-22.
+  #pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      const bool on = 8 * n + g < n_heads;
+      const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb +
+                   (int64_t)(head0 + (on ? 8 * n + g : 0)) * a.q_sh;
+      float x[S::kKey][4 * S::kKeyWords], top = 0.f;
+  #pragma unroll
+      for (int i = 0; i < S::kKey; ++i) {
+        constexpr int kEach = 16 / sizeof(T);  // elements of a load
+        const int d0 = (t + 4 * i) * 4 * S::kKeyWords;
+  #pragma unroll
+        for (int e = 0; e < 4 * S::kKeyWords; e += kEach) {
+          alignas(16) T y[kEach] = {};
+          if (on && d0 + e < a.D) {
+            if (a.q_whole) {
+              *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(q + d0 + e);
+            } else {
+  #pragma unroll
+              for (int c = 0; c < kEach; ++c) y[c] = q[d0 + e + c];
+            }
+          }
+  #pragma unroll
+          for (int c = 0; c < kEach; ++c) x[i][e + c] = to_float(y[c]);
         }
-    const float mine = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
+  #pragma unroll
+        for (int e = 0; e < 4 * S::kKeyWords; ++e) {
+          const float y = fabsf(x[i][e]);
+          if (y <= 3.402823466e38f) top = fmaxf(top, y);
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int k = top > 0.f ? 13 + 127 - (int)(__float_as_uint(top) >> 23) : 0;
+      k = max(min(k, 120), -120);
+      const float lift = __uint_as_float((uint32_t)(k + 127) << 23);
+  #pragma unroll
+      for (int i = 0; i < S::kKey; ++i)
+  #pragma unroll
+        for (int e = 0; e < 4 * S::kKeyWords; e += 4)
+  #pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float u = x[i][e + 2 * c] * lift, v = x[i][e + 2 * c + 1] * lift;
+            uint32_t (&to)[kParts] = qf[n][i * S::kKeyWords + e / 4][c];
+            to[0] = qt_pack(u, v);
+            if constexpr (kSplit) to[1] = qt_pack(qt_rest(u), qt_rest(v));
+          }
+      const float back = a.scale_log2 * __uint_as_float((uint32_t)(127 - k) << 23);
+  #pragma unroll
+      for (int r = 0; r < 2; ++r) unit[n][r] = __shfl_sync(0xffffffffu, back, (2 * t + r) * 4);
+    }
+
 #pragma unroll
-    for (int r = 0; r < 2; ++r) unit[n][r] = __shfl_sync(0xffffffffu, mine, (2 * t + r) * 4);
+    for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+      for (int j = 0; j < 2 * S::kWords; ++j)
+        acc[n][j][0] = acc[n][j][1] = acc[n][j][2] = acc[n][j][3] = 0.f;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) m[n][r] = w_top[n][r] = -INFINITY, l[n][r] = 0.f;
+    }
   }
 
-  // columns (d, d + 1) x heads (2t, 2t + 1)
-  float acc[kTiles][2 * S::kWords][4];
-  float m[kTiles][2], l[kTiles][2], w_top[kTiles][2];     // maxima of the scores and of the
-#pragma unroll                                            // scores with the value scale
-  for (int n = 0; n < kTiles; ++n) {
-#pragma unroll
-    for (int j = 0; j < 2 * S::kWords; ++j) acc[n][j][0] = acc[n][j][1] = acc[n][j][2] = acc[n][j][3] = 0.f;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) m[n][r] = w_top[n][r] = -INFINITY, l[n][r] = 0.f;
-  }
-  int stage = 0;
-  for (int tile = lo + warp; tile < hi; tile += QT_WARPS) {
-    qt_wait<QT_STAGES - 2>();
-    __syncwarp();
-    request(tile + (QT_STAGES - 1) * QT_WARPS, stage == 0 ? QT_STAGES - 1 : stage - 1);
-    const uint8_t* at = ring + stage * S::kStage;
-    stage = stage + 1 == QT_STAGES ? 0 : stage + 1;
-
+  // The staged tile `at`; key scale and log2 of the value scale of tokens g and g + 8.
+  __device__ __forceinline__ void tile(const uint8_t* at, const uint32_t (&key)[2],
+                                       const float (&value)[2]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     float s[kTiles][4];                     // tokens (g, g + 8) x heads (2t, 2t + 1)
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
@@ -349,20 +310,17 @@ __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
           }
       }
     }
-    const uint32_t* scales = reinterpret_cast<const uint32_t*>(at + 2 * S::kTile);
     float z[kTiles][4];
     bool grown = false;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const uint32_t key = scales[g + 8 * r];
-      const float value = qt_log2(__uint_as_float(scales[16 + g + 8 * r]));
 #pragma unroll
       for (int n = 0; n < kTiles; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float& x = s[n][2 * r + c];
-          x = key == QT_ABSENT ? -INFINITY : x * unit[n][c] * __uint_as_float(key);
-          z[n][2 * r + c] = x + value;
+          x = key[r] == QT_ABSENT ? -INFINITY : x * unit[n][c] * __uint_as_float(key[r]);
+          z[n][2 * r + c] = x + value[r];
           grown |= x > m[n][c] + QT_SLACK || z[n][2 * r + c] > w_top[n][c] + QT_SLACK;
         }
     }
@@ -444,29 +402,195 @@ __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
     }
   }
 
+  // Every lane's share of the weights' sums, of all tokens.
+  __device__ __forceinline__ void sum_weights() {
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[n][r] += __shfl_xor_sync(0xffffffffu, l[n][r], o);
+  }
+};
+
+template <typename T, int DP, int kTiles, int kPiece, bool kRuns>
+__global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
+  using S = QtShape<DP>;
+  constexpr int kHeads = 8 * kTiles;
+  extern __shared__ __align__(128) uint8_t qt_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int chunks = (a.group + kHeads - 1) / kHeads;
+  const int b = blockIdx.x / (a.kv_heads * chunks), h = blockIdx.x / chunks % a.kv_heads;
+  const int head0 = h * a.group + blockIdx.x % chunks * kHeads;
+  const int n_heads = min(kHeads, (h + 1) * a.group - head0);
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+  const int past = quant_length(a, b), tiles = (past + 15) / 16;
+  const int lo = (int)((int64_t)tiles * blockIdx.y / gridDim.y);
+  const int hi = (int)((int64_t)tiles * (blockIdx.y + 1) / gridDim.y);
+  const int mine = max(0, (hi - lo - warp + QT_WARPS - 1) / QT_WARPS);   // this warp's tiles
+  uint8_t* ring = qt_smem + warp * S::kRing;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const int32_t* table = a.bt + (int64_t)b * a.bt_s;
+  const uint8_t* const kh = a.kc + h * a.c_sh;
+  const uint8_t* const vh = a.vc + h * a.c_sh;
+  constexpr int kLanes = DP / kPiece, kRows = 32 / kLanes;   // lanes of a row, rows of a round
+  const int lane_row = lane / kLanes, byte = lane % kLanes * kPiece;
+  const bool inside = byte < a.D;
+  const auto tile_of = [&](int j) { return lo + warp + j * QT_WARPS; };
+  const auto column = [&](int token) {
+    return a.magic ? (int)(__umulhi((uint32_t)token, a.magic) >> a.shift) : token;
+  };
+
+  // kRuns (pages of whole runs of 8 tokens): lane i looks up the two runs of sixteen
+  // tiles ahead at once - place, key scale and log2 of the value scale - and they are
+  // handed round by shuffles; `next` is requested in steps while `now` is in use.
+  // Else lanes i and i + 16 look up token i of the next tile to be requested.
+  struct Runs {
+    int64_t at;
+    uint32_t key;
+    float value;
+  };
+  int page = -1;
+  const auto look = [&](int j) {             // the page of this lane's run, or token
+    const int token = kRuns ? tile_of(j + (lane >> 1)) * 16 + (lane & 1) * 8
+                            : tile_of(j) * 16 + (lane & 15);
+    const bool ask = kRuns ? j + (lane >> 1) < mine : j < mine;
+    page = ask && token < past ? __ldg(table + column(token)) : -1;
+    return ask && token < past ? token : -1;
+  };
+  const auto place = [&](int token) {        // of the page looked up; -1: there is none
+    const bool there = page >= 0 && page < a.pages;
+    if (token >= 0 && !there) set_status(a.status, GRS_ERR_BAD_PAGE);
+    return there ? (int64_t)page * a.c_sp + (int64_t)(token - column(token) * a.page) * a.c_st
+                 : -1;
+  };
+  const auto scales_of = [&](Runs& r) {
+    const int64_t at = (int64_t)page * a.s_sp + h;
+    r.key = r.at >= 0 ? __float_as_uint(__ldg(a.ks + at)) : QT_ABSENT;
+    r.value = r.at >= 0 ? __ldg(a.vs + at) : 0.f;
+  };
+  Runs now = {}, next = {};
+  int token = look(0);
+  if constexpr (kRuns) {
+    now.at = place(token);
+    scales_of(now);
+    token = look(16);
+    next.at = place(token);
+    scales_of(next);
+    now.value = qt_log2(now.value);
+    next.value = qt_log2(next.value);
+  }
+  int batch = 0;                             // first tile of `now`
+  const auto request = [&](int j, int stage) {
+    if (j >= mine) {
+      qt_commit();
+      return;
+    }
+    const int left = past - tile_of(j) * 16; // tokens of this tile
+    const uint32_t base = ring_at + stage * S::kStage;
+    int64_t at;
+    if constexpr (kRuns) {
+      at = j - batch < 16 ? now.at : next.at;
+    } else {
+      at = place(token);
+      // scales: the keys' by the first 16 lanes, the values' by the others
+      const uint32_t scale = base + 2 * S::kTile + 4 * lane;
+      if (at >= 0)
+        qt_fetch<4>(scale, (lane < 16 ? a.ks : a.vs) + page * a.s_sp + h, true);
+      else
+        asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(scale), "r"(lane < 16 ? QT_ABSENT : 0u)
+                     : "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / kRows; ++i) {
+      const int row = i * kRows + lane_row;
+      int64_t from;
+      bool fetch = inside;
+      if constexpr (kRuns) {
+        from = __shfl_sync(0xffffffffu, at, ((j & 15) << 1) + (row >> 3));
+        fetch = fetch && from >= 0 && row < left;
+        from += (row & 7) * a.c_st;
+      } else {
+        from = __shfl_sync(0xffffffffu, at, row);
+        fetch = fetch && from >= 0;
+      }
+      from = fetch ? from + byte : 0;
+      qt_fetch<kPiece>(base + S::key_at(row, byte), kh + from, fetch);
+      qt_fetch<kPiece>(base + S::kTile + S::value_at(row, byte), vh + from, fetch);
+    }
+    qt_commit();
+    if constexpr (!kRuns) token = look(j + 1);
+  };
+#pragma unroll
+  for (int i = 0; i < QT_STAGES - 1; ++i) request(i, i);
+
+  QtState<T, DP, kTiles> state;
+  state.begin(a, b, head0, n_heads);
+  int stage = 0;
+  for (int j = 0; j < mine; ++j) {
+    if constexpr (kRuns) {
+      // the last tiles' requests are ahead in `next`; the one after it is looked up in
+      // three steps, so that no load is waited for
+      const int at = j & 15;
+      if (at == 0 && j > 0) {
+        now = next;
+        batch = j;
+        token = look(j + 16);
+      } else if (at == 4 && j > 16) {
+        next.at = place(token);
+        scales_of(next);
+      } else if (at == 8 && j > 16) {
+        next.value = qt_log2(next.value);
+      }
+    }
+    qt_wait<QT_STAGES - 2>();
+    __syncwarp();
+    request(j + QT_STAGES - 1, stage == 0 ? QT_STAGES - 1 : stage - 1);
+    const uint8_t* at = ring + stage * S::kStage;
+    stage = stage + 1 == QT_STAGES ? 0 : stage + 1;
+
+    const uint32_t* scales = reinterpret_cast<const uint32_t*>(at + 2 * S::kTile);
+    const int left = past - tile_of(j) * 16;
+    uint32_t key[2];
+    float value[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      if constexpr (kRuns) {
+        key[r] = __shfl_sync(0xffffffffu, now.key, ((j & 15) << 1) + r);
+        value[r] = __shfl_sync(0xffffffffu, now.value, ((j & 15) << 1) + r);
+        if (g + 8 * r >= left) key[r] = QT_ABSENT;
+      } else {
+        key[r] = scales[g + 8 * r];
+        value[r] = qt_log2(__uint_as_float(scales[16 + g + 8 * r]));
+      }
+    }
+    state.tile(at, key, value);
+  }
+
   // the warps' sums meet in shared memory
   qt_wait<0>();
   __syncthreads();
   float* sums = reinterpret_cast<float*>(qt_smem);        // [warps][kHeads][kSum]
   float* tops = sums + QT_WARPS * kHeads * S::kSum;       // [warps][kHeads][3]
+  state.sum_weights();
 #pragma unroll
   for (int n = 0; n < kTiles; ++n)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) l[n][r] += __shfl_xor_sync(0xffffffffu, l[n][r], o);
       const int head = 8 * n + 2 * t + r;
       float* row = sums + (warp * kHeads + head) * S::kSum;
       constexpr int kRead = S::kWords < 4 ? S::kWords : 4;
 #pragma unroll
       for (int j = 0; j < S::kWords; ++j)
         *reinterpret_cast<float4*>(row + 128 * (j / 4) + 4 * kRead * g + 4 * (j % 4)) = make_float4(
-            acc[n][2 * j][r], acc[n][2 * j][r + 2], acc[n][2 * j + 1][r], acc[n][2 * j + 1][r + 2]);
+            state.acc[n][2 * j][r], state.acc[n][2 * j][r + 2], state.acc[n][2 * j + 1][r],
+            state.acc[n][2 * j + 1][r + 2]);
       if (g == 0) {
         float* top = tops + (warp * kHeads + head) * 3;
-        top[0] = m[n][r];
-        top[1] = l[n][r];
-        top[2] = w_top[n][r];
+        top[0] = state.m[n][r];
+        top[1] = state.l[n][r];
+        top[2] = state.w_top[n][r];
       }
     }
   __syncthreads();
@@ -516,32 +640,327 @@ __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
   }
 }
 
-// A sequence's slices joined by their weights: a warp per (sequence, head).
+// ---- long contexts: a stream of tiles per warp -----------------------------------
+// The tiles of all sequences in a row are cut into as many equal ranges as the SMs hold
+// warps for each K/V head, whatever the sequences' lengths; a warp goes through its
+// range of one head, from one sequence into the next without draining its ring, and
+// the warps of the other heads of those tokens run beside it, so that whole pages are
+// read at once.  A sequence that one range holds is written at once; parts of one go to
+// the workspace, at most two of a range, and are joined by quant_join_kernel.
+constexpr int QS_MOST = 1024;               // sequences: their first tiles are in shared memory
+
+template <typename T, int DP, int kTiles>
+struct QsShape {
+  // CTAs that share an SM (by registers) and tiles that a warp has in flight and in use
+  static constexpr bool kSplit = std::is_same<T, float>::value;
+  static constexpr int kCtas = DP > 128 ? 2 : DP > 64 ? (kTiles == 1 && !kSplit ? 4 : kTiles == 1 ? 3 : 2)
+                             : kTiles == 1 ? (DP > 32 ? 5 : 7) : kSplit ? 3 : 4;
+  static constexpr int kStages = DP >= 128 ? 3 : 4;
+  static constexpr int kStage = 2 * QtShape<DP>::kTile;
+};
+
+// First tiles of the sequences, shifted left by four bits, with the tokens of the last
+// tile (0: 16) below; shared memory, `starts[batch]` is all tiles.  Two barriers.
+__device__ __forceinline__ void quant_starts(const QuantArgs& a, int* starts, int* sums) {
+  constexpr int kThreads = 32 * QT_WARPS, kEach = QS_MOST / kThreads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = (a.batch + kThreads - 1) / kThreads, room = a.columns * a.page;
+  int past[kEach], total = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int b = threadIdx.x * each + i;
+    past[i] = 0;
+    if (i < each && b < a.batch) {
+      const int length = __ldg(a.lengths + b);
+      past[i] = min(max(length, 0), room);
+      if (blockIdx.x == 0 && past[i] != length) set_status(a.status, GRS_ERR_LENGTH);
+      if (a.pages == 0 && past[i] > 0) {
+        if (blockIdx.x == 0) set_status(a.status, GRS_ERR_BAD_PAGE);
+        past[i] = 0;
+      }
+    }
+    total += (past[i] + 15) / 16;
+  }
+  int before = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  if (lane == 31) sums[warp] = before;
+  __syncthreads();
+  before -= total;
+  for (int i = 0; i < warp; ++i) before += sums[i];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int b = threadIdx.x * each + i;
+    if (i < each && b <= a.batch) starts[b] = before << 4 | (past[i] & 15);
+    before += (past[i] + 15) / 16;
+  }
+  if (threadIdx.x == kThreads - 1 && a.batch == kThreads * each) starts[a.batch] = before << 4;
+  __syncthreads();
+}
+
+// Ranges in use: none is empty, four tiles each at least (but for the last tiles).
+__device__ __forceinline__ int quant_used(int ranges, int64_t total) {
+  return (int)max((int64_t)1, min((int64_t)ranges, total / 4));
+}
+
 template <typename T>
-__global__ void __launch_bounds__(128) quant_join_kernel(QuantArgs a) {
+__device__ __forceinline__ void quant_store(T* to, const float (&x)[4], bool whole) {
+  if (!whole) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = from_float<T>(x[i]);
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+    *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo),
+                                               *reinterpret_cast<const uint32_t*>(&hi));
+  }
+}
+
+template <typename T, int DP, int kTiles, int kPiece>
+__global__ void __launch_bounds__(32 * QT_WARPS, (QsShape<T, DP, kTiles>::kCtas))
+    quant_stream_kernel(QuantArgs a) {
+  using S = QtShape<DP>;
+  using Q = QsShape<T, DP, kTiles>;
+  constexpr int kHeads = 8 * kTiles, kStages = Q::kStages;
+  extern __shared__ __align__(128) uint8_t qt_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  uint8_t* ring = qt_smem + warp * kStages * Q::kStage;
+  int* starts = reinterpret_cast<int*>(qt_smem + QT_WARPS * kStages * Q::kStage);
+  quant_starts(a, starts, reinterpret_cast<int*>(qt_smem));
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i <= a.batch; i += 32 * QT_WARPS) a.starts[i] = starts[i];
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {       // rows without keys
+    if (starts[b] >> 4 != starts[b + 1] >> 4) continue;
+    for (int i = threadIdx.x; i < a.heads * a.D; i += 32 * QT_WARPS)
+      static_cast<T*>(a.out)[b * a.o_sb + i / a.D * a.o_sh + i % a.D] = from_float<T>(0.f);
+  }
+
+  const int chunks = (a.group + kHeads - 1) / kHeads, units = a.kv_heads * chunks;
+  const int64_t job = (int64_t)blockIdx.x * QT_WARPS + warp;
+  const int range = (int)(job / units), part = (int)(job % units), h = part / chunks;
+  const int64_t total = starts[a.batch] >> 4;
+  const int ranges = quant_used(a.ranges, total);
+  if (range >= ranges) return;
+  const int lo = (int)(total * range / ranges), hi = (int)(total * (range + 1) / ranges);
+  if (lo >= hi) return;
+  const int head0 = h * a.group + part % chunks * kHeads;
+  const int n_heads = min(kHeads, (h + 1) * a.group - head0);
+  int seq = 0;                               // the last sequence that starts at or before lo
+  for (int left = a.batch; left > 1;) {
+    const int half = left / 2;
+    if (starts[seq + half] >> 4 <= lo) {
+      seq += half;
+      left -= half;
+    } else {
+      left = half;
+    }
+  }
+  int current = seq;                         // of the warp; seq: of this lane's look-ups
+
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const uint8_t* const kh = a.kc + h * a.c_sh;
+  const uint8_t* const vh = a.vc + h * a.c_sh;
+  constexpr int kLanes = DP / kPiece, kRows = 32 / kLanes;   // lanes of a row, rows of a round
+  const int lane_row = lane / kLanes, byte = lane % kLanes * kPiece;
+  const bool inside = byte < a.D;
+  const int mine = hi - lo;
+
+  // Lane i looks up the two runs of 8 tokens of sixteen tiles ahead at once - place,
+  // tokens of the tile, key scale and log2 of the value scale - and they are handed round
+  // by shuffles; `next` is looked up in steps while `now` is in use.
+  struct Runs {
+    int64_t at;
+    int left;
+    uint32_t key;
+    float value;
+  };
+  Runs now, next;
+  int page = -1, token = -1;
+  const auto look = [&](int j) {
+    const int f = lo + j + (lane >> 1);
+    page = token = -1;
+    next.left = 0;
+    if (f >= hi) return;
+    while (starts[seq + 1] >> 4 <= f) ++seq;
+    const int tile = f - (starts[seq] >> 4), fill = starts[seq] & 15;
+    next.left = f + 1 == starts[seq + 1] >> 4 && fill ? fill : 16;
+    if ((lane & 1) * 8 >= next.left) return;
+    token = tile * 16 + (lane & 1) * 8;
+    const int column = a.magic ? (int)(__umulhi((uint32_t)token, a.magic) >> a.shift) : token;
+    page = __ldg(a.bt + (int64_t)seq * a.bt_s + column);
+    token -= column * a.page;                // the run's first row in its page
+  };
+  const auto place = [&] {
+    const bool there = page >= 0 && page < a.pages;
+    if (token >= 0 && !there) set_status(a.status, GRS_ERR_BAD_PAGE);
+    next.at = there ? (int64_t)page * a.c_sp + (int64_t)token * a.c_st : -1;
+    const int64_t at = (int64_t)page * a.s_sp + h;
+    next.key = there ? __float_as_uint(__ldg(a.ks + at)) : QT_ABSENT;
+    next.value = there ? __ldg(a.vs + at) : 0.f;
+  };
+  look(0);
+  place();
+  now = next;
+  look(16);
+  place();
+  now.value = qt_log2(now.value);
+  next.value = qt_log2(next.value);
+  int batch = 0;                             // first tile of `now`
+  const auto request = [&](int j, int stage) {
+    if (j >= mine) {
+      qt_commit();
+      return;
+    }
+    const bool near = j - batch < 16;
+    const int64_t at = near ? now.at : next.at;
+    const int left = __shfl_sync(0xffffffffu, near ? now.left : next.left, (j & 15) << 1);
+    const uint32_t base = ring_at + stage * Q::kStage;
+#pragma unroll
+    for (int i = 0; i < 16 / kRows; ++i) {
+      const int row = i * kRows + lane_row;
+      int64_t from = __shfl_sync(0xffffffffu, at, ((j & 15) << 1) + (row >> 3));
+      const bool fetch = inside && from >= 0 && row < left;
+      from = fetch ? from + (row & 7) * a.c_st + byte : 0;
+      qt_fetch<kPiece>(base + S::key_at(row, byte), kh + from, fetch);
+      qt_fetch<kPiece>(base + S::kTile + S::value_at(row, byte), vh + from, fetch);
+    }
+    qt_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) request(i, i);
+
+  QtState<T, DP, kTiles> state;
+  state.begin(a, current, head0, n_heads);
+  // Writes the current sequence's rows, or its part in this range.
+  const auto finish = [&] {
+    state.sum_weights();
+    const int first = starts[current] >> 4, last = starts[current + 1] >> 4;
+    const bool whole = first >= lo && last <= hi;
+    const int64_t slot = 2 * (int64_t)range + (first >= lo ? 1 : 0);
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int head = 8 * n + 2 * t + r;
+        if (head >= n_heads) continue;
+        const float norm = state.l[n][r], top = state.m[n][r], high = state.w_top[n][r];
+        const float base = top == -INFINITY ? 0.f : top, w_base = high == -INFINITY ? 0.f : high;
+        // the references' difference in two halves: either alone may leave the range
+        const float half = exp2f(0.5f * (w_base - base - QT_LIFT));
+        const float inv = norm == 0.f ? 0.f : half / norm;
+        const int64_t row = slot * a.heads + head0 + head;
+        T* to = static_cast<T*>(a.out) + (int64_t)current * a.o_sb + (int64_t)(head0 + head) * a.o_sh;
+        constexpr int kRead = S::kWords < 4 ? S::kWords : 4;
+#pragma unroll
+        for (int j = 0; j < S::kWords; ++j) {
+          const int d = 128 * (j / 4) + 4 * kRead * g + 4 * (j % 4);
+          if (d >= a.D) continue;
+          const float x[4] = {state.acc[n][2 * j][r] * inv * half,
+                              state.acc[n][2 * j][r + 2] * inv * half,
+                              state.acc[n][2 * j + 1][r] * inv * half,
+                              state.acc[n][2 * j + 1][r + 2] * inv * half};
+          if (whole)
+            quant_store<T>(to + d, x, a.o_whole);
+          else
+            quant_store<float>(a.part + row * a.D + d, x, true);
+        }
+        if (!whole && g == 0) a.part_lse[row] = norm == 0.f ? -INFINITY : base + log2f(norm);
+      }
+  };
+  int end = min(starts[current + 1] >> 4, hi) - lo, stage = 0;
+  for (int j = 0; j < mine; ++j) {
+    const int at16 = j & 15;
+    if (at16 == 0 && j > 0) {
+      now = next;
+      batch = j;
+      look(j + 16);
+    } else if (at16 == 4 && j > 16) {
+      place();
+    } else if (at16 == 8 && j > 16) {
+      next.value = qt_log2(next.value);
+    }
+    qt_wait<kStages - 2>();
+    __syncwarp();
+    request(j + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+    if (j == end) {
+      finish();
+      do ++current; while (starts[current + 1] >> 4 <= lo + j);
+      end = min(starts[current + 1] >> 4, hi) - lo;
+      state.begin(a, current, head0, n_heads);
+    }
+    const int left = __shfl_sync(0xffffffffu, now.left, at16 << 1);
+    uint32_t key[2];
+    float value[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      key[r] = __shfl_sync(0xffffffffu, now.key, (at16 << 1) + r);
+      value[r] = __shfl_sync(0xffffffffu, now.value, (at16 << 1) + r);
+      if (g + 8 * r >= left) key[r] = QT_ABSENT;
+    }
+    state.tile(ring + stage * Q::kStage, key, value);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  }
+  finish();
+}
+
+// A row's partial sums joined by their weights: `team` (1 or 4) of a CTA's four warps per
+// (sequence, head).
+template <typename T>
+__global__ void __launch_bounds__(128) quant_join_kernel(QuantArgs a, int team) {
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const int64_t stride = (int64_t)a.batch * a.heads;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= stride) return;
+  __shared__ float4 xs[4][32];
+  __shared__ float norms[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t rows = (int64_t)a.batch * a.heads;
+  const int64_t row = team == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + warp;
+  if (row >= rows) return;                  // whole CTAs, or warps that meet nobody
+  const int b = (int)(row / a.heads), head = (int)(row % a.heads);
+  int parts = a.slices, first = 0;
+  if (a.ranges) {
+    const int64_t total = a.starts[a.batch] >> 4;
+    const int ranges = quant_used(a.ranges, total);
+    const int from = a.starts[b] >> 4, to = a.starts[b + 1] >> 4;
+    if (from == to) return;
+    const auto range_of = [&](int tile) {   // the range that holds it
+      int r = (int)min((int64_t)tile * ranges / total, (int64_t)ranges - 1);
+      while (total * (r + 1) / ranges <= tile) ++r;
+      while (total * r / ranges > tile) --r;
+      return r;
+    };
+    first = range_of(from);
+    parts = range_of(to - 1) - first + 1;
+    if (parts == 1) return;                 // written already
+  }
+  const auto at = [&](int i) {              // row of part i
+    if (!a.ranges) return i * rows + row;
+    return (2 * (int64_t)(first + i) + (i == 0 ? 1 : 0)) * a.heads + head;
+  };
   float top = -INFINITY;
-  for (int i = lane; i < a.slices; i += 32) top = fmaxf(top, a.part_lse[i * stride + row]);
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[at(i)]);
   top = warp_max(top);
   const float base = top == -INFINITY ? 0.f : top;
-  for (int d = 4 * lane; d < (a.D + 127) / 128 * 128; d += 128) {
+  const int step = team, mine0 = team == 4 ? warp : 0;
+  for (int d0 = 0; d0 < a.D; d0 += 128) {
+    const int d = d0 + 4 * lane;
     float norm = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = 0; p0 < a.slices; p0 += 32) {
-      const float w = p0 + lane < a.slices ? exp2f(a.part_lse[(p0 + lane) * stride + row] - base) : 0.f;
+    for (int p0 = mine0; p0 < parts; p0 += 32 * step) {
+      const int mine = p0 + lane * step;
+      const float w = mine < parts ? exp2f(a.part_lse[at(mine)] - base) : 0.f;
       norm += warp_sum(w);
-      const int n = min(32, a.slices - p0);
+      const int n = min(32, (parts - p0 + step - 1) / step);
       for (int i0 = 0; i0 < n; i0 += 8) {
         float4 y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (i0 + i < n && d < a.D)
-            y[i] = *reinterpret_cast<const float4*>(a.part + ((p0 + i0 + i) * stride + row) * a.D + d);
+            y[i] = *reinterpret_cast<const float4*>(a.part + at(p0 + (i0 + i) * step) * a.D + d);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -553,14 +972,43 @@ __global__ void __launch_bounds__(128) quant_join_kernel(QuantArgs a) {
         }
       }
     }
-    const float inv = norm == 0.f ? 0.f : 1.f / norm;
-    if (d < a.D) {
-      T* to = static_cast<T*>(a.out) + row / a.heads * a.o_sb + row % a.heads * a.o_sh + d;
-      const float o[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+    if (team == 4) {
+      if (d0) __syncthreads();              // the last columns' sums are read
+      xs[warp][lane] = x;
+      if (lane == 0) norms[warp] = norm;
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) to[i] = from_float<T>(o[i]);
+      for (int i = 0; i < 4; ++i) {
+        if (i == warp) continue;
+        const float4 y = xs[i][lane];
+        x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        norm += norms[i];
+      }
     }
+    const float inv = norm == 0.f ? 0.f : 1.f / norm;
+    const float o[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+    if (d < a.D && (team == 1 || warp == 0))
+      quant_store<T>(static_cast<T*>(a.out) + b * a.o_sb + head * a.o_sh + d, o, a.o_whole);
   }
+}
+
+template <typename T>
+static int quant_join(const QuantArgs& p, int parts, cudaStream_t stream) {
+  const int64_t rows = (int64_t)p.batch * p.heads;
+  const int team = parts > 8 ? 4 : 1;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)(team == 4 ? rows : (rows + 3) / 4));
+  config.blockDim = dim3(128);
+  config.stream = counted(stream);
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  if (cudaLaunchKernelEx(&config, quant_join_kernel<T>, p, team) != cudaSuccess)
+    return GRS_ERR_CUDA;
+  GRS_CUDA_CHECK_LAUNCH();
+  return GRS_OK;
 }
 
 // Whether a CTA takes 16 query heads of a group (two column tiles); above width 128
@@ -576,13 +1024,27 @@ static int quant_slices(int batch, int heads, int kv_heads, int D, int64_t room)
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, 128, room / 256}));
 }
 
+// Ranges of the stream form, or 0: sequences that fit its table, and tiles enough to give
+// the warps of all SMs (by the type and width, at most 28 an SM) several each, if the
+// tables are full.  Otherwise four warps share a sequence's head: 5 sequences of 129
+// tokens take one launch there.
+static int quant_ranges(int batch, int heads, int kv_heads, int D, int64_t room, int warps) {
+  const int group = heads / kv_heads, chunk = quant_wide(group, D) ? 16 : 8;
+  const int64_t units = (int64_t)kv_heads * ((group + chunk - 1) / chunk);
+  const int64_t tiles = batch * ((room + 15) / 16);
+  if (batch > QS_MOST || tiles >= 1 << 27 || tiles * units < 4 * (int64_t)warps) return 0;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(warps / units, (tiles + 3) / 4));
+}
+template <typename T, int DP, int kTiles>
+constexpr int quant_warps() { return 148 * QsShape<T, DP, kTiles>::kCtas * QT_WARPS; }
+
 static bool quant_aligned(const QuantArgs& p, int bytes) {
   const uint64_t bits = reinterpret_cast<uintptr_t>(p.kc) | reinterpret_cast<uintptr_t>(p.vc) |
                         (uint64_t)p.c_sp | (uint64_t)p.c_st | (uint64_t)p.c_sh | (uint64_t)p.D;
   return bits % bytes == 0;
 }
 
-template <typename T, int DP, int kTiles, int kPiece>
+template <typename T, int DP, int kTiles, int kPiece, bool kRuns>
 static int quant_mma_run(const QuantArgs& p, cudaStream_t stream) {
   using S = QtShape<DP>;
   constexpr int kSums = QT_WARPS * 8 * kTiles * (S::kSum + 3) * 4;
@@ -592,34 +1054,53 @@ static int quant_mma_run(const QuantArgs& p, cudaStream_t stream) {
   const int64_t rows = (int64_t)p.batch * p.heads;
   if (tasks > INT_MAX || rows > INT_MAX) return GRS_ERR_SHAPE;
   if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(quant_mma_kernel<T, DP, kTiles, kPiece>,
+      cudaFuncSetAttribute(quant_mma_kernel<T, DP, kTiles, kPiece, kRuns>,
                            cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return GRS_ERR_CUDA;
-  quant_mma_kernel<T, DP, kTiles, kPiece>
+  quant_mma_kernel<T, DP, kTiles, kPiece, kRuns>
       <<<dim3((unsigned)tasks, p.slices), 32 * QT_WARPS, smem, counted(stream)>>>(p);
   GRS_CUDA_CHECK_LAUNCH();
-  if (p.slices > 1) {
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)((rows + 3) / 4));
-    config.blockDim = dim3(128);
-    config.stream = counted(stream);
-    config.attrs = &attr;
-    config.numAttrs = 1;
-    if (cudaLaunchKernelEx(&config, quant_join_kernel<T>, p) != cudaSuccess) return GRS_ERR_CUDA;
-    GRS_CUDA_CHECK_LAUNCH();
-  }
+  if (p.slices > 1) return quant_join<T>(p, p.slices, stream);
   return GRS_OK;
 }
 
-template <typename T, int kTiles, int kPiece>
+template <typename T, int DP, int kTiles, int kPiece>
+static int quant_stream_run(QuantArgs p, cudaStream_t stream) {
+  using Q = QsShape<T, DP, kTiles>;
+  const int units = p.kv_heads * ((p.group + 8 * kTiles - 1) / (8 * kTiles));
+  p.slices = 1;
+  p.part_lse = p.part + 2 * (int64_t)p.ranges * p.heads * p.D;
+  p.starts = reinterpret_cast<int32_t*>(p.part_lse + 2 * (int64_t)p.ranges * p.heads);
+  const int smem = QT_WARPS * Q::kStages * Q::kStage + (p.batch + 1) * 4;
+  const int most = QT_WARPS * Q::kStages * Q::kStage + (QS_MOST + 1) * 4;
+  if (cudaFuncSetAttribute(quant_stream_kernel<T, DP, kTiles, kPiece>,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
+    return GRS_ERR_CUDA;
+  const int64_t ctas = ((int64_t)p.ranges * units + QT_WARPS - 1) / QT_WARPS;
+  if (ctas > INT_MAX || (int64_t)p.batch * p.heads > INT_MAX) return GRS_ERR_SHAPE;
+  quant_stream_kernel<T, DP, kTiles, kPiece>
+      <<<(unsigned)ctas, 32 * QT_WARPS, smem, counted(stream)>>>(p);
+  GRS_CUDA_CHECK_LAUNCH();
+  return quant_join<T>(p, p.ranges / p.batch, stream);
+}
+
+template <typename T, int kTiles, int kPiece, bool kRuns>
 static int quant_mma_width(const QuantArgs& p, cudaStream_t stream) {
-  if (p.D <= 32) return quant_mma_run<T, 32, kTiles, kPiece>(p, stream);
-  if (p.D <= 64) return quant_mma_run<T, 64, kTiles, kPiece>(p, stream);
-  if (kTiles == 2 || p.D <= 128) return quant_mma_run<T, 128, kTiles, kPiece>(p, stream);
-  return quant_mma_run<T, 256, 1, kPiece>(p, stream);
+  const auto go = [&](auto width, auto tiles) -> int {
+    constexpr int DP = decltype(width)::value, kT = decltype(tiles)::value;
+    if constexpr (kRuns) {
+      QuantArgs q = p;
+      q.ranges = quant_ranges(p.batch, p.heads, p.kv_heads, p.D, (int64_t)p.columns * p.page,
+                              quant_warps<T, DP, kT>());
+      if (q.ranges) return quant_stream_run<T, DP, kT, kPiece>(q, stream);
+    }
+    return quant_mma_run<T, DP, kT, kPiece, kRuns>(p, stream);
+  };
+  const std::integral_constant<int, kTiles> tiles;
+  if (p.D <= 32) return go(std::integral_constant<int, 32>{}, tiles);
+  if (p.D <= 64) return go(std::integral_constant<int, 64>{}, tiles);
+  if (kTiles == 2 || p.D <= 128) return go(std::integral_constant<int, 128>{}, tiles);
+  return go(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
 }
 
 template <typename T>
@@ -627,8 +1108,10 @@ static int quant_launch(const QuantArgs& p, cudaStream_t stream) {
   if (quant_aligned(p, 8)) {
     const auto go = [&](auto tiles) -> int {
       constexpr int kTiles = decltype(tiles)::value;
-      return quant_aligned(p, 16) ? quant_mma_width<T, kTiles, 16>(p, stream)
-                                  : quant_mma_width<T, kTiles, 8>(p, stream);
+      if (p.page % 8 == 0)
+        return quant_aligned(p, 16) ? quant_mma_width<T, kTiles, 16, true>(p, stream)
+                                    : quant_mma_width<T, kTiles, 8, true>(p, stream);
+      return quant_mma_width<T, kTiles, 8, false>(p, stream);
     };
     return quant_wide(p.group, p.D) ? go(std::integral_constant<int, 2>{})
                                     : go(std::integral_constant<int, 1>{});
@@ -645,8 +1128,16 @@ static int quant_launch(const QuantArgs& p, cudaStream_t stream) {
 extern "C" int64_t grs_quantized_attention_workspace_bytes(int batch, int heads, int kv_heads,
                                                            int head_width, int64_t page_tokens) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
-  const int slices = grs::quant_slices(batch, heads, kv_heads, head_width, page_tokens);
-  return slices > 1 ? (int64_t)slices * batch * heads * (head_width + 1) * 4 : 0;
+  // any of the kernels may take the call, by the type and alignment of its tensors
+  const int64_t slices = grs::quant_slices(batch, heads, kv_heads, head_width, page_tokens);
+  int64_t words = slices > 1 ? slices * batch * heads * (head_width + 1) : 0;
+  for (int warps = 148 * 2 * grs::QT_WARPS; warps <= 148 * 7 * grs::QT_WARPS; warps += 148 * grs::QT_WARPS) {
+    const int64_t ranges =
+        grs::quant_ranges(batch, heads, kv_heads, head_width, page_tokens, warps);
+    if (ranges)
+      words = std::max(words, 2 * ranges * heads * (head_width + 1) + batch + 1);
+  }
+  return words * 4;
 }
 
 extern "C" int grs_quantized_attention(
@@ -684,6 +1175,11 @@ extern "C" int grs_quantized_attention(
     while ((1ll << (p.shift + 1)) < page_size) ++p.shift;
     p.magic = (uint32_t)(((1ull << (32 + p.shift)) + page_size - 1) / page_size);
   }
+  const int item = dtype == GRS_DTYPE_F32 ? 4 : 2;
+  p.q_whole = ((reinterpret_cast<uintptr_t>(query) | (uint64_t)(q_sb * item) |
+                (uint64_t)(q_sh * item) | (uint64_t)(head_width * item)) & 15) == 0;
+  p.o_whole = ((reinterpret_cast<uintptr_t>(output) | (uint64_t)(o_sb * item) |
+                (uint64_t)(o_sh * item)) & (4 * item - 1)) == 0;
   p.slices = quant_slices(batch, heads, kv_heads, head_width, room);
   p.part = static_cast<float*>(workspace);
   p.part_lse = p.part + (int64_t)p.slices * batch * heads * head_width;

@@ -16,73 +16,30 @@ struct RotateArgs {
 };
 
 constexpr int ROT_THREADS = 256;
-constexpr int ROT_AHEAD = 4;                // units of a thread in flight
 
 // One CTA per `rows` tokens.  The (cos, sin) of its tokens' pairs are computed once
-// into shared memory and serve every head; then each thread moves units (two
-// pieces of 16 bytes that turn together) of one place in the head through the
-// (token, head) rows, four at a time.
+// into shared memory; then every thread takes its own pairs' into registers and goes
+// through the heads of its token.
 template <typename T, int kVec, bool kInter>
-__global__ void __launch_bounds__(ROT_THREADS) rotate_kernel(RotateArgs a) {
-  using Units = RotaryUnits<kVec, kInter>;
-  using Piece = RotaryPiece<T, kVec>;
-  extern __shared__ float2 rot_turns[];
+__global__ void __launch_bounds__(ROT_THREADS, 3) rotate_kernel(RotateArgs a) {
+  extern __shared__ __align__(16) float rot_turns[];
   const int64_t first = (int64_t)blockIdx.x * a.rows;
   const int n = (int)min((int64_t)a.rows, a.tokens - first);
-  for (int i = threadIdx.x; i < n * a.pairs; i += ROT_THREADS) {
-    const int64_t at = first + i / a.pairs;
-    const int64_t p = a.wide ? static_cast<const int64_t*>(a.positions)[at]
-                             : static_cast<const int32_t*>(a.positions)[at];
-    const float2 t = rotary_cos_sin(rotary_phase(p, rotary_step(a.freq[i % a.pairs])));
-    rot_turns[i] = make_float2(t.x * a.magnitude, t.y * a.magnitude);
-  }
+  rotary_table<kVec, kInter, ROT_THREADS>(
+      rot_turns, a.freq, a.pairs, a.magnitude, n, [&](int row) -> int64_t {
+        return a.wide ? static_cast<const int64_t*>(a.positions)[first + row]
+                      : static_cast<const int32_t*>(a.positions)[first + row];
+      });
   __syncthreads();
-
-  const int units = Units::count(a.width, a.pairs), each = ROT_THREADS / units;
-  const int all = a.heads + a.kv_heads;
-  if (threadIdx.x >= each * units) return;
-  const Units unit(threadIdx.x % units, a.pairs);
-  int head = threadIdx.x / units % all, token = threadIdx.x / units / all;
-  while (token < n) {
-    Piece x[ROT_AHEAD], y[ROT_AHEAD];
-    T* to[ROT_AHEAD];
-    const float2* turns[ROT_AHEAD];
-#pragma unroll
-    for (int j = 0; j < ROT_AHEAD; ++j) {
-      to[j] = nullptr;
-      if (token >= n) continue;
-      const bool key = head >= a.heads;
-      const int64_t at = first + token, h = key ? head - a.heads : head;
-      const T* from = key ? static_cast<const T*>(a.k) + at * a.k_st + h * a.k_sh
-                          : static_cast<const T*>(a.q) + at * a.q_st + h * a.q_sh;
-      to[j] = key ? static_cast<T*>(a.ko) + at * a.ko_st + h * a.ko_sh
-                  : static_cast<T*>(a.qo) + at * a.qo_st + h * a.qo_sh;
-      turns[j] = rot_turns + token * a.pairs + unit.pair;
-      x[j] = *reinterpret_cast<const Piece*>(from + unit.a);
-      if (unit.two()) y[j] = *reinterpret_cast<const Piece*>(from + unit.b);
-      for (head += each; head >= all; head -= all) ++token;
-    }
-#pragma unroll
-    for (int j = 0; j < ROT_AHEAD; ++j) {
-      if (!to[j]) continue;
-      if (unit.pair >= 0) {
-        float u[kVec], v[kVec];
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          u[i] = to_float(x[j].e[i]);
-          v[i] = Units::kTwo ? to_float(y[j].e[i]) : 0.f;
-        }
-        rotary_turn<T, kVec, kInter>(turns[j], u, v);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          x[j].e[i] = from_float<T>(u[i]);
-          y[j].e[i] = from_float<T>(v[i]);
-        }
-      }
-      *reinterpret_cast<Piece*>(to[j] + unit.a) = x[j];
-      if (unit.two()) *reinterpret_cast<Piece*>(to[j] + unit.b) = y[j];
-    }
-  }
+  // one row of the grid for queries and one for keys, or one for both
+  if (blockIdx.y == 0)
+    rotary_rows<T, kVec, kInter, ROT_THREADS>(
+        rot_turns, a.pairs, a.width, n, a.heads, static_cast<const T*>(a.q) + first * a.q_st,
+        a.q_st, a.q_sh, static_cast<T*>(a.qo) + first * a.qo_st, a.qo_st, a.qo_sh);
+  if (a.kv_heads && blockIdx.y == gridDim.y - 1)
+    rotary_rows<T, kVec, kInter, ROT_THREADS>(
+        rot_turns, a.pairs, a.width, n, a.kv_heads, static_cast<const T*>(a.k) + first * a.k_st,
+        a.k_st, a.k_sh, static_cast<T*>(a.ko) + first * a.ko_st, a.ko_st, a.ko_sh);
 }
 
 template <typename T>
@@ -93,13 +50,14 @@ static int rotate_run(RotateArgs a, bool interleaved, cudaStream_t stream) {
   if (a.kv_heads)
     alignment = std::min({alignment, common_alignment(a.k, a.k_st * e, a.k_sh * e),
                           common_alignment(a.ko, a.ko_st * e, a.ko_sh * e)});
-  // eight tokens share a table, fewer when that would leave SMs without a CTA
-  a.rows = std::min(8, std::max(1, a.tokens / (4 * 148)));
+  // up to eight tokens share a table; fewer when one wave of CTAs holds them all
+  a.rows = std::min(8, (a.tokens + 3 * 148 - 1) / (3 * 148));
   const int64_t ctas = ((int64_t)a.tokens + a.rows - 1) / a.rows;
-  const int smem = a.rows * a.pairs * (int)sizeof(float2);
+  const int smem = a.rows * a.pairs * 2 * (int)sizeof(float);
   return rotary_dispatch<T>(a.width, a.pairs, interleaved, alignment, [&](auto vec, auto inter) -> int {
     rotate_kernel<T, decltype(vec)::value, decltype(inter)::value>
-        <<<(unsigned)ctas, ROT_THREADS, smem, counted(stream)>>>(a);
+        <<<dim3((unsigned)ctas, a.kv_heads && a.rows == 1 ? 2 : 1), ROT_THREADS, smem,
+           counted(stream)>>>(a);
     GRS_CUDA_CHECK_LAUNCH();
     return GRS_OK;
   });

@@ -20,13 +20,12 @@ struct AppendArgs {
   const void* positions; int wide;                    // int32 or int64 [tokens], or null
   const double* freq; int pairs; float magnitude, key_most;
   int tokens, sequences, group, kv_heads, width, pages, page;
-  int units, heads_each, rows, clear;
+  int units, heads_each, rows, code_bytes, clear;
   int32_t* status;
 };
 
 constexpr int AP_THREADS = 256;
 constexpr int AP_ROWS = 16;                 // rows of a CTA's table of turns
-constexpr int AP_AHEAD = 4;                 // units of a thread in flight
 
 // A page that receives tokens: rows [kept, kept + n) of page `to`, from the packed
 // tokens first .. first + n - 1, the first of them at `position`.  The rows before
@@ -83,104 +82,183 @@ __device__ __forceinline__ bool append_unit(const AppendArgs& a, int u, AppendUn
   return true;
 }
 
-// A lane's walk over the pieces of consecutive rows.
-struct PieceWalk {
-  int row, piece;
-  __device__ __forceinline__ PieceWalk(int start, int per_row)
-      : row(start / per_row), piece(start % per_row) {}
-  __device__ __forceinline__ void step(int by, int per_row) {
-    for (piece += by; piece >= per_row; piece -= per_row) ++row;
+// `rows` rows of `pieces` pieces of codes times `ratio` (1: copied), from one page to
+// another or in place.  Threads lane, lane + step, ... of a group; kHold pieces of each
+// in flight.
+template <int kBytes>
+struct CodePieces {
+  using Word = typename std::conditional<
+      kBytes == 16, uint4, typename std::conditional<kBytes == 8, uint2, uint8_t>::type>::type;
+  static constexpr int kHold = 4;
+  Word x[kHold];
+  // the pieces first, first + step, ...; returns how many of them there are
+  __device__ __forceinline__ void load(const uint8_t* from, int64_t stride, int pieces, int count,
+                                       int first, int step) {
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) {
+      const int i = first + j * step;
+      if (i < count)
+        x[j] = *reinterpret_cast<const Word*>(from + i / pieces * stride + i % pieces * kBytes);
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t* to, int64_t stride, int pieces, int count,
+                                        int first, int step, float ratio) {
+    const bool halves = (__float_as_uint(ratio) & 0x7fffffu) == 0 && ratio <= 1.f;
+    const __half2 scale = __float2half2_rn(ratio);
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) {
+      const int i = first + j * step;
+      if (i >= count) continue;
+      if (ratio != 1.f) {
+        if constexpr (kBytes == 1) {
+          x[j] = to_e4m3(from_e4m3(x[j]) * ratio);
+        } else {
+          uint32_t* v = reinterpret_cast<uint32_t*>(&x[j]);
+#pragma unroll
+          for (int k = 0; k < kBytes / 4; ++k)
+            v[k] = halves ? e4m3x2_times(v[k], scale) | e4m3x2_times(v[k] >> 16, scale) << 16
+                          : e4m3x4_times(v[k], ratio);
+        }
+      }
+      *reinterpret_cast<Word*>(to + i / pieces * stride + i % pieces * kBytes) = x[j];
+    }
   }
 };
 
-// The scale of one head's page, and its kept rows under that scale.  A warp.
-template <typename T, int kVec>
-__device__ __forceinline__ float append_scale(const AppendArgs& a, const AppendUnit& unit,
-                                              const T* rows, int64_t stride, float most,
-                                              uint8_t* cache, float* scale) {
-  using Codes = RotaryPiece<uint8_t, kVec>;
-  const int lane = threadIdx.x & 31, pieces = a.width / kVec;
-  float amax = 0.f;
-  PieceWalk w(lane, pieces);
-  while (w.row < unit.n) {
-    RotaryPiece<T, kVec> x[AP_AHEAD];
-#pragma unroll
-    for (int j = 0; j < AP_AHEAD; ++j) {
-      x[j] = {};
-      if (w.row >= unit.n) continue;
-      x[j] = *reinterpret_cast<const RotaryPiece<T, kVec>*>(rows + w.row * stride + w.piece * kVec);
-      w.step(32, pieces);
-    }
-#pragma unroll
-    for (int j = 0; j < AP_AHEAD; ++j)
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        const float y = fabsf(to_float(x[j].e[i]));
-        if (y <= 3.402823466e38f) amax = fmaxf(amax, y);
-      }
+// A lane's walk over the units of consecutive rows at `at`: whole rows side by side in
+// the warp, or a row in several rounds.  Units of 32 and less keep their lanes, whose
+// place then changes by whole strides only.
+template <typename T, int kVec, bool kInter>
+struct RowWalk {
+  using Units = RotaryUnits<kVec, kInter>;
+  T* at;                                    // the row
+  int64_t stride;                           // of a step
+  int row, index, by;                       // unit's index in the row; rows of a step, or 0
+  Units unit;
+  __device__ __forceinline__ RowWalk(T* base, int64_t st, int units, int pairs)
+      : unit((int)(threadIdx.x & 31) % min(units, 32), pairs) {
+    const int lane = threadIdx.x & 31;
+    by = 32 / units;
+    row = by ? lane / units : 0;
+    index = by ? 0 : lane;
+    if (row >= max(by, 1)) row = 1 << 30;   // lanes that are left over
+    at = base + (row < (1 << 30) ? row * st : 0);
+    stride = max(by, 1) * st;
   }
-  const float need = e4m3_scale(warp_max(amax) * most);
-  if (!unit.kept || unit.from < 0) {
-    if (lane == 0) scale[unit.to * a.s_sp] = need;
-    return need;
+  __device__ __forceinline__ bool inside(int n, int units) const {
+    return row < n && index < units;
   }
-  const float before = scale[unit.from * a.s_sp], now = fmaxf(before, need);
-  if (now != before || unit.from != unit.to) {
-    const float ratio = before / now;
-    const uint8_t* from = cache + (int64_t)unit.from * a.c_sp;
-    uint8_t* to = cache + (int64_t)unit.to * a.c_sp;
-    PieceWalk c(lane, pieces);
-    while (c.row < unit.kept) {
-      Codes x[AP_AHEAD];
-      int64_t at[AP_AHEAD];
-#pragma unroll
-      for (int j = 0; j < AP_AHEAD; ++j) {
-        at[j] = -1;
-        if (c.row >= unit.kept) continue;
-        at[j] = c.row * a.c_st + c.piece * kVec;
-        x[j] = *reinterpret_cast<const Codes*>(from + at[j]);
-        c.step(32, pieces);
+  __device__ __forceinline__ void step(int units, int pairs) {
+    if (by) {
+      row += by;
+      at += stride;
+    } else {
+      index += 32;
+      if (index >= (units + 31) / 32 * 32 + (int)(threadIdx.x & 31)) {
+        index = threadIdx.x & 31;
+        ++row;
+        at += stride;
       }
-#pragma unroll
-      for (int j = 0; j < AP_AHEAD; ++j) {
-        if (at[j] < 0) continue;
-        if (ratio != 1.f) {
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) x[j].e[i] = to_e4m3(from_e4m3(x[j].e[i]) * ratio);
-        }
-        *reinterpret_cast<Codes*>(to + at[j]) = x[j];
-      }
+      unit = Units(min(index, units - 1), pairs);
     }
   }
-  __syncwarp();                             // every lane has read the old scale
-  if (lane == 0) scale[unit.to * a.s_sp] = now;
-  return now;
-}
+  static __device__ __forceinline__ int rounds(int n, int units) {
+    return units <= 32 ? (n + 32 / units - 1) / (32 / units) : n * ((units + 31) / 32);
+  }
+};
 
-// One CTA per page that receives tokens and heads_each K/V heads with their query
-// heads.  8-bit pages: a warp per head takes the largest value of the page's new
-// rows (as they come: the scale does not hang on the rotation's rounding, a pair's
-// length bounds what it can become) and moves the rows that are there to the new
-// scale.  Then all threads turn, convert and write the new rows, with a table of
-// the rows' (cos, sin) in shared memory.
-template <typename T, int kVec, bool kInter, bool kCodes>
-__global__ void __launch_bounds__(AP_THREADS) append_kernel(AppendArgs a) {
+// The new rows of one head's page, key or value, by a warp: kHold units of a lane at
+// once.  8-bit pages: the largest value of all of them first, which gives the scale; the
+// blocks of kHold rounds are fetched upwards there and downwards afterwards, so that the
+// last one (the only one of up to 16 rows of 128 bf16 elements) is fetched once.
+template <typename T, int kVec, bool kInter, bool kCodes, int kHold>
+struct AppendHead {
   using Units = RotaryUnits<kVec, kInter>;
   using Piece = RotaryPiece<T, kVec>;
   using Store = typename std::conditional<kCodes, uint8_t, T>::type;
-  extern __shared__ float2 ap_turns[];
-  float* inverse = reinterpret_cast<float*>(ap_turns + a.rows * a.pairs);   // [2][heads_each]
-  const int warp = threadIdx.x >> 5;
-  const int h0 = blockIdx.y * a.heads_each, nh = min(a.heads_each, a.kv_heads - h0);
-  const int nq = a.q ? nh * a.group : 0;
+  Piece x[kHold], y[kHold];
 
-  if ((int)blockIdx.x >= a.units) {         // rows of no sequence
+  __device__ __forceinline__ void fetch(RowWalk<const T, kVec, kInter>& walk, int n, int units,
+                                        int pairs) {
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) {
+      x[j].clear();
+      y[j].clear();
+      if (walk.inside(n, units)) {
+        x[j].load(walk.at + walk.unit.a);
+        if (walk.unit.two()) y[j].load(walk.at + walk.unit.b);
+      }
+      walk.step(units, pairs);
+    }
+  }
+  // The largest absolute value held, as its bits; what is not finite is larger than
+  // any number, or with `finite` left out.
+  __device__ __forceinline__ uint32_t largest(bool finite) const {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) {
+      top = max(top, x[j].largest(finite));
+      if constexpr (Units::kTwo) top = max(top, y[j].largest(finite));
+    }
+    return top;
+  }
+  // `careful`: there may be values that are not finite
+  __device__ __forceinline__ void store(RowWalk<Store, kVec, kInter>& walk, int n, int units,
+                                        int pairs, const float* table, float inverse,
+                                        bool careful) {
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) {
+      if (walk.inside(n, units)) {
+        const Units& unit = walk.unit;
+        float u[kVec], v[kVec] = {};
+        x[j].get(u);
+        if constexpr (Units::kTwo) y[j].get(v);
+        if (table && unit.pair >= 0) {
+          RotaryTurns<kVec, kInter> turns;
+          turns.get(table + 2 * walk.row * pairs, unit.pair, pairs);
+          turns.turn(u, v);
+        }
+        if constexpr (kCodes) {
+          e4m3_store<kVec>(walk.at + unit.a, u, inverse, careful);
+          if (unit.two()) e4m3_store<kVec>(walk.at + unit.b, v, inverse, careful);
+        } else {
+          x[j].set(u);
+          x[j].store(walk.at + unit.a);
+          if (unit.two()) {
+            y[j].set(v);
+            y[j].store(walk.at + unit.b);
+          }
+        }
+      }
+      walk.step(units, pairs);
+    }
+  }
+};
+
+// One CTA per page that receives tokens and heads_each K/V heads with their query
+// heads.  A warp per key or value head: with 8-bit pages it finds the scale (on the
+// values as they come, not on the rotation's rounding: a pair's length bounds what it
+// becomes) and moves the rows that are there to it; then it turns, converts and writes
+// the new rows.  All threads turn the queries.  A table of the rows' (cos, sin) in
+// shared memory serves all of them.
+template <typename T, int kVec, bool kInter, bool kCodes>
+__global__ void __launch_bounds__(AP_THREADS, 2) append_kernel(AppendArgs a) {
+  using Units = RotaryUnits<kVec, kInter>;
+  using From = RowWalk<const T, kVec, kInter>;
+  using Store = typename std::conditional<kCodes, uint8_t, T>::type;
+  constexpr int kHold = Units::kTwo ? 4 : 8;
+  extern __shared__ __align__(16) float ap_turns[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int h0 = blockIdx.y * a.heads_each, nh = min(a.heads_each, a.kv_heads - h0);
+  const int q0 = h0 * a.group, nq = a.q ? nh * a.group : 0;
+
+  if ((int)blockIdx.x >= a.units) {         // query rows of no sequence
     const int begin = min(max(__ldg(a.offsets), 0), a.tokens);
     const int end = min(max(__ldg(a.offsets + a.sequences), begin), a.tokens);
     const int rest = begin + a.tokens - end, all = nq * a.width;
     for (int r = blockIdx.x - a.units; r < rest; r += gridDim.x - a.units) {
       T* row = static_cast<T*>(a.qo) + (int64_t)(r < begin ? r : end + r - begin) * a.qo_st +
-               (int64_t)h0 * a.group * a.qo_sh;
+               q0 * a.qo_sh;
       for (int i = threadIdx.x; i < all; i += AP_THREADS)
         row[i / a.width * a.qo_sh + i % a.width] = from_float<T>(0.f);
     }
@@ -188,116 +266,274 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(AppendArgs a) {
   }
   AppendUnit unit;
   if (!append_unit(a, blockIdx.x, unit)) return;
-  const auto cache = [&](bool value) { return static_cast<Store*>(value ? a.vc : a.kc); };
-  const auto fresh = [&](bool value) { return static_cast<const T*>(value ? a.v : a.k); };
 
-  if (unit.to >= 0) {
+  // this warp's head: a key's, or a value's
+  const bool value = warp >= nh, works = unit.to >= 0 && warp < 2 * nh;
+  const int h = h0 + (value ? warp - nh : warp), units = Units::count(a.width, a.pairs);
+  const int rounds = From::rounds(unit.n, units);
+  const int64_t st = value ? a.v_st : a.k_st;
+  const T* rows = static_cast<const T*>(value ? a.v : a.k) + unit.first * st +
+                  h * (value ? a.v_sh : a.k_sh);
+  Store* cache = static_cast<Store*>(value ? a.vc : a.kc) + (int64_t)unit.to * a.c_sp + h * a.c_sh;
+  AppendHead<T, kVec, kInter, kCodes, kHold> head;
+  float inverse = 1.f;
+  bool careful = false;
+  if (works) {
+    const bool moved = unit.kept && unit.from >= 0;
+    const Store* origin = cache + (int64_t)(unit.from - unit.to) * a.c_sp;
     if constexpr (kCodes) {
-      for (int task = warp; task < 2 * nh; task += AP_THREADS / 32) {
-        const bool which = task >= nh;
-        const int h = h0 + (which ? task - nh : task);
-        const int64_t st = which ? a.v_st : a.k_st, sh = which ? a.v_sh : a.k_sh;
-        const float s = append_scale<T, kVec>(
-            a, unit, fresh(which) + unit.first * st + h * sh, st, which ? 1.f : a.key_most,
-            cache(which) + h * a.c_sh, (which ? a.vs : a.ks) + h);
-        if ((threadIdx.x & 31) == 0) inverse[task] = 1.f / s;
+      float* scales = (value ? a.vs : a.ks) + h;
+      const float before = moved ? scales[unit.from * a.s_sp] : 0.f;
+      const auto largest = [&](bool finite) {
+        uint32_t top = 0;
+        From walk(rows, st, units, a.pairs);
+        for (int r = 0; r < rounds; r += kHold) {
+          head.fetch(walk, unit.n, units, a.pairs);
+          top = max(top, head.largest(finite));
+        }
+        return __reduce_max_sync(0xffffffffu, top);
+      };
+      uint32_t top = largest(false);
+      careful = top >= 0x7e800000u;         // 2^126: a turned pair may overflow
+      if (top >= 0x7f800000u) top = largest(true);
+      const float now =
+          fmaxf(before, e4m3_scale(__uint_as_float(top) * (value ? 1.f : a.key_most)));
+      inverse = 1.f / now;
+      if (moved && (now != before || unit.from != unit.to)) {
+        const auto move = [&](auto bytes) {
+          constexpr int kBytes = decltype(bytes)::value;
+          CodePieces<kBytes> codes;
+          const int pieces = a.width / kBytes, count = unit.kept * pieces;
+          for (int i = lane; i < count; i += 32 * codes.kHold) {
+            codes.load(origin, a.c_st, pieces, count, i, 32);
+            codes.store(cache, a.c_st, pieces, count, i, 32, before / now);
+          }
+        };
+        if (a.code_bytes == 16)
+          move(std::integral_constant<int, 16>{});
+        else if (a.code_bytes == 8)
+          move(std::integral_constant<int, 8>{});
+        else
+          move(std::integral_constant<int, 1>{});
       }
-    } else if (unit.kept && unit.from >= 0 && unit.from != unit.to) {
-      const int pieces = a.width / kVec;
-      for (int task = warp; task < 2 * nh * unit.kept; task += AP_THREADS / 32) {
-        const int head = task / unit.kept, row = task - head * unit.kept;
-        const bool which = head >= nh;
-        const int64_t at = row * a.c_st + (h0 + (which ? head - nh : head)) * a.c_sh;
-        for (int p = threadIdx.x & 31; p < pieces; p += 32)
-          *reinterpret_cast<Piece*>(cache(which) + (int64_t)unit.to * a.c_sp + at + p * kVec) =
-              *reinterpret_cast<const Piece*>(cache(which) + (int64_t)unit.from * a.c_sp + at +
-                                              p * kVec);
+      __syncwarp();                         // every lane has read the old scale
+      if (lane == 0) scales[unit.to * a.s_sp] = now;
+    } else if (moved && unit.from != unit.to) {
+      const int pieces = a.width / kVec, count = unit.kept * pieces;
+      for (int i = lane; i < count; i += 32) {
+        const int64_t at = i / pieces * a.c_st + i % pieces * kVec;
+        RotaryPiece<T, kVec> x;
+        x.load(reinterpret_cast<const T*>(origin) + at);
+        x.store(reinterpret_cast<T*>(cache) + at);
       }
     }
   }
 
-  const int units = Units::count(a.width, a.pairs), each = AP_THREADS / units;
-  const int all = nq + (unit.to >= 0 ? 2 * nh : 0);
-  const bool works = all > 0 && threadIdx.x < each * units;
-  const Units place(threadIdx.x % units, a.pairs);
-  for (int r0 = 0; r0 < unit.n; r0 += a.rows) {
-    const int n = min(a.rows, unit.n - r0);
-    __syncthreads();                        // the scales are known, the last table is read
-    for (int i = threadIdx.x; i < n * a.pairs; i += AP_THREADS) {
-      const int row = r0 + i / a.pairs, at = unit.first + row;
-      int64_t p = unit.position + row;
-      if (a.positions)
-        p = a.wide ? static_cast<const int64_t*>(a.positions)[at]
-                   : static_cast<const int32_t*>(a.positions)[at];
-      const float2 t = rotary_cos_sin(rotary_phase(p, rotary_step(a.freq[i % a.pairs])));
-      ap_turns[i] = make_float2(t.x * a.magnitude, t.y * a.magnitude);
+  // rows in blocks of the table's size, from the last (whose units may be held)
+  const int blocks = (unit.n + a.rows - 1) / a.rows;
+  for (int block = blocks - 1; block >= 0; --block) {
+    const int r0 = block * a.rows, n = min(a.rows, unit.n - r0);
+    if (block != blocks - 1) __syncthreads();             // the last table is read
+    rotary_table<kVec, kInter, AP_THREADS>(
+        ap_turns, a.freq, a.pairs, a.magnitude, n, [&](int row) -> int64_t {
+          if (!a.positions) return unit.position + r0 + row;
+          return a.wide ? static_cast<const int64_t*>(a.positions)[unit.first + r0 + row]
+                        : static_cast<const int32_t*>(a.positions)[unit.first + r0 + row];
+        });
+    __syncthreads();
+    if (works) {
+      const bool held = kCodes && blocks == 1 && rounds <= kHold;
+      From there(rows + r0 * st, st, units, a.pairs);
+      RowWalk<Store, kVec, kInter> walk(cache + (unit.kept + r0) * a.c_st, a.c_st, units, a.pairs);
+      for (int r = From::rounds(n, units); r > 0; r -= kHold) {
+        if (!held) head.fetch(there, n, units, a.pairs);
+        head.store(walk, n, units, a.pairs, value ? nullptr : ap_turns, inverse, careful);
+      }
+    }
+    if (nq) {
+      const int64_t first = unit.first + r0;
+      rotary_rows<T, kVec, kInter, AP_THREADS>(
+          ap_turns, a.pairs, a.width, n, nq,
+          static_cast<const T*>(a.q) + first * a.q_st + q0 * a.q_sh, a.q_st, a.q_sh,
+          static_cast<T*>(a.qo) + first * a.qo_st + q0 * a.qo_sh, a.qo_st, a.qo_sh);
+    }
+  }
+}
+
+// One token per sequence: a CTA per sequence and heads_each K/V heads with their query
+// heads.  A thread keeps one place in the head and takes every slots-th of the key,
+// value and query heads; the first rounds are fetched before anything else is known,
+// and the rows of the last page that are to be copied under the table of (cos, sin):
+// the call is a chain of latencies, not of bytes.
+template <typename T, int kVec, bool kInter, bool kCodes>
+__global__ void __launch_bounds__(AP_THREADS, 3) append_one_kernel(AppendArgs a) {
+  using Units = RotaryUnits<kVec, kInter>;
+  using Piece = RotaryPiece<T, kVec>;
+  using Store = typename std::conditional<kCodes, uint8_t, T>::type;
+  constexpr int kHeld = Units::kTwo ? 2 : 4;
+  extern __shared__ __align__(16) float ap_turns[];
+  uint32_t* tops = reinterpret_cast<uint32_t*>(ap_turns + 2 * a.pairs);   // [2 heads_each]
+  uint32_t* marks = tops + 2 * a.heads_each;                              // [2 heads_each]
+  float* inverses = reinterpret_cast<float*>(marks + 2 * a.heads_each);   // [2 heads_each]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x;
+  const int h0 = blockIdx.y * a.heads_each, nh = min(a.heads_each, a.kv_heads - h0);
+  const int all = 2 * nh + (a.q ? nh * a.group : 0);
+  const int units = Units::count(a.width, a.pairs), slots = AP_THREADS / units;
+  const int slot = threadIdx.x / units;
+  const Units unit(threadIdx.x - slot * units, a.pairs);
+  const auto head_at = [&](int i) {         // key heads, value heads, query heads
+    return i < nh       ? static_cast<const T*>(a.k) + b * a.k_st + (h0 + i) * a.k_sh
+           : i < 2 * nh ? static_cast<const T*>(a.v) + b * a.v_st + (h0 + i - nh) * a.v_sh
+                        : static_cast<const T*>(a.q) + b * a.q_st +
+                              (h0 * a.group + i - 2 * nh) * a.q_sh;
+  };
+  Piece x[kHeld], y[kHeld];
+  const auto fetch = [&](int i, Piece& u, Piece& v) {
+    if (slot >= slots || i >= all) return;
+    const T* at = head_at(i);
+    u.load(at + unit.a);
+    if (unit.two()) v.load(at + unit.b);
+  };
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r) fetch(slot + r * slots, x[r], y[r]);
+  for (int i = threadIdx.x; i < 2 * nh; i += AP_THREADS) tops[i] = marks[i] = 0;
+  AppendUnit page;
+  append_unit(a, b, page);
+  const bool kept = page.to >= 0 && page.kept && page.from >= 0, copied = kept && page.from != page.to;
+
+  // this warp's first head of the kept rows
+  const auto cache_of = [&](int task, int at) {
+    return static_cast<Store*>(task >= nh ? a.vc : a.kc) + (int64_t)at * a.c_sp +
+           (h0 + (task >= nh ? task - nh : task)) * a.c_sh;
+  };
+  const auto scale_of = [&](int task) {
+    return (task >= nh ? a.vs : a.ks) + h0 + (task >= nh ? task - nh : task);
+  };
+  float before = 0.f;
+  CodePieces<16> codes;
+  const int pieces = a.width / 16, count = page.kept * pieces;
+  const bool ahead = kCodes && copied && a.code_bytes == 16;
+  if (warp < 2 * nh) {
+    if (kCodes && kept) before = scale_of(warp)[page.from * a.s_sp];
+    if (ahead) codes.load(reinterpret_cast<const uint8_t*>(cache_of(warp, page.from)), a.c_st, pieces,
+                          count, lane, 32);
+  }
+  rotary_table<kVec, kInter, AP_THREADS>(ap_turns, a.freq, a.pairs, a.magnitude, 1, [&](int) -> int64_t {
+    if (!a.positions) return page.position;
+    return a.wide ? static_cast<const int64_t*>(a.positions)[b]
+                  : static_cast<const int32_t*>(a.positions)[b];
+  });
+  __syncthreads();
+  RotaryTurns<kVec, kInter> turns;
+  if (unit.pair >= 0) turns.get(ap_turns, unit.pair, a.pairs);
+  if constexpr (kCodes) {
+    const auto top_of = [&](int i, const Piece& u, const Piece& v) {
+      if (slot >= slots || i >= 2 * nh) return;
+      const auto both = [&](bool finite) {
+        const uint32_t top = u.largest(finite);
+        return unit.two() ? max(top, v.largest(finite)) : top;
+      };
+      uint32_t top = both(false);
+      if (top >= 0x7f800000u) {             // not finite
+        top = both(true);
+        marks[i] = 1;
+      }
+      atomicMax(&tops[i], top);
+    };
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) top_of(slot + r * slots, x[r], y[r]);
+    for (int i = slot + kHeld * slots; i < 2 * nh; i += slots) {
+      Piece u, v;
+      fetch(i, u, v);
+      top_of(i, u, v);
     }
     __syncthreads();
-    if (!works) continue;
-    int head = threadIdx.x / units % all, row = threadIdx.x / units / all;
-    while (row < n) {
-      Piece x[AP_AHEAD], y[AP_AHEAD];
-      int heads[AP_AHEAD], rows[AP_AHEAD];
-#pragma unroll
-      for (int j = 0; j < AP_AHEAD; ++j) {
-        heads[j] = -1;
-        if (row >= n) continue;
-        heads[j] = head;
-        rows[j] = row;
-        const int64_t at = unit.first + r0 + row;
-        const T* from = head < nq        ? static_cast<const T*>(a.q) + at * a.q_st +
-                                               (int64_t)(h0 * a.group + head) * a.q_sh
-                        : head < nq + nh ? fresh(false) + at * a.k_st + (h0 + head - nq) * a.k_sh
-                                         : fresh(true) + at * a.v_st + (h0 + head - nq - nh) * a.v_sh;
-        x[j] = *reinterpret_cast<const Piece*>(from + place.a);
-        if (place.two()) y[j] = *reinterpret_cast<const Piece*>(from + place.b);
-        for (head += each; head >= all; head -= all) ++row;
-      }
-#pragma unroll
-      for (int j = 0; j < AP_AHEAD; ++j) {
-        if (heads[j] < 0) continue;
-        const bool query = heads[j] < nq, value = heads[j] >= nq + nh;
-        float u[kVec], w[kVec];
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          u[i] = to_float(x[j].e[i]);
-          w[i] = Units::kTwo && place.pair >= 0 ? to_float(y[j].e[i]) : 0.f;
-        }
-        if (!value && place.pair >= 0)
-          rotary_turn<T, kVec, kInter>(ap_turns + rows[j] * a.pairs + place.pair, u, w);
-        if (query || !kCodes) {
-          T* to;
-          if (query)
-            to = static_cast<T*>(a.qo) + (int64_t)(unit.first + r0 + rows[j]) * a.qo_st +
-                 (int64_t)(h0 * a.group + heads[j]) * a.qo_sh;
-          else
-            to = reinterpret_cast<T*>(cache(value)) + (int64_t)unit.to * a.c_sp +
-                 (int64_t)(unit.kept + r0 + rows[j]) * a.c_st +
-                 (h0 + heads[j] - nq - (value ? nh : 0)) * a.c_sh;
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            x[j].e[i] = from_float<T>(u[i]);
-            y[j].e[i] = from_float<T>(w[i]);
+  }
+  for (int task = warp; task < 2 * nh && page.to >= 0; task += AP_THREADS / 32) {
+    if constexpr (kCodes) {
+      float* scale = scale_of(task);
+      if (kept && task != warp) before = scale[page.from * a.s_sp];
+      const float need = e4m3_scale(__uint_as_float(tops[task]) *
+                                    (task >= nh ? 1.f : a.key_most));
+      const float now = fmaxf(before, need);
+      if (kept && (now != before || copied)) {
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(cache_of(task, page.from));
+        uint8_t* to = reinterpret_cast<uint8_t*>(cache_of(task, page.to));
+        const auto move = [&](auto& held, int bytes, bool there) {
+          const int each = a.width / bytes, n = page.kept * each;
+          for (int i = lane; i < n; i += 32 * held.kHold) {
+            if (!there || i != lane) held.load(from, a.c_st, each, n, i, 32);
+            held.store(to, a.c_st, each, n, i, 32, before / now);
           }
-          *reinterpret_cast<Piece*>(to + place.a) = x[j];
-          if (place.two()) *reinterpret_cast<Piece*>(to + place.b) = y[j];
+        };
+        if (a.code_bytes == 16) {
+          move(codes, 16, ahead && task == warp);
+        } else if (a.code_bytes == 8) {
+          CodePieces<8> narrow;
+          move(narrow, 8, false);
         } else {
-          using Codes = RotaryPiece<uint8_t, kVec>;
-          const int h = heads[j] - nq - (value ? nh : 0);
-          const float inv = inverse[heads[j] - nq];
-          uint8_t* to = reinterpret_cast<uint8_t*>(cache(value)) + (int64_t)unit.to * a.c_sp +
-                        (int64_t)(unit.kept + r0 + rows[j]) * a.c_st + (h0 + h) * a.c_sh;
-          Codes c, d;
+          CodePieces<1> single;
+          move(single, 1, false);
+        }
+      }
+      __syncwarp();                         // every lane has read the old scale
+      if (lane == 0) {
+        scale[page.to * a.s_sp] = now;
+        inverses[task] = 1.f / now;
+      }
+    } else if (copied) {
+      const int each = a.width / kVec, n = page.kept * each;
+      const T* from = reinterpret_cast<const T*>(cache_of(task, page.from));
+      T* to = reinterpret_cast<T*>(cache_of(task, page.to));
+      constexpr int kCopies = 4;
+      for (int i0 = lane; i0 < n; i0 += 32 * kCopies) {
+        Piece z[kCopies];
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            c.e[i] = to_e4m3(u[i] * inv);
-            d.e[i] = to_e4m3(w[i] * inv);
-          }
-          *reinterpret_cast<Codes*>(to + place.a) = c;
-          if (place.two()) *reinterpret_cast<Codes*>(to + place.b) = d;
+        for (int j = 0; j < kCopies; ++j) {
+          const int i = i0 + 32 * j;
+          if (i < n) z[j].load(from + i / each * a.c_st + i % each * kVec);
+        }
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) {
+          const int i = i0 + 32 * j;
+          if (i < n) z[j].store(to + i / each * a.c_st + i % each * kVec);
         }
       }
     }
+  }
+  const auto write = [&](int i, Piece& u, Piece& v, bool queries) {
+    if (slot >= slots || i >= all || (i >= 2 * nh) != queries) return;
+    float p[kVec], q[kVec] = {};
+    u.get(p);
+    if constexpr (Units::kTwo) v.get(q);
+    if (unit.pair >= 0 && (i < nh || queries)) turns.turn(p, q);
+    if (queries || !kCodes) {
+      T* to = queries ? static_cast<T*>(a.qo) + b * a.qo_st + (h0 * a.group + i - 2 * nh) * a.qo_sh
+                      : reinterpret_cast<T*>(cache_of(i, page.to)) + page.kept * a.c_st;
+      u.set(p);
+      u.store(to + unit.a);
+      if (unit.two()) {
+        v.set(q);
+        v.store(to + unit.b);
+      }
+    } else {
+      uint8_t* to = reinterpret_cast<uint8_t*>(cache_of(i, page.to)) + page.kept * a.c_st;
+      const bool careful = marks[i] || tops[i] >= 0x7e800000u;   // a turned pair may overflow
+      e4m3_store<kVec>(to + unit.a, p, inverses[i], careful);
+      if (unit.two()) e4m3_store<kVec>(to + unit.b, q, inverses[i], careful);
+    }
+  };
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r) write(slot + r * slots, x[r], y[r], true);
+  if (kCodes) __syncthreads();              // the scales are known
+  if (page.to >= 0) {
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) write(slot + r * slots, x[r], y[r], false);
+  }
+  for (int i = slot + kHeld * slots; i < all; i += slots) {
+    Piece u, v;
+    fetch(i, u, v);
+    if (i >= 2 * nh || page.to >= 0) write(i, u, v, i >= 2 * nh);
   }
 }
 
@@ -319,22 +555,29 @@ static int append_run(AppendArgs a, bool interleaved, cudaStream_t stream) {
                             : a.sequences;
   if (units > INT_MAX - 64) return GRS_ERR_SHAPE;
   a.units = (int)units;
-  const int split = (int)std::min<int64_t>(a.kv_heads, std::max<int64_t>(1, 4 * 148 / std::max<int64_t>(1, units)));
-  a.heads_each = (a.kv_heads + split - 1) / split;
-  a.rows = a.offsets ? std::min(AP_ROWS, a.page) : 1;
-  const dim3 grid((unsigned)(units + (a.clear ? 64 : 0)),
-                  (a.kv_heads + a.heads_each - 1) / a.heads_each);
-  if (grid.y > 65535) return GRS_ERR_SHAPE;
-  const int64_t smem = (int64_t)a.rows * a.pairs * sizeof(float2) + 8 * (int64_t)a.heads_each;
-  if (smem > 48 * 1024) return GRS_ERR_SHAPE;
+  a.code_bytes = a.width % 16 == 0 && cache == 16 ? 16 : a.width % 8 == 0 && cache >= 8 ? 8 : 1;
+  if (a.offsets) {
+    a.heads_each = std::min(a.kv_heads, AP_THREADS / 64);   // a warp per key and value head
+    a.rows = std::min(AP_ROWS, a.page);
+  } else {
+    // all heads of a sequence, fewer while that leaves SMs without a CTA
+    const int split = std::min(a.kv_heads, std::max(1, 2 * 148 / a.sequences));
+    a.heads_each = std::min((a.kv_heads + split - 1) / split, 512);
+    a.rows = 1;
+  }
+  const int64_t groups = ((int64_t)a.kv_heads + a.heads_each - 1) / a.heads_each;
+  if (groups > 65535) return GRS_ERR_SHAPE;
+  const dim3 grid((unsigned)(units + (a.clear ? 64 : 0)), (unsigned)groups);
+  const int smem = (a.rows * a.pairs * 2 + (a.offsets ? 0 : 6 * a.heads_each)) * (int)sizeof(float);
   return rotary_dispatch<T>(a.width, a.pairs, interleaved, alignment,
                             [&](auto vec, auto inter) -> int {
     constexpr int kVec = decltype(vec)::value;
     constexpr bool kInter = decltype(inter)::value;
-    if (codes)
-      append_kernel<T, kVec, kInter, true><<<grid, AP_THREADS, smem, counted(stream)>>>(a);
-    else
-      append_kernel<T, kVec, kInter, false><<<grid, AP_THREADS, smem, counted(stream)>>>(a);
+    const auto kernel = a.offsets ? (codes ? append_kernel<T, kVec, kInter, true>
+                                           : append_kernel<T, kVec, kInter, false>)
+                                  : (codes ? append_one_kernel<T, kVec, kInter, true>
+                                           : append_one_kernel<T, kVec, kInter, false>);
+    kernel<<<grid, AP_THREADS, smem, counted(stream)>>>(a);
     GRS_CUDA_CHECK_LAUNCH();
     return GRS_OK;
   });

@@ -99,6 +99,63 @@ def test_pages(cuda_device, page, dtype):
     _clean(cuda_device)
 
 
+# tiles enough for ranges of tiles over all sequences, whatever their lengths
+STREAMS = [(40, 8, 8, 32, 3000), (30, 32, 8, 128, 1500), (1, 16, 8, 64, 40000),
+           (1000, 8, 8, 32, 70), (1024, 8, 4, 64, 90), (1025, 4, 4, 64, 90),
+           (12, 48, 4, 128, 3100), (9, 40, 4, 64, 4000), (9, 80, 4, 32, 5000),
+           (14, 4, 4, 256, 2600), (9, 8, 8, 40, 3800), (9, 4, 4, 136, 6000)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("batch,heads,kv_heads,width,longest", STREAMS)
+def test_many_tiles(cuda_device, batch, heads, kv_heads, width, longest, dtype):
+    """Ragged sequences, empty ones and ones of a token among them, first and last."""
+    g = torch.Generator().manual_seed(longest)
+    lengths = torch.randint(0, longest + 1, (batch,), generator=g, dtype=torch.int32)
+    lengths[torch.rand(batch, generator=g) < 0.2] = 0
+    lengths[batch // 2] = longest
+    if batch > 4:
+        lengths[[1, batch - 2]] = 1
+        lengths[[0, batch - 1]] = 0
+    args = _case(batch, batch=batch, heads=heads, kv_heads=kv_heads, width=width, longest=longest,
+                 page=8 if width == 64 else 24, lengths=lengths, dtype=dtype)
+    got = _call(cuda_device, args)
+    assert not got[(lengths == 0).to(cuda_device)].any()
+    _check(got, args)
+    _clean(cuda_device)
+
+
+@pytest.mark.parametrize("lengths", [[0] * 30, [0] * 29 + [1], [1] + [0] * 29, [2000] * 30,
+                                     [16] * 30, [17] * 30, [2000] + [0] * 28 + [2000]])
+def test_lengths_that_leave_tables_empty(cuda_device, lengths):
+    """Wide tables whose sequences fill them or do not."""
+    args = _case(len(lengths), batch=30, heads=8, kv_heads=8, width=64, longest=2000,
+                 lengths=torch.tensor(lengths, dtype=torch.int32))
+    _check(_call(cuda_device, args), args)
+
+
+def test_bad_pages_and_lengths_of_many_tiles(cuda_device):
+    args = _case(9, batch=20, heads=8, kv_heads=8, width=64, longest=2000,
+                 lengths=torch.full((20,), 2000, dtype=torch.int32))
+    args["block_table"][2, 1] = 1 << 30
+    args["block_table"][3, 100:] = -1
+    for code, change in ((-2, None), (-7, {0: -5, 7: 2001, 19: 1 << 30})):
+        if change:
+            args["block_table"].clamp_(0, args["key_cache"].shape[0] - 1)
+            for b, n in change.items():
+                args["lengths"][b] = n
+        status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+        got = _call(cuda_device, args, status=status)
+        assert int(status.item()) == code
+        _check(got, args)
+    more = dict(args, lengths=torch.ones(20, dtype=torch.int32))
+    for name in ("key", "value"):
+        more[name + "_cache"] = args[name + "_cache"][:0]
+        more[name + "_scale"] = args[name + "_scale"][:0]
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    assert not _call(cuda_device, more, status=status).any() and int(status.item()) == -2
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_empty_rows_are_zero(cuda_device, dtype):
     lengths = torch.tensor([0, 3, 0, 20, 0, 900], dtype=torch.int32)
@@ -313,13 +370,16 @@ def test_far_pages(cuda_device):
     _check(quantized_attention(**d), args)
 
 
-def test_captured_and_two_calls_at_once(cuda_device):
+@pytest.mark.parametrize("many", [False, True])
+def test_captured_and_two_calls_at_once(cuda_device, many):
     """Two captured graphs replayed together and an eager call, sliced, each with
     a workspace of its own; results do not depend on the run."""
     from graph_rewrite_system_b200.quantized_attention import quantized_attention
 
     dev = cuda_device
     size = dict(batch=3, heads=8, kv_heads=2, width=64, longest=2500)
+    if many:
+        size = dict(batch=20, heads=8, kv_heads=8, width=64, longest=2500)
     first, second = _case(15, **size), _case(16, **size)
     d = _to(dev, first)
     eager = quantized_attention(**d)
