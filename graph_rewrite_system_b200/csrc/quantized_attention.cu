@@ -31,12 +31,13 @@ struct QuantArgs {
 
 constexpr float QA_LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ int quant_length(const QuantArgs& a, int b) {
+__device__ __forceinline__ int quant_length(const QuantArgs& a, int b, bool by_warp = false) {
+  const bool tells = (threadIdx.x & (by_warp ? 31 : ~0)) == 0;
   const int room = a.columns * a.page, length = __ldg(a.lengths + b);
   const int past = min(max(length, 0), room);
-  if (past != length && threadIdx.x == 0) set_status(a.status, GRS_ERR_LENGTH);
+  if (past != length && tells) set_status(a.status, GRS_ERR_LENGTH);
   if (a.pages == 0 && past > 0) {           // no address to read from
-    if (threadIdx.x == 0) set_status(a.status, GRS_ERR_BAD_PAGE);
+    if (tells) set_status(a.status, GRS_ERR_BAD_PAGE);
     return 0;
   }
   return past;
@@ -123,6 +124,7 @@ constexpr int QT_STAGES = 3;
 constexpr float QT_LIFT = 9.f;              // weights are at most 2^(9 + 6): f16 holds them to
 constexpr float QT_SLACK = 6.f;             // 2^-24, 2^-33 of the largest
 constexpr uint32_t QT_ABSENT = 0xffffffffu; // key scale of a token that is not there
+constexpr float QT_UNSET = -3e38f;          // a reference before the first score
 
 __device__ __forceinline__ void qt_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                        uint32_t b1) {
@@ -197,8 +199,8 @@ struct QtShape {
   }
 };
 
-// A warp's work on one sequence and kTiles * 8 query heads.
-template <typename T, int DP, int kTiles>
+// A warp's work on one sequence and kTiles * 8 query heads, kSub tiles of 16 tokens a step.
+template <typename T, int DP, int kTiles, int kSub>
 struct QtState {
   using S = QtShape<DP>;
   static constexpr bool kSplit = std::is_same<T, float>::value;   // operands in two f16 parts
@@ -210,37 +212,57 @@ struct QtState {
   float m[kTiles][2], l[kTiles][2];         // maxima and sums of the scores' weights
   float w_top[kTiles][2];                   // maxima of the scores with the value scale
 
-  __device__ __forceinline__ void begin(const QuantArgs& a, int b, int head0, int n_heads) {
+  // Elements of a query row in the order of its pieces, as they come.
+  struct Query {
+    static constexpr int kEach = 16 / sizeof(T), kLoads = 4 * S::kKeyWords / kEach;
+    uint4 words[kTiles][S::kKey][kLoads];
+  };
+  __device__ __forceinline__ static void fetch(const QuantArgs& a, int b, int head0, int n_heads,
+                                               Query& query) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    // Queries of head g, scaled by a power of two to at most 2^14: f16 then holds a
-    // bf16 element down to 2^-25 of the head's largest exactly, and two parts hold
-    // fp32 to 2^-22.
-  #pragma unroll
+#pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       const bool on = 8 * n + g < n_heads;
       const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb +
                    (int64_t)(head0 + (on ? 8 * n + g : 0)) * a.q_sh;
-      float x[S::kKey][4 * S::kKeyWords], top = 0.f;
-  #pragma unroll
-      for (int i = 0; i < S::kKey; ++i) {
-        constexpr int kEach = 16 / sizeof(T);  // elements of a load
-        const int d0 = (t + 4 * i) * 4 * S::kKeyWords;
-  #pragma unroll
-        for (int e = 0; e < 4 * S::kKeyWords; e += kEach) {
-          alignas(16) T y[kEach] = {};
-          if (on && d0 + e < a.D) {
-            if (a.q_whole) {
-              *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(q + d0 + e);
-            } else {
-  #pragma unroll
-              for (int c = 0; c < kEach; ++c) y[c] = q[d0 + e + c];
-            }
+#pragma unroll
+      for (int i = 0; i < S::kKey; ++i)
+#pragma unroll
+        for (int e = 0; e < Query::kLoads; ++e) {
+          const int d = (t + 4 * i) * 4 * S::kKeyWords + e * Query::kEach;
+          uint4& to = query.words[n][i][e];
+          to = make_uint4(0, 0, 0, 0);
+          if (!on || d >= a.D) continue;
+          if (a.q_whole) {
+            to = *reinterpret_cast<const uint4*>(q + d);
+          } else {
+            T* x = reinterpret_cast<T*>(&to);
+#pragma unroll
+            for (int c = 0; c < Query::kEach; ++c) x[c] = q[d + c];
           }
-  #pragma unroll
-          for (int c = 0; c < kEach; ++c) x[i][e + c] = to_float(y[c]);
         }
-  #pragma unroll
+    }
+  }
+
+  // Queries of head g, scaled by a power of two to at most 2^14: f16 then holds a
+  // bf16 element down to 2^-25 of the head's largest exactly, and two parts hold
+  // fp32 to 2^-22.
+  __device__ __forceinline__ void begin(const QuantArgs& a, const Query& query) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      float x[S::kKey][4 * S::kKeyWords], top = 0.f;
+#pragma unroll
+      for (int i = 0; i < S::kKey; ++i) {
+#pragma unroll
         for (int e = 0; e < 4 * S::kKeyWords; ++e) {
+          const uint4& from = query.words[n][i][e / Query::kEach];
+          const int c = e % Query::kEach;
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(&from);
+          if constexpr (sizeof(T) == 4)
+            x[i][e] = __uint_as_float(w[c]);
+          else
+            x[i][e] = __uint_as_float(c & 1 ? w[c / 2] & 0xffff0000u : w[c / 2] << 16);
           const float y = fabsf(x[i][e]);
           if (y <= 3.402823466e38f) top = fmaxf(top, y);
         }
@@ -272,133 +294,158 @@ struct QtState {
       for (int j = 0; j < 2 * S::kWords; ++j)
         acc[n][j][0] = acc[n][j][1] = acc[n][j][2] = acc[n][j][3] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) m[n][r] = w_top[n][r] = -INFINITY, l[n][r] = 0.f;
+      for (int r = 0; r < 2; ++r) m[n][r] = w_top[n][r] = QT_UNSET, l[n][r] = 0.f;
     }
   }
 
-  // The staged tile `at`; key scale and log2 of the value scale of tokens g and g + 8.
-  __device__ __forceinline__ void tile(const uint8_t* at, const uint32_t (&key)[2],
-                                       const float (&value)[2]) {
+  // The staged tiles at `keys` and `values`; key scale and log2 of the value scale of
+  // tokens g and g + 8 of each.
+  __device__ __forceinline__ void step(const uint8_t* keys, const uint8_t* values,
+                                       const uint32_t (&key)[kSub][2],
+                                       const float (&value)[kSub][2]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    float s[kTiles][4];                     // tokens (g, g + 8) x heads (2t, 2t + 1)
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-    for (int i = 0; i < S::kKey; ++i) {
-      uint32_t k[2][4];
+    float s[kSub][kTiles][4];               // tokens (g, g + 8) x heads (2t, 2t + 1)
+    float x[kSub][kTiles][4], z[kSub][kTiles][4];   // their exponents, without and with the
+    bool grown = false;                             // value scale, above the references
+    const auto exponents = [&](int u, bool above) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        if constexpr (DP >= 64) {
-          const uint4 x = *reinterpret_cast<const uint4*>(at + S::key_at(g + 8 * r, 16 * (t + 4 * i)));
-          k[r][0] = x.x, k[r][1] = x.y, k[r][2] = x.z, k[r][3] = x.w;
-        } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(at + S::key_at(g + 8 * r, 8 * t));
-          k[r][0] = x.x, k[r][1] = x.y;
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < S::kKeyWords; ++e) {
-        uint32_t f[4];
-        qt_widen(k[0][e], f[0], f[2]);
-        qt_widen(k[1][e], f[1], f[3]);
+        const bool there = key[u][r] != QT_ABSENT;
+        const float scale = there ? __uint_as_float(key[u][r]) : 0.f, base = there ? 0.f : -INFINITY;
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-          for (int p = 0; p < kParts; ++p) {
-            const auto& q = qf[n][i * S::kKeyWords + e];
-            qt_mma(s[n], f, q[0][p], q[1][p]);
+          for (int c = 0; c < 2; ++c) {
+            const float f = unit[n][c] * scale;
+            x[u][n][2 * r + c] = fmaf(s[u][n][2 * r + c], f, above ? base - m[n][c] : base);
+            z[u][n][2 * r + c] =
+                fmaf(s[u][n][2 * r + c], f,
+                     above ? (base + value[u][r]) - (w_top[n][c] - QT_LIFT) : base + value[u][r]);
           }
       }
-    }
-    float z[kTiles][4];
-    bool grown = false;
+    };
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int u = 0; u < kSub; ++u) {
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n)
+      for (int n = 0; n < kTiles; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.f;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float& x = s[n][2 * r + c];
-          x = key[r] == QT_ABSENT ? -INFINITY : x * unit[n][c] * __uint_as_float(key[r]);
-          z[n][2 * r + c] = x + value[r];
-          grown |= x > m[n][c] + QT_SLACK || z[n][2 * r + c] > w_top[n][c] + QT_SLACK;
+      for (int i = 0; i < S::kKey; ++i) {
+        uint32_t k[2][4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint8_t* at = keys + u * S::kTile;
+          if constexpr (DP >= 64) {
+            const uint4 x = *reinterpret_cast<const uint4*>(at + S::key_at(g + 8 * r, 16 * (t + 4 * i)));
+            k[r][0] = x.x, k[r][1] = x.y, k[r][2] = x.z, k[r][3] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(at + S::key_at(g + 8 * r, 8 * t));
+            k[r][0] = x.x, k[r][1] = x.y;
+          }
         }
+#pragma unroll
+        for (int e = 0; e < S::kKeyWords; ++e) {
+          uint32_t f[4];
+          qt_widen(k[0][e], f[0], f[2]);
+          qt_widen(k[1][e], f[1], f[3]);
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+              const auto& q = qf[n][i * S::kKeyWords + e];
+              qt_mma(s[u][n], f, q[0][p], q[1][p]);
+            }
+        }
+      }
+      exponents(u, true);
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          grown |= x[u][n][c] > QT_SLACK || z[u][n][c] > QT_LIFT + QT_SLACK;
     }
-    if (__any_sync(0xffffffffu, grown)) {
+    if (__any_sync(0xffffffffu, grown)) {   // new references: the largest so far
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) exponents(u, false);
 #pragma unroll
       for (int n = 0; n < kTiles; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float x = fmaxf(s[n][c], s[n][c + 2]), y = fmaxf(z[n][c], z[n][c + 2]);
+          float top = m[n][c], high = w_top[n][c];
+#pragma unroll
+          for (int u = 0; u < kSub; ++u) {
+            top = fmaxf(top, fmaxf(x[u][n][c], x[u][n][c + 2]));
+            high = fmaxf(high, fmaxf(z[u][n][c], z[u][n][c + 2]));
+          }
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
           }
-          x = fmaxf(x, m[n][c]);
-          y = fmaxf(y, w_top[n][c]);
-          if (x != -INFINITY) l[n][c] *= qt_exp2(m[n][c] - x);
-          const float keep = y == -INFINITY ? 1.f : qt_exp2(w_top[n][c] - y);
+          l[n][c] *= qt_exp2(m[n][c] - top);
+          const float keep = qt_exp2(w_top[n][c] - high);
 #pragma unroll
           for (int j = 0; j < 2 * S::kWords; ++j) {
             acc[n][j][c] *= keep;
             acc[n][j][c + 2] *= keep;
           }
-          m[n][c] = x;
-          w_top[n][c] = y;
+          m[n][c] = top;
+          w_top[n][c] = high;
         }
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) exponents(u, true);
     }
-    uint32_t p[kTiles][2][kParts];          // weights of tokens 2t, 2t + 1 (+ 8) of head g
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      float w[4];
+    for (int u = 0; u < kSub; ++u) {
+      uint32_t p[kTiles][2][kParts];        // weights of tokens 2t, 2t + 1 (+ 8) of head g
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float top = m[n][c & 1], high = w_top[n][c & 1];
-        l[n][c & 1] += qt_exp2(s[n][c] - (top == -INFINITY ? 0.f : top));
-        w[c] = qt_exp2(z[n][c] - (high == -INFINITY ? 0.f : high - QT_LIFT));
-      }
+      for (int n = 0; n < kTiles; ++n) {
+        float w[4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        p[n][r][0] = qt_transpose(qt_pack(w[2 * r], w[2 * r + 1]));
-        if constexpr (kSplit)
-          p[n][r][1] = qt_transpose(qt_pack(qt_rest(w[2 * r]), qt_rest(w[2 * r + 1])));
-      }
-    }
-    // values of tokens 2t, 2t + 1, 2t + 8, 2t + 9
-    const uint8_t* values = at + S::kTile;
+        for (int c = 0; c < 4; ++c) {
+          l[n][c & 1] += qt_exp2(x[u][n][c]);
+          w[c] = qt_exp2(z[u][n][c]);
+        }
 #pragma unroll
-    for (int i = 0; i < (DP + 127) / 128; ++i) {
-      constexpr int kRead = S::kWords < 4 ? S::kWords : 4;   // words of a read
-      uint32_t v[4][kRead];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const uint8_t* x = values + S::value_at(2 * t + (n & 1) + 8 * (n >> 1),
-                                                128 * i + 4 * kRead * g);
-        if constexpr (kRead == 4) {
-          const uint4 y = *reinterpret_cast<const uint4*>(x);
-          v[n][0] = y.x, v[n][1] = y.y, v[n][2] = y.z, v[n][3] = y.w;
-        } else if constexpr (kRead == 2) {
-          const uint2 y = *reinterpret_cast<const uint2*>(x);
-          v[n][0] = y.x, v[n][1] = y.y;
-        } else {
-          v[n][0] = *reinterpret_cast<const uint32_t*>(x);
+        for (int r = 0; r < 2; ++r) {
+          p[n][r][0] = qt_transpose(qt_pack(w[2 * r], w[2 * r + 1]));
+          if constexpr (kSplit)
+            p[n][r][1] = qt_transpose(qt_pack(qt_rest(w[2 * r]), qt_rest(w[2 * r + 1])));
         }
       }
+      // values of tokens 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-      for (int e = 0; e < kRead; ++e)
+      for (int i = 0; i < (DP + 127) / 128; ++i) {
+        constexpr int kRead = S::kWords < 4 ? S::kWords : 4;   // words of a read
+        uint32_t v[4][kRead];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const unsigned pick = c ? 0x7362u : 0x5140u;
-          uint32_t f[4];
-          qt_widen(__byte_perm(v[0][e], v[1][e], pick), f[0], f[1]);
-          qt_widen(__byte_perm(v[2][e], v[3][e], pick), f[2], f[3]);
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-            for (int k = 0; k < kParts; ++k)
-              qt_mma(acc[n][2 * (4 * i + e) + c], f, p[n][0][k], p[n][1][k]);
+        for (int n = 0; n < 4; ++n) {
+          const uint8_t* x = values + u * S::kTile +
+                             S::value_at(2 * t + (n & 1) + 8 * (n >> 1), 128 * i + 4 * kRead * g);
+          if constexpr (kRead == 4) {
+            const uint4 y = *reinterpret_cast<const uint4*>(x);
+            v[n][0] = y.x, v[n][1] = y.y, v[n][2] = y.z, v[n][3] = y.w;
+          } else if constexpr (kRead == 2) {
+            const uint2 y = *reinterpret_cast<const uint2*>(x);
+            v[n][0] = y.x, v[n][1] = y.y;
+          } else {
+            v[n][0] = *reinterpret_cast<const uint32_t*>(x);
+          }
         }
+#pragma unroll
+        for (int e = 0; e < kRead; ++e)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const unsigned pick = c ? 0x7362u : 0x5140u;
+            uint32_t f[4];
+            qt_widen(__byte_perm(v[0][e], v[1][e], pick), f[0], f[1]);
+            qt_widen(__byte_perm(v[2][e], v[3][e], pick), f[2], f[3]);
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+              for (int k = 0; k < kParts; ++k)
+                qt_mma(acc[n][2 * (4 * i + e) + c], f, p[n][0][k], p[n][1][k]);
+          }
+      }
     }
   }
 
@@ -429,6 +476,8 @@ __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
   const int lo = (int)((int64_t)tiles * blockIdx.y / gridDim.y);
   const int hi = (int)((int64_t)tiles * (blockIdx.y + 1) / gridDim.y);
   const int mine = max(0, (hi - lo - warp + QT_WARPS - 1) / QT_WARPS);   // this warp's tiles
+  typename QtState<T, DP, kTiles, 1>::Query query;
+  QtState<T, DP, kTiles, 1>::fetch(a, b, head0, n_heads, query);
   uint8_t* ring = qt_smem + warp * S::kRing;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   const int32_t* table = a.bt + (int64_t)b * a.bt_s;
@@ -525,8 +574,8 @@ __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
 #pragma unroll
   for (int i = 0; i < QT_STAGES - 1; ++i) request(i, i);
 
-  QtState<T, DP, kTiles> state;
-  state.begin(a, b, head0, n_heads);
+  QtState<T, DP, kTiles, 1> state;
+  state.begin(a, query);
   int stage = 0;
   for (int j = 0; j < mine; ++j) {
     if constexpr (kRuns) {
@@ -552,20 +601,20 @@ __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
 
     const uint32_t* scales = reinterpret_cast<const uint32_t*>(at + 2 * S::kTile);
     const int left = past - tile_of(j) * 16;
-    uint32_t key[2];
-    float value[2];
+    uint32_t key[1][2];
+    float value[1][2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       if constexpr (kRuns) {
-        key[r] = __shfl_sync(0xffffffffu, now.key, ((j & 15) << 1) + r);
-        value[r] = __shfl_sync(0xffffffffu, now.value, ((j & 15) << 1) + r);
-        if (g + 8 * r >= left) key[r] = QT_ABSENT;
+        key[0][r] = __shfl_sync(0xffffffffu, now.key, ((j & 15) << 1) + r);
+        value[0][r] = __shfl_sync(0xffffffffu, now.value, ((j & 15) << 1) + r);
+        if (g + 8 * r >= left) key[0][r] = QT_ABSENT;
       } else {
-        key[r] = scales[g + 8 * r];
-        value[r] = qt_log2(__uint_as_float(scales[16 + g + 8 * r]));
+        key[0][r] = scales[g + 8 * r];
+        value[0][r] = qt_log2(__uint_as_float(scales[16 + g + 8 * r]));
       }
     }
-    state.tile(at, key, value);
+    state.step(at, at + S::kTile, key, value);
   }
 
   // the warps' sums meet in shared memory
@@ -596,13 +645,13 @@ __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
   __syncthreads();
   const int64_t stride = (int64_t)a.batch * a.heads;
   for (int head = warp; head < n_heads; head += QT_WARPS) {
-    float top = -INFINITY, high = -INFINITY;
+    float top = QT_UNSET, high = QT_UNSET;
 #pragma unroll
     for (int i = 0; i < QT_WARPS; ++i) {
       top = fmaxf(top, tops[(i * kHeads + head) * 3]);
       high = fmaxf(high, tops[(i * kHeads + head) * 3 + 2]);
     }
-    const float base = top == -INFINITY ? 0.f : top, w_base = high == -INFINITY ? 0.f : high;
+    const float base = top == QT_UNSET ? 0.f : top, w_base = high == QT_UNSET ? 0.f : high;
     float norm = 0.f, w[QT_WARPS];
 #pragma unroll
     for (int i = 0; i < QT_WARPS; ++i) {
@@ -647,20 +696,27 @@ __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
 // the warps of the other heads of those tokens run beside it, so that whole pages are
 // read at once.  A sequence that one range holds is written at once; parts of one go to
 // the workspace, at most two of a range, and are joined by quant_join_kernel.
+constexpr int QS_SHORT = 256;               // tokens of a table row that one warp takes,
+constexpr int QS_MANY = 3500;               // four times as many if there are so many warps
 constexpr int QS_MOST = 1024;               // sequences: their first tiles are in shared memory
 
 template <typename T, int DP, int kTiles>
 struct QsShape {
-  // CTAs that share an SM (by registers) and tiles that a warp has in flight and in use
+  // CTAs that share an SM (by registers), tokens of a step, steps that a warp has in
+  // flight and in use: fewer warps with more steps in flight read faster (64 sequences of
+  // up to 4099 tokens: four CTAs of three 16-token steps 63 us, three of four 61.5)
   static constexpr bool kSplit = std::is_same<T, float>::value;
-  static constexpr int kCtas = DP > 128 ? 2 : DP > 64 ? (kTiles == 1 && !kSplit ? 4 : kTiles == 1 ? 3 : 2)
-                             : kTiles == 1 ? (DP > 32 ? 5 : 7) : kSplit ? 3 : 4;
-  static constexpr int kStages = DP >= 128 ? 3 : 4;
-  static constexpr int kStage = 2 * QtShape<DP>::kTile;
+  static constexpr int kCtas = DP > 128 ? 2 : DP > 64 ? (kTiles == 1 ? 3 : 2)
+                             : kTiles == 1 ? (DP > 32 ? 4 : 5) : kSplit ? 2 : 3;
+  static constexpr int kSub = DP > 64 || kTiles == 2 ? 1 : 2, kSpan = 16 * kSub;
+  static constexpr int kStages = DP > 128 || (DP == 64 && kSub == 2) ? 3 : 4;
+  static constexpr int kStage = 2 * kSub * QtShape<DP>::kTile;
+  static constexpr int kBits = kSub == 1 ? 4 : 5;         // log2 of kSpan
 };
 
-// First tiles of the sequences, shifted left by four bits, with the tokens of the last
-// tile (0: 16) below; shared memory, `starts[batch]` is all tiles.  Two barriers.
+// First steps of the sequences, shifted left by kBits, with the tokens of the last step
+// (0: all) below; shared memory, `starts[batch]` is all steps.  Two barriers.
+template <int kBits>
 __device__ __forceinline__ void quant_starts(const QuantArgs& a, int* starts, int* sums) {
   constexpr int kThreads = 32 * QT_WARPS, kEach = QS_MOST / kThreads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -679,7 +735,7 @@ __device__ __forceinline__ void quant_starts(const QuantArgs& a, int* starts, in
         past[i] = 0;
       }
     }
-    total += (past[i] + 15) / 16;
+    total += (past[i] + (1 << kBits) - 1) >> kBits;
   }
   int before = total;
 #pragma unroll
@@ -694,17 +750,28 @@ __device__ __forceinline__ void quant_starts(const QuantArgs& a, int* starts, in
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int b = threadIdx.x * each + i;
-    if (i < each && b <= a.batch) starts[b] = before << 4 | (past[i] & 15);
-    before += (past[i] + 15) / 16;
+    if (i < each && b <= a.batch) starts[b] = before << kBits | (past[i] & ((1 << kBits) - 1));
+    before += (past[i] + (1 << kBits) - 1) >> kBits;
   }
-  if (threadIdx.x == kThreads - 1 && a.batch == kThreads * each) starts[a.batch] = before << 4;
+  if (threadIdx.x == kThreads - 1 && a.batch == kThreads * each) starts[a.batch] = before << kBits;
   __syncthreads();
 }
 
-// Ranges in use: none is empty, four tiles each at least (but for the last tiles).
-__device__ __forceinline__ int quant_used(int ranges, int64_t total) {
-  return (int)max((int64_t)1, min((int64_t)ranges, total / 4));
-}
+// How all steps are cut: ranges of four steps at least, the first `rest` of them one
+// longer than the others.
+struct QsCut {
+  int ranges, each, rest;
+  __device__ __forceinline__ QsCut(int most, int total) {
+    ranges = max(1, min(most, total / 4));
+    each = total / ranges;
+    rest = total - each * ranges;
+  }
+  __device__ __forceinline__ int first(int range) const { return each * range + min(range, rest); }
+  __device__ __forceinline__ int holds(int tile) const {   // the range that does
+    const int longer = rest * (each + 1);
+    return tile < longer ? tile / (each + 1) : rest + (tile - longer) / each;
+  }
+};
 
 template <typename T>
 __device__ __forceinline__ void quant_store(T* to, const float (&x)[4], bool whole) {
@@ -720,47 +787,68 @@ __device__ __forceinline__ void quant_store(T* to, const float (&x)[4], bool who
   }
 }
 
-template <typename T, int DP, int kTiles, int kPiece>
+// kWhole: every warp has one sequence (short ones; no table of first steps, no parts).
+template <typename T, int DP, int kTiles, int kPiece, bool kWhole>
 __global__ void __launch_bounds__(32 * QT_WARPS, (QsShape<T, DP, kTiles>::kCtas))
     quant_stream_kernel(QuantArgs a) {
   using S = QtShape<DP>;
   using Q = QsShape<T, DP, kTiles>;
-  constexpr int kHeads = 8 * kTiles, kStages = Q::kStages;
+  using State = QtState<T, DP, kTiles, Q::kSub>;
+  constexpr int kHeads = 8 * kTiles, kStages = Q::kStages, kSub = Q::kSub, kBits = Q::kBits;
+  constexpr int kAhead = 16 / kSub;          // steps that the lanes look up at once
   extern __shared__ __align__(128) uint8_t qt_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  if (!kWhole) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   uint8_t* ring = qt_smem + warp * kStages * Q::kStage;
-  int* starts = reinterpret_cast<int*>(qt_smem + QT_WARPS * kStages * Q::kStage);
-  quant_starts(a, starts, reinterpret_cast<int*>(qt_smem));
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= a.batch; i += 32 * QT_WARPS) a.starts[i] = starts[i];
-  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {       // rows without keys
-    if (starts[b] >> 4 != starts[b + 1] >> 4) continue;
-    for (int i = threadIdx.x; i < a.heads * a.D; i += 32 * QT_WARPS)
-      static_cast<T*>(a.out)[b * a.o_sb + i / a.D * a.o_sh + i % a.D] = from_float<T>(0.f);
-  }
-
+  const int* starts = reinterpret_cast<int*>(qt_smem + QT_WARPS * kStages * Q::kStage);
   const int chunks = (a.group + kHeads - 1) / kHeads, units = a.kv_heads * chunks;
-  const int64_t job = (int64_t)blockIdx.x * QT_WARPS + warp;
-  const int range = (int)(job / units), part = (int)(job % units), h = part / chunks;
-  const int64_t total = starts[a.batch] >> 4;
-  const int ranges = quant_used(a.ranges, total);
-  if (range >= ranges) return;
-  const int lo = (int)(total * range / ranges), hi = (int)(total * (range + 1) / ranges);
-  if (lo >= hi) return;
+  const int job = blockIdx.x * QT_WARPS + warp;
+  const int range = job / units, part = job - range * units, h = part / chunks;
   const int head0 = h * a.group + part % chunks * kHeads;
   const int n_heads = min(kHeads, (h + 1) * a.group - head0);
-  int seq = 0;                               // the last sequence that starts at or before lo
-  for (int left = a.batch; left > 1;) {
-    const int half = left / 2;
-    if (starts[seq + half] >> 4 <= lo) {
-      seq += half;
-      left -= half;
-    } else {
-      left = half;
+  int lo, hi, seq = 0, whole_fill = 0;
+  if constexpr (kWhole) {
+    if (range >= a.batch) return;
+    const int past = quant_length(a, range, true);
+    seq = range;
+    lo = 0;
+    hi = (past + Q::kSpan - 1) >> kBits;
+    whole_fill = past & (Q::kSpan - 1);
+    if (hi == 0) {                           // no keys
+      for (int i = lane; i < n_heads * a.D; i += 32)
+        static_cast<T*>(a.out)[seq * a.o_sb + (head0 + i / a.D) * a.o_sh + i % a.D] =
+            from_float<T>(0.f);
+      return;
+    }
+  } else {
+    quant_starts<kBits>(a, const_cast<int*>(starts), reinterpret_cast<int*>(qt_smem));
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i <= a.batch; i += 32 * QT_WARPS) a.starts[i] = starts[i] >> kBits;
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {     // rows without keys
+      if (starts[b] >> kBits != starts[b + 1] >> kBits) continue;
+      for (int i = threadIdx.x; i < a.heads * a.D; i += 32 * QT_WARPS)
+        static_cast<T*>(a.out)[b * a.o_sb + i / a.D * a.o_sh + i % a.D] = from_float<T>(0.f);
+    }
+    const QsCut cut(a.ranges, starts[a.batch] >> kBits);
+    if (range >= cut.ranges) return;
+    lo = cut.first(range);
+    hi = cut.first(range + 1);
+    if (lo >= hi) return;
+    for (int left = a.batch; left > 1;) {    // the last sequence that starts at or before lo
+      const int half = left / 2;
+      if (starts[seq + half] >> kBits <= lo) {
+        seq += half;
+        left -= half;
+      } else {
+        left = half;
+      }
     }
   }
+  const auto first_of = [&](int b) { return kWhole ? 0 : starts[b] >> kBits; };
+  const auto last_of = [&](int b) { return kWhole ? hi : starts[b + 1] >> kBits; };
   int current = seq;                         // of the warp; seq: of this lane's look-ups
+  typename State::Query query;
+  State::fetch(a, current, head0, n_heads, query);
 
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   const uint8_t* const kh = a.kc + h * a.c_sh;
@@ -768,11 +856,12 @@ __global__ void __launch_bounds__(32 * QT_WARPS, (QsShape<T, DP, kTiles>::kCtas)
   constexpr int kLanes = DP / kPiece, kRows = 32 / kLanes;   // lanes of a row, rows of a round
   const int lane_row = lane / kLanes, byte = lane % kLanes * kPiece;
   const bool inside = byte < a.D;
+  const int64_t lane_at = (lane_row & 7) * a.c_st + byte;
   const int mine = hi - lo;
 
-  // Lane i looks up the two runs of 8 tokens of sixteen tiles ahead at once - place,
-  // tokens of the tile, key scale and log2 of the value scale - and they are handed round
-  // by shuffles; `next` is looked up in steps while `now` is in use.
+  // Lane i looks up one run of 8 tokens, all of them kAhead steps' at once - place, tokens
+  // of the step, key scale and log2 of the value scale - and they are handed round by
+  // shuffles; `next` is looked up in stages while `now` is in use.
   struct Runs {
     int64_t at;
     int left;
@@ -782,15 +871,17 @@ __global__ void __launch_bounds__(32 * QT_WARPS, (QsShape<T, DP, kTiles>::kCtas)
   Runs now, next;
   int page = -1, token = -1;
   const auto look = [&](int j) {
-    const int f = lo + j + (lane >> 1);
+    const int f = lo + j + lane / (2 * kSub);
     page = token = -1;
     next.left = 0;
     if (f >= hi) return;
-    while (starts[seq + 1] >> 4 <= f) ++seq;
-    const int tile = f - (starts[seq] >> 4), fill = starts[seq] & 15;
-    next.left = f + 1 == starts[seq + 1] >> 4 && fill ? fill : 16;
-    if ((lane & 1) * 8 >= next.left) return;
-    token = tile * 16 + (lane & 1) * 8;
+    if constexpr (!kWhole)
+      while (last_of(seq) <= f) ++seq;
+    const int fill = kWhole ? whole_fill : starts[seq] & (Q::kSpan - 1);
+    const int row = lane % (2 * kSub) * 8;
+    next.left = f + 1 == last_of(seq) && fill ? fill : Q::kSpan;
+    if (row >= next.left) return;
+    token = (f - first_of(seq)) * Q::kSpan + row;
     const int column = a.magic ? (int)(__umulhi((uint32_t)token, a.magic) >> a.shift) : token;
     page = __ldg(a.bt + (int64_t)seq * a.bt_s + column);
     token -= column * a.page;                // the run's first row in its page
@@ -803,45 +894,70 @@ __global__ void __launch_bounds__(32 * QT_WARPS, (QsShape<T, DP, kTiles>::kCtas)
     next.key = there ? __float_as_uint(__ldg(a.ks + at)) : QT_ABSENT;
     next.value = there ? __ldg(a.vs + at) : 0.f;
   };
-  look(0);
-  place();
-  now = next;
-  look(16);
-  place();
-  now.value = qt_log2(now.value);
-  next.value = qt_log2(next.value);
-  int batch = 0;                             // first tile of `now`
+  {
+    look(0);                                 // the second look-up's pages with the first's
+    const int page0 = page, token0 = token, left0 = next.left;
+    look(kAhead);
+    const int page1 = page, token1 = token, left1 = next.left;
+    page = page0;
+    token = token0;
+    place();
+    now = next;
+    now.left = left0;
+    page = page1;
+    token = token1;
+    place();
+    next.left = left1;
+    now.value = qt_log2(now.value);
+    next.value = qt_log2(next.value);
+  }
+  int batch = 0;                             // first step of `now`
   const auto request = [&](int j, int stage) {
     if (j >= mine) {
       qt_commit();
       return;
     }
-    const bool near = j - batch < 16;
+    const bool near = j - batch < kAhead;
     const int64_t at = near ? now.at : next.at;
-    const int left = __shfl_sync(0xffffffffu, near ? now.left : next.left, (j & 15) << 1);
+    const int run0 = j % kAhead * 2 * kSub;
+    const int left = __shfl_sync(0xffffffffu, near ? now.left : next.left, run0);
     const uint32_t base = ring_at + stage * Q::kStage;
 #pragma unroll
-    for (int i = 0; i < 16 / kRows; ++i) {
-      const int row = i * kRows + lane_row;
-      int64_t from = __shfl_sync(0xffffffffu, at, ((j & 15) << 1) + (row >> 3));
+    for (int i = 0; i < Q::kSpan / kRows; ++i) {
+      const int row = i * kRows + lane_row, tile = row / 16 * S::kTile;
+      // a lane's row in its run is the same in every round, or in every other one
+      const int64_t shift = kRows % 8 == 0 ? lane_at : kRows == 4 ? lane_at + i % 2 * 4 * a.c_st
+                                                                  : (row & 7) * a.c_st + byte;
+      const int64_t from = __shfl_sync(0xffffffffu, at, run0 + (row >> 3));
       const bool fetch = inside && from >= 0 && row < left;
-      from = fetch ? from + (row & 7) * a.c_st + byte : 0;
-      qt_fetch<kPiece>(base + S::key_at(row, byte), kh + from, fetch);
-      qt_fetch<kPiece>(base + S::kTile + S::value_at(row, byte), vh + from, fetch);
+      const int64_t place = fetch ? from + shift : 0;
+      qt_fetch<kPiece>(base + tile + S::key_at(row % 16, byte), kh + place, fetch);
+      qt_fetch<kPiece>(base + kSub * S::kTile + tile + S::value_at(row % 16, byte), vh + place,
+                       fetch);
     }
     qt_commit();
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) request(i, i);
 
-  QtState<T, DP, kTiles> state;
-  state.begin(a, current, head0, n_heads);
+  State state;
+  // The next sequence of this range, whose queries are fetched under the current one's steps.
+  int following = current;
+  const auto begin = [&] {
+    state.begin(a, query);
+    if constexpr (!kWhole) {
+      if (last_of(current) >= hi) return;
+      following = current + 1;
+      while (last_of(following) <= last_of(current)) ++following;
+      State::fetch(a, following, head0, n_heads, query);
+    }
+  };
+  begin();
   // Writes the current sequence's rows, or its part in this range.
   const auto finish = [&] {
     state.sum_weights();
-    const int first = starts[current] >> 4, last = starts[current + 1] >> 4;
-    const bool whole = first >= lo && last <= hi;
-    const int64_t slot = 2 * (int64_t)range + (first >= lo ? 1 : 0);
+    const bool whole = kWhole || (first_of(current) >= lo && last_of(current) <= hi);
+    const int64_t slot = 2 * (int64_t)range + (first_of(current) >= lo ? 1 : 0);
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
@@ -849,12 +965,12 @@ __global__ void __launch_bounds__(32 * QT_WARPS, (QsShape<T, DP, kTiles>::kCtas)
         const int head = 8 * n + 2 * t + r;
         if (head >= n_heads) continue;
         const float norm = state.l[n][r], top = state.m[n][r], high = state.w_top[n][r];
-        const float base = top == -INFINITY ? 0.f : top, w_base = high == -INFINITY ? 0.f : high;
+        const float base = top == QT_UNSET ? 0.f : top, w_base = high == QT_UNSET ? 0.f : high;
         // the references' difference in two halves: either alone may leave the range
-        const float half = exp2f(0.5f * (w_base - base - QT_LIFT));
-        const float inv = norm == 0.f ? 0.f : half / norm;
+        const float half = qt_exp2(0.5f * (w_base - base - QT_LIFT));
+        const float inv = norm == 0.f ? 0.f : __fdividef(half, norm);
         const int64_t row = slot * a.heads + head0 + head;
-        T* to = static_cast<T*>(a.out) + (int64_t)current * a.o_sb + (int64_t)(head0 + head) * a.o_sh;
+        T* to = static_cast<T*>(a.out) + current * a.o_sb + (head0 + head) * a.o_sh;
         constexpr int kRead = S::kWords < 4 ? S::kWords : 4;
 #pragma unroll
         for (int j = 0; j < S::kWords; ++j) {
@@ -872,37 +988,40 @@ __global__ void __launch_bounds__(32 * QT_WARPS, (QsShape<T, DP, kTiles>::kCtas)
         if (!whole && g == 0) a.part_lse[row] = norm == 0.f ? -INFINITY : base + log2f(norm);
       }
   };
-  int end = min(starts[current + 1] >> 4, hi) - lo, stage = 0;
+  int end = min(last_of(current), hi) - lo, stage = 0;
   for (int j = 0; j < mine; ++j) {
-    const int at16 = j & 15;
-    if (at16 == 0 && j > 0) {
+    const int at = j % kAhead;
+    if (at == 0 && j > 0) {
       now = next;
       batch = j;
-      look(j + 16);
-    } else if (at16 == 4 && j > 16) {
+      look(j + kAhead);
+    } else if (at == kAhead / 4 && j > kAhead) {
       place();
-    } else if (at16 == 8 && j > 16) {
+    } else if (at == kAhead / 2 && j > kAhead) {
       next.value = qt_log2(next.value);
     }
     qt_wait<kStages - 2>();
     __syncwarp();
     request(j + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
-    if (j == end) {
+    if (!kWhole && j == end) {
       finish();
-      do ++current; while (starts[current + 1] >> 4 <= lo + j);
-      end = min(starts[current + 1] >> 4, hi) - lo;
-      state.begin(a, current, head0, n_heads);
+      current = following;
+      end = min(last_of(current), hi) - lo;
+      begin();
     }
-    const int left = __shfl_sync(0xffffffffu, now.left, at16 << 1);
-    uint32_t key[2];
-    float value[2];
+    const int left = __shfl_sync(0xffffffffu, now.left, at * 2 * kSub);
+    uint32_t key[kSub][2];
+    float value[kSub][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      key[r] = __shfl_sync(0xffffffffu, now.key, (at16 << 1) + r);
-      value[r] = __shfl_sync(0xffffffffu, now.value, (at16 << 1) + r);
-      if (g + 8 * r >= left) key[r] = QT_ABSENT;
-    }
-    state.tile(ring + stage * Q::kStage, key, value);
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        key[u][r] = __shfl_sync(0xffffffffu, now.key, at * 2 * kSub + 2 * u + r);
+        value[u][r] = __shfl_sync(0xffffffffu, now.value, at * 2 * kSub + 2 * u + r);
+        if (16 * u + g + 8 * r >= left) key[u][r] = QT_ABSENT;
+      }
+    const uint8_t* keys = ring + stage * Q::kStage;
+    state.step(keys, keys + kSub * S::kTile, key, value);
     stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   finish();
@@ -922,36 +1041,33 @@ __global__ void __launch_bounds__(128) quant_join_kernel(QuantArgs a, int team) 
   const int b = (int)(row / a.heads), head = (int)(row % a.heads);
   int parts = a.slices, first = 0;
   if (a.ranges) {
-    const int64_t total = a.starts[a.batch] >> 4;
-    const int ranges = quant_used(a.ranges, total);
-    const int from = a.starts[b] >> 4, to = a.starts[b + 1] >> 4;
+    const int total = a.starts[a.batch], from = a.starts[b], to = a.starts[b + 1];
     if (from == to) return;
-    const auto range_of = [&](int tile) {   // the range that holds it
-      int r = (int)min((int64_t)tile * ranges / total, (int64_t)ranges - 1);
-      while (total * (r + 1) / ranges <= tile) ++r;
-      while (total * r / ranges > tile) --r;
-      return r;
-    };
-    first = range_of(from);
-    parts = range_of(to - 1) - first + 1;
+    const QsCut cut(a.ranges, total);
+    first = cut.holds(from);
+    parts = cut.holds(to - 1) - first + 1;
     if (parts == 1) return;                 // written already
   }
   const auto at = [&](int i) {              // row of part i
     if (!a.ranges) return i * rows + row;
     return (2 * (int64_t)(first + i) + (i == 0 ? 1 : 0)) * a.heads + head;
   };
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[at(i)]);
+  const int step = team, mine0 = team == 4 ? warp : 0;
+  // a lane's first part, before anything waits for the others'
+  const float early = mine0 + lane * step < parts ? a.part_lse[at(mine0 + lane * step)] : -INFINITY;
+  float top = early;
+  if (step > 1 || parts > 32)
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[at(i)]);
   top = warp_max(top);
   const float base = top == -INFINITY ? 0.f : top;
-  const int step = team, mine0 = team == 4 ? warp : 0;
   for (int d0 = 0; d0 < a.D; d0 += 128) {
     const int d = d0 + 4 * lane;
     float norm = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int p0 = mine0; p0 < parts; p0 += 32 * step) {
       const int mine = p0 + lane * step;
-      const float w = mine < parts ? exp2f(a.part_lse[at(mine)] - base) : 0.f;
+      const float lse = p0 == mine0 ? early : mine < parts ? a.part_lse[at(mine)] : -INFINITY;
+      const float w = exp2f(lse - base);
       norm += warp_sum(w);
       const int n = min(32, (parts - p0 + step - 1) / step);
       for (int i0 = 0; i0 < n; i0 += 8) {
@@ -1024,16 +1140,25 @@ static int quant_slices(int batch, int heads, int kv_heads, int D, int64_t room)
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, 128, room / 256}));
 }
 
-// Ranges of the stream form, or 0: sequences that fit its table, and tiles enough to give
-// the warps of all SMs (by the type and width, at most 28 an SM) several each, if the
+// Ranges of the stream form, or 0: sequences that fit its table, and steps enough to give
+// the warps of all SMs (by the type and width, at most 20 an SM) several each, if the
 // tables are full.  Otherwise four warps share a sequence's head: 5 sequences of 129
 // tokens take one launch there.
 static int quant_ranges(int batch, int heads, int kv_heads, int D, int64_t room, int warps) {
   const int group = heads / kv_heads, chunk = quant_wide(group, D) ? 16 : 8;
   const int64_t units = (int64_t)kv_heads * ((group + chunk - 1) / chunk);
   const int64_t tiles = batch * ((room + 15) / 16);
-  if (batch > QS_MOST || tiles >= 1 << 27 || tiles * units < 4 * (int64_t)warps) return 0;
+  if (batch > QS_MOST || tiles >= 1 << 26 || tiles * units < 4 * (int64_t)warps) return 0;
   return (int)std::max<int64_t>(1, std::min<int64_t>(warps / units, (tiles + 3) / 4));
+}
+// Whether a warp takes a whole sequence's head: short ones, enough of them (32/8 heads of
+// 128, 1000 sequences of up to 256 / 512 / 1000 tokens: 58 / 98 / 181 us against 83 / 119 /
+// 191 by ranges; 500 of up to 500 57 against 66; 619 of 15 to 30, 56/8 heads, 17 against 45).
+static bool quant_whole(int batch, int heads, int kv_heads, int D, int64_t room) {
+  const int group = heads / kv_heads, chunk = quant_wide(group, D) ? 16 : 8;
+  const int64_t units = (int64_t)kv_heads * ((group + chunk - 1) / chunk);
+  return (room <= QS_SHORT && batch * units >= 4 * 148) ||
+         (room <= 4 * QS_SHORT && batch * units >= QS_MANY);
 }
 template <typename T, int DP, int kTiles>
 constexpr int quant_warps() { return 148 * QsShape<T, DP, kTiles>::kCtas * QT_WARPS; }
@@ -1064,24 +1189,26 @@ static int quant_mma_run(const QuantArgs& p, cudaStream_t stream) {
   return GRS_OK;
 }
 
-template <typename T, int DP, int kTiles, int kPiece>
+template <typename T, int DP, int kTiles, int kPiece, bool kWhole>
 static int quant_stream_run(QuantArgs p, cudaStream_t stream) {
   using Q = QsShape<T, DP, kTiles>;
-  const int units = p.kv_heads * ((p.group + 8 * kTiles - 1) / (8 * kTiles));
+  const int64_t units = (int64_t)p.kv_heads * ((p.group + 8 * kTiles - 1) / (8 * kTiles));
+  constexpr int kRings = QT_WARPS * Q::kStages * Q::kStage;
+  constexpr int kMostBytes = kRings + (kWhole ? 0 : (QS_MOST + 1) * 4);
   p.slices = 1;
   p.part_lse = p.part + 2 * (int64_t)p.ranges * p.heads * p.D;
   p.starts = reinterpret_cast<int32_t*>(p.part_lse + 2 * (int64_t)p.ranges * p.heads);
-  const int smem = QT_WARPS * Q::kStages * Q::kStage + (p.batch + 1) * 4;
-  const int most = QT_WARPS * Q::kStages * Q::kStage + (QS_MOST + 1) * 4;
-  if (cudaFuncSetAttribute(quant_stream_kernel<T, DP, kTiles, kPiece>,
-                           cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
+  if (kMostBytes > 48 * 1024 &&
+      cudaFuncSetAttribute(quant_stream_kernel<T, DP, kTiles, kPiece, kWhole>,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes) != cudaSuccess)
     return GRS_ERR_CUDA;
-  const int64_t ctas = ((int64_t)p.ranges * units + QT_WARPS - 1) / QT_WARPS;
-  if (ctas > INT_MAX || (int64_t)p.batch * p.heads > INT_MAX) return GRS_ERR_SHAPE;
-  quant_stream_kernel<T, DP, kTiles, kPiece>
-      <<<(unsigned)ctas, 32 * QT_WARPS, smem, counted(stream)>>>(p);
+  const int64_t jobs = units * (kWhole ? p.batch : p.ranges);
+  if (jobs > INT_MAX - QT_WARPS || (int64_t)p.batch * p.heads > INT_MAX) return GRS_ERR_SHAPE;
+  quant_stream_kernel<T, DP, kTiles, kPiece, kWhole>
+      <<<(unsigned)((jobs + QT_WARPS - 1) / QT_WARPS), 32 * QT_WARPS,
+         kRings + (kWhole ? 0 : (p.batch + 1) * 4), counted(stream)>>>(p);
   GRS_CUDA_CHECK_LAUNCH();
-  return quant_join<T>(p, p.ranges / p.batch, stream);
+  return kWhole ? (int)GRS_OK : quant_join<T>(p, p.ranges / p.batch, stream);
 }
 
 template <typename T, int kTiles, int kPiece, bool kRuns>
@@ -1089,10 +1216,12 @@ static int quant_mma_width(const QuantArgs& p, cudaStream_t stream) {
   const auto go = [&](auto width, auto tiles) -> int {
     constexpr int DP = decltype(width)::value, kT = decltype(tiles)::value;
     if constexpr (kRuns) {
+      const int64_t room = (int64_t)p.columns * p.page;
+      if (quant_whole(p.batch, p.heads, p.kv_heads, p.D, room))
+        return quant_stream_run<T, DP, kT, kPiece, true>(p, stream);
       QuantArgs q = p;
-      q.ranges = quant_ranges(p.batch, p.heads, p.kv_heads, p.D, (int64_t)p.columns * p.page,
-                              quant_warps<T, DP, kT>());
-      if (q.ranges) return quant_stream_run<T, DP, kT, kPiece>(q, stream);
+      q.ranges = quant_ranges(p.batch, p.heads, p.kv_heads, p.D, room, quant_warps<T, DP, kT>());
+      if (q.ranges) return quant_stream_run<T, DP, kT, kPiece, false>(q, stream);
     }
     return quant_mma_run<T, DP, kT, kPiece, kRuns>(p, stream);
   };
