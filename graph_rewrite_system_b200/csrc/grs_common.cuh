@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/grs_b200.h"
 
 #define GRS_CUDA_CHECK_LAUNCH()                                   \
@@ -64,6 +66,21 @@ __host__ __device__ __forceinline__ uint64_t edge_component(int64_t src, int64_t
                                                             int64_t sp, int64_t dp) {
   return mix64((2ull << 62) | ((uint64_t)src << 36) | ((uint64_t)dst << 12) |
                (((uint64_t)sp & 63ull) << 6) | ((uint64_t)dp & 63ull));
+}
+
+// Lets a kernel ask for up to `bytes` of dynamic shared memory; asked of the driver once
+// for each kernel and device (about a microsecond of host time).
+template <auto kKernel>
+inline bool allow_shared(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }

@@ -1178,9 +1178,7 @@ static int quant_mma_run(const QuantArgs& p, cudaStream_t stream) {
   const int64_t tasks = (int64_t)p.batch * p.kv_heads * chunks;
   const int64_t rows = (int64_t)p.batch * p.heads;
   if (tasks > INT_MAX || rows > INT_MAX) return GRS_ERR_SHAPE;
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(quant_mma_kernel<T, DP, kTiles, kPiece, kRuns>,
-                           cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  if (smem > 48 * 1024 && !allow_shared<quant_mma_kernel<T, DP, kTiles, kPiece, kRuns>>(smem))
     return GRS_ERR_CUDA;
   quant_mma_kernel<T, DP, kTiles, kPiece, kRuns>
       <<<dim3((unsigned)tasks, p.slices), 32 * QT_WARPS, smem, counted(stream)>>>(p);
@@ -1199,8 +1197,7 @@ static int quant_stream_run(QuantArgs p, cudaStream_t stream) {
   p.part_lse = p.part + 2 * (int64_t)p.ranges * p.heads * p.D;
   p.starts = reinterpret_cast<int32_t*>(p.part_lse + 2 * (int64_t)p.ranges * p.heads);
   if (kMostBytes > 48 * 1024 &&
-      cudaFuncSetAttribute(quant_stream_kernel<T, DP, kTiles, kPiece, kWhole>,
-                           cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes) != cudaSuccess)
+      !allow_shared<quant_stream_kernel<T, DP, kTiles, kPiece, kWhole>>(kMostBytes))
     return GRS_ERR_CUDA;
   const int64_t jobs = units * (kWhole ? p.batch : p.ranges);
   if (jobs > INT_MAX - QT_WARPS || (int64_t)p.batch * p.heads > INT_MAX) return GRS_ERR_SHAPE;

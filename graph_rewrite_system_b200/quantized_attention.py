@@ -27,24 +27,32 @@ def _workspace_bytes(*sizes: int) -> int:
     return _lib.lib().grs_quantized_attention_workspace_bytes(*sizes)
 
 
-def _scales(name: str, t: torch.Tensor, device: int, pages: int, kv_heads: int) -> int:
-    """Row stride of fp32 scales [pages, kv_heads]."""
-    if (t.dtype is not torch.float32 or t.shape != (pages, kv_heads) or t.get_device() != device
-            or (kv_heads > 1 and t.stride(1) != 1)):
-        _lib.require_cuda(t)
-        raise ValueError(f"{name} must be fp32 [pages, kv_heads] with contiguous rows on the "
-                         "inputs' device")
-    return t.stride(0)
+def _scales(key_scale: torch.Tensor, value_scale: torch.Tensor, device: int, pages: int,
+            kv_heads: int) -> int:
+    """Row stride of fp32 key and value scales [pages, kv_heads] of one layout."""
+    row = None
+    for name, t in (("key_scale", key_scale), ("value_scale", value_scale)):
+        stride = t.stride()
+        if (t.dtype is not torch.float32 or t.shape != (pages, kv_heads)
+                or t.get_device() != device or (stride[1] != 1 and kv_heads > 1)):
+            _lib.require_cuda(t)
+            raise ValueError(f"{name} must be fp32 [pages, kv_heads] with contiguous rows on the "
+                             "inputs' device")
+        if row is not None and stride[0] != row and pages > 1:
+            raise ValueError("key/value scales must share a layout")
+        row = stride[0]
+    return row
 
 
 def _table(name: str, t: torch.Tensor, device: int, rows: int) -> tuple[int, int]:
     """Columns and row stride of an int32 block table."""
-    if (t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != rows
-            or t.get_device() != device or (t.shape[1] > 1 and t.stride(1) != 1)):
+    shape, stride = t.shape, t.stride()
+    if (t.dtype is not torch.int32 or len(shape) != 2 or shape[0] != rows
+            or t.get_device() != device or (stride[1] != 1 and shape[1] > 1)):
         _lib.require_cuda(t)
         raise ValueError(f"{name} must be int32 [sequences, columns] with contiguous rows on the "
                          "inputs' device")
-    return t.shape[1], t.stride(0)
+    return shape[1], stride[0]
 
 
 def _lengths(t: torch.Tensor, device: int, rows: int) -> int:
@@ -55,19 +63,21 @@ def _lengths(t: torch.Tensor, device: int, rows: int) -> int:
     return t.data_ptr()
 
 
-def _cache(key_cache: torch.Tensor, value_cache: torch.Tensor, device: int, dtype: torch.dtype,
-           kv_heads: int, width: int) -> tuple:
-    """Strides of a key and a value cache [pages, page, kv_heads, D] of one layout."""
-    shape, stride = key_cache.shape, key_cache.stride()
-    for t in (key_cache, value_cache):
-        if t.get_device() != device or t.dtype is not dtype:
-            _lib.require_cuda(t)
-            raise ValueError(f"caches must be {dtype} on the inputs' device")
-        if t.dim() != 4 or t.shape != shape or t.shape[2] != kv_heads or t.shape[3] != width:
-            raise ValueError(f"caches must be [pages, page, {kv_heads}, {width}]")
-        if width > 1 and t.stride(3) != 1:
-            raise ValueError("caches need a contiguous head width")
-    if any(a != b for a, b, n in zip(stride, value_cache.stride(), shape) if n > 1):
+def _cache(key_cache: torch.Tensor, value_cache: torch.Tensor, shape: tuple, device: int,
+           dtype: torch.dtype, kv_heads: int, width: int) -> tuple:
+    """Strides of a key cache of that shape, [pages, page, kv_heads, D], and a value
+    cache of its layout."""
+    stride = key_cache.stride()
+    if (key_cache.dtype is not dtype or value_cache.dtype is not dtype
+            or key_cache.get_device() != device or value_cache.get_device() != device):
+        _lib.require_cuda(key_cache, value_cache)
+        raise ValueError(f"caches must be {dtype} on the inputs' device")
+    if value_cache.shape != shape or shape[2] != kv_heads or shape[3] != width:
+        raise ValueError(f"caches must be [pages, page, {kv_heads}, {width}]")
+    if stride[3] != 1 and width > 1:
+        raise ValueError("caches need a contiguous head width")
+    other = value_cache.stride()
+    if stride != other and any(a != b for a, b, n in zip(stride, other, shape) if n > 1):
         raise ValueError("key/value caches must share a layout")
     if shape[0] >= 1 << 31 or not 0 < shape[1] < 1 << 30:
         raise ValueError("at most 2^31 pages of 1 to 2^30 tokens")
@@ -113,29 +123,30 @@ def quantized_attention(
         with place:
             return quantized_attention(query, key_cache, value_cache, key_scale, value_scale,
                                        block_table, lengths, scale=scale, out=out, status=status)
-    if query.dim() != 3 or key_cache.dim() != 4:
+    shape, dtype, pool = query.shape, query.dtype, key_cache.shape
+    if len(shape) != 3 or len(pool) != 4:
         raise ValueError("query must be [batch, heads, D], caches [pages, page, kv_heads, D]")
-    shape, dtype = query.shape, query.dtype
     batch, heads, width = shape
-    pages, page, kv_heads, _ = key_cache.shape
+    pages, page, kv_heads, _ = pool
     if batch >= 1 << 30:
         raise ValueError("at most 2^30 sequences")
     code = _check_heads(query, heads, kv_heads, width)
     q = query.stride()
     if q[2] != 1 and width > 1:
         raise ValueError("query needs a contiguous head width")
-    c = _cache(key_cache, value_cache, device, _E4M3, kv_heads, width)
-    s = _scales("key_scale", key_scale, device, pages, kv_heads)
-    if s != _scales("value_scale", value_scale, device, pages, kv_heads) and pages > 1:
-        raise ValueError("key/value scales must share a layout")
+    c = _cache(key_cache, value_cache, pool, device, _E4M3, kv_heads, width)
+    s = _scales(key_scale, value_scale, device, pages, kv_heads)
     columns, row = _table("block_table", block_table, device, batch)
     past = _lengths(lengths, device, batch)
     if columns * page >= 1 << 30:
         raise ValueError("a block table row holds at most 2^30 tokens")
     scale = _check_scale(scale, width)
     if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-        o = (heads * width, width)
+        out = torch.empty_like(query)         # half the time of asking for the format
+        o = out.stride()
+        if o[0] < o[1]:
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)
+            o = out.stride()
     else:
         o = _out_rows(out, device, dtype, shape, query)
     if not batch:

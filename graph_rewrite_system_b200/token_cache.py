@@ -102,19 +102,17 @@ def append_tokens(
         raise ValueError("at most 2^30 tokens and heads, and one head at least")
     k = _rows("key", key, device, dtype, shape)
     v = _rows("value", value, device, dtype, shape)
-    if key_cache.dim() != 4:
+    pool = key_cache.shape
+    if len(pool) != 4:
         raise ValueError("caches must be [pages, page, kv_heads, D]")
-    pages, page = key_cache.shape[:2]
+    pages, page = pool[:2]
     cache_code, scale_row, key_at, value_at = code, 0, 0, 0
     if key_cache.dtype is _E4M3:
         if key_scale is None or value_scale is None:
             raise ValueError("8-bit caches come with key and value scales")
         cache_code = 2
-        c = _cache(key_cache, value_cache, device, _E4M3, kv_heads, width)
-        scale_row = _scales("key_scale", key_scale, device, pages, kv_heads)
-        if (scale_row != _scales("value_scale", value_scale, device, pages, kv_heads)
-                and pages > 1):
-            raise ValueError("key/value scales must share a layout")
+        c = _cache(key_cache, value_cache, pool, device, _E4M3, kv_heads, width)
+        scale_row = _scales(key_scale, value_scale, device, pages, kv_heads)
         if pages > 1 and scale_row < kv_heads:
             raise ValueError("scales must not overlap themselves")
         key_at, value_at = key_scale.data_ptr(), value_scale.data_ptr()
@@ -123,15 +121,17 @@ def append_tokens(
     else:
         if key_scale is not None or value_scale is not None:
             raise ValueError("scales come with 8-bit caches")
-        c = _cache(key_cache, value_cache, device, dtype, kv_heads, width)
-    need = 1
-    for size, step in sorted(zip(key_cache.shape, c), key=lambda p: p[1]):
-        if size > 1 and step < need:
-            raise ValueError("a cache must not overlap itself")
-        need = max(need, step * size)
-    if key_cache.data_ptr() == value_cache.data_ptr() and key_cache.numel():
+        c = _cache(key_cache, value_cache, pool, device, dtype, kv_heads, width)
+    if c[2] < width or c[1] < c[2] * kv_heads or c[0] < c[1] * page:
+        need = 1                              # not pages of rows of heads: any order will do
+        for size, step in sorted(zip(pool, c), key=lambda p: p[1]):
+            if size > 1 and step < need:
+                raise ValueError("a cache must not overlap itself")
+            need = max(need, step * size)
+    keys_at, values_at = key_cache.data_ptr(), value_cache.data_ptr()
+    if keys_at == values_at and keys_at:
         raise ValueError("key and value caches must not be one tensor")
-    rows = lengths.shape[0] if lengths.dim() else -1
+    rows = len(lengths) if lengths.dim() else -1
     past = _lengths(lengths, device, rows)
     if rows >= 1 << 29:
         raise ValueError("at most 2^29 sequences")
@@ -167,9 +167,10 @@ def append_tokens(
     q = qo = (0, 0)
     fresh = query_out is None
     if query is not None:
-        if query.dim() != 3:
+        asked = query.shape
+        if len(asked) != 3:
             raise ValueError("query must be [tokens, heads, D]")
-        heads = query.shape[1]
+        heads = asked[1]
         if not 0 < heads < 1 << 30 or heads % kv_heads:
             raise ValueError("query heads must be a multiple of the key/value heads")
         q = _rows("query", query, device, dtype, (tokens, heads, width))
@@ -186,7 +187,7 @@ def append_tokens(
         _entry = _lib.words_entry("grs_append_tokens")
     code = _entry(_pack(
         code, cache_code, query_at, q[0], q[1], query_to, qo[0], qo[1], fresh, key.data_ptr(),
-        k[0], k[1], value.data_ptr(), v[0], v[1], key_cache.data_ptr(), value_cache.data_ptr(),
+        k[0], k[1], value.data_ptr(), v[0], v[1], keys_at, values_at,
         c[0], c[1], c[2], key_at, value_at, scale_row, block_table.data_ptr(), row, source,
         source_row, columns, past, begins, places, wide, turns, pairs, bool(interleaved),
         magnitude, tokens, rows, heads, kv_heads, width, pages, page, word,
