@@ -47,31 +47,30 @@ __device__ __forceinline__ uint32_t e4m3x2_times(uint32_t codes, __half2 ratio) 
 }
 
 // Four codes times any ratio, in fp32.
-__device__ __forceinline__ uint32_t e4m3x4_times(uint32_t codes, float ratio) {
+static __device__ __noinline__ uint32_t e4m3x4_times(uint32_t codes, float ratio) {
   uint32_t out = 0;
 #pragma unroll
   for (int i = 0; i < 32; i += 8)
     out |= (uint32_t)to_e4m3(from_e4m3((uint8_t)(codes >> i)) * ratio) << i;
   return out;
 }
-// kVec values over a scale, stored as one word; `careful`: some may not be finite.
+// kVec values over a scale, stored as one word.  x * 0 + x * inverse: an infinity becomes
+// NaN without a branch.
 template <int kVec>
-__device__ __forceinline__ void e4m3_store(uint8_t* at, const float (&y)[kVec], float inverse,
-                                           bool careful) {
-  float x[kVec];
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) x[i] = y[i];
-  if (careful) {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) x[i] = e4m3_checked(x[i]);
-  }
+__device__ __forceinline__ void e4m3_store(uint8_t* at, const float (&x)[kVec], float inverse) {
   if constexpr (kVec == 1) {
-    *at = to_e4m3(x[0] * inverse);
+    *at = (uint8_t)to_e4m3x2(fmaf(x[0], inverse, x[0] * 0.f), 0.f);
   } else {
+    const uint64_t by = (uint64_t)__float_as_uint(inverse) << 32 | __float_as_uint(inverse);
     uint32_t w[(kVec + 3) / 4] = {};
 #pragma unroll
-    for (int i = 0; i < kVec; i += 2)
-      w[i / 4] |= to_e4m3x2(x[i] * inverse, x[i + 1] * inverse) << 8 * (i % 4);
+    for (int i = 0; i < kVec; i += 2) {
+      uint64_t y = (uint64_t)__float_as_uint(x[i + 1]) << 32 | __float_as_uint(x[i]), z;
+      asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(z) : "l"(y), "l"(0ull));
+      asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(y) : "l"(y), "l"(by), "l"(z));
+      w[i / 4] |= to_e4m3x2(__uint_as_float((uint32_t)y), __uint_as_float((uint32_t)(y >> 32)))
+                  << 8 * (i % 4);
+    }
     if constexpr (kVec == 2)
       *reinterpret_cast<uint16_t*>(at) = (uint16_t)w[0];
     else if constexpr (kVec == 4)

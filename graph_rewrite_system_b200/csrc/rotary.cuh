@@ -306,6 +306,14 @@ __device__ __forceinline__ void rotary_rows(const float* table, int pairs, int w
   }
 }
 
+// Out of line, with registers of its own, where it is one call of several.
+template <typename T, int kVec, bool kInter, int kThreads>
+static __device__ __noinline__ void rotary_rows_apart(const float* table, int pairs, int width,
+                                                      int n, int heads, const T* from, int64_t st,
+                                                      int64_t sh, T* to, int64_t ot, int64_t oh) {
+  rotary_rows<T, kVec, kInter, kThreads>(table, pairs, width, n, heads, from, st, sh, to, ot, oh);
+}
+
 // The widest piece that `takes` the layout: calls f with its width (16 bytes, 8, or one
 // element) and whether pairs lie side by side.
 template <typename T, typename F>

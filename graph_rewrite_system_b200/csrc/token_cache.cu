@@ -24,8 +24,8 @@ struct AppendArgs {
   int32_t* status;
 };
 
-constexpr int AP_THREADS = 256;
-constexpr int AP_ROWS = 16;                 // rows of a CTA's table of turns
+// Threads of a CTA: at least one for each unit of a head.
+constexpr int append_threads(int vec) { return vec == 1 ? 256 : 128; }
 
 // A page that receives tokens: rows [kept, kept + n) of page `to`, from the packed
 // tokens first .. first + n - 1, the first of them at `position`.  The rows before
@@ -82,33 +82,39 @@ __device__ __forceinline__ bool append_unit(const AppendArgs& a, int u, AppendUn
   return true;
 }
 
-// `rows` rows of `pieces` pieces of codes times `ratio` (1: copied), from one page to
-// another or in place.  Threads lane, lane + step, ... of a group; kHold pieces of each
-// in flight.
+// The kept rows of one head's page, times `ratio` (1: copied), from one page to another or
+// in place: pieces of kBytes codes, whole rows side by side in a warp's lanes, kHold pieces
+// of a lane at once.
 template <int kBytes>
-struct CodePieces {
+struct KeptCodes {
   using Word = typename std::conditional<
       kBytes == 16, uint4, typename std::conditional<kBytes == 8, uint2, uint8_t>::type>::type;
   static constexpr int kHold = 4;
   Word x[kHold];
-  // the pieces first, first + step, ...; returns how many of them there are
-  __device__ __forceinline__ void load(const uint8_t* from, int64_t stride, int pieces, int count,
-                                       int first, int step) {
+  int64_t at;                               // of the first piece
+  int row, by;                              // first row, rows of a step
+  __device__ __forceinline__ KeptCodes(int64_t stride, int width, int part) {
+    const int lane = threadIdx.x & 31, pieces = min(width / kBytes - 32 * part, 32);
+    row = lane / pieces;
+    by = 32 / pieces;
+    at = row * stride + (lane - row * pieces + 32 * part) * kBytes;
+    if (row >= by) row = 1 << 30;           // lanes that are left over
+  }
+  __device__ __forceinline__ void load(const uint8_t* from, int64_t stride, int rows, int round) {
 #pragma unroll
     for (int j = 0; j < kHold; ++j) {
-      const int i = first + j * step;
-      if (i < count)
-        x[j] = *reinterpret_cast<const Word*>(from + i / pieces * stride + i % pieces * kBytes);
+      const int step = (round * kHold + j) * by;
+      if (row + step < rows) x[j] = *reinterpret_cast<const Word*>(from + at + step * stride);
     }
   }
-  __device__ __forceinline__ void store(uint8_t* to, int64_t stride, int pieces, int count,
-                                        int first, int step, float ratio) {
+  __device__ __forceinline__ void store(uint8_t* to, int64_t stride, int rows, int round,
+                                        float ratio) {
     const bool halves = (__float_as_uint(ratio) & 0x7fffffu) == 0 && ratio <= 1.f;
     const __half2 scale = __float2half2_rn(ratio);
 #pragma unroll
     for (int j = 0; j < kHold; ++j) {
-      const int i = first + j * step;
-      if (i >= count) continue;
+      const int step = (round * kHold + j) * by;
+      if (row + step >= rows) continue;
       if (ratio != 1.f) {
         if constexpr (kBytes == 1) {
           x[j] = to_e4m3(from_e4m3(x[j]) * ratio);
@@ -120,10 +126,30 @@ struct CodePieces {
                           : e4m3x4_times(v[k], ratio);
         }
       }
-      *reinterpret_cast<Word*>(to + i / pieces * stride + i % pieces * kBytes) = x[j];
+      *reinterpret_cast<Word*>(to + at + step * stride) = x[j];
+    }
+  }
+  static __device__ __forceinline__ void move(const uint8_t* from, uint8_t* to, int64_t stride,
+                                              int rows, int width, float ratio) {
+    for (int part = 0; part * 32 * kBytes < width; ++part) {
+      KeptCodes codes(stride, width, part);
+      for (int round = 0; round * kHold * codes.by < rows; ++round) {
+        codes.load(from, stride, rows, round);
+        codes.store(to, stride, rows, round, ratio);
+      }
     }
   }
 };
+// Out of line: it is rare, or short, beside the code around it.
+static __device__ __noinline__ void append_move(const uint8_t* from, uint8_t* to, int64_t stride, int rows,
+                                         int width, int bytes, float ratio) {
+  if (bytes == 16)
+    KeptCodes<16>::move(from, to, stride, rows, width, ratio);
+  else if (bytes == 8)
+    KeptCodes<8>::move(from, to, stride, rows, width, ratio);
+  else
+    KeptCodes<1>::move(from, to, stride, rows, width, ratio);
+}
 
 // A lane's walk over the units of consecutive rows at `at`: whole rows side by side in
 // the warp, or a row in several rounds.  Units of 32 and less keep their lanes, whose
@@ -202,10 +228,8 @@ struct AppendHead {
     }
     return top;
   }
-  // `careful`: there may be values that are not finite
   __device__ __forceinline__ void store(RowWalk<Store, kVec, kInter>& walk, int n, int units,
-                                        int pairs, const float* table, float inverse,
-                                        bool careful) {
+                                        int pairs, const float* table, float inverse) {
 #pragma unroll
     for (int j = 0; j < kHold; ++j) {
       if (walk.inside(n, units)) {
@@ -219,8 +243,8 @@ struct AppendHead {
           turns.turn(u, v);
         }
         if constexpr (kCodes) {
-          e4m3_store<kVec>(walk.at + unit.a, u, inverse, careful);
-          if (unit.two()) e4m3_store<kVec>(walk.at + unit.b, v, inverse, careful);
+          e4m3_store<kVec>(walk.at + unit.a, u, inverse);
+          if (unit.two()) e4m3_store<kVec>(walk.at + unit.b, v, inverse);
         } else {
           x[j].set(u);
           x[j].store(walk.at + unit.a);
@@ -242,12 +266,16 @@ struct AppendHead {
 // the new rows.  All threads turn the queries.  A table of the rows' (cos, sin) in
 // shared memory serves all of them.
 template <typename T, int kVec, bool kInter, bool kCodes>
-__global__ void __launch_bounds__(AP_THREADS, 2) append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(append_threads(kVec), kVec == 1 ? 2 : 4)
+    append_kernel(AppendArgs a) {
+  constexpr int kThreads = append_threads(kVec);
   using Units = RotaryUnits<kVec, kInter>;
   using From = RowWalk<const T, kVec, kInter>;
   using Store = typename std::conditional<kCodes, uint8_t, T>::type;
   constexpr int kHold = Units::kTwo ? 4 : 8;
   extern __shared__ __align__(16) float ap_turns[];
+  float* inverses = ap_turns + 2 * a.rows * a.pairs;      // [2 heads_each]
+  float* ratios = inverses + 2 * a.heads_each;            // [2 heads_each]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int h0 = blockIdx.y * a.heads_each, nh = min(a.heads_each, a.kv_heads - h0);
   const int q0 = h0 * a.group, nq = a.q ? nh * a.group : 0;
@@ -259,7 +287,7 @@ __global__ void __launch_bounds__(AP_THREADS, 2) append_kernel(AppendArgs a) {
     for (int r = blockIdx.x - a.units; r < rest; r += gridDim.x - a.units) {
       T* row = static_cast<T*>(a.qo) + (int64_t)(r < begin ? r : end + r - begin) * a.qo_st +
                q0 * a.qo_sh;
-      for (int i = threadIdx.x; i < all; i += AP_THREADS)
+      for (int i = threadIdx.x; i < all; i += kThreads)
         row[i / a.width * a.qo_sh + i % a.width] = from_float<T>(0.f);
     }
     return;
@@ -267,97 +295,131 @@ __global__ void __launch_bounds__(AP_THREADS, 2) append_kernel(AppendArgs a) {
   AppendUnit unit;
   if (!append_unit(a, blockIdx.x, unit)) return;
 
-  // this warp's head: a key's, or a value's
-  const bool value = warp >= nh, works = unit.to >= 0 && warp < 2 * nh;
-  const int h = h0 + (value ? warp - nh : warp), units = Units::count(a.width, a.pairs);
-  const int rounds = From::rounds(unit.n, units);
-  const int64_t st = value ? a.v_st : a.k_st;
-  const T* rows = static_cast<const T*>(value ? a.v : a.k) + unit.first * st +
-                  h * (value ? a.v_sh : a.k_sh);
-  Store* cache = static_cast<Store*>(value ? a.vc : a.kc) + (int64_t)unit.to * a.c_sp + h * a.c_sh;
+  // key heads, then value heads, in turn by the warps
+  const int units = Units::count(a.width, a.pairs), rounds = From::rounds(unit.n, units);
+  const int tasks = unit.to >= 0 ? 2 * nh : 0, blocks = (unit.n + a.rows - 1) / a.rows;
+  const bool held = blocks == 1 && rounds <= kHold;       // a task's rows in registers
+  const auto stride_of = [&](int task) { return task >= nh ? a.v_st : a.k_st; };
+  const auto rows_of = [&](int task) {
+    const bool value = task >= nh;
+    return static_cast<const T*>(value ? a.v : a.k) + unit.first * stride_of(task) +
+           (h0 + (value ? task - nh : task)) * (value ? a.v_sh : a.k_sh);
+  };
+  const auto cache_of = [&](int task, int page) {
+    const bool value = task >= nh;
+    return static_cast<Store*>(value ? a.vc : a.kc) + (int64_t)page * a.c_sp +
+           (h0 + (value ? task - nh : task)) * a.c_sh;
+  };
   AppendHead<T, kVec, kInter, kCodes, kHold> head;
-  float inverse = 1.f;
-  bool careful = false;
-  if (works) {
-    const bool moved = unit.kept && unit.from >= 0;
-    const Store* origin = cache + (int64_t)(unit.from - unit.to) * a.c_sp;
-    if constexpr (kCodes) {
-      float* scales = (value ? a.vs : a.ks) + h;
-      const float before = moved ? scales[unit.from * a.s_sp] : 0.f;
-      const auto largest = [&](bool finite) {
-        uint32_t top = 0;
-        From walk(rows, st, units, a.pairs);
+  const auto fetch = [&](int task) {
+    From walk(rows_of(task), stride_of(task), units, a.pairs);
+    head.fetch(walk, unit.n, units, a.pairs);
+  };
+  // 8-bit pages: the scale of a task's page and its inverse; what moves the kept rows to it
+  // (-1: they stay) is left for the end, when nothing else is held
+  const bool moved = unit.kept && unit.from >= 0;
+  const auto scale = [&](int task) {
+    if constexpr (!kCodes) return 1.f;
+    const bool value = task >= nh;
+    float* scales = (value ? a.vs : a.ks) + h0 + (value ? task - nh : task);
+    const float before = moved ? scales[unit.from * a.s_sp] : 0.f;
+    const auto largest = [&](bool finite) {
+      uint32_t top = 0;
+      if (held) {
+        top = head.largest(finite);
+      } else {
+        From walk(rows_of(task), stride_of(task), units, a.pairs);
         for (int r = 0; r < rounds; r += kHold) {
           head.fetch(walk, unit.n, units, a.pairs);
           top = max(top, head.largest(finite));
         }
-        return __reduce_max_sync(0xffffffffu, top);
-      };
-      uint32_t top = largest(false);
-      careful = top >= 0x7e800000u;         // 2^126: a turned pair may overflow
-      if (top >= 0x7f800000u) top = largest(true);
-      const float now =
-          fmaxf(before, e4m3_scale(__uint_as_float(top) * (value ? 1.f : a.key_most)));
-      inverse = 1.f / now;
-      if (moved && (now != before || unit.from != unit.to)) {
-        const auto move = [&](auto bytes) {
-          constexpr int kBytes = decltype(bytes)::value;
-          CodePieces<kBytes> codes;
-          const int pieces = a.width / kBytes, count = unit.kept * pieces;
-          for (int i = lane; i < count; i += 32 * codes.kHold) {
-            codes.load(origin, a.c_st, pieces, count, i, 32);
-            codes.store(cache, a.c_st, pieces, count, i, 32, before / now);
-          }
-        };
-        if (a.code_bytes == 16)
-          move(std::integral_constant<int, 16>{});
-        else if (a.code_bytes == 8)
-          move(std::integral_constant<int, 8>{});
-        else
-          move(std::integral_constant<int, 1>{});
       }
-      __syncwarp();                         // every lane has read the old scale
-      if (lane == 0) scales[unit.to * a.s_sp] = now;
-    } else if (moved && unit.from != unit.to) {
+      return __reduce_max_sync(0xffffffffu, top);
+    };
+    uint32_t top = largest(false);
+    if (top >= 0x7f800000u) top = largest(true);
+    const float now = fmaxf(before, e4m3_scale(__uint_as_float(top) * (value ? 1.f : a.key_most)));
+    __syncwarp();                           // every lane has read the old scale
+    if (lane == 0) {
+      scales[unit.to * a.s_sp] = now;
+      ratios[task] = moved && (now != before || unit.from != unit.to) ? before / now : -1.f;
+    }
+    return 1.f / now;
+  };
+  if constexpr (!kCodes) {
+    if (moved && unit.from != unit.to) {
       const int pieces = a.width / kVec, count = unit.kept * pieces;
-      for (int i = lane; i < count; i += 32) {
-        const int64_t at = i / pieces * a.c_st + i % pieces * kVec;
-        RotaryPiece<T, kVec> x;
-        x.load(reinterpret_cast<const T*>(origin) + at);
-        x.store(reinterpret_cast<T*>(cache) + at);
-      }
+      for (int task = warp; task < tasks; task += kThreads / 32)
+        for (int i = lane; i < count; i += 32) {
+          const int64_t at = i / pieces * a.c_st + i % pieces * kVec;
+          RotaryPiece<T, kVec> x;
+          x.load(reinterpret_cast<const T*>(cache_of(task, unit.from)) + at);
+          x.store(reinterpret_cast<T*>(cache_of(task, unit.to)) + at);
+        }
     }
   }
+  if (kCodes && held && warp < tasks) fetch(warp);    // under the table
+  if (kCodes && !held)
+    for (int task = warp; task < tasks; task += kThreads / 32) {
+      const float inverse = scale(task);
+      if (lane == 0) inverses[task] = inverse;
+    }
 
-  // rows in blocks of the table's size, from the last (whose units may be held)
-  const int blocks = (unit.n + a.rows - 1) / a.rows;
-  for (int block = blocks - 1; block >= 0; --block) {
+  for (int block = 0; block < blocks; ++block) {          // rows of a table
     const int r0 = block * a.rows, n = min(a.rows, unit.n - r0);
-    if (block != blocks - 1) __syncthreads();             // the last table is read
-    rotary_table<kVec, kInter, AP_THREADS>(
+    if (block) __syncthreads();             // the last table is read
+    rotary_table<kVec, kInter, kThreads>(
         ap_turns, a.freq, a.pairs, a.magnitude, n, [&](int row) -> int64_t {
           if (!a.positions) return unit.position + r0 + row;
           return a.wide ? static_cast<const int64_t*>(a.positions)[unit.first + r0 + row]
                         : static_cast<const int32_t*>(a.positions)[unit.first + r0 + row];
         });
     __syncthreads();
-    if (works) {
-      const bool held = kCodes && blocks == 1 && rounds <= kHold;
-      From there(rows + r0 * st, st, units, a.pairs);
-      RowWalk<Store, kVec, kInter> walk(cache + (unit.kept + r0) * a.c_st, a.c_st, units, a.pairs);
+    const int64_t first = unit.first + r0;
+    if constexpr (!kCodes) {
+      if (tasks) {
+        const int64_t at = (int64_t)unit.to * a.c_sp + (unit.kept + r0) * a.c_st + h0 * a.c_sh;
+        rotary_rows_apart<T, kVec, kInter, kThreads>(
+            ap_turns, a.pairs, a.width, n, nh,
+            static_cast<const T*>(a.k) + first * a.k_st + h0 * a.k_sh, a.k_st, a.k_sh,
+            static_cast<T*>(a.kc) + at, a.c_st, a.c_sh);
+        rotary_rows_apart<T, kVec, kInter, kThreads>(
+            ap_turns, 0, a.width, n, nh,
+            static_cast<const T*>(a.v) + first * a.v_st + h0 * a.v_sh, a.v_st, a.v_sh,
+            static_cast<T*>(a.vc) + at, a.c_st, a.c_sh);
+      }
+    }
+    for (int task = warp; kCodes && task < tasks; task += kThreads / 32) {
+      float inverse = 1.f;
+      if (held) {
+        if (task != warp) fetch(task);
+        inverse = scale(task);
+      } else {
+        inverse = inverses[task];
+      }
+      From there(rows_of(task) + r0 * stride_of(task), stride_of(task), units, a.pairs);
+      RowWalk<Store, kVec, kInter> walk(cache_of(task, unit.to) + (unit.kept + r0) * a.c_st, a.c_st,
+                                        units, a.pairs);
       for (int r = From::rounds(n, units); r > 0; r -= kHold) {
         if (!held) head.fetch(there, n, units, a.pairs);
-        head.store(walk, n, units, a.pairs, value ? nullptr : ap_turns, inverse, careful);
+        head.store(walk, n, units, a.pairs, task >= nh ? nullptr : ap_turns, inverse);
       }
     }
     if (nq) {
-      const int64_t first = unit.first + r0;
-      rotary_rows<T, kVec, kInter, AP_THREADS>(
+      rotary_rows_apart<T, kVec, kInter, kThreads>(
           ap_turns, a.pairs, a.width, n, nq,
           static_cast<const T*>(a.q) + first * a.q_st + q0 * a.q_sh, a.q_st, a.q_sh,
           static_cast<T*>(a.qo) + first * a.qo_st + q0 * a.qo_sh, a.qo_st, a.qo_sh);
     }
   }
+  if (kCodes && moved)
+    for (int task = warp; task < tasks; task += kThreads / 32) {
+      __syncwarp();
+      if (ratios[task] != -1.f)
+        append_move(reinterpret_cast<const uint8_t*>(cache_of(task, unit.from)),
+                    reinterpret_cast<uint8_t*>(cache_of(task, unit.to)), a.c_st, unit.kept, a.width,
+                    a.code_bytes, ratios[task]);
+    }
 }
 
 // One token per sequence: a CTA per sequence and heads_each K/V heads with their query
@@ -366,19 +428,21 @@ __global__ void __launch_bounds__(AP_THREADS, 2) append_kernel(AppendArgs a) {
 // and the rows of the last page that are to be copied under the table of (cos, sin):
 // the call is a chain of latencies, not of bytes.
 template <typename T, int kVec, bool kInter, bool kCodes>
-__global__ void __launch_bounds__(AP_THREADS, 3) append_one_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(append_threads(kVec), kVec == 1 ? 2 : 4)
+    append_one_kernel(AppendArgs a) {
+  constexpr int kThreads = append_threads(kVec);
   using Units = RotaryUnits<kVec, kInter>;
   using Piece = RotaryPiece<T, kVec>;
   using Store = typename std::conditional<kCodes, uint8_t, T>::type;
-  constexpr int kHeld = Units::kTwo ? 2 : 4;
+  constexpr int kHeld = Units::kTwo ? 3 : 6;
   extern __shared__ __align__(16) float ap_turns[];
   uint32_t* tops = reinterpret_cast<uint32_t*>(ap_turns + 2 * a.pairs);   // [2 heads_each]
-  uint32_t* marks = tops + 2 * a.heads_each;                              // [2 heads_each]
-  float* inverses = reinterpret_cast<float*>(marks + 2 * a.heads_each);   // [2 heads_each]
+  float* inverses = reinterpret_cast<float*>(tops + 2 * a.heads_each);    // [2 heads_each]
+  float* ratios = inverses + 2 * a.heads_each;                            // [2 heads_each]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x;
   const int h0 = blockIdx.y * a.heads_each, nh = min(a.heads_each, a.kv_heads - h0);
   const int all = 2 * nh + (a.q ? nh * a.group : 0);
-  const int units = Units::count(a.width, a.pairs), slots = AP_THREADS / units;
+  const int units = Units::count(a.width, a.pairs), slots = kThreads / units;
   const int slot = threadIdx.x / units;
   const Units unit(threadIdx.x - slot * units, a.pairs);
   const auto head_at = [&](int i) {         // key heads, value heads, query heads
@@ -396,7 +460,7 @@ __global__ void __launch_bounds__(AP_THREADS, 3) append_one_kernel(AppendArgs a)
   };
 #pragma unroll
   for (int r = 0; r < kHeld; ++r) fetch(slot + r * slots, x[r], y[r]);
-  for (int i = threadIdx.x; i < 2 * nh; i += AP_THREADS) tops[i] = marks[i] = 0;
+  for (int i = threadIdx.x; i < 2 * nh; i += kThreads) tops[i] = 0;
   AppendUnit page;
   append_unit(a, b, page);
   const bool kept = page.to >= 0 && page.kept && page.from >= 0, copied = kept && page.from != page.to;
@@ -410,15 +474,14 @@ __global__ void __launch_bounds__(AP_THREADS, 3) append_one_kernel(AppendArgs a)
     return (task >= nh ? a.vs : a.ks) + h0 + (task >= nh ? task - nh : task);
   };
   float before = 0.f;
-  CodePieces<16> codes;
-  const int pieces = a.width / 16, count = page.kept * pieces;
   const bool ahead = kCodes && copied && a.code_bytes == 16;
+  KeptCodes<16> codes(a.c_st, ahead ? a.width : 16, 0);
   if (warp < 2 * nh) {
     if (kCodes && kept) before = scale_of(warp)[page.from * a.s_sp];
-    if (ahead) codes.load(reinterpret_cast<const uint8_t*>(cache_of(warp, page.from)), a.c_st, pieces,
-                          count, lane, 32);
+    if (ahead)
+      codes.load(reinterpret_cast<const uint8_t*>(cache_of(warp, page.from)), a.c_st, page.kept, 0);
   }
-  rotary_table<kVec, kInter, AP_THREADS>(ap_turns, a.freq, a.pairs, a.magnitude, 1, [&](int) -> int64_t {
+  rotary_table<kVec, kInter, kThreads>(ap_turns, a.freq, a.pairs, a.magnitude, 1, [&](int) -> int64_t {
     if (!a.positions) return page.position;
     return a.wide ? static_cast<const int64_t*>(a.positions)[b]
                   : static_cast<const int32_t*>(a.positions)[b];
@@ -434,10 +497,7 @@ __global__ void __launch_bounds__(AP_THREADS, 3) append_one_kernel(AppendArgs a)
         return unit.two() ? max(top, v.largest(finite)) : top;
       };
       uint32_t top = both(false);
-      if (top >= 0x7f800000u) {             // not finite
-        top = both(true);
-        marks[i] = 1;
-      }
+      if (top >= 0x7f800000u) top = both(true);   // not finite
       atomicMax(&tops[i], top);
     };
 #pragma unroll
@@ -449,37 +509,27 @@ __global__ void __launch_bounds__(AP_THREADS, 3) append_one_kernel(AppendArgs a)
     }
     __syncthreads();
   }
-  for (int task = warp; task < 2 * nh && page.to >= 0; task += AP_THREADS / 32) {
+  for (int task = warp; task < 2 * nh && page.to >= 0; task += kThreads / 32) {
     if constexpr (kCodes) {
       float* scale = scale_of(task);
       if (kept && task != warp) before = scale[page.from * a.s_sp];
       const float need = e4m3_scale(__uint_as_float(tops[task]) *
                                     (task >= nh ? 1.f : a.key_most));
       const float now = fmaxf(before, need);
-      if (kept && (now != before || copied)) {
+      const float ratio = before / now;
+      if (ahead) {
         const uint8_t* from = reinterpret_cast<const uint8_t*>(cache_of(task, page.from));
         uint8_t* to = reinterpret_cast<uint8_t*>(cache_of(task, page.to));
-        const auto move = [&](auto& held, int bytes, bool there) {
-          const int each = a.width / bytes, n = page.kept * each;
-          for (int i = lane; i < n; i += 32 * held.kHold) {
-            if (!there || i != lane) held.load(from, a.c_st, each, n, i, 32);
-            held.store(to, a.c_st, each, n, i, 32, before / now);
-          }
-        };
-        if (a.code_bytes == 16) {
-          move(codes, 16, ahead && task == warp);
-        } else if (a.code_bytes == 8) {
-          CodePieces<8> narrow;
-          move(narrow, 8, false);
-        } else {
-          CodePieces<1> single;
-          move(single, 1, false);
+        for (int round = 0; round * codes.kHold * codes.by < page.kept; ++round) {
+          if (task != warp || round) codes.load(from, a.c_st, page.kept, round);
+          codes.store(to, a.c_st, page.kept, round, ratio);
         }
       }
       __syncwarp();                         // every lane has read the old scale
       if (lane == 0) {
         scale[page.to * a.s_sp] = now;
         inverses[task] = 1.f / now;
+        ratios[task] = kept && !ahead && (now != before || copied) ? ratio : -1.f;
       }
     } else if (copied) {
       const int each = a.width / kVec, n = page.kept * each;
@@ -518,9 +568,8 @@ __global__ void __launch_bounds__(AP_THREADS, 3) append_one_kernel(AppendArgs a)
       }
     } else {
       uint8_t* to = reinterpret_cast<uint8_t*>(cache_of(i, page.to)) + page.kept * a.c_st;
-      const bool careful = marks[i] || tops[i] >= 0x7e800000u;   // a turned pair may overflow
-      e4m3_store<kVec>(to + unit.a, p, inverses[i], careful);
-      if (unit.two()) e4m3_store<kVec>(to + unit.b, q, inverses[i], careful);
+      e4m3_store<kVec>(to + unit.a, p, inverses[i]);
+      if (unit.two()) e4m3_store<kVec>(to + unit.b, q, inverses[i]);
     }
   };
 #pragma unroll
@@ -535,6 +584,13 @@ __global__ void __launch_bounds__(AP_THREADS, 3) append_one_kernel(AppendArgs a)
     fetch(i, u, v);
     if (i >= 2 * nh || page.to >= 0) write(i, u, v, i >= 2 * nh);
   }
+  // kept rows that were not fetched ahead, now that nothing else is held
+  if (kCodes && page.to >= 0)
+    for (int task = warp; task < 2 * nh; task += kThreads / 32)
+      if (ratios[task] != -1.f)
+        append_move(reinterpret_cast<const uint8_t*>(cache_of(task, page.from)),
+                    reinterpret_cast<uint8_t*>(cache_of(task, page.to)), a.c_st, page.kept, a.width,
+                    a.code_bytes, ratios[task]);
 }
 
 template <typename T>
@@ -557,8 +613,13 @@ static int append_run(AppendArgs a, bool interleaved, cudaStream_t stream) {
   a.units = (int)units;
   a.code_bytes = a.width % 16 == 0 && cache == 16 ? 16 : a.width % 8 == 0 && cache >= 8 ? 8 : 1;
   if (a.offsets) {
-    a.heads_each = std::min(a.kv_heads, AP_THREADS / 64);   // a warp per key and value head
-    a.rows = std::min(AP_ROWS, a.page);
+    // a key and a value head for each pair of warps, up to four times as many while that
+    // leaves CTAs for every SM (two prompts of 42 tokens, 21/3 heads of 64: 11.3 -> 7 us)
+    const int most = (a.kv_heads + 1) / 2;   // groups
+    const int wanted = (int)std::max<int64_t>(4 * 148 / std::max<int64_t>(units, 1), (a.kv_heads + 7) / 8);
+    const int split = std::max(1, std::min(most, wanted));
+    a.heads_each = (a.kv_heads + split - 1) / split;
+    a.rows = std::min({a.page, 64, 4096 / std::max(1, a.pairs)});   // a table of up to 32 KB
   } else {
     // all heads of a sequence, fewer while that leaves SMs without a CTA
     const int split = std::min(a.kv_heads, std::max(1, 2 * 148 / a.sequences));
@@ -568,7 +629,7 @@ static int append_run(AppendArgs a, bool interleaved, cudaStream_t stream) {
   const int64_t groups = ((int64_t)a.kv_heads + a.heads_each - 1) / a.heads_each;
   if (groups > 65535) return GRS_ERR_SHAPE;
   const dim3 grid((unsigned)(units + (a.clear ? 64 : 0)), (unsigned)groups);
-  const int smem = (a.rows * a.pairs * 2 + (a.offsets ? 0 : 6 * a.heads_each)) * (int)sizeof(float);
+  const int smem = (a.rows * a.pairs * 2 + (a.offsets ? 4 : 6) * a.heads_each) * (int)sizeof(float);
   return rotary_dispatch<T>(a.width, a.pairs, interleaved, alignment,
                             [&](auto vec, auto inter) -> int {
     constexpr int kVec = decltype(vec)::value;
@@ -577,7 +638,7 @@ static int append_run(AppendArgs a, bool interleaved, cudaStream_t stream) {
                                            : append_kernel<T, kVec, kInter, false>)
                                   : (codes ? append_one_kernel<T, kVec, kInter, true>
                                            : append_one_kernel<T, kVec, kInter, false>);
-    kernel<<<grid, AP_THREADS, smem, counted(stream)>>>(a);
+    kernel<<<grid, append_threads(kVec), smem, counted(stream)>>>(a);
     GRS_CUDA_CHECK_LAUNCH();
     return GRS_OK;
   });
