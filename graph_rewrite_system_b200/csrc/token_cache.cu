@@ -15,7 +15,7 @@ struct AppendArgs {
   const void* v; int64_t v_st, v_sh;
   void* kc; void* vc; int64_t c_sp, c_st, c_sh;       // strides in elements
   float* ks; float* vs; int64_t s_sp;                 // scales [pages, kv_heads], or null
-  const int32_t* table; int64_t t_s; const int32_t* source; int64_t source_s; int columns;
+  const int32_t* table; int64_t t_s; const int32_t* source; int64_t source_s; int source_columns, columns;
   const int32_t* lengths; const int32_t* offsets;     // offsets null: a token per sequence
   const void* positions; int wide;                    // int32 or int64 [tokens], or null
   const double* freq; int pairs; float magnitude, key_most;
@@ -75,7 +75,8 @@ __device__ __forceinline__ bool append_unit(const AppendArgs& a, int u, AppendUn
   }
   out.from = out.to;
   if (out.kept && a.source && out.to >= 0) {
-    out.from = __ldg(a.source + (int64_t)b * a.source_s + column);
+    out.from = column < a.source_columns
+                   ? __ldg(a.source + (int64_t)b * a.source_s + column) : -1;
     if (out.from < 0 || out.from >= a.pages) out.from = -1, error = GRS_ERR_BAD_PAGE;
   }
   if (error != GRS_OK && threadIdx.x == 0) set_status(a.status, error);
@@ -652,7 +653,7 @@ extern "C" int grs_append_tokens(
     const void* value, int64_t v_st, int64_t v_sh, void* key_cache, void* value_cache,
     int64_t c_sp, int64_t c_st, int64_t c_sh, float* key_scale, float* value_scale, int64_t s_sp,
     const int32_t* block_table, int64_t bt_stride, const int32_t* source_table,
-    int64_t source_stride, int max_blocks, const int32_t* lengths, const int32_t* offsets,
+    int64_t source_stride, int source_blocks, int max_blocks, const int32_t* lengths, const int32_t* offsets,
     const void* positions, int positions_are_i64, const double* frequencies, int pairs,
     int interleaved, double magnitude, int tokens, int sequences, int heads, int kv_heads,
     int head_width, int num_pages, int page_size, int32_t* status, void* stream) {
@@ -664,6 +665,7 @@ extern "C" int grs_append_tokens(
       kv_heads >= kMost || heads < 0 || heads >= kMost || heads % kv_heads ||
       (query && heads == 0) || head_width <= 0 || head_width > 256 || pairs < 0 ||
       2 * pairs > head_width || !std::isfinite(magnitude) || num_pages < 0 || max_blocks < 0 ||
+      source_blocks < 0 ||
       page_size <= 0 || page_size >= kMost || (int64_t)max_blocks * page_size >= kMost ||
       (!offsets && tokens != sequences))
     return GRS_ERR_SHAPE;
@@ -679,7 +681,7 @@ extern "C" int grs_append_tokens(
   a.kc = key_cache; a.vc = value_cache; a.c_sp = c_sp; a.c_st = c_st; a.c_sh = c_sh;
   a.ks = codes ? key_scale : nullptr; a.vs = codes ? value_scale : nullptr; a.s_sp = s_sp;
   a.table = block_table; a.t_s = bt_stride; a.source = source_table; a.source_s = source_stride;
-  a.columns = max_blocks; a.lengths = lengths; a.offsets = offsets;
+  a.source_columns = source_blocks; a.columns = max_blocks; a.lengths = lengths; a.offsets = offsets;
   a.positions = positions; a.wide = positions_are_i64;
   a.freq = frequencies; a.pairs = pairs; a.magnitude = (float)magnitude;
   // sqrt(2), rounded up: a pair's length over its larger element

@@ -67,13 +67,13 @@ def append_tokens(
     that are there move to a new scale.  Infinite values are held as NaN.  The
     rows of a page behind the new ones are left as they were.
 
-    source_table (int32 [B, columns] or wider): the rows that a sequence has in
+    source_table (int32 [B, any columns that hold the lengths]): the rows that a sequence has in
     its first page to receive tokens are copied from the page that this table
     names there - the parent's, after a fork - as are their scales.  No page may
     receive tokens of two sequences, or receive tokens and be another's source.
 
     Tokens whose pages lie outside the cache or whose place the table does not
-    hold are not written, which ``status`` records (default: the device word
+    hold are not written (kept rows without a source stay unspecified), which ``status`` records (default: the device word
     that ``check_decode_status`` reads).  Query rows of no sequence are left as
     they were in a given ``query_out`` and zero in a new one; ``query_out`` may
     be the query itself.  The call does not synchronise and can be captured into
@@ -138,11 +138,9 @@ def append_tokens(
     columns, row = _table("block_table", block_table, device, rows)
     if columns * page >= 1 << 30:
         raise ValueError("a block table row holds at most 2^30 tokens")
-    source = source_row = 0
+    source = source_row = source_columns = 0
     if source_table is not None:
-        wide, source_row = _table("source_table", source_table, device, rows)
-        if wide < columns:
-            raise ValueError("source_table must have the block table's columns")
+        source_columns, source_row = _table("source_table", source_table, device, rows)
         source = source_table.data_ptr()
     begins = 0
     if offsets is not None:
@@ -189,7 +187,7 @@ def append_tokens(
         code, cache_code, query_at, q[0], q[1], query_to, qo[0], qo[1], fresh, key.data_ptr(),
         k[0], k[1], value.data_ptr(), v[0], v[1], keys_at, values_at,
         c[0], c[1], c[2], key_at, value_at, scale_row, block_table.data_ptr(), row, source,
-        source_row, columns, past, begins, places, wide, turns, pairs, bool(interleaved),
+        source_row, source_columns, columns, past, begins, places, wide, turns, pairs, bool(interleaved),
         magnitude, tokens, rows, heads, kv_heads, width, pages, page, word,
         _lib.stream_on(device)))
     if code:

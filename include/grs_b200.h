@@ -691,7 +691,8 @@ GRS_API int grs_rotate_positions(int dtype, const void* query, int64_t q_st, int
  * for turned keys, before they are turned) in 448, or the old scale if rows are
  * there and it is larger; those rows move to a new scale.  Infinities become NaN.
  * source_table (or null): the rows that a sequence has in its first page to
- * receive tokens are copied from that table's page.  No page receives tokens of
+ * receive tokens are copied from that table's page (int32 [sequences,
+ * source_blocks]; wide enough for the tokens that are there).  No page receives tokens of
  * two sequences, and none that receives tokens is another's source.
  * Pages outside the cache set GRS_ERR_BAD_PAGE and lengths or tokens that the
  * table cannot hold GRS_ERR_LENGTH in `status`; their tokens are not written. */
@@ -701,7 +702,7 @@ GRS_API int grs_append_tokens(
     const void* value, int64_t v_st, int64_t v_sh, void* key_cache, void* value_cache,
     int64_t c_sp, int64_t c_st, int64_t c_sh, float* key_scale, float* value_scale, int64_t s_sp,
     const int32_t* block_table, int64_t bt_stride, const int32_t* source_table,
-    int64_t source_stride, int max_blocks, const int32_t* lengths, const int32_t* offsets,
+    int64_t source_stride, int source_blocks, int max_blocks, const int32_t* lengths, const int32_t* offsets,
     const void* positions, int positions_are_i64, const double* frequencies, int pairs,
     int interleaved, double magnitude, int tokens, int sequences, int heads, int kv_heads,
     int head_width, int num_pages, int page_size, int32_t* status, void* stream);

@@ -309,6 +309,21 @@ def test_rows_of_no_sequence(cuda_device, tail):
     _check(after, query, args)
 
 
+def test_narrow_source_table(cuda_device):
+    """The parents' table ends where their tokens do; kept rows that it does not hold
+    are reported, the new ones written."""
+    args = _case(21, past=[3, 20, 16, 35], pages=E4M3, fork=True)
+    wide = args["source_table"]
+    args["source_table"] = torch.cat([wide, torch.full((4, 1), -5, dtype=torch.int32)], 1)[:, :3]
+    _check(*_call(cuda_device, args), args)
+    d = dict(args, source_table=wide[:, :2].contiguous())
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    after, query = _call(cuda_device, d, status=status)
+    assert int(status.item()) == -2
+    args["source_table"][3, 2] = -1           # as a page outside the cache
+    _check(after, query, args)
+
+
 def test_no_tokens_and_no_pages(cuda_device):
     args = _case(12, new=[0, 0], past=[3, 0], pages=E4M3)
     after, query = _call(cuda_device, args)

@@ -108,7 +108,7 @@ PLAIN = dict(key_cache=_z(5, 8, 2, 32), value_cache=_z(5, 8, 2, 32), key_scale=N
     dict(block_table=_i(2, 3).T), dict(block_table=_i(3, 1).expand(3, 1 << 27)),
     dict(lengths=_i(2)), dict(lengths=_i(3, dtype=torch.int64)), dict(lengths=_i(6)[::2]),
     dict(offsets=_i(3)), dict(offsets=_i(4, dtype=torch.int64)), dict(offsets=_i(8)[::2]),
-    dict(key=_z(4, 2, 32), value=_z(4, 2, 32), query=None), dict(source_table=_i(3, 1)),
+    dict(key=_z(4, 2, 32), value=_z(4, 2, 32), query=None), dict(source_table=_i(2, 3).T),
     dict(source_table=_i(2, 2)), dict(frequencies=None), dict(frequencies=_f(17)),
     dict(frequencies=None, query=None, positions=_i(3)), dict(positions=_i(4)),
     dict(magnitude=float("nan")), dict(query=_z(3, 3, 32)), dict(query=_z(2, 4, 32)),
@@ -197,7 +197,8 @@ def test_c_abi_refusals():
     assert lib.grs_rotate_positions(*{**rotate, "tokens": 0}.values()) == 0
     append = dict(dtype=0, cache=2, q=256, q_st=1, q_sh=1, qo=256, qo_st=1, qo_sh=1, clear=0,
                   k=256, k_st=1, k_sh=1, v=256, v_st=1, v_sh=1, kc=256, vc=256, c_sp=1, c_st=1,
-                  c_sh=1, ks=256, vs=256, s_sp=1, bt=256, bt_s=1, src=None, src_s=0, blocks=2,
+                  c_sh=1, ks=256, vs=256, s_sp=1, bt=256, bt_s=1, src=None, src_s=0,
+                  src_blocks=0, blocks=2,
                   lengths=256, offsets=None, pos=None, wide=0, freq=256, pairs=16, inter=0,
                   mag=1.0, tokens=1, seqs=1, heads=4, kv=2, width=32, pages=5, page=16,
                   status=None, stream=None)
@@ -205,7 +206,7 @@ def test_c_abi_refusals():
                    dict(seqs=-1), dict(seqs=2), dict(seqs=far), dict(kv=0), dict(heads=3),
                    dict(heads=0), dict(width=0), dict(width=257), dict(pairs=17), dict(pairs=-1),
                    dict(page=0), dict(page=far), dict(blocks=far), dict(blocks=-1), dict(pages=-1),
-                   dict(k=None), dict(v=None), dict(kc=None), dict(vc=None), dict(ks=None),
+                   dict(src_blocks=-1), dict(k=None), dict(v=None), dict(kc=None), dict(vc=None), dict(ks=None),
                    dict(vs=None), dict(bt=None), dict(lengths=None), dict(freq=None),
                    dict(qo=None), dict(mag=float("nan"))):
         assert lib.grs_append_tokens(*{**append, **change}.values()) == shape, change
