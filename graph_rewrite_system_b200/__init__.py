@@ -12,10 +12,14 @@ Beside them, for prompts and beams of a token model:
 * ``prompt_attention`` - causal attention over packed prompts, grouped heads
 * ``prefix_attention`` - decode attention of a batch behind one long prefix
 * ``token_logits``     - repetition penalties, biases and grammar masks
+* ``rotary``           - rotary positions of queries and keys
+* ``token_cache``      - keys and values into pages, bf16, fp32 or 8 bits, turned on the way
+* ``quantized_attention`` - decode attention over 8-bit pages
 
 Importing a submodule that launches kernels loads the library; a missing
 library raises ImportError (there is no CPU fallback).
 """
 
 __all__ = ["paged_attention", "paged_cache", "gpu_proposals", "prompt_attention",
-           "prefix_attention", "token_logits", "synthetic", "types"]
+           "prefix_attention", "token_logits", "rotary", "token_cache", "quantized_attention",
+           "synthetic", "types"]

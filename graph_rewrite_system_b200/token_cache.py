@@ -13,6 +13,8 @@ Inference only: no gradient is recorded.  The sm_100a kernels live in
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 
 from . import _lib
@@ -70,7 +72,8 @@ def append_tokens(
     source_table (int32 [B, any columns that hold the lengths]): the rows that a sequence has in
     its first page to receive tokens are copied from the page that this table
     names there - the parent's, after a fork - as are their scales.  No page may
-    receive tokens of two sequences, or receive tokens and be another's source.
+    receive tokens of two sequences, or receive tokens and be another's source;
+    the caches overlap none of the inputs.
 
     Tokens whose pages lie outside the cache or whose place the table does not
     hold are not written (kept rows without a source stay unspecified), which ``status`` records (default: the device word
@@ -220,6 +223,9 @@ class TokenKVCache(PagePool):
             raise ValueError("all cache dimensions must be positive")
         if dtype not in (torch.bfloat16, torch.float32, _E4M3):
             raise ValueError("TokenKVCache arenas are bf16, fp32 or float8_e4m3fn")
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         super().__init__(capacity, page_size, device)
         self.layers, self.heads, self.head_width, self.dtype = layers, heads, head_width, dtype
         self.keys = torch.empty(layers, capacity, page_size, heads, head_width,
@@ -229,6 +235,30 @@ class TokenKVCache(PagePool):
         if dtype is _E4M3:
             self.key_scales = torch.ones(layers, capacity, heads, device=self.device)
             self.value_scales = torch.ones_like(self.key_scales)
+
+    # The pool's own launches go where append and attend go: to the stream that this
+    # thread pinned on the device, with memory of that stream.
+    def _stream(self) -> int:
+        return _lib.stream_on(self.device.index)
+
+    def _here(self):
+        return _lib.elsewhere(self.device.index) or nullcontext()
+
+    def reset(self) -> None:
+        with self._here():
+            super().reset()
+
+    def check_status(self) -> None:
+        with self._here():
+            super().check_status()
+
+    def alloc_pages(self, n: int) -> torch.Tensor:
+        with self._here():
+            return super().alloc_pages(n)
+
+    def release_device(self, table: torch.Tensor, lengths: torch.Tensor) -> None:
+        with self._here():
+            super().release_device(table, lengths)
 
     def _layer(self, layer: int) -> tuple:
         scales = (None, None)
@@ -248,14 +278,15 @@ class TokenKVCache(PagePool):
         width, row = _table("parent_table", parent_table, self.device.index, n)
         past = _lengths(parent_lengths, self.device.index, n)
         columns = columns or width + 1
-        table = torch.empty(n, columns, device=self.device, dtype=torch.int32)
-        lengths = torch.empty(n, device=self.device, dtype=torch.int32)
-        if n:
-            _lib.check(_lib.lib().grs_cache_fork(
-                self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
-                self.capacity, parent_table.data_ptr(), row, width, past, n, self.page_size,
-                table.data_ptr(), columns, lengths.data_ptr(), columns, self._status.data_ptr(),
-                self._stream()), "fork")
+        with self._here():
+            table = torch.empty(n, columns, device=self.device, dtype=torch.int32)
+            lengths = torch.empty(n, device=self.device, dtype=torch.int32)
+            if n:
+                _lib.check(_lib.lib().grs_cache_fork(
+                    self._refcounts.data_ptr(), self._free.data_ptr(),
+                    self._free_count.data_ptr(), self.capacity, parent_table.data_ptr(), row,
+                    width, past, n, self.page_size, table.data_ptr(), columns,
+                    lengths.data_ptr(), columns, self._status.data_ptr(), self._stream()), "fork")
         return table
 
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor,
