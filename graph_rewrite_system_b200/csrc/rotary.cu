@@ -50,11 +50,17 @@ static int rotate_run(RotateArgs a, bool interleaved, cudaStream_t stream) {
   if (a.kv_heads)
     alignment = std::min({alignment, common_alignment(a.k, a.k_st * e, a.k_sh * e),
                           common_alignment(a.ko, a.ko_st * e, a.ko_sh * e)});
-  // up to eight tokens share a table; fewer when one wave of CTAs holds them all
-  a.rows = std::min(8, (a.tokens + 3 * 148 - 1) / (3 * 148));
-  const int64_t ctas = ((int64_t)a.tokens + a.rows - 1) / a.rows;
-  const int smem = a.rows * a.pairs * 2 * (int)sizeof(float);
   return rotary_dispatch<T>(a.width, a.pairs, interleaved, alignment, [&](auto vec, auto inter) -> int {
+    // tokens that share a CTA's table: eight, more of few heads (2048 units of work), fewer
+    // when one wave of CTAs holds them all; up to 32 KB (12242 tokens of 6 heads of 96: 18
+    // -> 8.7 us)
+    const int units = RotaryUnits<decltype(vec)::value, decltype(inter)::value>::count(
+        a.width, a.pairs);
+    const int64_t work = (int64_t)(a.heads + a.kv_heads) * units;
+    const int most = std::min((int)std::max<int64_t>(8, 2048 / work), std::min(64, 4096 / a.pairs));
+    a.rows = std::min(most, (a.tokens + 3 * 148 - 1) / (3 * 148));
+    const int64_t ctas = ((int64_t)a.tokens + a.rows - 1) / a.rows;
+    const int smem = a.rows * a.pairs * 2 * (int)sizeof(float);
     rotate_kernel<T, decltype(vec)::value, decltype(inter)::value>
         <<<dim3((unsigned)ctas, a.kv_heads && a.rows == 1 ? 2 : 1), ROT_THREADS, smem,
            counted(stream)>>>(a);

@@ -314,7 +314,7 @@ static __device__ __noinline__ void rotary_rows_apart(const float* table, int pa
   rotary_rows<T, kVec, kInter, kThreads>(table, pairs, width, n, heads, from, st, sh, to, ot, oh);
 }
 
-// The widest piece that `takes` the layout: calls f with its width (16 bytes, 8, or one
+// The widest piece that `takes` the layout: calls f with its width (16 bytes, 8, 4, or one
 // element) and whether pairs lie side by side.
 template <typename T, typename F>
 static int rotary_dispatch(int width, int pairs, bool interleaved, int alignment, F f) {
@@ -325,6 +325,9 @@ static int rotary_dispatch(int width, int pairs, bool interleaved, int alignment
       return f(std::integral_constant<int, kWide>{}, inter);
     if (alignment % 8 == 0 && RotaryUnits<kHalf, kInter>::takes(width, pairs))
       return f(std::integral_constant<int, kHalf>{}, inter);
+    if constexpr (kHalf > 2)
+      if (alignment % 4 == 0 && RotaryUnits<2, kInter>::takes(width, pairs))
+        return f(std::integral_constant<int, 2>{}, inter);
     return f(std::integral_constant<int, 1>{}, inter);
   };
   return interleaved ? with(std::true_type{}) : with(std::false_type{});
