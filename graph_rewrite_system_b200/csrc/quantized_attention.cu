@@ -696,8 +696,7 @@ __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
 // the warps of the other heads of those tokens run beside it, so that whole pages are
 // read at once.  A sequence that one range holds is written at once; parts of one go to
 // the workspace, at most two of a range, and are joined by quant_join_kernel.
-constexpr int QS_SHORT = 256;               // tokens of a table row that one warp takes,
-constexpr int QS_MANY = 3500;               // four times as many if there are so many warps
+constexpr int QS_SHORT = 1024;              // tokens of a table row that one warp takes
 constexpr int QS_MOST = 1024;               // sequences: their first tiles are in shared memory
 
 template <typename T, int DP, int kTiles>
@@ -1151,14 +1150,15 @@ static int quant_ranges(int batch, int heads, int kv_heads, int D, int64_t room,
   if (batch > QS_MOST || tiles >= 1 << 26 || tiles * units < 4 * (int64_t)warps) return 0;
   return (int)std::max<int64_t>(1, std::min<int64_t>(warps / units, (tiles + 3) / 4));
 }
-// Whether a warp takes a whole sequence's head: short ones, enough of them (32/8 heads of
-// 128, 1000 sequences of up to 256 / 512 / 1000 tokens: 58 / 98 / 181 us against 83 / 119 /
-// 191 by ranges; 500 of up to 500 57 against 66; 619 of 15 to 30, 56/8 heads, 17 against 45).
+// Whether a warp takes a whole sequence's head: short ones, enough of them (bf16; tokens
+// are up to the number given; 32/8 heads of 128: 1000 sequences of 256 / 512 / 1000 tokens
+// 58 / 98 / 181 us against 83 / 119 / 191 by ranges, 500 of 500 57 against 66, 200 of 1000
+// 60 against 52; 14/2 heads of 40: 800 of 700 33 against 38; 40/4 heads of 64: 300 of 500
+// 25 against 36; 8/8 heads of 32: 200 of 1000 31 against 27).
 static bool quant_whole(int batch, int heads, int kv_heads, int D, int64_t room) {
   const int group = heads / kv_heads, chunk = quant_wide(group, D) ? 16 : 8;
   const int64_t units = (int64_t)kv_heads * ((group + chunk - 1) / chunk);
-  return (room <= QS_SHORT && batch * units >= 4 * 148) ||
-         (room <= 4 * QS_SHORT && batch * units >= QS_MANY);
+  return room <= QS_SHORT && batch * units >= std::max<int64_t>(4 * 148, 2 * room);
 }
 template <typename T, int DP, int kTiles>
 constexpr int quant_warps() { return 148 * QsShape<T, DP, kTiles>::kCtas * QT_WARPS; }

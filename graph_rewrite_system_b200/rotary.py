@@ -159,7 +159,9 @@ def rotate_positions(
         raise ValueError("head widths from 1 to 256 are supported")
     if tokens >= 1 << 30 or not 0 < heads < 1 << 30:
         raise ValueError("at most 2^30 tokens and heads, and one head at least")
-    q = _rows("query", query, device, dtype, shape)
+    q = query.stride()
+    if q[2] != 1 and width > 1:
+        raise ValueError("query needs a contiguous head width")
     k, kv_heads = (0, 0), 0
     if key is not None:
         kv_heads = keys[1]

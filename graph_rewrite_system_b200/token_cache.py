@@ -103,7 +103,9 @@ def append_tokens(
         raise ValueError("head widths from 1 to 256 are supported")
     if tokens >= 1 << 30 or not 0 < kv_heads < 1 << 30:
         raise ValueError("at most 2^30 tokens and heads, and one head at least")
-    k = _rows("key", key, device, dtype, shape)
+    k = key.stride()
+    if k[2] != 1 and width > 1:
+        raise ValueError("key needs a contiguous head width")
     v = _rows("value", value, device, dtype, shape)
     pool = key_cache.shape
     if len(pool) != 4:
@@ -134,7 +136,7 @@ def append_tokens(
     keys_at, values_at = key_cache.data_ptr(), value_cache.data_ptr()
     if keys_at == values_at and keys_at:
         raise ValueError("key and value caches must not be one tensor")
-    rows = len(lengths) if lengths.dim() else -1
+    rows = lengths.numel()
     past = _lengths(lengths, device, rows)
     if rows >= 1 << 29:
         raise ValueError("at most 2^29 sequences")
