@@ -265,7 +265,10 @@ struct AppendHead {
 // values as they come, not on the rotation's rounding: a pair's length bounds what it
 // becomes) and moves the rows that are there to it; then it turns, converts and writes
 // the new rows.  All threads turn the queries.  A table of the rows' (cos, sin) in
-// shared memory serves all of them.
+// shared memory serves all of them.  16384 tokens, 32/8 heads of 128, into bf16 pages:
+// 72 us = 5.6 TB/s, by HBM; 13930 tokens of 16 prompts into 8-bit pages 77 us = 4.4 TB/s,
+// by latency: the rows wait in registers for their scale, which leaves 16 warps an SM
+// (12 of 170 registers 102 us, 20 of 96 spill, 123).
 template <typename T, int kVec, bool kInter, bool kCodes>
 __global__ void __launch_bounds__(append_threads(kVec), kVec == 1 ? 2 : 4)
     append_kernel(AppendArgs a) {
@@ -284,12 +287,12 @@ __global__ void __launch_bounds__(append_threads(kVec), kVec == 1 ? 2 : 4)
   if ((int)blockIdx.x >= a.units) {         // query rows of no sequence
     const int begin = min(max(__ldg(a.offsets), 0), a.tokens);
     const int end = min(max(__ldg(a.offsets + a.sequences), begin), a.tokens);
-    const int rest = begin + a.tokens - end, all = nq * a.width;
+    const int rest = begin + a.tokens - end;
     for (int r = blockIdx.x - a.units; r < rest; r += gridDim.x - a.units) {
       T* row = static_cast<T*>(a.qo) + (int64_t)(r < begin ? r : end + r - begin) * a.qo_st +
                q0 * a.qo_sh;
-      for (int i = threadIdx.x; i < all; i += kThreads)
-        row[i / a.width * a.qo_sh + i % a.width] = from_float<T>(0.f);
+      for (int h = warp; h < nq; h += kThreads / 32)
+        for (int i = lane; i < a.width; i += 32) row[h * a.qo_sh + i] = from_float<T>(0.f);
     }
     return;
   }
@@ -427,7 +430,8 @@ __global__ void __launch_bounds__(append_threads(kVec), kVec == 1 ? 2 : 4)
 // heads.  A thread keeps one place in the head and takes every slots-th of the key,
 // value and query heads; the first rounds are fetched before anything else is known,
 // and the rows of the last page that are to be copied under the table of (cos, sin):
-// the call is a chain of latencies, not of bytes.
+// the call is a chain of latencies, not of bytes.  1000 forked tokens, 32/8 heads of 128,
+// into 8-bit pages: 22 us, of which 52 MB are 8; five tokens 3 us.
 template <typename T, int kVec, bool kInter, bool kCodes>
 __global__ void __launch_bounds__(append_threads(kVec), kVec == 1 ? 2 : 4)
     append_one_kernel(AppendArgs a) {

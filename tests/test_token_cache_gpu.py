@@ -309,6 +309,26 @@ def test_rows_of_no_sequence(cuda_device, tail):
     _check(after, query, args)
 
 
+def test_rows_past_31_bits(cuda_device):
+    """A token of no sequence whose query row has 2^31 elements is zeroed."""
+    from graph_rewrite_system_b200.token_cache import append_tokens
+
+    heads, width = 1 << 24, 128
+    if torch.cuda.mem_get_info()[0] < 3 * 2 * heads * width:
+        pytest.skip("needs 13 GB")
+    query = torch.ones(1, heads, width, dtype=BF16, device=cuda_device)
+    key = torch.ones(1, 1, width, dtype=BF16, device=cuda_device)
+    pages = torch.zeros(2, 3, 16, 1, width, dtype=BF16, device=cuda_device)
+    none = torch.zeros(0, dtype=torch.int32, device=cuda_device)
+    used = torch.ones_like(query)             # its memory serves the next output
+    del used
+    turned = append_tokens(key, key, pages[0], pages[1], none.view(0, 2), none,
+                           offsets=torch.zeros(1, dtype=torch.int32, device=cuda_device),
+                           frequencies=_freq(width).to(cuda_device), query=query)
+    assert turned.shape == query.shape and not turned.any()
+    assert not pages.any()
+
+
 def test_narrow_source_table(cuda_device):
     """The parents' table ends where their tokens do; kept rows that it does not hold
     are reported, the new ones written."""
