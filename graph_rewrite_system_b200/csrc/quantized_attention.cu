@@ -46,7 +46,8 @@ __device__ __forceinline__ int quant_length(const QuantArgs& a, int b, bool by_w
 // ---- any layout ---------------------------------------------------------------
 // One CTA of four warps per sequence and query head, every warp taking each fourth
 // run of 32 tokens: a lane per key for the scores, a lane per column for the
-// values, byte loads.  For widths that are no multiple of 8 and rows off 8 bytes.
+// values, byte loads.  For widths that are no multiple of 8 and rows off 8 bytes; bound
+// by its loads, one code each.
 template <typename T>
 __global__ void __launch_bounds__(128) quant_rows_kernel(QuantArgs a) {
   constexpr int ND = 8;
@@ -114,11 +115,13 @@ __global__ void __launch_bounds__(128) quant_rows_kernel(QuantArgs a) {
 // ---- tensor cores ---------------------------------------------------------------
 // A warp streams tiles of 16 tokens of one (sequence, K/V head) through a ring of
 // its own in shared memory: cp.async fetches the rows in 16-byte pieces wherever
-// their pages lie, two tiles ahead.  Keys, then value columns, are the 16 rows of
+// their pages lie, two or three steps ahead.  Keys, then value columns, are the 16 rows of
 // mma.m16n8k16, the group's query heads its columns.  The order in which a product
 // sums its inner dimension is free, so a lane takes whole pieces of a row, and a
 // lane's column index picks its piece of the value rows; two tokens' codes are
-// interleaved by byte permutes before they are widened.
+// interleaved by byte permutes before they are widened.  Lane i looks up one run of 8
+// tokens for 16 tiles at once, and shuffles hand places and scales round (a look-up per
+// token and tile: 79 us against 70 for 64 sequences of up to 4099 tokens).
 constexpr int QT_WARPS = 4;
 constexpr int QT_STAGES = 3;
 constexpr float QT_LIFT = 9.f;              // weights are at most 2^(9 + 6): f16 holds them to
@@ -460,6 +463,9 @@ struct QtState {
   }
 };
 
+// Four warps on one slice of a sequence and K/V head, every fourth tile each, joined in
+// shared memory: one launch for few tokens (5 sequences of 129 tokens 4.7 us, of which
+// most is the chain length, look-up, copy, product).  kRuns: pages are multiples of 8.
 template <typename T, int DP, int kTiles, int kPiece, bool kRuns>
 __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
   using S = QtShape<DP>;
@@ -695,7 +701,13 @@ __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
 // range of one head, from one sequence into the next without draining its ring, and
 // the warps of the other heads of those tokens run beside it, so that whole pages are
 // read at once.  A sequence that one range holds is written at once; parts of one go to
-// the workspace, at most two of a range, and are joined by quant_join_kernel.
+// the workspace, at most two of a range, and are joined by quant_join_kernel.  Two, three
+// or five ranges a warp balance no better than their starts cost (73, 79, 91 us against 63).
+// bf16, 32/8 heads of 128: 64 sequences of 300 to 4099 tokens 60 us (310 MB, 5.2 TB/s; 55 %
+// of the issue slots), 512 of 2048 to 4096 483 us = 6.6 TB/s, a plain copy's rate, 2 of up to
+// 131000 86 to 94 us.  Narrow heads and fp32 are bound by instructions: 200 sequences of up
+// to 1001 tokens of 8 heads of 32 take 27 us in bf16 and 29 to 30 in fp32, which HBM would
+// read in 6 to 8.
 constexpr int QS_SHORT = 1024;              // tokens of a table row that one warp takes
 constexpr int QS_MOST = 1024;               // sequences: their first tiles are in shared memory
 
@@ -1027,7 +1039,8 @@ __global__ void __launch_bounds__(32 * QT_WARPS, (QsShape<T, DP, kTiles>::kCtas)
 }
 
 // A row's partial sums joined by their weights: `team` (1 or 4) of a CTA's four warps per
-// (sequence, head).
+// (sequence, head).  The parts are still in L2; the launch overlaps the end of the kernel
+// before it, and adds about 4 us to 64 sequences of 32 heads of 128.
 template <typename T>
 __global__ void __launch_bounds__(128) quant_join_kernel(QuantArgs a, int team) {
   asm volatile("griddepcontrol.wait;\n" ::: "memory");

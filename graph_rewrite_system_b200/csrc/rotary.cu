@@ -19,7 +19,9 @@ constexpr int ROT_THREADS = 256;
 
 // One CTA per `rows` tokens.  The (cos, sin) of its tokens' pairs are computed once
 // into shared memory; then every thread takes its own pairs' into registers and goes
-// through the heads of its token.
+// through the heads of its token (read from shared memory for every head: bank conflicts,
+// 99 us against 58).  Bound by HBM: 16384 bf16 tokens of 32 + 8 heads of 128 (336 MB)
+// take 58 us = 5.8 TB/s, 0.88 of a plain copy; one token 2.7 us.
 template <typename T, int kVec, bool kInter>
 __global__ void __launch_bounds__(ROT_THREADS, 3) rotate_kernel(RotateArgs a) {
   extern __shared__ __align__(16) float rot_turns[];
