@@ -405,13 +405,10 @@ def run(state):
     if op == "append":
         from graph_rewrite_system_b200.token_cache import append_tokens
 
-        offsets = state["offsets"]
-        if offsets is None and case["tail"]:             # padded: more rows than sequences
-            offsets = torch.arange(case["sequences"] + 1, device="cuda", dtype=torch.int32)
         query = append_tokens(
             state["key"], state["value"], state["key_cache"], state["value_cache"],
             state["block_table"], state["lengths"], key_scale=state["key_scale"],
-            value_scale=state["value_scale"], offsets=offsets,
+            value_scale=state["value_scale"], offsets=state["offsets"],
             source_table=state["source_table"], frequencies=state["frequencies"],
             interleaved=case["interleaved"], magnitude=case["magnitude"], query=state["query"])
         if state["key_scale"] is None:
