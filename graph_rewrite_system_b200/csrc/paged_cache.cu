@@ -23,7 +23,10 @@ struct CacheArenas {
   int layers, capacity, page, hd, width, elem;  // hd = H * D; elem = bytes per element
 };
 
-__device__ __forceinline__ int blocks_for(int length, int page) { return (length + page - 1) / page; }
+// Pages of a row; the sum of a length and a page may pass 32 bits.
+__device__ __forceinline__ int blocks_for(int length, int page) {
+  return length > 0 ? (length - 1) / page + 1 : (length + page - 1) / page;
+}
 
 // One thread per parent: retain shared pages, allocate the child page, write
 // the child block-table row and length.
@@ -49,7 +52,7 @@ __global__ void cache_fork_kernel(int32_t* __restrict__ refcounts,
     clengths[i] = 0;
     return;
   }
-  if (keep + 1 > ccols) { set_status(status, GRS_ERR_SHAPE); return; }
+  if (keep >= ccols) { set_status(status, GRS_ERR_SHAPE); return; }
   // Error paths record a status and write page 0 so that no table ever holds
   // an out-of-range page id.
   for (int j = 0; j < keep; ++j) {
