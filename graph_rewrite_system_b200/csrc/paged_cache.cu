@@ -10,6 +10,7 @@
 // (paged_cache.py:99-105): that decrement is the page's last one in scan
 // order, found with an atomicMax over scan positions, and a single-CTA ordered
 // compaction appends the pages.
+#include <algorithm>
 #include <climits>
 
 #include "grs_common.cuh"
@@ -29,7 +30,11 @@ __device__ __forceinline__ int blocks_for(int length, int page) {
 }
 
 // One thread per parent: retain shared pages, allocate the child page, write
-// the child block-table row and length.
+// the child block-table row and length.  kWhole: all children or none - with an
+// error in the status word (cache_fork_check_kernel's, or an earlier one) nothing is
+// retained or taken, and the rows name no page (-1; zeros where the row's own length
+// is the error).
+template <bool kWhole>
 __global__ void cache_fork_kernel(int32_t* __restrict__ refcounts,
                                   const int32_t* __restrict__ free_list,
                                   const int32_t* __restrict__ free_count, int capacity,
@@ -49,7 +54,12 @@ __global__ void cache_fork_kernel(int32_t* __restrict__ refcounts,
   if (len < 0 || nb > pcols) {
     set_status(status, GRS_ERR_LENGTH);
     for (int j = 0; j < ccols; ++j) crow[j] = 0;
-    clengths[i] = 0;
+    if (!kWhole || clengths) clengths[i] = 0;
+    return;
+  }
+  if (kWhole && *status != GRS_OK) {
+    for (int j = 0; j < ccols; ++j) crow[j] = -1;
+    if (clengths) clengths[i] = 0;
     return;
   }
   if (keep >= ccols) { set_status(status, GRS_ERR_SHAPE); return; }
@@ -87,13 +97,46 @@ __global__ void cache_fork_kernel(int32_t* __restrict__ refcounts,
   }
   crow[keep] = page_id;
   for (int j = keep + 1; j < ccols; ++j) crow[j] = 0;
-  clengths[i] = len + 1;
+  if (!kWhole || clengths) clengths[i] = len + 1;
+}
+
+// Whether every child of a fork can have its row: a thread per parent's page, and one per
+// child for its length, columns and page of the free list.  Changes nothing.
+__global__ void cache_fork_check_kernel(const int32_t* __restrict__ refcounts,
+                                        const int32_t* __restrict__ free_list,
+                                        const int32_t* __restrict__ free_count, int capacity,
+                                        const int32_t* __restrict__ ptable, int64_t pstride,
+                                        int pcols, const int32_t* __restrict__ plengths, int n,
+                                        int page, int ccols, int32_t* __restrict__ status) {
+  const int64_t each = (int64_t)pcols + 1, all = n * each;
+  for (int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; idx < all;
+       idx += (int64_t)gridDim.x * blockDim.x) {
+    const int i = (int)(idx / each), j = (int)(idx - i * each);
+    const int len = plengths[i], keep = len / page;
+    const bool held = len >= 0 && blocks_for(len, page) <= pcols;
+    int error = GRS_OK;
+    if (j == pcols) {
+      const int at = *free_count - 1 - i;
+      const int candidate = at >= 0 && at < capacity ? free_list[at] : -1;
+      if (!held)
+        error = GRS_ERR_LENGTH;
+      else if (keep >= ccols)
+        error = GRS_ERR_SHAPE;
+      else if (at < 0)
+        error = GRS_ERR_EXHAUSTED;
+      else if (candidate < 0 || candidate >= capacity || refcounts[candidate] != 0)
+        error = GRS_ERR_CORRUPT;
+    } else if (held && j < keep) {
+      const int p = ptable[i * pstride + j];
+      if (p < 0 || p >= capacity || refcounts[p] <= 0) error = GRS_ERR_BAD_PAGE;
+    }
+    if (error != GRS_OK) set_status(status, error);
+  }
 }
 
 // The pages that the fork of n children took, off the free count.
-__global__ void cache_taken_kernel(int32_t* free_count, int n) {
-  const int fc = *free_count;
-  *free_count = fc >= n ? fc - n : 0;
+__global__ void cache_taken_kernel(int32_t* free_count, int n, const int32_t* status) {
+  if (*status == GRS_OK) *free_count -= n;
 }
 
 // Copy `rows` rows of `row_bytes` bytes from page src to page dst within one
@@ -443,13 +486,21 @@ extern "C" int grs_cache_fork(int32_t* refcounts, int32_t* free_list, int32_t* f
                               int32_t* child_table, int64_t child_stride, int32_t* child_lengths,
                               int child_cols, int32_t* status, void* stream) {
   cudaStream_t s = (cudaStream_t)stream;
-  if (n < 0 || capacity <= 0 || page_size <= 0 || child_cols <= 0) return GRS_ERR_SHAPE;
+  if (n < 0 || capacity <= 0 || page_size <= 0 || parent_cols < 0 || child_cols <= 0)
+    return GRS_ERR_SHAPE;
   if (n == 0) return GRS_OK;
-  cache_fork_kernel<<<ceil_div(n, 128), 128, 0, grs::counted(s)>>>(
+  if (!status) return GRS_ERR_SHAPE;
+  const int64_t checks = n * ((int64_t)parent_cols + 1);
+  cache_fork_check_kernel<<<(int)std::min<int64_t>((checks + 255) / 256, 16 * 148), 256, 0,
+                            grs::counted(s)>>>(
+      refcounts, free_list, free_count, capacity, parent_table, parent_stride, parent_cols,
+      parent_lengths, n, page_size, child_cols, status);
+  GRS_CUDA_CHECK_LAUNCH();
+  cache_fork_kernel<true><<<ceil_div(n, 128), 128, 0, grs::counted(s)>>>(
       refcounts, free_list, free_count, capacity, parent_table, parent_stride, parent_cols,
       parent_lengths, n, page_size, child_table, child_stride, child_lengths, child_cols, status);
   GRS_CUDA_CHECK_LAUNCH();
-  cache_taken_kernel<<<1, 1, 0, grs::counted(s)>>>(free_count, n);
+  cache_taken_kernel<<<1, 1, 0, grs::counted(s)>>>(free_count, n, status);
   GRS_CUDA_CHECK_LAUNCH();
   return GRS_OK;
 }
@@ -470,7 +521,7 @@ extern "C" int grs_cache_append(int elem_bytes, int32_t* refcounts, int32_t* fre
     return GRS_ERR_SHAPE;
   if ((new_readout_keys == nullptr) != (new_readout_values == nullptr)) return GRS_ERR_SHAPE;
   if (n == 0) return GRS_OK;
-  cache_fork_kernel<<<ceil_div(n, 128), 128, 0, grs::counted(s)>>>(refcounts, free_list, free_count, capacity,
+  cache_fork_kernel<false><<<ceil_div(n, 128), 128, 0, grs::counted(s)>>>(refcounts, free_list, free_count, capacity,
                                                       parent_table, parent_stride, INT_MAX,
                                                       parent_lengths, n, page_size, child_table, child_stride,
                                                       child_lengths, child_cols, status);

@@ -275,20 +275,26 @@ class TokenKVCache(PagePool):
         the parent's full pages and owns a page of the free list for the token.
         parent_table int32 [n, cols], parent_lengths int32 [n].  The kept rows of
         the parent's last page follow with ``append(source_table=parent_table)``
-        in every layer.  Errors land in the status word."""
+        in every layer.
+
+        All children or none: where a parent's table does not hold its length
+        or names a page that is not allocated, ``columns`` leave a child no
+        room or the pages run out - or an error is recorded that
+        ``check_status`` has not raised yet - no page is shared or taken and the
+        rows name none (-1; zeros where the parent's own length is the error).
+        Once ``check_status`` has raised it, the fork can be tried again."""
         n = parent_lengths.shape[0]
         width, row = _table("parent_table", parent_table, self.device.index, n)
         past = _lengths(parent_lengths, self.device.index, n)
         columns = columns or width + 1
         with self._here():
             table = torch.empty(n, columns, device=self.device, dtype=torch.int32)
-            lengths = torch.empty(n, device=self.device, dtype=torch.int32)
             if n:
                 _lib.check(_lib.lib().grs_cache_fork(
                     self._refcounts.data_ptr(), self._free.data_ptr(),
                     self._free_count.data_ptr(), self.capacity, parent_table.data_ptr(), row,
-                    width, past, n, self.page_size, table.data_ptr(), columns,
-                    lengths.data_ptr(), columns, self._status.data_ptr(), self._stream()), "fork")
+                    width, past, n, self.page_size, table.data_ptr(), columns, None, columns,
+                    self._status.data_ptr(), self._stream()), "fork")
         return table
 
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor,

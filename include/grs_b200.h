@@ -710,7 +710,12 @@ GRS_API int grs_append_tokens(
 /* The fork of grs_cache_append alone: child i shares the full pages of its
  * parent row and gets a page of its own, from the free list, for its next token
  * (behind the parent's full pages).  Nothing is copied: grs_append_tokens takes
- * the parent's table as its source_table. */
+ * the parent's table as its source_table.  All children or none: with an error in
+ * `status` - this fork's (lengths that the parents' rows do not hold, pages that are
+ * not allocated, rows without room for the child's page, too few free pages) or one
+ * that was there before - reference counts and free list stay as they are, and the
+ * children's rows name no page (-1; zeros where the row's own length is the error).
+ * status is required; child_lengths may be null. */
 GRS_API int grs_cache_fork(int32_t* refcounts, int32_t* free_list, int32_t* free_count,
                            int capacity, const int32_t* parent_table, int64_t parent_stride,
                            int parent_cols, const int32_t* parent_lengths, int n, int page_size,
