@@ -22,6 +22,7 @@ struct AppendArgs {
   int tokens, sequences, group, kv_heads, width, pages, page;
   int units, heads_each, rows, code_bytes, clear;
   int32_t* status;
+  const int32_t* shut;                                // or null: nothing is written while set
 };
 
 // Threads of a CTA: at least one for each unit of a head.
@@ -65,7 +66,8 @@ __device__ __forceinline__ bool append_unit(const AppendArgs& a, int u, AppendUn
   out.n = high - low;
   out.position = low;
   out.kept = low - column * a.page;
-  out.to = -1;
+  out.to = out.from = -1;
+  if (a.shut && *a.shut != 0) return true;            // queries are turned all the same
   int error = GRS_OK;
   if (length != past || column >= a.columns) {
     error = GRS_ERR_LENGTH;
@@ -653,7 +655,7 @@ static int append_run(AppendArgs a, bool interleaved, cudaStream_t stream) {
 
 extern "C" int grs_append_tokens(
     int dtype, int cache_dtype, const void* query, int64_t q_st, int64_t q_sh, void* query_out,
-    int64_t qo_st, int64_t qo_sh, int clear_rest, const void* key, int64_t k_st, int64_t k_sh,
+    int64_t qo_st, int64_t qo_sh, int flags, const void* key, int64_t k_st, int64_t k_sh,
     const void* value, int64_t v_st, int64_t v_sh, void* key_cache, void* value_cache,
     int64_t c_sp, int64_t c_st, int64_t c_sh, float* key_scale, float* value_scale, int64_t s_sp,
     const int32_t* block_table, int64_t bt_stride, const int32_t* source_table,
@@ -671,7 +673,7 @@ extern "C" int grs_append_tokens(
       2 * pairs > head_width || !std::isfinite(magnitude) || num_pages < 0 || max_blocks < 0 ||
       source_blocks < 0 ||
       page_size <= 0 || page_size >= kMost || (int64_t)max_blocks * page_size >= kMost ||
-      (!offsets && tokens != sequences))
+      (!offsets && tokens != sequences) || (flags & GRS_APPEND_GUARDED && !status))
     return GRS_ERR_SHAPE;
   if (tokens == 0) return GRS_OK;
   if (!key || !value || (query && !query_out) || (pairs && !frequencies) ||
@@ -692,7 +694,8 @@ extern "C" int grs_append_tokens(
   a.key_most = pairs ? (float)std::max(1.0, 1.41421366 * std::fabs(magnitude)) : 1.f;
   a.tokens = tokens; a.sequences = sequences; a.group = heads / kv_heads; a.kv_heads = kv_heads;
   a.width = head_width; a.pages = num_pages; a.page = page_size;
-  a.clear = clear_rest && query && offsets; a.status = status;
+  a.clear = flags & GRS_APPEND_CLEAR_REST && query && offsets; a.status = status;
+  a.shut = flags & GRS_APPEND_GUARDED ? status + 1 : nullptr;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (sequences == 0 && !a.clear) return GRS_OK;
   return dtype == GRS_DTYPE_F32 ? append_run<float>(a, interleaved != 0, s)

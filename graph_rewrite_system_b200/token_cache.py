@@ -26,6 +26,7 @@ from .rotary import _check_magnitude, _frequencies, _positions, _turned_out
 
 _pack = _lib.words_of("grs_append_tokens").pack
 _entry = None
+_GUARDED = 2                                  # GRS_APPEND_GUARDED
 
 
 def append_tokens(
@@ -183,13 +184,16 @@ def append_tokens(
         raise ValueError("query_out comes with a query")
     if not tokens:
         return query_out
+    flags = int(fresh)
     word = None if status is not None else _STATUS_AT.get(device)
     if word is None:
+        if status is not None and status.shape == (2,) and status.is_contiguous():
+            status, flags = status[:1], flags | _GUARDED
         word = _status_for(key, device, status)
     if _entry is None:
         _entry = _lib.words_entry("grs_append_tokens")
     code = _entry(_pack(
-        code, cache_code, query_at, q[0], q[1], query_to, qo[0], qo[1], fresh, key.data_ptr(),
+        code, cache_code, query_at, q[0], q[1], query_to, qo[0], qo[1], flags, key.data_ptr(),
         k[0], k[1], value.data_ptr(), v[0], v[1], keys_at, values_at,
         c[0], c[1], c[2], key_at, value_at, scale_row, block_table.data_ptr(), row, source,
         source_row, source_columns, columns, past, begins, places, wide, turns, pairs, bool(interleaved),
@@ -211,12 +215,20 @@ class TokenKVCache(PagePool):
 
     A decode step of beams, parents gathered by the search::
 
-        table = cache.fork_device(parent_table, lengths)   # and release the parents after it
+        table = cache.fork_device(parent_table, lengths)
         for layer in range(layers):
             ...
             query = cache.append(layer, key, value, table, lengths, source_table=parent_table,
                                  query=query, frequencies=frequencies)
             context = cache.attend(layer, query, table, lengths + 1)
+        cache.check_status()
+        cache.release_device(old_table, old_lengths)       # the parents' own rows
+
+    A fork, allocation or release that fails shuts the pages: until
+    ``check_status`` raises its error, later forks make no children and ``append``
+    writes nothing, so a step that ran out of pages leaves its parents as they were.
+    Every layer's ``append`` reads the parents' last pages: released before the last
+    of them, they must not be given out again until then.
     """
 
     def __init__(self, *, layers: int, capacity: int, page_size: int, heads: int,
@@ -237,6 +249,9 @@ class TokenKVCache(PagePool):
         if dtype is _E4M3:
             self.key_scales = torch.ones(layers, capacity, heads, device=self.device)
             self.value_scales = torch.ones_like(self.key_scales)
+        # errors of append and attend, and of the pool's own calls, which guard the append
+        self._words = torch.zeros(2, device=self.device, dtype=torch.int32)
+        self._calls, self._status = self._words[:1], self._words[1:]
 
     # The pool's own launches go where append and attend go: to the stream that this
     # thread pinned on the device, with memory of that stream.
@@ -248,11 +263,21 @@ class TokenKVCache(PagePool):
 
     def reset(self) -> None:
         with self._here():
+            self._calls.zero_()
             super().reset()
 
-    def check_status(self) -> None:
+    def status_tensor(self) -> torch.Tensor:
+        """An error recorded so far (int32 [1], 0 = ok) without synchronising."""
         with self._here():
-            super().check_status()
+            return self._words.amin(0, keepdim=True)
+
+    def check_status(self) -> None:
+        """Raise an error recorded by a kernel since the last check, the pool's first."""
+        with self._here():
+            calls, pool = self._words.tolist()
+            if calls or pool:
+                self._words.zero_()
+                _lib.check(pool or calls, type(self).__name__)
 
     def alloc_pages(self, n: int) -> torch.Tensor:
         with self._here():
@@ -302,7 +327,7 @@ class TokenKVCache(PagePool):
         """``append_tokens`` into one layer's pages (its keyword arguments)."""
         keys, values, key_scale, value_scale = self._layer(layer)
         return append_tokens(key, value, keys, values, block_table, lengths, key_scale=key_scale,
-                             value_scale=value_scale, status=self._status, **options)
+                             value_scale=value_scale, status=self._words, **options)
 
     def attend(self, layer: int, query: torch.Tensor, block_table: torch.Tensor,
                lengths: torch.Tensor, *, scale: float | None = None,
@@ -313,7 +338,7 @@ class TokenKVCache(PagePool):
         keys, values, key_scale, value_scale = self._layer(layer)
         if key_scale is not None:
             return quantized_attention(query, keys, values, key_scale, value_scale, block_table,
-                                       lengths, scale=scale, out=out, status=self._status)
+                                       lengths, scale=scale, out=out, status=self._calls)
         none = keys.new_empty(0, self.heads, self.head_width)
         return shared_prefix_attention(query, none, none, keys, values, block_table, lengths,
-                                       scale=scale, out=out, status=self._status)
+                                       scale=scale, out=out, status=self._calls)

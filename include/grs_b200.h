@@ -682,8 +682,11 @@ GRS_API int grs_rotate_positions(int dtype, const void* query, int64_t q_st, int
  * (null: one each) and lengths[b] tokens in its pages; its token i is written
  * as token lengths[b] + i.  Keys, and queries into query_out (query may be
  * null; query_out may be query), are turned as by grs_rotate_positions, at that
- * position or at positions[token] (pairs 0: not turned).  Query rows of no
- * sequence are left as they were, or zeroed with clear_rest.
+ * position or at positions[token] (pairs 0: not turned).  flags: query rows of no
+ * sequence are left as they were, or zeroed with GRS_APPEND_CLEAR_REST; with
+ * GRS_APPEND_GUARDED nothing is written to the caches and their scales while
+ * status[1] is not zero - the status word of the forks that made the table (status
+ * is two words then; queries are turned all the same).
  * cache_dtype: the inputs', or GRS_DTYPE_E4M3 with the scales [num_pages,
  * kv_heads] (row stride s_sp): a code stands for code * scale.  The scale of a
  * page and head is the smallest power of two, from 2^-118 to 2^119, that holds
@@ -696,9 +699,10 @@ GRS_API int grs_rotate_positions(int dtype, const void* query, int64_t q_st, int
  * two sequences, and none that receives tokens is another's source.
  * Pages outside the cache set GRS_ERR_BAD_PAGE and lengths or tokens that the
  * table cannot hold GRS_ERR_LENGTH in `status`; their tokens are not written. */
+enum { GRS_APPEND_CLEAR_REST = 1, GRS_APPEND_GUARDED = 2 };
 GRS_API int grs_append_tokens(
     int dtype, int cache_dtype, const void* query, int64_t q_st, int64_t q_sh, void* query_out,
-    int64_t qo_st, int64_t qo_sh, int clear_rest, const void* key, int64_t k_st, int64_t k_sh,
+    int64_t qo_st, int64_t qo_sh, int flags, const void* key, int64_t k_st, int64_t k_sh,
     const void* value, int64_t v_st, int64_t v_sh, void* key_cache, void* value_cache,
     int64_t c_sp, int64_t c_st, int64_t c_sh, float* key_scale, float* value_scale, int64_t s_sp,
     const int32_t* block_table, int64_t bt_stride, const int32_t* source_table,

@@ -125,3 +125,141 @@ def test_forks_without_columns(cuda_device):
     with pytest.raises(RuntimeError, match="length"):
         cache.check_status()
     assert cache.allocated_pages == 3
+
+
+def _bits(t):
+    return t.contiguous().view(torch.uint8).clone()
+
+
+def _arenas(cache):
+    return [_bits(t) for t in (cache.keys, cache.values, cache.key_scales, cache.value_scales)
+            if t is not None]
+
+
+def _fill(cache, seed):
+    """Finite rows and scales in every page."""
+    g = torch.Generator().manual_seed(seed)
+    for t in (cache.keys, cache.values):
+        t.copy_(torch.randn(t.shape, generator=g).to(t.dtype))
+    if cache.key_scales is not None:
+        cache.key_scales.fill_(0.5), cache.value_scales.fill_(2.0)
+
+
+def _step(cache, table, lengths, source, qkv, frequencies, offsets=None):
+    """New tokens of every layer and, for one each, their attention."""
+    outs = []
+    for layer in range(cache.layers):
+        q, k, v = qkv[layer].split([4, 2, 2], 1)
+        q = cache.append(layer, k, v, table, lengths, source_table=source, query=q,
+                         frequencies=frequencies, offsets=offsets)
+        outs.append(q)
+        if offsets is None:
+            outs.append(cache.attend(layer, q, table, lengths + 1))
+    return outs
+
+
+def _inputs(dev, tokens, dtype, seed=1):
+    from graph_rewrite_system_b200.rotary import rotary_frequencies
+
+    g = torch.Generator().manual_seed(seed)
+    kind = FP32 if dtype is FP32 else BF16
+    return (torch.randn(2, tokens, 8, 16, generator=g).to(kind).to(dev),
+            rotary_frequencies(16, device=dev))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32, E4M3])
+@pytest.mark.parametrize("kind", FAILURES)
+def test_steps_after_failed_forks_write_nothing(cuda_device, kind, dtype):
+    """Pages and scales of all layers, bit by bit, page 0 of a living row among them;
+    tried again, the step is that of a cache whose fork did not fail."""
+    dev = cuda_device
+    qkv, f = _inputs(dev, 2, dtype)
+    cache, other = (_cache(dev, dtype=dtype, layers=2) for _ in range(2))
+    _fill(cache, 3), _fill(other, 3)
+    table, lengths, asked, past, options, error = _failing(cache, kind)
+    assert int(table.min()) == 0
+    before = _arenas(cache)
+    child = cache.fork_device(asked, past, **options)
+    for columns in (child, torch.nn.functional.pad(child, (0, 2))):
+        _step(cache, columns, lengths, table, qkv, f)
+        _step(cache, columns, past, asked, qkv, f)
+        _step(cache, columns, lengths, None, qkv, f,
+              offsets=torch.tensor([0, 0, 2], dtype=torch.int32, device=dev))
+    assert all(torch.equal(a, b) for a, b in zip(_arenas(cache), before))
+    assert int(cache.status_tensor().item()) < 0
+    with pytest.raises((RuntimeError, ValueError), match=error):
+        cache.check_status()
+    assert int(cache.status_tensor().item()) == 0
+    if kind == "exhausted":
+        cache.reset()
+        assert torch.equal(cache.alloc_pages(4).view(2, 2), table)
+    own = other.alloc_pages(4).view(2, 2)
+    assert torch.equal(own, table)
+    for c in (cache, other):
+        child = c.fork_device(table, lengths)
+        c.outs = _step(c, child, lengths, table, qkv, f)
+        c.check_status()
+    assert all(torch.equal(a, b) for a, b in zip(cache.outs, other.outs))
+    assert all(torch.equal(a, b) for a, b in zip(_arenas(cache), _arenas(other)))
+    assert not all(torch.equal(a, b) for a, b in zip(_arenas(cache), before))
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_prompts_after_failed_allocations_write_nothing(cuda_device, dtype):
+    dev = cuda_device
+    qkv, f = _inputs(dev, 9, dtype)
+    cache = _cache(dev, capacity=4, dtype=dtype, layers=2)
+    _fill(cache, 4)
+    mine = cache.alloc_pages(3).view(1, 3)
+    before = _arenas(cache)
+    table = cache.alloc_pages(3).view(1, 3)               # one page is left
+    zero = torch.zeros(1, dtype=torch.int32, device=dev)
+    offsets = torch.tensor([0, 9], dtype=torch.int32, device=dev)
+    _step(cache, table, zero, None, qkv, f, offsets)
+    assert all(torch.equal(a, b) for a, b in zip(_arenas(cache), before))
+    with pytest.raises(RuntimeError, match="exhausted"):
+        cache.check_status()
+    _step(cache, mine, zero, None, qkv, f, offsets)
+    cache.check_status()
+    assert not all(torch.equal(a, b) for a, b in zip(_arenas(cache), before))
+
+
+def test_errors_of_an_append_do_not_shut_the_pages(cuda_device):
+    """A row without its page is reported; the others, and later calls, are written."""
+    dev = cuda_device
+    qkv, f = _inputs(dev, 2, BF16)
+    cache = _cache(dev, layers=2)
+    _fill(cache, 5)
+    table = cache.alloc_pages(2).view(2, 1)
+    bad = table.clone()
+    bad[0] = -1
+    zero = torch.zeros(2, dtype=torch.int32, device=dev)
+    _step(cache, bad, zero, None, qkv, f)
+    first = _arenas(cache)
+    page = int(table[1, 0])
+    assert torch.equal(cache.values[:, page, 0], qkv[:, 1, 6:])
+    _step(cache, table, zero, None, qkv, f)
+    assert not all(torch.equal(a, b) for a, b in zip(_arenas(cache), first))
+    with pytest.raises(RuntimeError, match="unallocated"):
+        cache.check_status()
+    cache.check_status()
+
+
+def test_a_guard_shuts_the_caches(cuda_device):
+    """append_tokens with a status of two words, whatever is set in the second."""
+    from graph_rewrite_system_b200.token_cache import append_tokens
+
+    dev = cuda_device
+    qkv, f = _inputs(dev, 3, BF16)
+    q, k, v = qkv[0].split([4, 2, 2], 1)
+    pages = torch.zeros(2, 4, 8, 2, 16, dtype=BF16, device=dev)
+    table = torch.arange(3, dtype=torch.int32, device=dev).view(3, 1)
+    lengths = torch.zeros(3, dtype=torch.int32, device=dev)
+    call = lambda status: append_tokens(k, v, pages[0], pages[1], table, lengths, query=q,
+                                        frequencies=f, status=status)
+    for guard in (-1, 1, 1 << 30):
+        words = torch.tensor([0, guard], dtype=torch.int32, device=dev)
+        turned = call(words)
+        assert not pages.any() and int(words[0]) == 0
+    words = torch.zeros(2, dtype=torch.int32, device=dev)
+    assert torch.equal(call(words), turned) and torch.equal(pages[1, :3, 0], v)

@@ -243,3 +243,28 @@ def test_c_abi_refusals():
         expected = getattr(lib, f"grs_{name}")(*{**args, **change}.values())
         assert getattr(lib, f"grs_{name}_words")(table) == expected, (name, change)
         assert getattr(lib, f"grs_{name}_words")(None) == shape
+
+
+def test_guarded_append_refusals(lifted):
+    from graph_rewrite_system_b200.token_cache import append_tokens
+
+    for status in (_i(3), _i(2, 1), _i(4)[::2], _i(2, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="status"):
+            append_tokens(**{**APPEND, "status": status})
+
+
+def test_c_abi_refusals_of_guards_and_forks_without_status():
+    from graph_rewrite_system_b200 import _lib
+
+    values = dict(dtype=0, cache=2, q=256, q_st=1, q_sh=1, qo=256, qo_st=1, qo_sh=1, flags=2,
+                  k=256, k_st=1, k_sh=1, v=256, v_st=1, v_sh=1, kc=256, vc=256, c_sp=1, c_st=1,
+                  c_sh=1, ks=256, vs=256, s_sp=1, bt=256, bt_s=1, src=None, src_s=0, src_blocks=0,
+                  blocks=2, lengths=256, offsets=None, pos=None, wide=0, freq=256, pairs=16,
+                  inter=0, mag=1.0, tokens=1, seqs=1, heads=4, kv=2, width=32, pages=5, page=16,
+                  status=None, stream=None).values()
+    assert _lib.lib().grs_append_tokens(*values) == -4
+    fork = dict(refs=256, free=256, count=256, capacity=4, table=256, stride=1, cols=1, lengths=256,
+                n=1, page=4, child=256, c_stride=2, c_lengths=256, c_cols=2, status=None,
+                stream=None)
+    for change in (dict(), dict(cols=-1, status=256)):
+        assert _lib.lib().grs_cache_fork(*{**fork, **change}.values()) == -4, change
