@@ -20,6 +20,7 @@ Two layers:
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import numpy as np
@@ -46,42 +47,53 @@ class PagePool:
             raise RuntimeError(f"{type(self).__name__} lives in CUDA memory (no CPU fallback)")
         self.capacity, self.page_size, self.device = capacity, page_size, device
         i32 = dict(device=device, dtype=torch.int32)
-        self._refcounts = torch.empty(capacity, **i32)
-        self._free = torch.empty(capacity, **i32)
-        self._free_count = torch.empty(1, **i32)
-        self._last_pos = torch.empty(capacity, **i32)
-        self._status = torch.zeros(1, **i32)
-        _lib.check(_lib.lib().grs_cache_init(
-            self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
-            self._last_pos.data_ptr(), capacity, self._stream()), type(self).__name__)
+        with self._here():
+            self._refcounts = torch.empty(capacity, **i32)
+            self._free = torch.empty(capacity, **i32)
+            self._free_count = torch.empty(1, **i32)
+            self._last_pos = torch.empty(capacity, **i32)
+            self._status = torch.zeros(1, **i32)
+            self._all_free()
 
-    def reset(self) -> None:
-        """Return every page to the free list (the state of a new cache)."""
-        self._status.zero_()
+    def _all_free(self) -> None:
         _lib.check(_lib.lib().grs_cache_init(
             self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
             self._last_pos.data_ptr(), self.capacity, self._stream()), type(self).__name__)
+
+    def reset(self) -> None:
+        """Return every page to the free list (the state of a new cache)."""
+        with self._here():
+            self._status.zero_()
+            self._all_free()
 
     def status_tensor(self) -> torch.Tensor:
         """The device status word (0 = ok) without synchronising."""
         return self._status
 
-    # ---- state views (device -> host) -------------------------------------
+    # Where the pool's launches go, and the context that its torch calls enter: every
+    # call of one kind or the other goes to one stream.
     def _stream(self) -> int:
         return torch.cuda.current_stream(self.device).cuda_stream
 
+    def _here(self):
+        return nullcontext()
+
+    # ---- state views (device -> host) -------------------------------------
     @property
     def refcounts(self) -> list[int]:
-        return self._refcounts.tolist()
+        with self._here():
+            return self._refcounts.tolist()
 
     @property
     def free(self) -> list[int]:
-        count = int(self._free_count.item())
-        return self._free[:count].tolist()
+        with self._here():
+            count = int(self._free_count.item())
+            return self._free[:count].tolist()
 
     @property
     def allocated_pages(self) -> int:
-        return self.capacity - int(self._free_count.item())
+        with self._here():
+            return self.capacity - int(self._free_count.item())
 
     def free_count_tensor(self) -> torch.Tensor:
         """The device free-page count (int32 [1]) itself, no synchronisation."""
@@ -89,7 +101,8 @@ class PagePool:
 
     def allocated_pages_tensor(self) -> torch.Tensor:
         """Allocated page count as a device scalar (no synchronisation)."""
-        return self.capacity - self._free_count
+        with self._here():
+            return self.capacity - self._free_count
 
     @staticmethod
     def empty_handle() -> PrefixHandle:
@@ -97,35 +110,38 @@ class PagePool:
 
     def check_status(self) -> None:
         """Raise the first error recorded by a kernel since the last check."""
-        code = int(self._status.item())
-        if code:
-            self._status.zero_()
-            _lib.check(code, type(self).__name__)
+        with self._here():
+            code = int(self._status.item())
+            if code:
+                self._status.zero_()
+                _lib.check(code, type(self).__name__)
 
     def release_device(self, table: torch.Tensor, lengths: torch.Tensor) -> None:
         """Release handles given as device rows, in row order (no sync)."""
         n = lengths.shape[0]
         if n == 0:
             return
-        table = table.to(torch.int32)
-        if table.stride(-1) != 1:
-            table = table.contiguous()
-        lengths = lengths.to(torch.int32).contiguous()
-        _lib.check(_lib.lib().grs_cache_release(
-            self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
-            self._last_pos.data_ptr(), self.capacity, table.data_ptr(), table.stride(0),
-            lengths.data_ptr(), n, table.shape[1], self.page_size, self._status.data_ptr(),
-            self._stream()), "release")
+        with self._here():
+            table = table.to(torch.int32)
+            if table.stride(-1) != 1:
+                table = table.contiguous()
+            lengths = lengths.to(torch.int32).contiguous()
+            _lib.check(_lib.lib().grs_cache_release(
+                self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
+                self._last_pos.data_ptr(), self.capacity, table.data_ptr(), table.stride(0),
+                lengths.data_ptr(), n, table.shape[1], self.page_size, self._status.data_ptr(),
+                self._stream()), "release")
 
     def alloc_pages(self, n: int) -> torch.Tensor:
         """Allocate n pages (refcount 1, free-list order) for contents copied
         in from another cache; returns their ids (device int32)."""
-        pages = torch.empty(n, device=self.device, dtype=torch.int32)
-        if n:
-            _lib.check(_lib.lib().grs_cache_alloc(
-                self._refcounts.data_ptr(), self._free.data_ptr(), self._free_count.data_ptr(),
-                self.capacity, n, pages.data_ptr(), self._status.data_ptr(), self._stream()),
-                "alloc_pages")
+        with self._here():
+            pages = torch.empty(n, device=self.device, dtype=torch.int32)
+            if n:
+                _lib.check(_lib.lib().grs_cache_alloc(
+                    self._refcounts.data_ptr(), self._free.data_ptr(),
+                    self._free_count.data_ptr(), self.capacity, n, pages.data_ptr(),
+                    self._status.data_ptr(), self._stream()), "alloc_pages")
         return pages
 
     def _handle_rows(self, handles: list[PrefixHandle], min_cols: int = 1):
@@ -139,16 +155,18 @@ class PagePool:
                 raise ValueError("prefix handle names a page outside the cache")
             rows[i, : len(h.blocks)] = h.blocks
             lengths[i] = h.length
-        table = torch.from_numpy(rows).to(self.device, non_blocking=True)
-        length_tensor = torch.from_numpy(lengths).to(self.device, non_blocking=True)
+        with self._here():
+            table = torch.from_numpy(rows).to(self.device, non_blocking=True)
+            length_tensor = torch.from_numpy(lengths).to(self.device, non_blocking=True)
         return table, length_tensor
 
     def release(self, handle: PrefixHandle) -> None:
         if not handle.blocks:
             return
-        table, lengths = self._handle_rows([handle])
-        self.release_device(table, lengths)
-        self.check_status()
+        with self._here():                    # the rows' memory goes back where it came from
+            table, lengths = self._handle_rows([handle])
+            self.release_device(table, lengths)
+            self.check_status()
 
     def block_table(self, handles: list[PrefixHandle]) -> tuple[torch.Tensor, torch.Tensor]:
         """Padded physical page ids (>= 1 column) and logical lengths (int32)."""

@@ -242,19 +242,20 @@ class TokenKVCache(PagePool):
             device = torch.device("cuda", torch.cuda.current_device())
         super().__init__(capacity, page_size, device)
         self.layers, self.heads, self.head_width, self.dtype = layers, heads, head_width, dtype
-        self.keys = torch.empty(layers, capacity, page_size, heads, head_width,
-                                device=self.device, dtype=dtype)
-        self.values = torch.empty_like(self.keys)
         self.key_scales = self.value_scales = None
-        if dtype is _E4M3:
-            self.key_scales = torch.ones(layers, capacity, heads, device=self.device)
-            self.value_scales = torch.ones_like(self.key_scales)
-        # errors of append and attend, and of the pool's own calls, which guard the append
-        self._words = torch.zeros(2, device=self.device, dtype=torch.int32)
+        with self._here():
+            self.keys = torch.empty(layers, capacity, page_size, heads, head_width,
+                                    device=self.device, dtype=dtype)
+            self.values = torch.empty_like(self.keys)
+            if dtype is _E4M3:
+                self.key_scales = torch.ones(layers, capacity, heads, device=self.device)
+                self.value_scales = torch.ones_like(self.key_scales)
+            # errors of append and attend, and of the pool's own calls, which guard the append
+            self._words = torch.zeros(2, device=self.device, dtype=torch.int32)
         self._calls, self._status = self._words[:1], self._words[1:]
 
-    # The pool's own launches go where append and attend go: to the stream that this
-    # thread pinned on the device, with memory of that stream.
+    # All that the cache does, its making among it, goes where append and attend go: to
+    # the stream that this thread pinned on the device, with memory of that stream.
     def _stream(self) -> int:
         return _lib.stream_on(self.device.index)
 
@@ -278,14 +279,6 @@ class TokenKVCache(PagePool):
             if calls or pool:
                 self._words.zero_()
                 _lib.check(pool or calls, type(self).__name__)
-
-    def alloc_pages(self, n: int) -> torch.Tensor:
-        with self._here():
-            return super().alloc_pages(n)
-
-    def release_device(self, table: torch.Tensor, lengths: torch.Tensor) -> None:
-        with self._here():
-            super().release_device(table, lengths)
 
     def _layer(self, layer: int) -> tuple:
         scales = (None, None)
