@@ -837,8 +837,9 @@ __global__ void __launch_bounds__(32 * QT_WARPS, (QsShape<T, DP, kTiles>::kCtas)
       for (int i = threadIdx.x; i <= a.batch; i += 32 * QT_WARPS) a.starts[i] = starts[i] >> kBits;
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {     // rows without keys
       if (starts[b] >> kBits != starts[b + 1] >> kBits) continue;
-      for (int i = threadIdx.x; i < a.heads * a.D; i += 32 * QT_WARPS)
-        static_cast<T*>(a.out)[b * a.o_sb + i / a.D * a.o_sh + i % a.D] = from_float<T>(0.f);
+      for (int h = warp; h < a.heads; h += QT_WARPS)            // (a row may pass 2^31 elements)
+        for (int d = lane; d < a.D; d += 32)
+          static_cast<T*>(a.out)[b * a.o_sb + h * a.o_sh + d] = from_float<T>(0.f);
     }
     const QsCut cut(a.ranges, starts[a.batch] >> kBits);
     if (range >= cut.ranges) return;

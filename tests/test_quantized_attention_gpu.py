@@ -403,3 +403,28 @@ def test_captured_and_two_calls_at_once(cuda_device, many):
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], other)
         _check(outs[0], args)
     assert torch.equal(outs[0], eager)
+
+
+def test_empty_rows_past_31_bits(cuda_device):
+    """A row without keys that has 2^31 elements is zeroed, between two that have keys
+    (ranges of tiles; every head's output is the value of its only key)."""
+    from graph_rewrite_system_b200.quantized_attention import quantized_attention
+
+    heads, width = 1 << 24, 128
+    if torch.cuda.mem_get_info()[0] < 5 * 2 * heads * width + 4 * heads * (width + 1) * 4:
+        pytest.skip("needs 60 GB")
+    dev = cuda_device
+    query = torch.ones(1, 1, 1, dtype=BF16, device=dev).expand(2, heads, width).contiguous()
+    codes = torch.ones(2, 3, 8, 1, width, device=dev).to(E4M3)
+    scales = torch.ones(2, 3, 1, device=dev)
+    for lengths in ([0, 1], [1, 0], [0, 0]):
+        out = torch.full_like(query, 5.0)
+        got = quantized_attention(
+            query, codes[0], codes[1], scales[0], scales[1],
+            torch.zeros(2, 200, dtype=torch.int32, device=dev),
+            torch.tensor(lengths, dtype=torch.int32, device=dev), out=out)
+        for row, length in zip(got, lengths):
+            assert bool((row == float(length)).all())
+        del out, got
+    del query
+    torch.cuda.empty_cache()
