@@ -19,14 +19,18 @@ namespace grs {
 struct RotaryStep {
   uint64_t hi, lo;
 };
+// A whole number from -2^63 to 2^63, modulo 2^64: half a turn, 2^63, is no int64.
+__device__ __forceinline__ uint64_t rotary_units(double x) {
+  return x < 0 ? (uint64_t)__double2ll_rn(x) : __double2ull_rn(x);
+}
 __device__ __forceinline__ RotaryStep rotary_step(double f) {
   constexpr double hi = 0x1.45f306dc9c883p-3, lo = -0x1.6b01ec5417056p-57;
   const double t = f * hi;
-  const double rest = fma(f, hi, -t) + f * lo;
+  double rest = fma(f, hi, -t) + f * lo;
+  rest -= rint(rest);                       // whole turns of f from 2^53 on
   const double a = (t - rint(t)) * 0x1p64, whole = rint(a);     // both exact
   const double b = (a - whole) + rest * 0x1p64, low = floor(b);
-  return {(uint64_t)__double2ll_rn(whole) + (uint64_t)__double2ll_rn(low),
-          __double2ull_rz((b - low) * 0x1p64)};
+  return {rotary_units(whole) + rotary_units(low), __double2ull_rz((b - low) * 0x1p64)};
 }
 // The phase of a position, a fraction of a turn in units of 2^-64.
 __device__ __forceinline__ uint64_t rotary_phase(int64_t position, RotaryStep step) {

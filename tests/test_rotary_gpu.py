@@ -194,3 +194,27 @@ def test_far_rows(cuda_device):
     f = _freq(64)
     got = rotate_positions(far, None, p.to(cuda_device), f.to(cuda_device), query_out=far)
     _check(got[0], q, p, f)
+
+
+@pytest.mark.parametrize("far", [1000, 2 ** 45, 2 ** 62])
+def test_steps_of_half_a_turn(cuda_device, far):
+    """Frequencies whose step rounds to half a turn and whole ones, at positions where
+    one unit of the step's last place would be seen."""
+    pi = 3.141592653589793
+    f = torch.tensor([pi, 5 * pi, 9 * pi, 3 * pi, -pi, -5 * pi, 2 * pi, 7 * pi],
+                     dtype=torch.float64)
+    q, k, p = _case(11, 30, 2, 1, 16, FP32, far, torch.int64)
+    p[0], p[1] = far, -far
+    got = _call(cuda_device, q, k, p, f)
+    _check(got[0], q, p, f)
+    _check(got[1], k, p, f)
+
+
+def test_frequencies_of_many_turns(cuda_device):
+    """Up to 2^60 radians a position; 1 / (2 pi) is held to 2^-108, which leaves them
+    2^-40 of a turn at these positions."""
+    f = torch.tensor([1e15, 2.0 ** 52 * 7, 1e17, -3e17, 2.0 ** 60, 1e9, 0.3, -1e16],
+                     dtype=torch.float64)
+    q, k, p = _case(12, 30, 2, 1, 16, FP32, 100)
+    got = _call(cuda_device, q, k, p, f)
+    _check(got[0], q, p, f)
