@@ -673,6 +673,7 @@ extern "C" int grs_append_tokens(
       2 * pairs > head_width || !std::isfinite(magnitude) || num_pages < 0 || max_blocks < 0 ||
       source_blocks < 0 ||
       page_size <= 0 || page_size >= kMost || (int64_t)max_blocks * page_size >= kMost ||
+      (!codes && source_table && (int64_t)page_size * head_width > INT_MAX) ||
       (!offsets && tokens != sequences) || (flags & GRS_APPEND_GUARDED && !status))
     return GRS_ERR_SHAPE;
   if (tokens == 0) return GRS_OK;

@@ -128,6 +128,8 @@ def append_tokens(
         if key_scale is not None or value_scale is not None:
             raise ValueError("scales come with 8-bit caches")
         c = _cache(key_cache, value_cache, pool, device, dtype, kv_heads, width)
+        if source_table is not None and page * width >= 1 << 31:
+            raise ValueError("rows are copied between pages of less than 2^31 elements a head")
     if c[2] < width or c[1] < c[2] * kv_heads or c[0] < c[1] * page:
         need = 1                              # not pages of rows of heads: any order will do
         for size, step in sorted(zip(pool, c), key=lambda p: p[1]):

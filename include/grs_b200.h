@@ -695,7 +695,8 @@ GRS_API int grs_rotate_positions(int dtype, const void* query, int64_t q_st, int
  * there and it is larger; those rows move to a new scale.  Infinities become NaN.
  * source_table (or null): the rows that a sequence has in its first page to
  * receive tokens are copied from that table's page (int32 [sequences,
- * source_blocks]; wide enough for the tokens that are there).  No page receives tokens of
+ * source_blocks]; wide enough for the tokens that are there; pages of the inputs' type
+ * then have less than 2^31 elements a head).  No page receives tokens of
  * two sequences, and none that receives tokens is another's source.
  * Pages outside the cache set GRS_ERR_BAD_PAGE and lengths or tokens that the
  * table cannot hold GRS_ERR_LENGTH in `status`; their tokens are not written. */

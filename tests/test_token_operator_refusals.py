@@ -268,3 +268,28 @@ def test_c_abi_refusals_of_guards_and_forks_without_status():
                 stream=None)
     for change in (dict(), dict(cols=-1, status=256)):
         assert _lib.lib().grs_cache_fork(*{**fork, **change}.values()) == -4, change
+
+
+def test_pages_whose_rows_pass_31_bits(lifted):
+    """Kept rows are counted in pieces, up to an element each, in 32 bits."""
+    from graph_rewrite_system_b200.token_cache import append_tokens
+
+    huge = lambda: _z(1, 1, 1, 256).expand(2, 1 << 23, 1, 256)
+    args = dict(key=_z(3, 1, 256), value=_z(3, 1, 256), key_cache=huge(), value_cache=huge(),
+                block_table=_i(3, 2), lengths=_i(3), status=_i(1))
+    with pytest.raises(ValueError, match="2\\^31 elements"):
+        append_tokens(**args, source_table=_i(3, 2))
+    with pytest.raises(ValueError, match="overlap"):       # and without a source the next check
+        append_tokens(**args)
+
+
+def test_c_abi_refuses_pages_whose_rows_pass_31_bits():
+    from graph_rewrite_system_b200 import _lib
+
+    values = dict(dtype=0, cache=0, q=None, q_st=1, q_sh=1, qo=None, qo_st=1, qo_sh=1, flags=0,
+                  k=256, k_st=1, k_sh=1, v=256, v_st=1, v_sh=1, kc=256, vc=256, c_sp=1, c_st=1,
+                  c_sh=1, ks=None, vs=None, s_sp=0, bt=256, bt_s=1, src=256, src_s=1, src_blocks=2,
+                  blocks=2, lengths=256, offsets=None, pos=None, wide=0, freq=None, pairs=0,
+                  inter=0, mag=1.0, tokens=1, seqs=1, heads=0, kv=1, width=256, pages=2,
+                  page=1 << 23, status=None, stream=None).values()
+    assert _lib.lib().grs_append_tokens(*values) == -4
