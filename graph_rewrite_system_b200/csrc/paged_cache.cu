@@ -30,14 +30,14 @@ __device__ __forceinline__ int blocks_for(int length, int page) {
 }
 
 // One thread per parent: retain shared pages, allocate the child page, write
-// the child block-table row and length.  kWhole: all children or none - with an
-// error in the status word (cache_fork_check_kernel's, or an earlier one) nothing is
-// retained or taken, and the rows name no page (-1; zeros where the row's own length
-// is the error).
+// the child block-table row and length.  kWhole: all children or none, behind
+// cache_fork_check_kernel, which left each child's page in its row - with an error in
+// the status word (its own, or an earlier one) nothing is retained or taken, and the
+// rows name no page (-1; zeros where the row's own length is the error).
 template <bool kWhole>
 __global__ void cache_fork_kernel(int32_t* __restrict__ refcounts,
                                   const int32_t* __restrict__ free_list,
-                                  const int32_t* __restrict__ free_count, int capacity,
+                                  int32_t* __restrict__ free_count, int capacity,
                                   const int32_t* __restrict__ ptable, int64_t pstride, int pcols,
                                   const int32_t* __restrict__ plengths, int n, int page,
                                   int32_t* __restrict__ ctable, int64_t cstride,
@@ -82,12 +82,13 @@ __global__ void cache_fork_kernel(int32_t* __restrict__ refcounts,
     }
     crow[j] = p;
   }
-  const int fc = *free_count;
   int page_id = 0;
+  const int fc = kWhole ? n : *free_count;
+  if (kWhole && i == 0) *free_count -= n;   // no other thread reads it
   if (i >= fc) {
     set_status(status, GRS_ERR_EXHAUSTED);
   } else {
-    const int candidate = free_list[fc - 1 - i];
+    const int candidate = kWhole ? crow[keep] : free_list[fc - 1 - i];
     if (candidate < 0 || candidate >= capacity || refcounts[candidate] != 0) {
       set_status(status, GRS_ERR_CORRUPT);
     } else {
@@ -101,13 +102,15 @@ __global__ void cache_fork_kernel(int32_t* __restrict__ refcounts,
 }
 
 // Whether every child of a fork can have its row: a thread per parent's page, and one per
-// child for its length, columns and page of the free list.  Changes nothing.
+// child for its length, columns and page of the free list.  Writes that page into the
+// child's row, and changes nothing else.
 __global__ void cache_fork_check_kernel(const int32_t* __restrict__ refcounts,
                                         const int32_t* __restrict__ free_list,
                                         const int32_t* __restrict__ free_count, int capacity,
                                         const int32_t* __restrict__ ptable, int64_t pstride,
                                         int pcols, const int32_t* __restrict__ plengths, int n,
-                                        int page, int ccols, int32_t* __restrict__ status) {
+                                        int page, int32_t* __restrict__ ctable, int64_t cstride,
+                                        int ccols, int32_t* __restrict__ status) {
   const int64_t each = (int64_t)pcols + 1, all = n * each;
   for (int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; idx < all;
        idx += (int64_t)gridDim.x * blockDim.x) {
@@ -126,17 +129,13 @@ __global__ void cache_fork_check_kernel(const int32_t* __restrict__ refcounts,
         error = GRS_ERR_EXHAUSTED;
       else if (candidate < 0 || candidate >= capacity || refcounts[candidate] != 0)
         error = GRS_ERR_CORRUPT;
+      if (error == GRS_OK) ctable[i * cstride + keep] = candidate;
     } else if (held && j < keep) {
       const int p = ptable[i * pstride + j];
       if (p < 0 || p >= capacity || refcounts[p] <= 0) error = GRS_ERR_BAD_PAGE;
     }
     if (error != GRS_OK) set_status(status, error);
   }
-}
-
-// The pages that the fork of n children took, off the free count.
-__global__ void cache_taken_kernel(int32_t* free_count, int n, const int32_t* status) {
-  if (*status == GRS_OK) *free_count -= n;
 }
 
 // Copy `rows` rows of `row_bytes` bytes from page src to page dst within one
@@ -494,13 +493,11 @@ extern "C" int grs_cache_fork(int32_t* refcounts, int32_t* free_list, int32_t* f
   cache_fork_check_kernel<<<(int)std::min<int64_t>((checks + 255) / 256, 16 * 148), 256, 0,
                             grs::counted(s)>>>(
       refcounts, free_list, free_count, capacity, parent_table, parent_stride, parent_cols,
-      parent_lengths, n, page_size, child_cols, status);
+      parent_lengths, n, page_size, child_table, child_stride, child_cols, status);
   GRS_CUDA_CHECK_LAUNCH();
   cache_fork_kernel<true><<<ceil_div(n, 128), 128, 0, grs::counted(s)>>>(
       refcounts, free_list, free_count, capacity, parent_table, parent_stride, parent_cols,
       parent_lengths, n, page_size, child_table, child_stride, child_lengths, child_cols, status);
-  GRS_CUDA_CHECK_LAUNCH();
-  cache_taken_kernel<<<1, 1, 0, grs::counted(s)>>>(free_count, n, status);
   GRS_CUDA_CHECK_LAUNCH();
   return GRS_OK;
 }
