@@ -124,8 +124,12 @@ __global__ void __launch_bounds__(128) quant_rows_kernel(QuantArgs a) {
 // token and tile: 79 us against 70 for 64 sequences of up to 4099 tokens).
 constexpr int QT_WARPS = 4;
 constexpr int QT_STAGES = 3;
-constexpr float QT_LIFT = 9.f;              // weights are at most 2^(9 + 6): f16 holds them to
-constexpr float QT_SLACK = 6.f;             // 2^-24, 2^-33 of the largest
+// Weights go into the value products in f16: the largest between 2^9 and 2^15, the smallest
+// that it holds 2^-24, 2^-33 of the largest.  One f16 is off by 2^-11 of a weight at most,
+// 2e-4 in the mean, beside the 1.7e-3 of the norm that rounding the output to bf16 costs;
+// fp32 takes two parts, 22 bits, for queries and weights.
+constexpr float QT_LIFT = 9.f;
+constexpr float QT_SLACK = 6.f;
 constexpr uint32_t QT_ABSENT = 0xffffffffu; // key scale of a token that is not there
 constexpr float QT_UNSET = -3e38f;          // a reference before the first score
 
@@ -704,12 +708,14 @@ __global__ void __launch_bounds__(32 * QT_WARPS) quant_mma_kernel(QuantArgs a) {
 // the workspace, at most two of a range, and are joined by quant_join_kernel.  Two, three
 // or five ranges a warp balance no better than their starts cost (73, 79, 91 us against 63).
 // bf16, 32/8 heads of 128: 64 sequences of 300 to 4099 tokens 60 us (310 MB, 5.2 TB/s; 55 %
-// of the issue slots), 512 of 2048 to 4096 483 us = 6.6 TB/s, a plain copy's rate, 2 of up to
+// of the issue slots), 512 of 2048 to 4096 484 us = 6.6 TB/s, a plain copy's rate (568, 5.6
+// TB/s, after 40 ms of load and more: the clocks sink under the power limit), 2 of up to
 // 131000 86 to 94 us.  Narrow heads and fp32 are bound by instructions: 200 sequences of up
 // to 1001 tokens of 8 heads of 32 take 27 us in bf16 and 29 to 30 in fp32, which HBM would
-// read in 6 to 8.
+// read in 6 to 8 (249 and 275 a tile; fp32 spills 108 bytes at the 96 registers of five CTAs).
 constexpr int QS_SHORT = 1024;              // tokens of a table row that one warp takes
 constexpr int QS_MOST = 1024;               // sequences: their first tiles are in shared memory
+// (1024 of 300 to 2000 tokens 385 us by ranges, 1025 in slices of four warps 397)
 
 template <typename T, int DP, int kTiles>
 struct QsShape {
@@ -1168,7 +1174,8 @@ static int quant_ranges(int batch, int heads, int kv_heads, int D, int64_t room,
 // are up to the number given; 32/8 heads of 128: 1000 sequences of 256 / 512 / 1000 tokens
 // 58 / 98 / 181 us against 83 / 119 / 191 by ranges, 500 of 500 57 against 66, 200 of 1000
 // 60 against 52; 14/2 heads of 40: 800 of 700 33 against 38; 40/4 heads of 64: 300 of 500
-// 25 against 36; 8/8 heads of 32: 200 of 1000 31 against 27).
+// 25 against 36; 8/8 heads of 32: 200 of 1000 31 against 27).  The table's width stands for
+// the lengths, which are on the device: wider tables lose that difference.
 static bool quant_whole(int batch, int heads, int kv_heads, int D, int64_t room) {
   const int group = heads / kv_heads, chunk = quant_wide(group, D) ? 16 : 8;
   const int64_t units = (int64_t)kv_heads * ((group + chunk - 1) / chunk);

@@ -65,8 +65,8 @@ def append_tokens(
     fp32 [pages, Hkv], which the call writes: a code stands for code * scale.
     The scale of a page and head is the smallest power of two (from 2^-118 to
     2^119) that holds the largest finite value of its new rows within 448 (for
-    turned keys the value before turning, times sqrt(2) * max(1, |magnitude|)
-    at most), or the page's old scale if rows are there and it is larger; rows
+    turned keys the value before turning, times max(1, sqrt(2) * |magnitude|)),
+    or the page's old scale if rows are there and it is larger; rows
     that are there move to a new scale.  Infinite values are held as NaN.  The
     rows of a page behind the new ones are left as they were.
 
@@ -74,7 +74,8 @@ def append_tokens(
     its first page to receive tokens are copied from the page that this table
     names there - the parent's, after a fork - as are their scales.  No page may
     receive tokens of two sequences, or receive tokens and be another's source;
-    the caches overlap none of the inputs.
+    the caches overlap none of the inputs; pages that are not 8-bit hold less than
+    2^31 elements a head.
 
     Tokens whose pages lie outside the cache or whose place the table does not
     hold are not written (kept rows without a source stay unspecified), which ``status`` records (default: the device word

@@ -690,7 +690,7 @@ GRS_API int grs_rotate_positions(int dtype, const void* query, int64_t q_st, int
  * cache_dtype: the inputs', or GRS_DTYPE_E4M3 with the scales [num_pages,
  * kv_heads] (row stride s_sp): a code stands for code * scale.  The scale of a
  * page and head is the smallest power of two, from 2^-118 to 2^119, that holds
- * the largest finite value of its new rows (times sqrt(2) max(1, |magnitude|)
+ * the largest finite value of its new rows (times max(1, sqrt(2) |magnitude|)
  * for turned keys, before they are turned) in 448, or the old scale if rows are
  * there and it is larger; those rows move to a new scale.  Infinities become NaN.
  * source_table (or null): the rows that a sequence has in its first page to
